@@ -11,9 +11,9 @@ import os
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libbzpf.so")
 
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 
-vp, i32, i64, f32 = C.c_void_p, C.c_int, C.c_int64, C.c_float
+vp, i32, i64, f32, f64 = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_double
 
 # name -> argtypes (restype is int unless listed in _RESTYPES)
 SIGNATURES = {
@@ -21,6 +21,12 @@ SIGNATURES = {
     "bzpf_last_error": [],
     "bzpf_row_pitch": [i64],
     "bzpf_layernorm": [vp, i32, vp, vp, f32, vp, i32, i64, i32, vp],
+    "bzpf_layernorm_bwd_ws": [i64, i32],
+    "bzpf_layernorm_bwd": [vp, i32, vp, i32, vp, f32, vp, vp, vp, vp, i64, i64, i32, vp],
+    "bzpf_dropout": [vp, i32, f64, vp, i32, i32, i64, i64, vp, i32, i64, i64, vp],
+    "bzpf_dropout_add_ln": [vp, vp, i32, f64, vp, i32, i32, i64, i64, vp, vp, f32, vp, vp, i32, i64, i32, vp],
+    "bzpf_dropout_add_ln_bwd": [vp, vp, i32, vp, vp, f32, f64, vp, i32, i32, i64, i64, vp, vp, i32, vp, vp, vp, i64, i64,
+                                i32, vp],
     "bzpf_add_ln": [vp, vp, i32, f32, i32, vp, vp, f32, vp, i32, i32, i64, i32, vp],
     "bzpf_count_nonfinite": [vp, i32, i64, vp, vp],
     "bzpf_linear_gated": [vp, vp, vp, vp, i64, i64, vp, i32, i64, i32, i32, vp],
@@ -65,7 +71,7 @@ SIGNATURES = {
     "bzpf_pair_bias": [vp, vp, vp, f32, vp, vp, i32, i64, i32, i32, vp],
 }
 _RESTYPES = {"bzpf_version": C.c_char_p, "bzpf_last_error": C.c_char_p, "bzpf_row_pitch": i64,
-             "bzpf_pwa_wsplit_bytes": i64}
+             "bzpf_pwa_wsplit_bytes": i64, "bzpf_layernorm_bwd_ws": i64}
 
 _lib = None
 

@@ -1,4 +1,5 @@
 // C-ABI entry points (declared in include/bzpf.h): argument validation, dispatch to the launchers, error capture.
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 
@@ -28,6 +29,11 @@ int done(hipError_t e, const char* what) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool dt_ok(int dt) { return dt == BZPF_F32 || dt == BZPF_F16; }
+// The training entry points: bf16 too, but not fp16 and bf16 in one call; pointers at element alignment.
+bool dt3_ok(int dt) { return dt_ok(dt) || dt == BZPF_BF16; }
+bool pair_ok(int a, int b) { return dt3_ok(a) && dt3_ok(b) && (a == b || a == BZPF_F32 || b == BZPF_F32); }
+bool aligned_el(const void* p, int dt) { return (reinterpret_cast<uintptr_t>(p) & (dt == BZPF_F32 ? 3u : 1u)) == 0; }
+bool width_ok(int64_t D) { return D >= bzpf::ROW_MIN_D && D <= bzpf::ROW_MAX_D; }
 hipStream_t S(void* s) { return static_cast<hipStream_t>(s); }
 
 }  // namespace
@@ -36,6 +42,7 @@ hipStream_t S(void* s) { return static_cast<hipStream_t>(s); }
   do {                     \
     if (!(cond)) return fail(BZPF_EINVAL, __VA_ARGS__); \
   } while (0)
+#define REQUIRE_EL(p, dt) REQUIRE((p) != nullptr && aligned_el(p, dt), "%s: %s must be non-null and aligned to its elements", __func__, #p)
 #define REQUIRE_PTR(p) REQUIRE((p) != nullptr && aligned16(p), "%s: %s must be a non-null 16-byte aligned pointer", __func__, #p)
 
 extern "C" {
@@ -48,14 +55,118 @@ int64_t bzpf_row_pitch(int64_t N) { return bzpf::row_pitch(N); }
 
 int bzpf_layernorm(const void* x, int x_dt, const float* w, const float* b, float eps, void* y, int y_dt,
                    int64_t rows, int D, void* stream) {
-  REQUIRE_PTR(x);
-  REQUIRE_PTR(y);
-  REQUIRE(dt_ok(x_dt) && dt_ok(y_dt), "bzpf_layernorm: bad dtype %d/%d", x_dt, y_dt);
-  REQUIRE(D % 64 == 0 && D >= 64 && D <= 1024 && (D / 64 <= 6 || D / 64 == 8 || D / 64 == 12 || D / 64 == 16),
-          "bzpf_layernorm: unsupported D=%d", D);
+  REQUIRE(pair_ok(x_dt, y_dt), "bzpf_layernorm: bad dtype %d/%d", x_dt, y_dt);
+  REQUIRE(width_ok(D), "bzpf_layernorm: unsupported D=%d", D);
   REQUIRE(rows >= 0, "bzpf_layernorm: rows < 0");
   if (rows == 0) return BZPF_OK;
-  return done(bzpf::launch_layernorm(x, x_dt, w, b, eps, y, y_dt, rows, D, S(stream)), "bzpf_layernorm");
+  REQUIRE_EL(x, x_dt);
+  REQUIRE_EL(y, y_dt);
+  REQUIRE(aligned_el(w, BZPF_F32) && aligned_el(b, BZPF_F32), "bzpf_layernorm: w or b misaligned");
+  const bool narrow = D % 64 == 0 && (D / 64 <= 6 || D / 64 == 8 || D / 64 == 12 || D / 64 == 16);
+  if (narrow && dt_ok(x_dt) && dt_ok(y_dt) && aligned16(x) && aligned16(y) && aligned16(w) && aligned16(b))
+    return done(bzpf::launch_layernorm(x, x_dt, w, b, eps, y, y_dt, rows, D, S(stream)), "bzpf_layernorm");
+  return done(bzpf::launch_layernorm_rows(x, x_dt, w, b, eps, y, y_dt, rows, D, S(stream)), "bzpf_layernorm");
+}
+
+int64_t bzpf_layernorm_bwd_ws(int64_t rows, int D) {
+  return rows >= 0 && width_ok(D) ? bzpf::row_grad_ws_bytes(rows, D) : -1;
+}
+
+int bzpf_layernorm_bwd(const void* dy, int dy_dt, const void* x, int x_dt, const float* w, float eps, void* dx,
+                       float* dw, float* db, float* ws, int64_t ws_bytes, int64_t rows, int D, void* stream) {
+  REQUIRE(pair_ok(x_dt, dy_dt), "bzpf_layernorm_bwd: bad dtype %d/%d", x_dt, dy_dt);
+  REQUIRE(width_ok(D), "bzpf_layernorm_bwd: unsupported D=%d", D);
+  REQUIRE(rows >= 1, "bzpf_layernorm_bwd: rows < 1");
+  REQUIRE_EL(dy, dy_dt);
+  REQUIRE_EL(x, x_dt);
+  REQUIRE_EL(dx, x_dt);
+  REQUIRE(aligned_el(w, BZPF_F32) && aligned_el(dw, BZPF_F32) && aligned_el(db, BZPF_F32) && aligned_el(ws, BZPF_F32),
+          "bzpf_layernorm_bwd: w, dw, db or ws misaligned");
+  const int64_t need = dw || db ? bzpf::row_grad_ws_bytes(rows, D) : 0;
+  REQUIRE(need == 0 || (ws && ws_bytes >= need), "bzpf_layernorm_bwd: ws holds %lld bytes of %lld",
+          (long long)(ws ? ws_bytes : 0), (long long)need);
+  return done(bzpf::launch_layernorm_bwd(dy, dy_dt, x, x_dt, w, eps, dx, dw, db, ws, rows, D, S(stream)),
+              "bzpf_layernorm_bwd");
+}
+
+}  // extern "C"
+
+namespace {
+
+// Fills `d` from the arguments of an entry point, or returns false with the message set.
+bool make_drop(const char* who, double p, const int64_t* rng, int site, int shared, int64_t rows, int64_t I, int64_t J,
+               int64_t D, bzpf::Drop* d) {
+  const auto bad = [&](const char* what) { return fail(BZPF_EINVAL, "%s: %s", who, what) == BZPF_OK; };
+  if (!(p >= 0.0 && p <= 1.0)) return bad("p must lie in [0, 1]");
+  if (site < 0 || site > 65535) return bad("site must lie in [0, 65535]");
+  if (shared < 0 || shared > 2) return bad("shared must be 0 (element), 1 (row) or 2 (column)");
+  const int64_t below = llround(p * 4294967296.0);
+  *d = bzpf::Drop{rng, (uint32_t)(below - 1), (uint32_t)site, p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f,
+                  below == 0 ? bzpf::DROP_OFF : shared == 0 ? bzpf::DROP_ELEMENT
+                  : shared == 1 ? bzpf::DROP_ROW : bzpf::DROP_COLUMN, I, J};
+  if (d->mode == bzpf::DROP_OFF) return true;
+  if (rng == nullptr || (reinterpret_cast<uintptr_t>(rng) & 7u)) return bad("rng must be a non-null pointer to two int64");
+  if (shared && (I < 1 || J < 1 || rows % I || rows / I % J)) return bad("rows must be a multiple of I * J");
+  if (rows > ((int64_t)1 << 48) / ((D + 3) / 4)) return bad("more draws than 2^48 blocks");
+  return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+int bzpf_dropout(const void* x, int x_dt, double p, const int64_t* rng, int site, int shared, int64_t I, int64_t J,
+                 void* y, int y_dt, int64_t rows, int64_t D, void* stream) {
+  REQUIRE(pair_ok(x_dt, y_dt), "bzpf_dropout: bad dtype %d/%d", x_dt, y_dt);
+  REQUIRE(rows >= 0 && D >= 1, "bzpf_dropout: rows=%lld D=%lld", (long long)rows, (long long)D);
+  if (rows == 0) return BZPF_OK;
+  bzpf::Drop d;
+  if (!make_drop("bzpf_dropout", p, rng, site, shared, rows, I, J, D, &d)) return BZPF_EINVAL;
+  REQUIRE_EL(x, x_dt);
+  REQUIRE_EL(y, y_dt);
+  return done(bzpf::launch_dropout(x, x_dt, d, y, y_dt, rows, D, S(stream)), "bzpf_dropout");
+}
+
+int bzpf_dropout_add_ln(const float* z, const void* y, int y_dt, double p, const int64_t* rng, int site, int shared,
+                        int64_t I, int64_t J, const float* w, const float* b, float eps, float* z_new, void* ln,
+                        int ln_dt, int64_t rows, int D, void* stream) {
+  REQUIRE(pair_ok(y_dt, ln_dt), "bzpf_dropout_add_ln: bad dtype %d/%d", y_dt, ln_dt);
+  REQUIRE(width_ok(D), "bzpf_dropout_add_ln: unsupported D=%d", D);
+  REQUIRE(rows >= 0, "bzpf_dropout_add_ln: rows < 0");
+  if (rows == 0) return BZPF_OK;
+  bzpf::Drop d;
+  if (!make_drop("bzpf_dropout_add_ln", p, rng, site, shared, rows, I, J, D, &d)) return BZPF_EINVAL;
+  REQUIRE_EL(z, BZPF_F32);
+  REQUIRE_EL(y, y_dt);
+  REQUIRE_EL(z_new, BZPF_F32);
+  REQUIRE_EL(ln, ln_dt);
+  REQUIRE(aligned_el(w, BZPF_F32) && aligned_el(b, BZPF_F32), "bzpf_dropout_add_ln: w or b misaligned");
+  return done(bzpf::launch_dropout_add_ln(z, y, y_dt, d, w, b, eps, z_new, ln, ln_dt, rows, D, S(stream)),
+              "bzpf_dropout_add_ln");
+}
+
+int bzpf_dropout_add_ln_bwd(const float* dz_new, const void* dln, int ln_dt, const float* z_new, const float* w,
+                            float eps, double p, const int64_t* rng, int site, int shared, int64_t I, int64_t J,
+                            float* dz, void* dy, int y_dt, float* dw, float* db, float* ws, int64_t ws_bytes,
+                            int64_t rows, int D, void* stream) {
+  REQUIRE(pair_ok(y_dt, ln_dt), "bzpf_dropout_add_ln_bwd: bad dtype %d/%d", y_dt, ln_dt);
+  REQUIRE(width_ok(D), "bzpf_dropout_add_ln_bwd: unsupported D=%d", D);
+  REQUIRE(rows >= 1, "bzpf_dropout_add_ln_bwd: rows < 1");
+  bzpf::Drop d;
+  if (!make_drop("bzpf_dropout_add_ln_bwd", p, rng, site, shared, rows, I, J, D, &d)) return BZPF_EINVAL;
+  REQUIRE(aligned_el(dz_new, BZPF_F32), "bzpf_dropout_add_ln_bwd: dz_new misaligned");
+  REQUIRE_EL(dln, ln_dt);
+  REQUIRE_EL(z_new, BZPF_F32);
+  REQUIRE_EL(dz, BZPF_F32);
+  REQUIRE_EL(dy, y_dt);
+  REQUIRE(aligned_el(w, BZPF_F32) && aligned_el(dw, BZPF_F32) && aligned_el(db, BZPF_F32) && aligned_el(ws, BZPF_F32),
+          "bzpf_dropout_add_ln_bwd: w, dw, db or ws misaligned");
+  const int64_t need = dw || db ? bzpf::row_grad_ws_bytes(rows, D) : 0;
+  REQUIRE(need == 0 || (ws && ws_bytes >= need), "bzpf_dropout_add_ln_bwd: ws holds %lld bytes of %lld",
+          (long long)(ws ? ws_bytes : 0), (long long)need);
+  return done(bzpf::launch_dropout_add_ln_bwd(dz_new, dln, ln_dt, z_new, w, eps, d, dz, dy, y_dt, dw, db, ws, rows, D,
+                                              S(stream)),
+              "bzpf_dropout_add_ln_bwd");
 }
 
 int bzpf_count_nonfinite(const void* x, int dt, int64_t n, int* count, void* stream) {

@@ -6,12 +6,41 @@
 
 namespace bzpf {
 
-enum { DT_F32 = 0, DT_F16 = 1 };
+enum { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2 };
 
 hipError_t launch_layernorm(const void* x, int x_dt, const float* w, const float* b, float eps, void* y, int y_dt,
                             int64_t rows, int D, hipStream_t st);
 hipError_t launch_add_ln(float* z, const void* y, int y_dt, float scale, int trans_y, const float* w, const float* b,
                          float eps, void* ln, int ln_dt, int trans_out, int64_t N, int D, hipStream_t st);
+constexpr int ROW_MIN_D = 8, ROW_MAX_D = 8192;  // widths of the row kernels below
+// LayerNorm at any such width and type (bzpf_lnorm.hip), and its backward pass: dx, and the sums dw / db of the
+// weight and bias (each may be null). ws: row_grad_ws_bytes(rows, D) bytes of partial sums, one [2][D] for each workgroup.
+hipError_t launch_layernorm_rows(const void* x, int x_dt, const float* w, const float* b, float eps, void* y, int y_dt,
+                                 int64_t rows, int D, hipStream_t st);
+int64_t row_grad_ws_bytes(int64_t rows, int D);
+hipError_t launch_layernorm_bwd(const void* dy, int dy_dt, const void* x, int x_dt, const float* w, float eps, void* dx,
+                                float* dw, float* db, float* ws, int64_t rows, int D, hipStream_t st);
+hipError_t launch_row_grad_sum(const float* ws, int64_t blocks, int D, float* dw, float* db, hipStream_t st);
+// How a call drops: a draw u < `last` + 1 = round(p 2^32) drops its element (p = 1 fits so; p = 0 is DROP_OFF), the rest
+// is scaled by 1 / (1 - p). rng: (seed, offset) on the device, read by the kernel, so that a replayed graph draws anew
+// once its owner has written another offset. I, J: the extents of the [.., I, J, D] tensor, for the shared draws.
+enum { DROP_OFF = 0, DROP_ELEMENT = 1, DROP_ROW = 2, DROP_COLUMN = 3 };
+struct Drop {
+  const int64_t* rng;
+  uint32_t last;
+  uint32_t site;
+  float scale;
+  int mode;
+  int64_t I, J;
+};
+hipError_t launch_dropout(const void* x, int x_dt, const Drop& drop, void* y, int y_dt, int64_t rows, int64_t D,
+                          hipStream_t st);
+hipError_t launch_dropout_add_ln(const float* z, const void* y, int y_dt, const Drop& drop, const float* w,
+                                 const float* b, float eps, float* z_new, void* ln, int ln_dt, int64_t rows, int D,
+                                 hipStream_t st);
+hipError_t launch_dropout_add_ln_bwd(const float* dz_new, const void* dln, int ln_dt, const float* z_new,
+                                     const float* w, float eps, const Drop& drop, float* dz, void* dy, int y_dt,
+                                     float* dw, float* db, float* ws, int64_t rows, int D, hipStream_t st);
 hipError_t launch_count_nonfinite(const void* x, int dt, int64_t n, int* count, hipStream_t st);
 
 hipError_t launch_trimul_proj(const void* xn, const void* w, const float* mask, float scale, int incoming, void* ab,

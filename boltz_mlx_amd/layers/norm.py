@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import torch
 
+from boltz_mlx_amd import autograd as A
 from boltz_mlx_amd import kernels as K
 
 
@@ -22,3 +23,7 @@ class LayerNorm(torch.nn.LayerNorm):
     def to_storage(self, x: torch.Tensor) -> torch.Tensor:
         """LN(x) in the pair path's storage dtype (fp32, or fp16 in f16 mode)."""
         return K.layer_norm(x, self.weight, self.bias, self.eps, out_dtype=K.storage_dtype())
+
+    def with_grad(self, x: torch.Tensor, out_dtype=torch.float32) -> torch.Tensor:
+        """LN(x) in out_dtype with gradients for x and the parameters (forward() and the others carry none)."""
+        return A.layer_norm(x, self.weight, self.bias, self.eps, out_dtype)

@@ -6,7 +6,8 @@
  * failure) with a message in bzpf_last_error(). Nothing here allocates or frees device memory and nothing
  * synchronises: the caller owns every buffer (inputs, outputs and intermediates) and the stream order.
  *
- * Storage types: BZPF_F32 (fp32) or BZPF_F16 (fp16 operands, fp32 accumulation / statistics / softmax). The pair
+ * Storage types: BZPF_F32 (fp32) or BZPF_F16 (fp16 operands, fp32 accumulation / statistics / softmax); LayerNorm and
+ * the training entry points take BZPF_BF16 too, but not fp16 and bf16 in one call. The pair
  * representation z is always fp32 [N, N, 128] row-major. Pointers are 16-byte aligned; D = c_z = 128 for the
  * pair kernels.
  *
@@ -24,6 +25,7 @@ extern "C" {
 
 #define BZPF_F32 0
 #define BZPF_F16 1
+#define BZPF_BF16 2
 
 #define BZPF_OK 0
 #define BZPF_EINVAL (-1)
@@ -39,11 +41,51 @@ const char* bzpf_last_error(void);
  * bias): N rounded up to 64. */
 int64_t bzpf_row_pitch(int64_t N);
 
-/* Row LayerNorm over D channels (D % 64 == 0, D <= 1024): two-pass fp32 statistics, (x-mean)*rsqrt(var+eps)*w+b;
- * w / b may be NULL. Replaces kernels.layer_norm (boltz_mlx/kernels.py:482-507) and LayerNorm.__call__/.f16
- * (boltz_mlx/layers/norm.py:9-17). */
+/* Row LayerNorm over D channels (8 <= D <= 8192): two-pass fp32 statistics, (x-mean)*rsqrt(var+eps)*w+b; w / b may be
+ * NULL. Pointers need only be aligned to their elements. Replaces kernels.layer_norm (boltz_mlx/kernels.py:482-507) and
+ * LayerNorm.__call__/.f16 (boltz_mlx/layers/norm.py:9-17). */
 int bzpf_layernorm(const void* x, int x_dt, const float* w, const float* b, float eps, void* y, int y_dt,
                    int64_t rows, int D, void* stream);
+
+/* Backward pass of bzpf_layernorm over rows >= 1 (the reference runs inference only): from dy (y's type) and the input x,
+ * whose statistics are formed again,
+ *   dx = rstd (g - mean(g) - xh mean(g xh)), g = dy w (x's type); dw = sum over rows of dy xh; db = sum over rows of dy.
+ * dw / db (fp32 [D]) may each be NULL. ws: bzpf_layernorm_bwd_ws(rows, D) bytes for the workgroups' partial sums (0: none
+ * needed; -1: a width or row count that is refused), of which ws_bytes are there; it may be NULL when dw and db are.
+ * Sums in fp32 in a fixed order: equal inputs give equal bits. */
+int64_t bzpf_layernorm_bwd_ws(int64_t rows, int D);
+int bzpf_layernorm_bwd(const void* dy, int dy_dt, const void* x, int x_dt, const float* w, float eps, void* dx,
+                       float* dw, float* db, float* ws, int64_t ws_bytes, int64_t rows, int D, void* stream);
+
+/* Dropout of x [rows, D] (any D >= 1): y = u < p ? 0 : x / (1 - p), p in [0, 1] to 2^-32; a dropped element is 0 whatever
+ * x holds. The backward pass is the same call on dy. No mask is stored: u is a word of Philox4x32-10 (Salmon et al.,
+ * "Parallel random numbers: as easy as 1, 2, 3", 2011), a function of
+ *   key      rng[0] (the seed), rng: two int64 on the device, read by the kernel (may be NULL when p = 0);
+ *   counter  (n bits 0-31, n bits 32-47 | site << 16, rng[1] bits 0-31, rng[1] bits 32-63), 0 <= site < 65536,
+ * so that distinct (seed, offset, site) draw apart. The word of element (r, c):
+ *   shared = 0: word c % 4 of block n = r ceil(D / 4) + c / 4, a draw for each element;
+ *   shared = 1: one draw for each row i of the [.., I, J, D] tensor (all j and c share it): g = r / J;
+ *   shared = 2: one for each column j: g = r / (I J) * J + r % J; in both word g % 4 of block n = g / 4.
+ * (The reference runs inference only; the two shared forms are the trunk's row- and
+ * column-wise dropout.) */
+int bzpf_dropout(const void* x, int x_dt, double p, const int64_t* rng, int site, int shared, int64_t I, int64_t J,
+                 void* y, int y_dt, int64_t rows, int64_t D, void* stream);
+
+/* The residual update with dropout and the LayerNorm that follows (the training form of bzpf_add_ln):
+ *   z_new = z + dropout(y);  ln = LN(z_new; w, b, eps)
+ * over rows of D channels (8 <= D <= 8192); z and z_new fp32 (two buffers), y and ln of their types, dropout as in
+ * bzpf_dropout. */
+int bzpf_dropout_add_ln(const float* z, const void* y, int y_dt, double p, const int64_t* rng, int site, int shared,
+                        int64_t I, int64_t J, const float* w, const float* b, float eps, float* z_new, void* ln,
+                        int ln_dt, int64_t rows, int D, void* stream);
+
+/* Its backward pass over rows >= 1: from the gradients dz_new (fp32; NULL: zero) and dln of the two outputs and z_new,
+ *   dz = dz_new + (the LayerNorm's gradient of dln);  dy = dropout(dz), with the forward call's draws; dw, db and ws as in
+ * bzpf_layernorm_bwd (the same workspace size). */
+int bzpf_dropout_add_ln_bwd(const float* dz_new, const void* dln, int ln_dt, const float* z_new, const float* w,
+                            float eps, double p, const int64_t* rng, int site, int shared, int64_t I, int64_t J,
+                            float* dz, void* dy, int y_dt, float* dw, float* db, float* ws, int64_t ws_bytes,
+                            int64_t rows, int D, void* stream);
 
 /* *count += the number of inf / nan among the n elements of x (fp32 or fp16; device int counter, no host sync): the
  * fp16 overflow guard's check of the residual streams. Replaces kernels.guard_residual / guard_take

@@ -1,0 +1,557 @@
+"""The training operators on the GPU (LayerNorm at any width with its backward pass, dropout, the residual update) against
+the float64 oracle.
+
+Tolerances, from the kernels' arithmetic: u = 2^-24 is fp32's half step. A row's sum of D <= 8192 terms passes at most 15
+additions (3 inside a chunk, 4 chunks, 6 steps over a wave, 2 over the waves), so it errs by 16u times the mean of the
+terms' sizes after the division:
+  mean: 16u M, M the row's largest |x|;  xh: (1 + |xh|) E with E = u (16 M rstd + 14);
+  y: |w| (1 + |xh|) E + 2u (|xh w| + |b|);
+  dx, with G the row's largest |dy w|: c1 errs by 17u G, c2 by G (18u + 2E) (the mean of |xh| is at most 1), so the whole by
+  rstd G (1 + |xh|) (6E + 60u);
+  dw: each term errs by |dy| (1 + |xh|) E, the sum by its depth (the rows of one thread, its wave, the workgroups) times u
+  times the terms' sizes.
+Outputs in fewer bits add their half step (fp16 2^-11, bf16 2^-8, relative) and fp16's smallest half step 2^-25."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from oracle import training as T  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+STEP = {F32: 0.0, F16: 2.0 ** -11, BF16: 2.0 ** -8}
+TINY = {F32: 1e-37, F16: 2.0 ** -25, BF16: 1e-37}
+TYPES = [(F32, F32), (F32, F16), (F32, BF16), (F16, F16), (BF16, BF16), (F16, F32), (BF16, F32)]
+# every row layout's first and last width, whole chunks and odd ones
+WIDTHS = [8, 9, 15, 63, 64, 65, 77, 100, 128, 129, 250, 256, 257, 384, 511, 513, 768, 1000, 1021, 1025, 1536, 2048, 2049,
+          2055, 4096, 4097, 8185, 8192]
+ROWS = [1, 2, 3, 5, 31, 33, 70]
+
+
+def K():
+    from boltz_mlx_amd import kernels
+
+    return kernels
+
+
+def rand(seed, *shape, scale=1.0, dtype=F32):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (scale * torch.randn(shape, generator=g, device="cuda")).to(dtype)
+
+
+def acts(seed, rows, D, dtype):
+    """Rows with a mean and a scale of their own."""
+    return (rand(seed, rows, D) * (0.5 + rand(seed + 1, rows, 1).abs()) + rand(seed + 2, rows, 1)).to(dtype)
+
+
+def np64(t):
+    return None if t is None else t.detach().double().cpu().numpy()
+
+
+def close(got, ref, tol, dtype=None):
+    dtype = dtype or got.dtype
+    err = np.abs(np64(got) - ref)
+    lim = tol + (STEP[dtype] * (np.abs(ref) + tol) + TINY[dtype] + U * np.abs(ref))
+    bad = ~(err <= lim)
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4].tolist(), float((err / lim).max()))
+
+
+def row_terms(x, eps=1e-5):
+    """(xh, rstd, E) of the rows, as the docstring has them."""
+    c = x - x.mean(-1, keepdims=True)
+    rstd = 1 / np.sqrt((c * c).mean(-1, keepdims=True) + eps)
+    return c * rstd, rstd, U * (16 * np.abs(x).max(-1, keepdims=True) * rstd + 14)
+
+
+def ln_tol(x, w, b):
+    xh, _, E = row_terms(x)
+    w = 1.0 if w is None else w
+    return np.abs(w) * (1 + np.abs(xh)) * E + 2 * U * (np.abs(xh * w) + (0 if b is None else np.abs(b)))
+
+
+def dx_tol(dy, x, w):
+    xh, rstd, E = row_terms(x)
+    G = np.abs(dy if w is None else dy * w).max(-1, keepdims=True)
+    return rstd * G * (1 + np.abs(xh)) * (6 * E + 60 * U)
+
+
+def dw_tol(dy, x):
+    xh, _, E = row_terms(x)
+    depth = len(x) // 256 + 128
+    return (np.abs(dy) * (1 + np.abs(xh)) * E).sum(0) + depth * U * np.abs(dy * xh).sum(0), depth * U * np.abs(dy).sum(0)
+
+
+def params(seed, D, affine=True):
+    return (1 + rand(seed, D, scale=0.1), rand(seed + 1, D, scale=0.1)) if affine else (None, None)
+
+
+def check_grads(dx, dw, db, dy, x, w):
+    dy, x, w = np64(dy), np64(x), np64(w)
+    rx, rw, rb = T.ln_grads(dy, x, w)
+    close(dx, rx, dx_tol(dy, x, w))
+    tw, tb = dw_tol(dy, x)
+    if dw is not None:
+        close(dw, rw, tw)
+    if db is not None:
+        close(db, rb, tb)
+
+
+# -------------------------------------------------------------------------------------------------- LayerNorm
+
+@pytest.mark.parametrize("D", WIDTHS)
+def test_layer_norm_widths(D):
+    for k, (tx, ty) in enumerate(TYPES):
+        rows = ROWS[(k + D) % len(ROWS)]
+        x, (w, b) = acts(D + k, rows, D, tx), params(D, D)
+        y = K().layer_norm(x, w, b, 1e-5, out_dtype=ty)
+        assert y.dtype == ty and y.shape == x.shape
+        close(y, T.ln(np64(x), np64(w), np64(b)), ln_tol(np64(x), np64(w), np64(b)))
+
+
+@pytest.mark.parametrize("D", WIDTHS)
+def test_layer_norm_bwd_widths(D):
+    for k, (tx, ty) in enumerate(TYPES):
+        rows = ROWS[(k + D) % len(ROWS)]
+        x, dy, (w, _) = acts(D + k, rows, D, tx), rand(D + k + 9, rows, D, dtype=ty), params(D, D)
+        dx, dw, db = K().layer_norm_bwd(dy, x, w)
+        assert dx.dtype == tx and dw.dtype == db.dtype == F32
+        check_grads(dx, dw, db, dy, x, w)
+
+
+@pytest.mark.parametrize("rows, D", [(257, 64), (4099, 128), (20011, 72), (1500, 384), (3001, 1021), (1100, 2100),
+                                     (1030, 8192), (70001, 16)])
+def test_layer_norm_bwd_many_rows(rows, D):
+    """Several workgroups, each with several rows: the partial sums and their meeting."""
+    x, dy, (w, _) = acts(1, rows, D, F32), rand(2, rows, D, dtype=F16), params(3, D)
+    dx, dw, db = K().layer_norm_bwd(dy, x, w)
+    check_grads(dx, dw, db, dy, x, w)
+    again = K().layer_norm_bwd(dy, x, w)
+    assert all(torch.equal(a, b) for a, b in zip((dx, dw, db), again))  # a fixed order of sums
+
+
+def test_layer_norm_without_affine_and_needs():
+    x, dy = acts(5, 300, 200, BF16), rand(6, 300, 200, dtype=BF16)
+    close(K().layer_norm(x, None, None, out_dtype=BF16), T.ln(np64(x)), ln_tol(np64(x), None, None))
+    dx, dw, db = K().layer_norm_bwd(dy, x, None, need_weight=False, need_bias=False)
+    assert dw is None and db is None
+    check_grads(dx, None, None, dy, x, None)
+    w = 1 + rand(7, 200, scale=0.1)
+    full = K().layer_norm_bwd(dy, x, w)
+    for need in ((True, False), (False, True)):
+        part = K().layer_norm_bwd(dy, x, w, need_weight=need[0], need_bias=need[1])
+        assert torch.equal(part[0], full[0])
+        for got, ref, n in zip(part[1:], full[1:], need):
+            assert torch.equal(got, ref) if n else got is None
+
+
+def test_layer_norm_hard_rows():
+    """Rows with a large mean (the two-pass variance), constant rows (variance 0: eps alone), and rows with an infinity or
+    a NaN, which spoil themselves and no other."""
+    x = rand(8, 40, 96)
+    x[0:8] += 300.0
+    x[8:12] = 2.5
+    x[13, 7], x[14, 95], x[15, 0] = float("inf"), float("nan"), float("-inf")
+    dy, (w, b) = rand(9, 40, 96), params(10, 96)
+    spoilt = [13, 14, 15]
+    fine = [r for r in range(40) if r not in spoilt]
+    y, (dx, _, _) = K().layer_norm(x, w, b), K().layer_norm_bwd(dy, x, w)
+    assert torch.isnan(y[spoilt]).all() and torch.isnan(dx[spoilt]).all()
+    xf, df = np64(x)[fine], np64(dy)[fine]
+    close(y[fine], T.ln(xf, np64(w), np64(b)), ln_tol(xf, np64(w), np64(b)))
+    rx, rw, rb = T.ln_grads(df, xf, np64(w))
+    close(dx[fine], rx, dx_tol(df, xf, np64(w)))
+    _, dw, db = K().layer_norm_bwd(dy[fine], x[fine], w)
+    tw, tb = dw_tol(df, xf)
+    close(dw, rw, tw)
+    close(db, rb, tb)
+
+
+@pytest.mark.parametrize("D", [64, 77, 128, 384, 2056, 8191])
+def test_strides_offsets_and_neighbours(D):
+    """Views at odd offsets (element alignment only), transposed inputs, and the memory around the outputs untouched."""
+    from boltz_mlx_amd import _lib
+
+    rows = 37
+    base = acts(11, rows + 2, D, F16).flatten()
+    x = base[3:3 + rows * D].view(rows, D)
+    g = rand(12, D, rows, dtype=F16).t()
+    w = (1 + rand(13, D + 1, scale=0.1))[1:]
+    check_grads(*K().layer_norm_bwd(g, x, w), g, x, w)
+    close(K().layer_norm(x, w, None, out_dtype=F16), T.ln(np64(x), np64(w)), ln_tol(np64(x), np64(w), None))
+    # outputs inside larger buffers
+    gc = g.contiguous()
+    dx, dw = torch.full((rows * D + 40,), 7.0, dtype=F16, device="cuda"), torch.full((2 * D + 40,), 7.0, device="cuda")
+    ws = torch.full((max(1, _lib.load().bzpf_layernorm_bwd_ws(rows, D) // 4) + 16,), 7.0, device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    _lib.call("bzpf_layernorm_bwd", gc.data_ptr(), 1, x.data_ptr(), 1, w.data_ptr(), 1e-5, dx[11:].data_ptr(),
+              dw[9:].data_ptr(), dw[20 + D:].data_ptr(), ws.data_ptr(), 4 * (ws.numel() - 16), rows, D, st)
+    torch.cuda.synchronize()
+    check_grads(dx[11:11 + rows * D].view(rows, D), dw[9:9 + D], dw[20 + D:20 + 2 * D], gc, x, w)
+    for t in (dx[:11], dx[11 + rows * D:], dw[:9], dw[9 + D:20 + D], dw[20 + 2 * D:], ws[-16:]):
+        assert (t == 7.0).all()
+
+
+def test_no_rows():
+    x, w, rng = torch.empty(0, 4, 32, device="cuda"), torch.ones(32, device="cuda"), K().dropout_rng(1)
+    assert K().layer_norm(x, w, w).shape == x.shape
+    dx, dw, db = K().layer_norm_bwd(x, x, w)
+    assert dx.shape == x.shape and (dw == 0).all() and (db == 0).all()
+    assert K().dropout(x, 0.5, rng).shape == x.shape and K().dropout(x, 0.5, rng, shared="row").shape == x.shape
+    zn, xn = K().dropout_add_ln(x, x, w, w, 1e-5, 0.5, rng)
+    assert zn.shape == xn.shape == x.shape
+    dz, dy, dw, db = K().dropout_add_ln_bwd(x, x, x, w, 1e-5, 0.5, rng)
+    assert dz.shape == dy.shape == x.shape and (dw == 0).all() and (db == 0).all()
+
+
+def test_earlier_widths_keep_their_results():
+    """The widths and types that LayerNorm had before run the same kernel at any row count; a misaligned input takes the
+    other one, which agrees to rounding."""
+    x, (w, b) = acts(14, 130, 128, F32), params(15, 128)
+    buf = torch.empty(130 * 128 + 1, device="cuda")
+    buf[1:] = x.flatten()
+    a, c = K().layer_norm(x, w, b), K().layer_norm(buf[1:].view(130, 128), w, b)
+    ref, tol = T.ln(np64(x), np64(w), np64(b)), ln_tol(np64(x), np64(w), np64(b))
+    close(a, ref, tol)
+    close(c, ref, tol)
+
+
+# -------------------------------------------------------------------------------------------------- dropout
+
+def dropped_of(t, p, rng, site=0, shared=None, **rows):
+    seed, off = (int(v) for v in rng.tolist())
+    return T.dropped(tuple(t.shape), p, seed, off, site, shared, **rows).reshape(-1, t.shape[-1])
+
+
+DEEP = [(2, 17, 5, 77), (3, 40, 31, 128), (2, 3, 4, 1025), (4, 3, 1)]
+
+
+@pytest.mark.parametrize("shape, shared", [(s, None) for s in [(1,), (7,), (8,), (100003,), (3, 1), (5, 3), (4, 9),
+                                                               (33, 64)] + DEEP] +
+                         [(s, m) for s in DEEP for m in ("row", "column")])
+def test_dropout(shape, shared):
+    for k, (tx, ty) in enumerate(TYPES):
+        rng = K().dropout_rng(2 ** 40 + 12345 * k, 2 ** 33 + k)
+        p = (0.1, 0.25, 0.5, 0.9)[k % 4]
+        x = rand(k, *shape, dtype=tx)
+        x[x == 0] = 1
+        y = K().dropout(x, p, rng, 7 * k, shared, out_dtype=ty)
+        assert y.dtype == ty and y.shape == x.shape
+        d = dropped_of(x, p, rng, 7 * k, shared).reshape(shape)
+        assert np.array_equal(np64(y) == 0, d)  # the same draws, and no kept element lost
+        close(y, T.dropout(np64(x), p, d), 2 * U * np.abs(np64(x)) / (1 - p))
+
+
+def test_dropout_ends_and_special_values():
+    x = rand(3, 20, 6, 50, dtype=F16)
+    x[::2, ::3, ::7] = float("inf")
+    x[1::2, ::3, ::5] = float("nan")
+    rng = K().dropout_rng(-5, -1)  # any int64 is a seed
+    assert torch.equal(K().dropout(x, 0.0, None), x) or torch.equal(torch.isnan(K().dropout(x, 0.0, None)), torch.isnan(x))
+    for shared in (None, "row", "column"):
+        assert (K().dropout(x, 1.0, rng, shared=shared) == 0).all()
+        y, d = K().dropout(x, 0.5, rng, 65535, shared), dropped_of(x, 0.5, rng, 65535, shared).reshape(x.shape)
+        assert (y[torch.tensor(d, device="cuda")] == 0).all()  # infinities and NaNs too
+        keep = torch.tensor(~d, device="cuda")
+        assert torch.equal(torch.isnan(y[keep]), torch.isnan(x[keep]))
+        assert torch.equal(torch.isinf(y[keep]), torch.isinf(x[keep]))
+    tiny = 2.0 ** -34  # rounds to no draw at all
+    assert torch.equal(K().dropout(x[0].nan_to_num(), tiny, rng), x[0].nan_to_num())
+
+
+def test_dropout_differs_by_seed_offset_and_site():
+    x, r = torch.ones(1000, 64, device="cuda"), K().dropout_rng
+    base = K().dropout(x, 0.5, r(1, 2), 3)
+    assert torch.equal(base, K().dropout(x, 0.5, r(1, 2), 3))
+    for other in (K().dropout(x, 0.5, r(2, 2), 3), K().dropout(x, 0.5, r(1, 3), 3), K().dropout(x, 0.5, r(1, 2), 4)):
+        share = (base == other).float().mean().item()
+        assert abs(share - 0.5) < 6 * 0.5 / 64000 ** 0.5  # independent fair draws agree in half of the places
+
+
+# -------------------------------------------------------------------------------------------------- residual update
+
+def check_residual(shape, ty, to, p, shared, seed, affine=True, zero_dz=False):
+    D = shape[-1]
+    z, y = acts(seed, int(np.prod(shape[:-1])), D, F32).view(shape), rand(seed + 3, *shape, dtype=ty)
+    w, b = params(seed + 4, D, affine)
+    rng, site = K().dropout_rng(seed * 77 + 2 ** 35, seed), seed % 9
+    zn, xn = K().dropout_add_ln(z, y, w, b, 1e-5, p, rng, site, shared, out_dtype=to)
+    assert zn.dtype == F32 and xn.dtype == to
+    d = dropped_of(z, p, rng, site, shared) if p > 0 else np.zeros((z.numel() // D, D), bool)
+    flat = lambda t: np64(t).reshape(-1, D)  # noqa: E731
+    close(zn.view(-1, D), flat(z) + T.dropout(flat(y), p, d), 3 * U * np.abs(flat(y)) / (1 - p))
+    zr = flat(zn)  # the LayerNorm of what the kernel wrote
+    close(xn.view(-1, D), T.ln(zr, np64(w), np64(b)), ln_tol(zr, np64(w), np64(b)))
+    dz_new, dln = None if zero_dz else rand(seed + 5, *shape), rand(seed + 6, *shape, dtype=to)
+    dz, dy, dw, db = K().dropout_add_ln_bwd(dz_new, dln, zn, w, 1e-5, p, rng, site, shared, y_dtype=ty,
+                                            need_weight=affine)
+    assert dz.dtype == F32 and dy.dtype == ty
+    rz, ry, rw, rb = T.residual_grads(None if zero_dz else flat(dz_new), flat(dln), zr, p, d, np64(w))
+    tol = dx_tol(flat(dln), zr, np64(w)) + 2 * U * np.abs(rz)
+    close(dz.view(-1, D), rz, tol)
+    assert (flat(dy)[d] == 0).all()
+    close(dy.view(-1, D), ry, (tol + 2 * U * np.abs(rz)) / (1 - p))
+    tw, tb = dw_tol(flat(dln), zr)
+    if affine:
+        close(dw, rw, tw)
+    else:
+        assert dw is None
+    close(db, rb, tb)
+
+
+@pytest.mark.parametrize("D", WIDTHS)
+def test_residual_widths(D):
+    for k, (ty, to) in enumerate(TYPES):
+        shared = (None, "row", "column")[(k + D) % 3]
+        check_residual((2, 3, ROWS[k], D), ty, to, (0.25, 0.1, 0.0, 0.6)[(k + D // 8) % 4], shared, k + D)
+
+
+@pytest.mark.parametrize("shape, shared", [((1, 65, 67, 128), "row"), ((1, 65, 67, 128), "column"), ((2, 50, 41, 77), None),
+                                           ((3, 31, 33, 64), "column"), ((1, 1, 1300, 384), None),
+                                           ((5, 1, 220, 1025), "row"), ((1, 3, 350, 4099), None)])
+def test_residual_many_rows(shape, shared):
+    check_residual(shape, BF16, BF16, 0.25, shared, 21)
+    check_residual(shape, F16, F32, 0.15, shared, 22, affine=False, zero_dz=True)
+
+
+def test_residual_keeps_the_stream_where_the_update_is_dropped():
+    z, y = rand(1, 4, 5, 6, 96), rand(2, 4, 5, 6, 96)
+    y[:, :, ::2] = float("nan")
+    rng = K().dropout_rng(11)
+    for shared in (None, "row", "column"):
+        zn, _ = K().dropout_add_ln(z, y, None, None, 1e-5, 0.5, rng, 1, shared)
+        d = torch.tensor(dropped_of(z, 0.5, rng, 1, shared).reshape(z.shape).copy(), device="cuda")
+        assert torch.equal(zn[d], z[d])
+        dz = torch.full_like(z, float("inf"))
+        _, dy, _, _ = K().dropout_add_ln_bwd(dz, torch.zeros_like(z), z, None, 1e-5, 0.5, rng, 1, shared,
+                                             need_weight=False)
+        assert (dy[d] == 0).all() and torch.isinf(dy[~d]).all()
+
+
+# -------------------------------------------------------------------------------------------------- sizes past 32 bits
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements (fp16): the last rows' values, gradients and draws."""
+    D, rows = 2048, 2 ** 20 + 77
+    x = torch.empty(rows, D, dtype=F16, device="cuda")
+    x.view(-1)[:2 ** 31].view(2 ** 20, D).copy_(acts(1, 2 ** 10, D, F16).repeat(2 ** 10, 1))
+    x[2 ** 20:] = acts(2, 77, D, F16)
+    w, rng = 1 + rand(3, D, scale=0.1), K().dropout_rng(5, 6)
+    tail = x[-80:]
+    y = K().dropout(x, 0.5, rng, 9)
+    d = dropped_of(x, 0.5, rng, 9, first_row=rows - 80, rows=80)
+    close(y[-80:], T.dropout(np64(tail), 0.5, d), 2 * U * np.abs(np64(tail)) * 2)
+    assert (np64(y[-80:])[d] == 0).all()
+    del y
+    dx, dw, db = K().layer_norm_bwd(x, x, w)  # the input as its own gradient
+    ref = T.ln_grads(np64(tail), np64(tail), np64(w))[0]
+    close(dx[-80:], ref, dx_tol(np64(tail), np64(tail), np64(w)))
+    assert torch.isfinite(dw).all() and torch.isfinite(db).all()
+    del dx
+    close(K().layer_norm(x, w, None, out_dtype=F16)[-80:], T.ln(np64(tail), np64(w)), ln_tol(np64(tail), np64(w), None))
+
+
+# -------------------------------------------------------------------------------------------------- autograd
+
+def test_autograd_against_float64_and_differences():
+    from boltz_mlx_amd import autograd as A
+
+    shape, p = (2, 5, 6, 40), 0.3
+    z, y = rand(1, *shape).requires_grad_(), rand(2, *shape).requires_grad_()
+    w, b = (t.requires_grad_() for t in params(3, 40))
+    rng = K().dropout_rng(17, 4)
+    gz, gl = rand(5, *shape), rand(6, *shape)
+
+    def f(z, y, w, b):
+        zn, xn = A.dropout_add_ln(z, A.layer_norm(y, w, b), w, b, 1e-5, p, rng, 2, "row", out_dtype=F32)
+        return zn, A.dropout(xn, p, rng, 3)
+
+    got = torch.autograd.grad(f(z, y, w, b), (z, y, w, b), (gz, gl))
+    leaves = [t.detach().double().cpu().requires_grad_() for t in (z, y, w, b)]
+    z6, y6, w6, b6 = leaves
+    d1 = torch.tensor(dropped_of(z, p, rng, 2, "row").reshape(shape).copy())
+    d2 = torch.tensor(dropped_of(z, p, rng, 3).reshape(shape).copy())
+    ln = torch.nn.functional.layer_norm
+    zn = z6 + torch.where(d1, 0.0, ln(y6, (40,), w6, b6) / (1 - p))
+    out = torch.where(d2, 0.0, ln(zn, (40,), w6, b6) / (1 - p))
+    ref = torch.autograd.grad((zn, out), leaves, (gz.double().cpu(), gl.double().cpu()))
+    for g, r in zip(got, ref):
+        # two LayerNorms in a chain: each errs by some 100u of the largest gradient, times the weights' and scales' growth
+        assert (g.double().cpu() - r).abs().max() <= 2000 * U * r.abs().max()
+    # along a direction: central differences of the kernels' own forward pass. Its value, a sum of 2400 terms with a mean
+    # size near 1, is formed in float64 from fp32 outputs that err by some 20u each: at h = 2^-6 the difference errs by
+    # 20u sqrt(2400) / h = 4e-3 and by the third derivative's h^2 / 6 (1e-3 for terms of unit size over 2400 terms).
+    v = [rand(7 + i, *t.shape) / t.numel() ** 0.5 for i, t in enumerate((z, y, w, b))]
+    h = 2.0 ** -6
+
+    def value(s):
+        with torch.no_grad():
+            a, c = f(*(t + s * h * dv for t, dv in zip((z, y, w, b), v)))
+            return (a.double() * gz).sum() + (c.double() * gl).sum()
+
+    slope = sum((g.double() * dv).sum() for g, dv in zip(got, v))
+    assert abs((value(1) - value(-1)) / (2 * h) - slope) < 0.02 + 0.01 * abs(slope)
+
+
+def test_autograd_needs_and_types():
+    from boltz_mlx_amd import autograd as A
+    from boltz_mlx_amd.layers.dropout import Dropout
+    from boltz_mlx_amd.layers.norm import LayerNorm
+
+    z, y, rng = rand(1, 3, 4, 64), rand(2, 3, 4, 64, dtype=BF16), K().dropout_rng(3)
+    ln = LayerNorm(64).cuda()
+    with torch.no_grad():
+        ln.weight.add_(rand(4, 64, scale=0.1))
+    drop = Dropout(0.25, "column", site=5).train()
+    zn, xn = drop.add_ln(z.unsqueeze(0), y.unsqueeze(0), ln, rng)
+    k_zn, k_xn = K().dropout_add_ln(z[None], y[None], ln.weight, ln.bias, ln.eps, 0.25, rng, 5, "column")
+    assert torch.equal(zn, k_zn) and torch.equal(xn, k_xn) and xn.dtype == BF16
+    zn.sum().backward()  # only the stream is used: the LayerNorm's parameters have no gradient
+    assert ln.weight.grad is None
+    yr = y.clone().requires_grad_()
+    zn, xn = drop.add_ln(z[None], yr[None], ln, rng)
+    (xn.float() ** 2).sum().backward()
+    assert yr.grad.dtype == BF16 and ln.weight.grad.shape == (64,)
+    zn, _ = drop.add_ln(z[None], yr[None], ln, rng)
+    (g,) = torch.autograd.grad(zn, yr, torch.ones_like(zn))
+    d = dropped_of(z[None], 0.25, rng, 5, "column").reshape(3, 4, 64)
+    assert np.array_equal(np64(g) == 0, d)
+    half = ln.weight.detach().half().requires_grad_()
+    (gw,) = torch.autograd.grad(A.layer_norm(z, half, None).sum(), half)
+    assert gw.dtype == F16
+    with pytest.raises(RuntimeError):  # the generator may not change between the passes
+        out = drop(yr[None], rng)
+        rng[1] += 1
+        out.sum().backward()
+    drop.eval()
+    assert drop(y, rng) is y
+    a, c = drop.add_ln(z, y, ln, rng)
+    assert torch.equal(a, z + y.float())
+    close(ln.with_grad(z), np64(ln(z)), 0 * np64(z))
+
+
+# -------------------------------------------------------------------------------------------------- streams and graphs
+
+def test_side_stream_and_two_calls_at_once():
+    x, dy, w = acts(1, 5000, 128, F32), rand(2, 5000, 128, dtype=F16), 1 + rand(3, 128, scale=0.1)
+    x2 = acts(9, 5000, 128, F32)
+    ref, ref2 = K().layer_norm_bwd(dy, x, w), K().layer_norm_bwd(dy, x2, w)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = []
+    for _ in range(4):
+        with torch.cuda.stream(s1):
+            a = K().layer_norm_bwd(dy, x, w)
+        with torch.cuda.stream(s2):
+            b = K().layer_norm_bwd(dy, x2, w)
+        outs.append((a, b))
+    torch.cuda.synchronize()
+    for a, b in outs:
+        assert all(torch.equal(p, q) for p, q in zip(a + b, ref + ref2))
+
+
+def test_captured_step_replays_with_new_inputs_and_draws():
+    """A whole update (forward and backward, autograd and kernels) in one graph: every replay, with new inputs and another
+    offset written between, gives what the eager calls give."""
+    from boltz_mlx_amd import autograd as A
+
+    shape, p = (1, 37, 41, 128), 0.25
+    z, y = rand(1, *shape), rand(2, *shape, dtype=F16)
+    w, b = params(3, 128)
+    rng, gz, gl = K().dropout_rng(8, 0), rand(4, *shape), rand(5, *shape, dtype=F16)
+
+    def step(leaves):
+        lz, ly, lw, lb = leaves
+        zn, xn = A.dropout_add_ln(lz, ly, lw, lb, 1e-5, p, rng, 1, "row")
+        t = A.dropout(A.layer_norm(zn, lw, lb, out_dtype=F16), p, rng, 2)
+        return (zn.detach(), xn.detach(), t.detach()) + torch.autograd.grad((zn, xn, t), leaves, (gz, gl, gl))
+
+    def fresh():
+        return [t.detach().requires_grad_() for t in (z, y, w, b)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(fresh())
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    leaves = fresh()
+    with torch.cuda.graph(graph):
+        outs = step(leaves)
+    seen = []
+    for k in range(4):
+        z.copy_(rand(10 + k, *shape))
+        y.copy_(rand(20 + k, *shape, dtype=F16))
+        rng[1] = k
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        want = step(fresh())
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
+        seen.append(got[2] == 0)
+    assert not torch.equal(seen[0], seen[1])
+
+
+def test_two_graphs_keep_their_own_workspaces():
+    x, dy, w = acts(1, 9000, 384, F32), rand(2, 9000, 384), 1 + rand(3, 384, scale=0.1)
+    xs = [acts(4 + k, 9000, 384, F32) for k in range(2)]
+    refs = [K().layer_norm_bwd(dy, t, w) for t in xs]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for t in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(K().layer_norm_bwd(dy, t, w))
+        graphs.append(g)
+    for order in ((0, 1), (1, 0), (0, 1)):
+        for k in order:
+            graphs[k].replay()
+        torch.cuda.synchronize()
+        for o, r in zip(outs, refs):
+            assert all(torch.equal(a, c) for a, c in zip(o, r))
+        (x * 2).sum()
+        torch.cuda.synchronize()
+
+
+# -------------------------------------------------------------------------------------------------- all together
+
+def test_a_block_of_updates_trains():
+    """Three pair updates in a chain (dropout per row, per column and per element, each with the next LayerNorm), as a
+    layer's training step has them: values and every parameter's gradient against float64 autograd."""
+    from boltz_mlx_amd.layers.dropout import Dropout
+    from boltz_mlx_amd.layers.norm import LayerNorm
+
+    shape, D = (2, 13, 13, 128), 128
+    drops = [Dropout(0.25, "row", 0), Dropout(0.25, "column", 1), Dropout(0.1, None, 2)]
+    lns = [LayerNorm(D).cuda() for _ in range(4)]
+    mats = [rand(30 + k, D, D, scale=D ** -0.5).requires_grad_() for k in range(3)]
+    for k, ln in enumerate(lns):
+        with torch.no_grad():
+            ln.weight.add_(rand(40 + k, D, scale=0.1))
+            ln.bias.add_(rand(50 + k, D, scale=0.1))
+    z0, rng, gz, gl = rand(1, *shape), K().dropout_rng(99, 3), rand(2, *shape), rand(3, *shape)
+    z, xn = z0, lns[0].with_grad(z0)
+    for drop, mat, ln in zip(drops, mats, lns[1:]):
+        z, xn = drop.add_ln(z, xn @ mat, ln, rng)
+    leaves = mats + [t for ln in lns for t in (ln.weight, ln.bias)]
+    got = torch.autograd.grad((z, xn), leaves, (gz, gl))
+    ref_leaves = [t.detach().double().cpu().requires_grad_() for t in leaves]
+    m6, p6 = ref_leaves[:3], ref_leaves[3:]
+    f = torch.nn.functional.layer_norm
+    r = z0.double().cpu()
+    x6 = f(r, (D,), p6[0], p6[1])
+    for k, drop in enumerate(drops):
+        d = torch.tensor(dropped_of(z0, drop.p, rng, drop.site, drop.shared).reshape(shape).copy())
+        r = r + torch.where(d, 0.0, (x6 @ m6[k]) / (1 - drop.p))
+        x6 = f(r, (D,), p6[2 * k + 2], p6[2 * k + 3])
+    # fp32 throughout; the matrix products err by sqrt(128) u of their terms, three updates deep: 1e-5 of the largest value
+    assert (z.double().cpu() - r).abs().max() <= 1e-5 * r.abs().max()
+    assert (xn.double().cpu() - x6).abs().max() <= 1e-5 * x6.abs().max()
+    for g, w in zip(got, torch.autograd.grad((r, x6), ref_leaves, (gz.double().cpu(), gl.double().cpu()))):
+        assert (g.double().cpu() - w).abs().max() <= 3e-5 * w.abs().max()

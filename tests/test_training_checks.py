@@ -1,0 +1,176 @@
+"""Refusals of the training operators: every argument is checked on the host before a launch. No device calls: the C entry
+points are given host addresses, which they must refuse before they could use them."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from boltz_mlx_amd import _lib
+from boltz_mlx_amd import kernels as K
+
+HOST = ctypes.create_string_buffer(4096)
+P = (ctypes.addressof(HOST) + 63) // 64 * 64  # an aligned address that no launch may see
+F32, F16, BF16 = 0, 1, 2
+
+
+def rc(name, *args):
+    return getattr(_lib.load(), name)(*args)
+
+
+def ln_bwd(dy=P, dy_dt=F32, x=P, x_dt=F32, w=P, dx=P, dw=P, db=P, ws=P, ws_bytes=1 << 30, rows=8, D=128):
+    return rc("bzpf_layernorm_bwd", dy, dy_dt, x, x_dt, w, 1e-5, dx, dw, db, ws, ws_bytes, rows, D, None)
+
+
+def drop(x=P, x_dt=F32, p=0.5, rng=P, site=0, shared=0, I=1, J=1, y=P, y_dt=F32, rows=12, D=16):
+    return rc("bzpf_dropout", x, x_dt, p, rng, site, shared, I, J, y, y_dt, rows, D, None)
+
+
+def res(z=P, y=P, y_dt=F32, p=0.5, rng=P, site=0, shared=0, I=1, J=1, w=P, b=P, zn=P, ln=P, ln_dt=F32, rows=12, D=16):
+    return rc("bzpf_dropout_add_ln", z, y, y_dt, p, rng, site, shared, I, J, w, b, 1e-5, zn, ln, ln_dt, rows, D, None)
+
+
+def res_bwd(dzn=P, dln=P, ln_dt=F32, zn=P, w=P, p=0.5, rng=P, site=0, shared=0, I=1, J=1, dz=P, dy=P, y_dt=F32, dw=P,
+            db=P, ws=P, ws_bytes=1 << 30, rows=12, D=16):
+    return rc("bzpf_dropout_add_ln_bwd", dzn, dln, ln_dt, zn, w, 1e-5, p, rng, site, shared, I, J, dz, dy, y_dt, dw, db,
+              ws, ws_bytes, rows, D, None)
+
+
+@pytest.mark.parametrize("change", [
+    {"dy": None}, {"x": None}, {"dx": None}, {"x": P + 2}, {"dw": P + 2}, {"ws": P + 1}, {"dy_dt": F16, "dy": P + 1},
+    {"dy_dt": 3}, {"x_dt": -1}, {"x_dt": F16, "dy_dt": BF16}, {"D": 7}, {"D": 0}, {"D": -8}, {"D": 8193}, {"rows": 0},
+    {"rows": -1}, {"rows": 100000, "ws": None}, {"rows": 100000, "ws_bytes": 64},
+])
+def test_layernorm_bwd_refuses(change):
+    assert ln_bwd(**change) == -1
+    assert b"bzpf_layernorm_bwd" in _lib.load().bzpf_last_error()
+
+
+@pytest.mark.parametrize("change", [
+    {"x": None}, {"y": None}, {"x": P + 1}, {"x_dt": F16, "y_dt": BF16}, {"x_dt": 7}, {"p": -0.1}, {"p": 1.5},
+    {"p": float("nan")}, {"rng": None}, {"rng": P + 4}, {"site": -1}, {"site": 65536}, {"shared": 3}, {"shared": -1},
+    {"shared": 1, "I": 5, "J": 2}, {"shared": 1, "I": 0, "J": 1}, {"shared": 2, "I": 4, "J": 5}, {"rows": -1}, {"D": 0},
+    {"rows": 1 << 48, "D": 5},
+])
+def test_dropout_refuses(change):
+    assert drop(**change) == -1
+    assert b"bzpf_dropout" in _lib.load().bzpf_last_error()
+
+
+@pytest.mark.parametrize("change", [
+    {"z": None}, {"y": None}, {"zn": None}, {"ln": None}, {"z": P + 2}, {"w": P + 2}, {"y_dt": F16, "ln_dt": BF16},
+    {"y_dt": 4}, {"D": 7}, {"D": 8193}, {"rows": -1}, {"p": 2.0}, {"rng": None}, {"shared": 1, "I": 3, "J": 8},
+])
+def test_dropout_add_ln_refuses(change):
+    assert res(**change) == -1
+    assert b"bzpf_dropout_add_ln" in _lib.load().bzpf_last_error()
+
+
+@pytest.mark.parametrize("change", [
+    {"dzn": P + 2}, {"dln": None}, {"zn": None}, {"dz": None}, {"dy": None}, {"y_dt": F16, "ln_dt": BF16}, {"D": 4},
+    {"D": 8200}, {"rows": 0}, {"p": -1.0}, {"rng": None}, {"site": 70000}, {"rows": 100000, "ws_bytes": 4},
+    {"rows": 100000, "ws": None},
+])
+def test_dropout_add_ln_bwd_refuses(change):
+    assert res_bwd(**change) == -1
+    assert b"bzpf_dropout_add_ln_bwd" in _lib.load().bzpf_last_error()
+
+
+def test_layernorm_refuses_and_takes_no_rows():
+    call = lambda **k: rc("bzpf_layernorm", *{**dict(x=P, xd=F32, w=P, b=P, eps=1e-5, y=P, yd=F32, rows=4, D=128,  # noqa: E731
+                                                     st=None), **k}.values())
+    for change in ({"x": None}, {"y": None}, {"xd": 3}, {"xd": F16, "yd": BF16}, {"D": 7}, {"D": 8193}, {"rows": -1},
+                   {"w": P + 2}, {"x": P + 1}):
+        assert call(**change) == -1, change
+    assert call(rows=0, x=None, y=None) == 0
+    assert drop(rows=0, x=None, y=None, rng=None) == 0
+    assert res(rows=0, z=None, y=None) == 0
+
+
+def test_workspace_sizes():
+    ws = _lib.load().bzpf_layernorm_bwd_ws
+    assert ws(1, 128) == 0 and ws(0, 128) == 0  # one workgroup writes the gradients itself
+    assert ws(-1, 128) == -1 and ws(10, 7) == -1 and ws(10, 8193) == -1
+    for rows, D in ((10 ** 6, 128), (10 ** 6, 8192), (5000, 77), (2 ** 40, 8)):
+        n = ws(rows, D)
+        assert n > 0 and n % (8 * D) == 0 and n // (8 * D) <= 1024  # whole [2][D] of fp32, at most 1024 workgroups
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """The wrappers' own checks without a device: nothing may reach a launch."""
+    monkeypatch.setattr(K, "_dev", lambda *ts: None)
+    monkeypatch.setattr(K, "_stream", lambda: 0)
+    calls = []
+    monkeypatch.setattr(K, "call", lambda *a: calls.append(a))
+    return calls
+
+
+def test_wrappers_refuse(host):
+    x, w, rng = torch.zeros(2, 3, 4, 16), torch.ones(16), torch.zeros(2, dtype=torch.int64)
+    bad = [
+        lambda: K.layer_norm(x, torch.ones(15), None), lambda: K.layer_norm(x, w, torch.ones(1, 16)),
+        lambda: K.layer_norm(torch.zeros(3, 0), None, None), lambda: K.layer_norm(torch.tensor(1.0), None, None),
+        lambda: K.layer_norm_bwd(x[0], x, w), lambda: K.layer_norm_bwd(x, x, torch.ones(17)),
+        lambda: K.dropout(x, 1.5, rng), lambda: K.dropout(x, -0.5, rng), lambda: K.dropout(x, float("nan"), rng),
+        lambda: K.dropout(x, 0.5, None), lambda: K.dropout(x, 0.5, rng.int()), lambda: K.dropout(x, 0.5, rng[:1]),
+        lambda: K.dropout(x, 0.5, rng, site=65536), lambda: K.dropout(x, 0.5, rng, shared="rows"),
+        lambda: K.dropout(x[0, 0], 0.5, rng, shared="row"),
+        lambda: K.dropout_add_ln(x.half(), x, w, w, 1e-5, 0.5, rng), lambda: K.dropout_add_ln(x, x[0], w, w, 1e-5, 0.5, rng),
+        lambda: K.dropout_add_ln(x, x, w[:3], w, 1e-5, 0.5, rng),
+        lambda: K.dropout_add_ln_bwd(x[0], x, x, w, 1e-5, 0.5, rng),
+        lambda: K.dropout_add_ln_bwd(x.half(), x, x, w, 1e-5, 0.5, rng),
+        lambda: K.dropout_add_ln_bwd(x, x, x.half(), w, 1e-5, 0.5, rng),
+    ]
+    for k, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {k} was taken")
+    for call in (lambda: K.layer_norm(x.double(), w, w), lambda: K.dropout(x.long(), 0.5, rng),
+                 lambda: K.layer_norm_bwd(x, x.double(), w)):
+        with pytest.raises(TypeError):
+            call()
+    assert not host
+
+
+def test_cpu_tensors_are_refused():
+    x, rng = torch.zeros(4, 16), torch.zeros(2, dtype=torch.int64)
+    for call in (lambda: K.layer_norm_bwd(x, x, None), lambda: K.dropout(x, 0.5, rng),
+                 lambda: K.dropout_add_ln(x, x, None, None, 1e-5, 0.0, None),
+                 lambda: K.dropout_add_ln_bwd(x, x, x, None, 1e-5, 0.0, None)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_converted_parameters_outlive_the_launch(host, monkeypatch):
+    """A weight that is not fp32 is converted for the call; its copy has to live until the launch is made."""
+    import weakref
+
+    copies, alive = [], []
+
+    def f32c(t):
+        c = t.float()
+        copies.append(weakref.ref(c))
+        return c
+
+    monkeypatch.setattr(K, "f32c", f32c)
+    monkeypatch.setattr(K, "call", lambda *a: alive.append([c() is not None for c in copies]))
+    x, w = torch.zeros(3, 16), torch.ones(16, dtype=torch.float16)
+    for call, n in ((lambda: K.layer_norm_bwd(x, x, w), 1), (lambda: K.dropout_add_ln(x, x, w, w, 1e-5, 0.0, None), 2),
+                    (lambda: K.dropout_add_ln_bwd(x, x, x, w, 1e-5, 0.0, None), 1)):
+        copies.clear(), alive.clear()
+        call()
+        assert alive == [[True] * n]
+
+
+def test_modules():
+    from boltz_mlx_amd.layers.dropout import Dropout
+
+    d = Dropout(0.25, shared="row", site=3)
+    x = torch.zeros(2, 3)
+    assert d.eval()(x, None) is x and Dropout(0.0).train()(x, None) is x
+    assert "0.25" in repr(d) and "row" in repr(d)
+    with pytest.raises(ValueError):
+        Dropout(1.5)
