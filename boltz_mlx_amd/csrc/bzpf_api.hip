@@ -107,6 +107,7 @@ bool make_drop(const char* who, double p, const int64_t* rng, int site, int shar
   if (d->mode == bzpf::DROP_OFF) return true;
   if (rng == nullptr || (reinterpret_cast<uintptr_t>(rng) & 7u)) return bad("rng must be a non-null pointer to two int64");
   if (shared && (I < 1 || J < 1 || rows % I || rows / I % J)) return bad("rows must be a multiple of I * J");
+  if (shared && rows > UINT32_MAX) return bad("shared draws need fewer than 2^32 rows");
   if (rows > ((int64_t)1 << 48) / ((D + 3) / 4)) return bad("more draws than 2^48 blocks");
   return true;
 }

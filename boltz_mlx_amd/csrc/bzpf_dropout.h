@@ -17,15 +17,19 @@ __device__ __forceinline__ Key drop_key(const Drop& d) {
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);  // one v_bitop3_b32 (truth table of a ^ b ^ c)
+}
+
 // The four words of block n: counter = (n bits 0-31, n bits 32-47 | site << 16, offset), key = seed.
 __device__ __forceinline__ u4 draw_block(uint64_t n, uint32_t site, Key k) {
   uint32_t c0 = (uint32_t)n, c1 = (uint32_t)(n >> 32) | site << 16, c2 = k.o0, c3 = k.o1;
 #pragma unroll
   for (int r = 0; r < 10; r++) {
     const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k.k0;
+    c0 = xor3((uint32_t)(p1 >> 32), c1, k.k0);
     c1 = (uint32_t)p1;
-    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k.k1;
+    c2 = xor3((uint32_t)(p0 >> 32), c3, k.k1);
     c3 = (uint32_t)p0;
     k.k0 += 0x9E3779B9u;
     k.k1 += 0xBB67AE85u;
@@ -33,34 +37,35 @@ __device__ __forceinline__ u4 draw_block(uint64_t n, uint32_t site, Key k) {
   return u4{c0, c1, c2, c3};
 }
 
-// The draw that a whole row r (of I * J rows a slice) shares: one for each row i or column j of the slice.
-__device__ __forceinline__ uint32_t draw_shared(const Drop& d, Key k, int64_t r) {
-  int64_t g;
-  if (((uint64_t)r | (uint64_t)d.I * (uint64_t)d.J) >> 32 == 0) {  // the 32-bit division is the shorter one
-    const uint32_t q = (uint32_t)r, J = (uint32_t)d.J;
-    g = d.mode == DROP_ROW ? q / J : (q / ((uint32_t)d.I * J)) * J + q % J;
-  } else {
-    g = d.mode == DROP_ROW ? r / d.J : (r / (d.I * d.J)) * d.J + r % d.J;
-  }
-  const u4 w = draw_block((uint64_t)g >> 2, d.site, k);
+// Whether the draw that a whole row r (of I * J rows a slice; fewer than 2^32 in all) shares drops it: one draw for each
+// row i or column j of the slice.
+__device__ __forceinline__ bool drops_row(const Drop& d, Key k, int64_t r) {
+  const uint32_t row = (uint32_t)r, J = (uint32_t)d.J, q = row / J;
+  const uint32_t g = d.mode == DROP_ROW ? q : q / (uint32_t)d.I * J + (row - q * J);
+  const u4 w = draw_block(g >> 2, d.site, k);
   const uint32_t a = g & 1 ? w[1] : w[0], b = g & 1 ? w[3] : w[2];
-  return g & 2 ? b : a;
+  return (g & 2 ? b : a) <= d.last;
 }
 
-// Applies the element draws to the eight columns v of a row, the first of them column `s` (0 to 3) of block n. Blocks
-// hold four columns counted from the row's start, so that s is 0 but for a chunk moved back from the row's end, which
-// then meets three blocks.
-__device__ __forceinline__ f8 drop_elements(const Drop& d, Key k, uint64_t n, int s, f8 v) {
-  const u4 a = draw_block(n, d.site, k), b = draw_block(n + 1, d.site, k);
-  uint32_t w[11] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3], 0, 0, 0};
-  if (s) {
-    const u4 c = draw_block(n + 2, d.site, k);
-    w[8] = c[0], w[9] = c[1], w[10] = c[2];
+// The element draws of VE columns of a row as bits (bit e set: column e is kept), the first of them column `s` (0 to 3) of
+// block n. Blocks hold four columns counted from the row's start, so that s is 0 but for a chunk moved back from the row's
+// end, which then meets one block more.
+template <int VE>
+__device__ __forceinline__ uint32_t kept(const Drop& d, Key k, uint64_t n, int s) {
+  const auto block = [&](int j) {
+    const u4 w = draw_block(n + j, d.site, k);
+    return (w[0] > d.last ? 1u : 0u) | (w[1] > d.last ? 2u : 0u) | (w[2] > d.last ? 4u : 0u) | (w[3] > d.last ? 8u : 0u);
+  };
+  uint32_t bits = block(0);
+  if (VE == 8) bits |= block(1) << 4;
+  if (s) bits = (bits | block(VE / 4) << VE) >> s;
+  return bits;
+}
+// v[e] / (1 - p) where bit `first` + e is set, else 0 (whatever v holds).
+template <int VE>
+__device__ __forceinline__ fv<VE> keep(const Drop& d, uint32_t bits, int first, fv<VE> v) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) w[e] = s == 1 ? w[e + 1] : s == 2 ? w[e + 2] : w[e + 3];
-  }
-#pragma unroll
-  for (int e = 0; e < 8; e++) v[e] = w[e] <= d.last ? 0.f : v[e] * d.scale;
+  for (int e = 0; e < VE; e++) v[e] = bits >> (first + e) & 1 ? v[e] * d.scale : 0.f;
   return v;
 }
 

@@ -7,37 +7,55 @@
 
 namespace bzpf {
 
-// One chunk of eight columns a thread; rows of any width. A chunk that passes the row's end takes its elements one by
-// one (rows may be shorter than a chunk here).
-template <typename TX, typename TY>
+// One chunk of VE columns a thread (two or four, their loads together, measured the same or slower). FLAT: D is a multiple
+// of VE, so chunk i is element VE i, block VE i / 4, and only a shared draw needs its row. Otherwise a chunk that would
+// pass the row's end is moved back to D - VE: its first elements are the neighbour's too, who writes the same values there
+// (each is one product, of the same factors). Rows shorter than a chunk (D < VE) are taken element by element.
+template <typename TX, typename TY, int MODE, bool FLAT>
 __global__ __launch_bounds__(256) void dropout_k(const TX* __restrict__ x, Drop drop, TY* __restrict__ y, int64_t rows,
                                                  int64_t D) {
-  const int64_t chunks = (D + 7) / 8, n = rows * chunks, per = (D + 3) / 4;
+  constexpr int VE = chunk_of<TX, TY>();
+  const int64_t chunks = (D + VE - 1) / VE, n = rows * chunks, per = (D + 3) / 4;
+  const bool small = n >> 32 == 0;
   Key key{};
-  if (drop.mode != DROP_OFF) key = drop_key(drop);
+  if (MODE != DROP_OFF) key = drop_key(drop);
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / chunks, at = 8 * (i - r * chunks);
-    const TX* const xp = x + r * D + at;
-    TY* const yp = y + r * D + at;
-    const int m = D - at < 8 ? (int)(D - at) : 8;
-    f8 v{};
-    if (m == 8) {
-      v = load8(xp);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 7; e++)
-        if (e < m) v[e] = (float)xp[e];
+    // the 32-bit division is a third as long
+    const int64_t r = FLAT && MODE < DROP_ROW ? 0 : small ? (int64_t)((uint32_t)i / (uint32_t)chunks) : i / chunks;
+    int64_t col = 0, at = VE * i;  // the chunk's column and its first element
+    if (!FLAT) {
+      col = VE * (i - r * chunks);
+      col = col + VE <= D ? col : D < VE ? 0 : D - VE;
+      at = r * D + col;
     }
-    if (drop.mode == DROP_ELEMENT) v = drop_elements(drop, key, (uint64_t)r * per + (at >> 2), 0, v);
-    if (drop.mode >= DROP_ROW) v = draw_shared(drop, key, r) <= drop.last ? f8{} : v * drop.scale;
-    if (m == 8) {
-      store8(yp, v);
+    fv<VE> v{};
+    if (FLAT || D >= VE) {
+      v = load_chunk<VE>(x + at);
     } else {
 #pragma unroll
-      for (int e = 0; e < 7; e++)
-        if (e < m) yp[e] = (TY)v[e];
+      for (int e = 0; e < VE - 1; e++)
+        if (e < D) v[e] = (float)x[at + e];
+    }
+    if (MODE == DROP_ELEMENT) {
+      const uint64_t block = FLAT ? (uint64_t)at >> 2 : (uint64_t)(r * per + (col >> 2));
+      v = keep<VE>(drop, kept<VE>(drop, key, block, (int)(col & 3)), 0, v);
+    }
+    if (MODE >= DROP_ROW) v = drops_row(drop, key, r) ? fv<VE>{} : v * drop.scale;
+    if (FLAT || D >= VE) {
+      store_chunk<VE>(y + at, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE - 1; e++)
+        if (e < D) y[at + e] = (TY)v[e];
     }
   }
+}
+
+template <typename TX, typename TY, bool FLAT>
+static auto dropout_kernel(int mode) {
+  return mode == DROP_OFF       ? dropout_k<TX, TY, DROP_OFF, FLAT>
+         : mode == DROP_ELEMENT ? dropout_k<TX, TY, DROP_ELEMENT, FLAT>
+                                : dropout_k<TX, TY, DROP_ROW, FLAT>;  // column draws too
 }
 
 hipError_t launch_dropout(const void* x, int x_dt, const Drop& drop, void* y, int y_dt, int64_t rows, int64_t D,
@@ -45,46 +63,44 @@ hipError_t launch_dropout(const void* x, int x_dt, const Drop& drop, void* y, in
   return with_types(x_dt, y_dt, [&](auto tx, auto ty) {
     typedef std::remove_cv_t<std::remove_pointer_t<decltype(tx)>> TX;
     typedef std::remove_cv_t<std::remove_pointer_t<decltype(ty)>> TY;
-    dropout_k<TX, TY><<<row_blocks(rows * ((D + 7) / 8), 256, 1 << 16), 256, 0, st>>>(
+    constexpr int VE = chunk_of<TX, TY>();
+    const auto kernel =
+        D % VE == 0 ? dropout_kernel<TX, TY, true>(drop.mode) : dropout_kernel<TX, TY, false>(drop.mode);
+    kernel<<<row_blocks(rows * ((D + VE - 1) / VE), 256, 1 << 16), 256, 0, st>>>(
         static_cast<const TX*>(x), drop, static_cast<TY*>(y), rows, D);
     return hipGetLastError();
   });
 }
 
-template <typename TY, typename TO, int L, int NV>
-__global__ __launch_bounds__(256) void dropout_add_ln_k(const float* __restrict__ z, const TY* __restrict__ y,
-                                                        Drop drop, const float* __restrict__ w,
-                                                        const float* __restrict__ b, float eps,
-                                                        float* __restrict__ z_new, TO* __restrict__ ln, int64_t rows,
-                                                        int D) {
-  __shared__ float red[8];
-  const RowSpan<L, NV> sp(threadIdx.x % L, D);
+template <typename TY, typename TO, int L, int E>
+__global__ __launch_bounds__(row_threads(L)) void dropout_add_ln_k(
+    const float* __restrict__ z, const TY* __restrict__ y, Drop drop, const float* __restrict__ w,
+    const float* __restrict__ b, float eps, float* __restrict__ z_new, TO* __restrict__ ln, int64_t rows, int D) {
+  __shared__ float red[2 * row_red(L)];
+  constexpr int R = row_threads(L) / L, VE = 4, NV = E / VE;
+  const RowSpan<L, NV, VE> sp(threadIdx.x % L, D);
   const int64_t per = (D + 3) / 4;
-  constexpr int R = 256 / L;
   Key key{};
   if (drop.mode != DROP_OFF) key = drop_key(drop);
+  fv<VE> pw[NV], pb[NV];
+  row_param(pw, sp, w, 1.f);
+  row_param(pb, sp, b, 0.f);
   for (int64_t r = (int64_t)blockIdx.x * R + threadIdx.x / L; r < rows; r += (int64_t)gridDim.x * R) {
-    f8 v[NV];
-    bool dropped = false;
-    if (drop.mode >= DROP_ROW) dropped = draw_shared(drop, key, r) <= drop.last;
+    fv<VE> v[NV];
+    const bool dropped = drop.mode >= DROP_ROW && drops_row(drop, key, r);
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-      v[k] = load8(z + r * D + sp.at[k]);
-      f8 t = load8(y + r * D + sp.at[k]);
+      v[k] = load_chunk<VE>(z + r * D + sp.at[k]);
+      fv<VE> t = load_chunk<VE>(y + r * D + sp.at[k]);
       if (drop.mode == DROP_ELEMENT)
-        t = drop_elements(drop, key, (uint64_t)r * per + (sp.at[k] >> 2), sp.at[k] & 3, t);
-      if (drop.mode >= DROP_ROW) t = dropped ? f8{} : t * drop.scale;
+        t = keep<VE>(drop, kept<VE>(drop, key, (uint64_t)r * per + (sp.at[k] >> 2), sp.at[k] & 3), 0, t);
+      if (drop.mode >= DROP_ROW) t = dropped ? fv<VE>{} : t * drop.scale;
       v[k] += t;
       sp.store(k, z_new + r * D, v[k]);
     }
-    const float rstd = centre_row<L, NV>(v, sp, D, eps, red);
+    const float rstd = centre_row(v, sp, D, eps, red);
 #pragma unroll
-    for (int k = 0; k < NV; k++) {
-      f8 o = v[k] * rstd;
-      if (w) o *= load8(w + sp.at[k]);
-      if (b) o += load8(b + sp.at[k]);
-      sp.store(k, ln + r * D, o);
-    }
+    for (int k = 0; k < NV; k++) sp.store(k, ln + r * D, v[k] * rstd * pw[k] + pb[k]);
   }
 }
 
@@ -96,7 +112,8 @@ hipError_t launch_dropout_add_ln(const float* z, const void* y, int y_dt, const 
       typedef decltype(lay) Lay;
       typedef std::remove_cv_t<std::remove_pointer_t<decltype(ty)>> TY;
       typedef std::remove_cv_t<std::remove_pointer_t<decltype(to)>> TO;
-      dropout_add_ln_k<TY, TO, Lay::L, Lay::NV><<<row_blocks(rows, 256 / Lay::L, 1 << 20), 256, 0, st>>>(
+      constexpr int T = row_threads(Lay::L);
+      dropout_add_ln_k<TY, TO, Lay::L, Lay::E><<<row_blocks(rows, T / Lay::L, 1 << 20), T, 0, st>>>(
           z, static_cast<const TY*>(y), drop, w, b, eps, z_new, static_cast<TO*>(ln), rows, D);
       return hipGetLastError();
     });

@@ -9,25 +9,23 @@
 
 namespace bzpf {
 
-template <typename TX, typename TY, int L, int NV>
-__global__ __launch_bounds__(256) void ln_rows_k(const TX* __restrict__ x, const float* __restrict__ w,
-                                                 const float* __restrict__ b, float eps, TY* __restrict__ y,
-                                                 int64_t rows, int D) {
-  __shared__ float red[8];
-  const RowSpan<L, NV> sp(threadIdx.x % L, D);
-  constexpr int R = 256 / L;
+template <typename TX, typename TY, int L, int E>
+__global__ __launch_bounds__(row_threads(L)) void ln_rows_k(const TX* __restrict__ x, const float* __restrict__ w,
+                                                            const float* __restrict__ b, float eps,
+                                                            TY* __restrict__ y, int64_t rows, int D) {
+  __shared__ float red[2 * row_red(L)];
+  constexpr int R = row_threads(L) / L, VE = chunk_of<TX, TY>(), NV = E / VE;
+  const RowSpan<L, NV, VE> sp(threadIdx.x % L, D);
+  fv<VE> pw[NV], pb[NV];
+  row_param(pw, sp, w, 1.f);
+  row_param(pb, sp, b, 0.f);
   for (int64_t r = (int64_t)blockIdx.x * R + threadIdx.x / L; r < rows; r += (int64_t)gridDim.x * R) {
-    f8 v[NV];
+    fv<VE> v[NV];
 #pragma unroll
-    for (int k = 0; k < NV; k++) v[k] = load8(x + r * D + sp.at[k]);
-    const float rstd = centre_row<L, NV>(v, sp, D, eps, red);
+    for (int k = 0; k < NV; k++) v[k] = load_chunk<VE>(x + r * D + sp.at[k]);
+    const float rstd = centre_row(v, sp, D, eps, red);
 #pragma unroll
-    for (int k = 0; k < NV; k++) {
-      f8 o = v[k] * rstd;
-      if (w) o *= load8(w + sp.at[k]);
-      if (b) o += load8(b + sp.at[k]);
-      sp.store(k, y + r * D, o);
-    }
+    for (int k = 0; k < NV; k++) sp.store(k, y + r * D, v[k] * rstd * pw[k] + pb[k]);
   }
 }
 
@@ -38,7 +36,8 @@ hipError_t launch_layernorm_rows(const void* x, int x_dt, const float* w, const 
       typedef decltype(lay) Lay;
       typedef std::remove_cv_t<std::remove_pointer_t<decltype(tx)>> TX;
       typedef std::remove_cv_t<std::remove_pointer_t<decltype(ty)>> TY;
-      ln_rows_k<TX, TY, Lay::L, Lay::NV><<<row_blocks(rows, 256 / Lay::L, 1 << 20), 256, 0, st>>>(
+      constexpr int T = row_threads(Lay::L);
+      ln_rows_k<TX, TY, Lay::L, Lay::E><<<row_blocks(rows, T / Lay::L, 1 << 20), T, 0, st>>>(
           static_cast<const TX*>(x), w, b, eps, static_cast<TY*>(y), rows, D);
       return hipGetLastError();
     });
@@ -56,19 +55,27 @@ hipError_t launch_layernorm_bwd(const void* dy, int dy_dt, const void* x, int x_
   });
 }
 
-// Sums of the workgroups' partial [2][D] (dw, then db) over `blocks` workgroups: 16 threads for each of 16 columns, each
-// adding every sixteenth partial sum, then the 16 in order.
-__global__ __launch_bounds__(256) void row_grad_sum_k(const float* __restrict__ ws, int64_t blocks, int D,
-                                                      float* __restrict__ dw, float* __restrict__ db) {
-  __shared__ float part[16][17];
+// Sums of the workgroups' partial [2][D] (dw, then db) over `blocks` <= 512 workgroups. A workgroup takes 16 columns: 64
+// threads a column each add every 64th partial sum, all loads in flight at once, then the 64 meet in a fixed order.
+__global__ __launch_bounds__(1024) void row_grad_sum_k(const float* __restrict__ ws, int blocks, int D,
+                                                       float* __restrict__ dw, float* __restrict__ db) {
+  __shared__ float part[64][17];
   const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
-  const int64_t col = (int64_t)blockIdx.x * 16 + c;
+  const int col = min(blockIdx.x * 16 + c, 2 * D - 1);
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) v[i] = g + 64 * i < blocks ? ws[(int64_t)(g + 64 * i) * 2 * D + col] : 0.f;
   float s = 0.f;
-  if (col < 2 * D)
-    for (int64_t i = g; i < blocks; i += 16) s += ws[i * 2 * D + col];
+#pragma unroll
+  for (int i = 0; i < 8; i++) s += v[i];
   part[g][c] = s;
   __syncthreads();
-  if (g == 0 && col < 2 * D) {
+  if (threadIdx.x < 256) {  // 16 threads a column, four partial sums each: the wave's lanes hold 4 rows of 16 columns
+    const int h = threadIdx.x >> 4;
+    part[h][c] = (part[h][c] + part[h + 16][c]) + (part[h + 32][c] + part[h + 48][c]);
+  }
+  __syncthreads();
+  if (threadIdx.x < 16 && blockIdx.x * 16 + c < 2 * D) {
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; i++) s += part[i][c];
@@ -78,7 +85,7 @@ __global__ __launch_bounds__(256) void row_grad_sum_k(const float* __restrict__ 
 }
 
 hipError_t launch_row_grad_sum(const float* ws, int64_t blocks, int D, float* dw, float* db, hipStream_t st) {
-  row_grad_sum_k<<<(unsigned)((2 * D + 15) / 16), 256, 0, st>>>(ws, blocks, D, dw, db);
+  row_grad_sum_k<<<(unsigned)((2 * D + 15) / 16), 1024, 0, st>>>(ws, (int)blocks, D, dw, db);
   return hipGetLastError();
 }
 

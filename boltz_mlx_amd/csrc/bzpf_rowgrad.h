@@ -27,17 +27,23 @@ struct RowGrad {
   int D;
 };
 
-// Workgroups of the backward pass: one for every four rows of each of its row places, up to 1024 (four for each
-// compute unit), so that the partial sums stay few.
+// Workgroups of the backward pass: enough for four rows in each of their row places, but not fewer than one for each
+// compute unit while rows last, nor more than two (one past D = 2048): each writes its partial sums, which the second
+// kernel reads. Measured with 256 / 512 / 768 workgroups in bf16 (fp32): 1 M rows of 128 195 / 140 / 133 us (270 / 288 /
+// 287), 16000 of 1024 26 / 26 / 26 (41 / 41 / 43), 6000 of 2048 33 / 27 / 24 (33 / 33 / 34); 4096 of 4096 with 256 / 512
+// 30 / 30 (44 / 47), 2048 of 8192 31 / 43 (47 / 56).
 static inline int64_t row_grad_blocks(int64_t rows, int D) {
-  const int per = D <= 64 ? 32 : D <= 128 ? 16 : D <= 256 ? 8 : D <= 2048 ? 4 : 1;  // rows that it holds at once
-  return row_blocks(rows, 4 * per, 1024);
+  const int per = row_places(D);
+  const int64_t all = row_blocks(rows, per, 256), four = row_blocks(rows, 4 * per, D <= 2048 ? 512 : 256);
+  return all > four ? all : four;
 }
 
 // The sum of v over the 64 / L lanes of a wave that hold the same columns of different rows.
 template <int L>
 __device__ __forceinline__ float column_sum(float v) {
-  if constexpr (L <= 8) v = dpp_add<0x128>(v);  // row_ror by 8: the other half of the DPP row
+  if constexpr (L <= 2) v = dpp_add<0x122>(v);  // row_ror by 2, 4 and 8: the other lanes of the DPP row
+  if constexpr (L <= 4) v = dpp_add<0x124>(v);
+  if constexpr (L <= 8) v = dpp_add<0x128>(v);
   if constexpr (L <= 16) {
     const unsigned u = __float_as_uint(v);
     const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
@@ -51,70 +57,115 @@ __device__ __forceinline__ float column_sum(float v) {
   return v;
 }
 
-// The workgroup's sums over its rows of s (chunks as in sp) into out [D].
+// sp.store of an fp32 chunk (two accesses where it has eight channels).
 template <int L, int NV>
-__device__ __forceinline__ void meet_columns(f8 (&s)[NV], const RowSpan<L, NV>& sp, int D, float* meet, float* out) {
-  if constexpr (L == 256) {
+__device__ __forceinline__ void store_param(const RowSpan<L, NV, 4>& sp, int k, float* row, fv<4> v) {
+  sp.store(k, row, v);
+}
+template <int L, int NV>
+__device__ __forceinline__ void store_param(const RowSpan<L, NV, 8>& sp, int k, float* row, fv<8> v) {
+  if (sp.whole(k) || sp.skip[k] == 0) {
+    store_chunk<4>(row + sp.at[k], fv<4>{v[0], v[1], v[2], v[3]});
+    store_chunk<4>(row + sp.at[k] + 4, fv<4>{v[4], v[5], v[6], v[7]});
+  } else {
 #pragma unroll
-    for (int k = 0; k < NV; k++) sp.store(k, out, s[k]);
+    for (int e = 1; e < 8; e++)
+      if (e >= sp.skip[k]) row[sp.at[k] + e] = v[e];
+  }
+}
+
+// The workgroup's sums over its rows of s (chunks as in sp) into out [D].
+template <int L, int NV, int VE>
+__device__ __forceinline__ void meet_columns(fv<VE> (&s)[NV], const RowSpan<L, NV, VE>& sp, int D, float* meet,
+                                             float* out) {
+  if constexpr (L > 64) {
+#pragma unroll
+    for (int k = 0; k < NV; k++) store_param(sp, k, out, s[k]);
   } else {
     __syncthreads();  // meet's last reader is done
 #pragma unroll
     for (int k = 0; k < NV; k++) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) s[k][e] = column_sum<L>(s[k][e]);
-      if ((threadIdx.x & 63) < L) sp.store(k, meet + (threadIdx.x >> 6) * D, s[k]);
+      for (int e = 0; e < VE; e++) s[k][e] = column_sum<L>(s[k][e]);
+      if ((threadIdx.x & 63) < L) store_param(sp, k, meet + (threadIdx.x >> 6) * D, s[k]);
     }
     __syncthreads();
     for (int c = threadIdx.x; c < D; c += 256) out[c] = (meet[c] + meet[D + c]) + (meet[2 * D + c] + meet[3 * D + c]);
   }
 }
 
-template <bool RES, typename TX, typename TG, typename TY, int L, int NV>
-__global__ __launch_bounds__(256) void row_grad_k(RowGrad<TX, TG, TY> a) {
-  constexpr int R = 256 / L;
-  __shared__ float red[16];
-  __shared__ float meet[L < 256 ? 4 * 8 * L * NV : 1];
+// Four waves a SIMD (128 registers) with 8 channels a lane, two with 16: what the sums, the row and the next row's loads
+// need without spilling.
+template <bool RES, typename TX, typename TG, typename TY, int L, int E>
+__global__ __launch_bounds__(row_threads(L), E == 8 ? 4 : 2) void row_grad_k(RowGrad<TX, TG, TY> a) {
+  constexpr int R = row_threads(L) / L, VE = RES ? 4 : chunk_of<TX, TG>(), NV = E / VE;
+  __shared__ float red[4 * row_red(L)];
+  __shared__ float meet[L <= 64 ? 4 * L * E : 1];
   const int D = a.D;
-  const RowSpan<L, NV> sp(threadIdx.x % L, D);
+  const RowSpan<L, NV, VE> sp(threadIdx.x % L, D);
   const int64_t per = (D + 3) / 4;
   const float inv = 1.0f / D;
   Key key{};
   if (RES && a.drop.mode != DROP_OFF) key = drop_key(a.drop);
-  f8 sw[NV], sb[NV];
+  fv<VE> sw[NV], sb[NV], w[NV];
+  row_param(w, sp, a.w, 1.f);
 #pragma unroll
-  for (int k = 0; k < NV; k++) sw[k] = sb[k] = f8{};
-  for (int64_t r = (int64_t)blockIdx.x * R + threadIdx.x / L; r < a.rows; r += (int64_t)gridDim.x * R) {
-    f8 v[NV], g[NV];
+  for (int k = 0; k < NV; k++) sw[k] = sb[k] = fv<VE>{};
+  // the next row's loads are in flight while this one's sums are formed
+  Raw<TX, VE> rx[NV];
+  Raw<TG, VE> rg[NV];
+  const auto fetch = [&](int64_t r) {
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-      v[k] = load8(a.x + r * D + sp.at[k]);
-      g[k] = load8(a.g + r * D + sp.at[k]);
+      rx[k].load(a.x + r * D + sp.at[k]);
+      rg[k].load(a.g + r * D + sp.at[k]);
     }
-    const float rstd = centre_row<L, NV>(v, sp, D, a.eps, red);
+  };
+  int64_t r = (int64_t)blockIdx.x * R + threadIdx.x / L;
+  const int64_t step = (int64_t)gridDim.x * R;
+  if (r < a.rows) fetch(r);
+  for (; r < a.rows; r += step) {
+    fv<VE> v[NV], g[NV];
+    Raw<float, 4> z[NV];
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+      if (RES && a.dz_new) z[k].load(a.dz_new + r * D + sp.at[k]);  // used last: it may be on its way meanwhile
+      v[k] = rx[k].get();
+      g[k] = rg[k].get();
+    }
+    if (r + step < a.rows) fetch(r + step);
+    uint32_t bits = 0;  // of the lane's E elements, those that are kept
+    if constexpr (RES) {
+      if (a.drop.mode == DROP_ELEMENT) {
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+          bits |= (kept<VE>(a.drop, key, (uint64_t)r * per + (sp.at[k] >> 2), sp.at[k] & 3) & ((1u << VE) - 1)) << (k * VE);
+      } else {
+        bits = a.drop.mode >= DROP_ROW && drops_row(a.drop, key, r) ? 0u : ~0u;
+      }
+    }
+    const float rstd = centre_row(v, sp, D, a.eps, red);
     float c1 = 0.f, c2 = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
       v[k] *= rstd;
       sw[k] += g[k] * v[k];
       sb[k] += g[k];
-      if (a.w) g[k] *= load8(a.w + sp.at[k]);
-      c1 += sum8(sp.own(k, g[k]));
-      c2 += sum8(sp.own(k, g[k] * v[k]));
+      g[k] *= w[k];
+      c1 += sp.sum(k, g[k]);
+      c2 += sp.sum(k, g[k] * v[k]);
     }
-    c1 = row_sum<L>(c1, red + 8) * inv;
-    c2 = row_sum<L>(c2, red + 12) * inv;
-    bool dropped = false;
-    if (RES && a.drop.mode >= DROP_ROW) dropped = draw_shared(a.drop, key, r) <= a.drop.last;
+    c1 = row_sum<L>(c1, red + 2 * row_red(L)) * inv;
+    c2 = row_sum<L>(c2, red + 3 * row_red(L)) * inv;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-      f8 o = (g[k] - c1 - v[k] * c2) * rstd;
-      if (RES && a.dz_new) o += load8(a.dz_new + r * D + sp.at[k]);
+      fv<VE> o = (g[k] - c1 - v[k] * c2) * rstd;
+      if constexpr (RES) {
+        if (a.dz_new) o += z[k].get();
+      }
       sp.store(k, a.dx + r * D, o);
       if constexpr (RES) {
-        if (a.drop.mode == DROP_ELEMENT)
-          o = drop_elements(a.drop, key, (uint64_t)r * per + (sp.at[k] >> 2), sp.at[k] & 3, o);
-        if (a.drop.mode >= DROP_ROW) o = dropped ? f8{} : o * a.drop.scale;
+        if (a.drop.mode != DROP_OFF) o = keep<VE>(a.drop, bits, k * VE, o);
         sp.store(k, a.dy + r * D, o);
       }
     }
@@ -122,8 +173,8 @@ __global__ __launch_bounds__(256) void row_grad_k(RowGrad<TX, TG, TY> a) {
   if (!a.dw && !a.db) return;
   float* const ow = gridDim.x > 1 ? a.ws + (int64_t)blockIdx.x * 2 * D : a.dw;
   float* const ob = gridDim.x > 1 ? a.ws + (int64_t)blockIdx.x * 2 * D + D : a.db;
-  if (ow) meet_columns<L, NV>(sw, sp, D, meet, ow);
-  if (ob) meet_columns<L, NV>(sb, sp, D, meet, ob);
+  if (ow) meet_columns(sw, sp, D, meet, ow);
+  if (ob) meet_columns(sb, sp, D, meet, ob);
 }
 
 template <bool RES, typename TX, typename TG, typename TY>
@@ -131,7 +182,7 @@ static hipError_t launch_row_grad(const RowGrad<TX, TG, TY>& a, hipStream_t st) 
   const unsigned blocks = (unsigned)row_grad_blocks(a.rows, a.D);
   const hipError_t e = with_row_layout(a.D, [&](auto lay) {
     typedef decltype(lay) Lay;
-    row_grad_k<RES, TX, TG, TY, Lay::L, Lay::NV><<<blocks, 256, 0, st>>>(a);
+    row_grad_k<RES, TX, TG, TY, Lay::L, Lay::E><<<blocks, row_threads(Lay::L), 0, st>>>(a);
     return hipGetLastError();
   });
   if (e != hipSuccess || blocks == 1 || (!a.dw && !a.db)) return e;

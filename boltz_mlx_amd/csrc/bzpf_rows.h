@@ -1,75 +1,95 @@
 // Rows of any width 8 <= D <= 8192 for the training kernels (LayerNorm, dropout, residual update): a row lies in the
-// registers of L lanes, lane q holding the 8-channel chunks q, q + L, .. (NV of them), so that every pass over the row
-// after the first is free of memory traffic.
+// registers of L lanes, lane q holding the chunks q, q + L, .. (NV of them) of VE channels, so that every pass over the
+// row after the first is free of memory traffic.
 #pragma once
 
 #include "bzpf_common.h"
 #include "bzpf_kernels.h"
 
 typedef __bf16 bf16_t;
-typedef float f8 __attribute__((ext_vector_type(8)));
 
 namespace bzpf {
 
-// Eight consecutive elements at element alignment (rows of odd widths, views at odd offsets): gfx950 loads and stores
-// 16 bytes at any element alignment in one instruction, and at a 16-byte boundary as fast as an aligned type.
-typedef float f4e __attribute__((ext_vector_type(4), aligned(4)));
-typedef half_t h8e __attribute__((ext_vector_type(8), aligned(2)));
-typedef bf16_t b8e __attribute__((ext_vector_type(8), aligned(2)));
-typedef bf16_t b8 __attribute__((ext_vector_type(8)));
+// Chunks are 16 bytes of the widest type of a call: 4 channels where one of its tensors is fp32, else 8. Then every load
+// and store of a wave covers whole lines: chunks of 8 fp32 channels take two instructions of alternate 16-byte pieces,
+// whose halves of a line reach memory apart.
+template <typename... T> constexpr int chunk_of() { return (... || (sizeof(T) == 4)) ? 4 : 8; }
 
-__device__ __forceinline__ f8 load8(const float* p) {
-  const f4e a = *reinterpret_cast<const f4e*>(p), b = *reinterpret_cast<const f4e*>(p + 4);
-  return f8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-}
-__device__ __forceinline__ f8 load8(const half_t* p) {
-  return __builtin_convertvector(static_cast<half8>(*reinterpret_cast<const h8e*>(p)), f8);
-}
-__device__ __forceinline__ f8 load8(const bf16_t* p) {
-  return __builtin_convertvector(static_cast<b8>(*reinterpret_cast<const b8e*>(p)), f8);
-}
-__device__ __forceinline__ void store8(float* p, f8 v) {
-  *reinterpret_cast<f4e*>(p) = f4e{v[0], v[1], v[2], v[3]};
-  *reinterpret_cast<f4e*>(p + 4) = f4e{v[4], v[5], v[6], v[7]};
-}
-__device__ __forceinline__ void store8(half_t* p, f8 v) {
-  *reinterpret_cast<h8e*>(p) = __builtin_convertvector(v, half8);
-}
-__device__ __forceinline__ void store8(bf16_t* p, f8 v) { *reinterpret_cast<b8e*>(p) = __builtin_convertvector(v, b8); }
+template <int VE> struct Chunk;
+template <> struct Chunk<4> { typedef float f __attribute__((ext_vector_type(4))); };
+template <> struct Chunk<8> { typedef float f __attribute__((ext_vector_type(8))); };
+template <int VE> using fv = typename Chunk<VE>::f;
 
-// Where a lane's chunks lie: chunk k covers the columns at[k] .. at[k] + 7. A chunk that would pass the row's end is
-// moved back to D - 8, and its first skip[k] elements belong to its neighbour (8 or more: the chunk lies wholly past
-// the end). Loads then need no branch; sums and stores leave the skipped elements out.
-template <int L, int NV>
+// VE consecutive elements of T at element alignment (rows of odd widths, views at odd offsets): gfx950 loads and stores 8
+// or 16 bytes at any element alignment in one instruction, and at a whole boundary as fast as an aligned type. A Raw is a
+// chunk as it is in memory, so that a load in flight holds the registers of its own type only.
+template <typename T, int VE> struct Raw {
+  typedef T V __attribute__((ext_vector_type(VE)));
+  typedef T U __attribute__((ext_vector_type(VE), aligned(sizeof(T))));
+  static_assert(VE * sizeof(T) <= 16, "one access");
+  V v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const U*>(p); }
+  __device__ __forceinline__ fv<VE> get() const { return __builtin_convertvector(v, fv<VE>); }
+};
+
+template <int VE, typename T>
+__device__ __forceinline__ fv<VE> load_chunk(const T* p) {
+  Raw<T, VE> r;
+  r.load(p);
+  return r.get();
+}
+// Outputs go out as non-temporal stores of whole lines: nothing of them waits in L2 for the write-back at the kernel's end.
+// Residual update of 20 M elements 42 us instead of 45 (5 M: 11.7, 14.2), LayerNorm backward 39 instead of 42 (13.6, 15.6),
+// dropout in fp16 22 instead of 24; at 128 M elements the gain is 2 to 4%.
+template <int VE, typename T>
+__device__ __forceinline__ void store_chunk(T* p, fv<VE> v) {
+  typedef typename Raw<T, VE>::V V;
+  typedef typename Raw<T, VE>::U U;
+  __builtin_nontemporal_store(static_cast<U>(__builtin_convertvector(v, V)), reinterpret_cast<U*>(p));
+}
+
+__device__ __forceinline__ float sum_of(fv<4> v) { return (v[0] + v[1]) + (v[2] + v[3]); }
+__device__ __forceinline__ float sum_of(fv<8> v) {
+  return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+}
+
+// Where a lane's chunks lie: chunk k covers the columns at[k] .. at[k] + VE - 1. A chunk that would pass the row's end is
+// moved back to D - VE, and its first skip[k] elements belong to its neighbour (VE or more: the chunk lies wholly past
+// the end). Loads then need no branch; sums and stores leave the skipped elements out. The first half of a lane's chunks
+// is never moved (a layout serves widths past half of its own), none is where D fills the layout.
+template <int L, int NV, int VE>
 struct RowSpan {
   int at[NV], skip[NV];
+  bool full;
   __device__ __forceinline__ RowSpan(int q, int D) {
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-      const int c = 8 * (q + L * k);
-      at[k] = min(c, D - 8);
+      const int c = VE * (q + L * k);
+      at[k] = min(c, D - VE);
       skip[k] = c - at[k];
     }
+    full = D == L * NV * VE;
   }
-  // v[k] without the skipped elements (zeros in their place)
-  __device__ __forceinline__ f8 own(int k, f8 v) const {
+  static constexpr bool whole(int k) { return k < NV / 2; }
+  // the sum of chunk k's own elements
+  __device__ __forceinline__ float sum(int k, fv<VE> v) const {
+    if (!whole(k) && !full) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = e >= skip[k] ? v[e] : 0.f;
-    return v;
+      for (int e = 0; e < VE; e++) v[e] = e >= skip[k] ? v[e] : 0.f;
+    }
+    return sum_of(v);
   }
   template <typename T>
-  __device__ __forceinline__ void store(int k, T* row, f8 v) const {
-    if (skip[k] == 0) {
-      store8(row + at[k], v);
-    } else if (skip[k] < 8) {
+  __device__ __forceinline__ void store(int k, T* row, fv<VE> v) const {
+    if (whole(k) || skip[k] == 0) {
+      store_chunk<VE>(row + at[k], v);
+    } else if (skip[k] < VE) {
 #pragma unroll
-      for (int e = 1; e < 8; e++)
+      for (int e = 1; e < VE; e++)
         if (e >= skip[k]) row[at[k] + e] = (T)v[e];
     }
   }
 };
-
-__device__ __forceinline__ float sum8(f8 v) { return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])); }
 
 template <int CTRL>
 __device__ __forceinline__ float dpp_add(float v) {
@@ -77,17 +97,20 @@ __device__ __forceinline__ float dpp_add(float v) {
   return v + __int_as_float(u);
 }
 
+// Threads of a workgroup whose rows take L lanes each: 256, or the L of one wide row.
+constexpr int row_threads(int L) { return L > 256 ? L : 256; }
+
 // The sum of v over the L lanes of a row, in every one of them, in a fixed order. Steps of 1 and 2 lanes are quad
 // permutations, 4 and 8 the mirrors of half a DPP row and of a whole one (the lanes that they pair hold equal sums by
-// then), 16 and 32 the row and half-wave swaps. L = 256: the four waves' sums meet in `red` (four floats; a kernel that
-// calls it several times in a loop gives each call its own four, at least two of them, so that the next call's barrier
-// stands between a slot's reads and its next write).
+// then), 16 and 32 the row and half-wave swaps. L > 64 (the workgroup holds one row): the waves' sums meet in `red` (one
+// float a wave; a kernel that calls it several times in a loop gives each call floats of its own, at least two such
+// sets, so that the next call's barrier stands between a set's reads and its next write).
 template <int L>
 __device__ __forceinline__ float row_sum(float v, float* red) {
-  static_assert(L == 8 || L == 16 || L == 32 || L == 64 || L == 256, "lanes per row");
-  v = dpp_add<0xB1>(v);   // quad_perm [1, 0, 3, 2]
-  v = dpp_add<0x4E>(v);   // quad_perm [2, 3, 0, 1]
-  v = dpp_add<0x141>(v);  // row_half_mirror
+  static_assert(L >= 2 && L <= 1024 && (L & (L - 1)) == 0, "lanes per row");
+  v = dpp_add<0xB1>(v);                          // quad_perm [1, 0, 3, 2]
+  if constexpr (L >= 4) v = dpp_add<0x4E>(v);    // quad_perm [2, 3, 0, 1]
+  if constexpr (L >= 8) v = dpp_add<0x141>(v);   // row_half_mirror
   if constexpr (L >= 16) v = dpp_add<0x140>(v);  // row_mirror
   if constexpr (L >= 32) {
     const unsigned u = __float_as_uint(v);
@@ -99,49 +122,81 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
     const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
     v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
   }
-  if constexpr (L == 256) {
+  if constexpr (L > 64) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = (red[0] + red[1]) + (red[2] + red[3]);
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < L / 64; i += 2) v += red[i] + red[i + 1];
   }
   return v;
+}
+constexpr int row_red(int L) { return L > 64 ? L / 64 : 1; }  // floats that one call of row_sum needs
+
+// A LayerNorm parameter at a lane's columns, or `none` where there is none: loaded before the rows, so that no load stands
+// between a row's sums and its use (the wait for it would also wait for the next row's loads, which were issued before).
+template <int L, int NV, int VE>
+__device__ __forceinline__ void row_param(fv<VE> (&v)[NV], const RowSpan<L, NV, VE>& sp, const float* p, float none) {
+#pragma unroll
+  for (int k = 0; k < NV; k++) {
+    if (p) {
+#pragma unroll
+      for (int j = 0; j < VE; j += 4) {
+        const fv<4> t = load_chunk<4>(p + sp.at[k] + j);
+        v[k][j] = t[0], v[k][j + 1] = t[1], v[k][j + 2] = t[2], v[k][j + 3] = t[3];
+      }
+    } else {
+      v[k] = fv<VE>{} + none;
+    }
+  }
 }
 
 // Centres the row in v and returns 1 / sqrt(var + eps), by two passes over the registers (mean, then the squared
 // deviations): both sums in fp32. Skipped elements are centred too and left out of the sums.
-template <int L, int NV>
-__device__ __forceinline__ float centre_row(f8 (&v)[NV], const RowSpan<L, NV>& sp, int D, float eps, float* red) {
+template <int L, int NV, int VE>
+__device__ __forceinline__ float centre_row(fv<VE> (&v)[NV], const RowSpan<L, NV, VE>& sp, int D, float eps,
+                                            float* red) {
   float s = 0.f;
 #pragma unroll
-  for (int k = 0; k < NV; k++) s += sum8(sp.own(k, v[k]));
+  for (int k = 0; k < NV; k++) s += sp.sum(k, v[k]);
   const float inv = 1.0f / D;
   const float mean = row_sum<L>(s, red) * inv;
   float ss = 0.f;
 #pragma unroll
   for (int k = 0; k < NV; k++) {
     v[k] -= mean;
-    ss += sum8(sp.own(k, v[k] * v[k]));
+    ss += sp.sum(k, v[k] * v[k]);
   }
-  return 1.0f / sqrtf(row_sum<L>(ss, red + 4) * inv + eps);
+  return __builtin_amdgcn_rsqf(row_sum<L>(ss, red + row_red(L)) * inv + eps);  // v_rsq_f32: 1 ulp
 }
 
-template <int L_, int NV_>
+// L lanes a row, E channels a lane (E / VE chunks).
+template <int L_, int E_>
 struct RowLayout {
-  static constexpr int L = L_, NV = NV_;
+  static constexpr int L = L_, E = E_;
 };
 
-// Calls fn with the row layout of width D: the fewest lanes that hold the row in one chunk each, then whole waves of 2
-// and 4 chunks a lane, then whole workgroups.
+// Calls fn with the row layout of width D. One wave or less a row while 16 channels a lane hold it (no barrier then), whole
+// workgroups beyond. Measured on the backward pass of 16 M elements in bf16 (fp32): D = 1024 as 64 x 16 26 us (43), as
+// 256 x 8 39 (45); D = 2048 as 256 x 8 33 (42), as 64 x 32 (over 256 registers) 43 (57); D = 4096 as 256 x 16 30 (43), as
+// 512 x 8 32 (43); D = 8192 as 512 x 16 31 (48), as 1024 x 8 34 (51).
 template <typename Fn>
-static inline hipError_t with_row_layout(int D, Fn&& fn) {
-  if (D <= 64) return fn(RowLayout<8, 1>());
-  if (D <= 128) return fn(RowLayout<16, 1>());
-  if (D <= 256) return fn(RowLayout<32, 1>());
-  if (D <= 512) return fn(RowLayout<64, 1>());
-  if (D <= 1024) return fn(RowLayout<64, 2>());
-  if (D <= 2048) return fn(RowLayout<64, 4>());
-  if (D <= 4096) return fn(RowLayout<256, 2>());
-  return fn(RowLayout<256, 4>());
+static inline auto with_row_layout(int D, Fn&& fn) {
+  if (D <= 16) return fn(RowLayout<2, 8>());
+  if (D <= 32) return fn(RowLayout<4, 8>());
+  if (D <= 64) return fn(RowLayout<8, 8>());
+  if (D <= 128) return fn(RowLayout<16, 8>());
+  if (D <= 256) return fn(RowLayout<32, 8>());
+  if (D <= 512) return fn(RowLayout<64, 8>());
+  if (D <= 1024) return fn(RowLayout<64, 16>());
+  if (D <= 2048) return fn(RowLayout<256, 8>());
+  if (D <= 4096) return fn(RowLayout<256, 16>());
+  return fn(RowLayout<512, 16>());
+}
+
+// Rows that a workgroup holds at once at width D.
+static inline int row_places(int D) {
+  return with_row_layout(D, [](auto lay) { return row_threads(decltype(lay)::L) / decltype(lay)::L; });
 }
 
 // Calls fn(a, b) with a null pointer of each of the two storage types: fp32, fp16, bf16, but not fp16 with bf16.
@@ -160,7 +215,7 @@ static inline hipError_t with_types(int a, int b, Fn&& fn) {
   return hipErrorInvalidValue;
 }
 
-// Workgroups for `rows` rows where one of 256 threads holds `per` rows at once: all of them up to `most`, the rest by
+// Workgroups for `rows` rows where one holds `per` rows at once: all of them up to `most`, the rest by
 // a loop with the grid's stride.
 static inline unsigned row_blocks(int64_t rows, int per, int64_t most) {
   const int64_t n = (rows + per - 1) / per;
