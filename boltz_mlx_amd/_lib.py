@@ -109,3 +109,20 @@ def call(name: str, *args) -> None:
     if rc != 0:
         msg = load().bzpf_last_error().decode()
         raise BzpfError(f"{name} failed ({rc}): {msg}")
+
+
+_train = None
+
+
+def train():
+    """The torch binding of the training operators (boltz_mlx_amd/_train.so). Raises if it has not been built."""
+    global _train
+    if _train is None:
+        load()  # torch's HIP runtime and the library that it calls
+        try:
+            from boltz_mlx_amd import _train as module
+        except ImportError as e:
+            raise BzpfError("boltz_mlx_amd/_train.so is missing or does not load: build it with "
+                            "`python -c 'import __graft_entry__ as g; g.build()'`") from e
+        _train = module
+    return _train

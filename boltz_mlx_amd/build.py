@@ -1,6 +1,7 @@
-"""Builds libbzpf.so (the gfx950 HIP kernels behind the C ABI in include/bzpf.h) in-tree with hipcc.
+"""Builds libbzpf.so (the gfx950 HIP kernels behind the C ABI in include/bzpf.h) in-tree with hipcc, and _train.so (the
+torch binding of its training operators, host code only).
 
-Each .hip source under csrc/ is compiled to an object in parallel, then linked into boltz_mlx_amd/libbzpf.so.
+Each source under csrc/ is compiled to an object in parallel, then linked into boltz_mlx_amd/libbzpf.so and _train.so.
 Packed-FP32 instruction selection is disabled for the device code.
 """
 
@@ -11,12 +12,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libbzpf.so")
+TRAIN = os.path.join(HERE, "_train.so")
 ARCH = os.environ.get("BZPF_ARCH", "gfx950")
 
 HIPCC = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
@@ -51,35 +54,60 @@ def sources() -> list[str]:
 FILE_FLAGS = {"bzpf_triattn_mfma.hip": ["-fno-honor-nans"]}
 
 
+def torch_flags() -> list[str]:
+    """g++ flags of a source that includes torch's extension header and the HIP runtime's (host code only): the compiler
+    and settings of torch's own build, whose types and exceptions the binding shares."""
+    import torch
+
+    inc = os.path.join(os.path.dirname(torch_lib_dir()), "include")
+    rocm = os.path.dirname(os.path.dirname(os.path.realpath(HIPCC)))
+    dirs = (inc, os.path.join(inc, "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"],
+            os.path.join(rocm, "include"))
+    return ["-O2", "-fPIC", "-std=c++17", "-Wall", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__=1",
+            "-DTORCH_API_INCLUDE_EXTENSION_H", "-DTORCH_EXTENSION_NAME=_train",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+            *(x for d in dirs for x in ("-isystem", d))]
+
+
 def _compile(src: str) -> str:
-    obj = os.path.join(BUILD, os.path.basename(src)[:-4] + ".o")
-    cmd = [HIPCC, *CFLAGS, *FILE_FLAGS.get(os.path.basename(src), []), "-c", src, "-o", obj]
+    name, ext = os.path.splitext(os.path.basename(src))
+    obj = os.path.join(BUILD, name + ".o")
+    cmd = ["g++", *torch_flags()] if ext == ".cpp" else [HIPCC, *CFLAGS, *FILE_FLAGS.get(os.path.basename(src), [])]
+    cmd += ["-c", src, "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
     noise = "is not a recognized feature for this target"
     err = "\n".join(line for line in (r.stderr or "").splitlines() if noise not in line)
     if r.returncode != 0:
-        raise RuntimeError(f"hipcc failed on {os.path.basename(src)}:\n{err}")
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed on {os.path.basename(src)}:\n{err}")
     if err.strip():
         print(err, file=sys.stderr)
     return obj
 
 
+def _link(out: str, objs: list[str], *libs: str) -> None:
+    """A shared object at `out`, against torch's libraries; it finds those and its neighbours where they are now."""
+    tlib = torch_lib_dir()
+    r = subprocess.run(["g++", "-shared", "-fPIC", *objs, "-o", out + ".tmp", f"-L{HERE}", f"-L{tlib}",
+                        "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}", *(f"-l:{lib}" for lib in libs)],
+                       capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link of {os.path.basename(out)} failed:\n{r.stderr}")
+    os.replace(out + ".tmp", out)
+
+
 def build(verbose: bool = True) -> str:
     os.makedirs(BUILD, exist_ok=True)
-    srcs = sources()
+    binding = os.path.join(CSRC, "bzpf_torch.cpp")
+    srcs = [binding, *sources()]  # the binding first: torch's headers take the longest
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
-        objs = list(ex.map(_compile, srcs))
-    tmp = LIB + ".tmp"
+        train, *objs = ex.map(_compile, srcs)
     # Link against the HIP runtime that torch loads (torch/lib/libamdhip64.so), so that the library and torch
     # share one runtime instance (and one device context) in the process.
-    tlib = torch_lib_dir()
-    r = subprocess.run(["g++", "-shared", "-fPIC", *objs, "-o", tmp, f"-L{tlib}", f"-Wl,-rpath,{tlib}",
-                        "-l:libamdhip64.so"], capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"link failed:\n{r.stderr}")
-    os.replace(tmp, LIB)
+    _link(LIB, objs, "libamdhip64.so")
+    _link(TRAIN, [train], "libbzpf.so", "libtorch_python.so", "libtorch.so", "libtorch_cpu.so", "libc10_hip.so", "libc10.so",
+          "libamdhip64.so")
     if verbose:
-        print(f"built {LIB} from {len(srcs)} sources")
+        print(f"built {LIB} and {os.path.basename(TRAIN)} from {len(srcs)} sources")
     return LIB
 
 

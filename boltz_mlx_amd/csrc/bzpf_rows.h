@@ -167,7 +167,9 @@ __device__ __forceinline__ float centre_row(fv<VE> (&v)[NV], const RowSpan<L, NV
     v[k] -= mean;
     ss += sp.sum(k, v[k] * v[k]);
   }
-  return __builtin_amdgcn_rsqf(row_sum<L>(ss, red + row_red(L)) * inv + eps);  // v_rsq_f32: 1 ulp
+  const float var = row_sum<L>(ss, red + row_red(L)) * inv + eps;
+  const bool tiny = var < 0x1p-100f;  // v_rsq_f32 (1 ulp) takes a denormal for 0
+  return __builtin_amdgcn_rsqf(tiny ? var * 0x1p100f : var) * (tiny ? 0x1p50f : 1.f);
 }
 
 // L lanes a row, E channels a lane (E / VE chunks).

@@ -22,7 +22,7 @@ from typing import NamedTuple
 import torch
 
 from boltz_mlx_amd import _lib
-from boltz_mlx_amd._lib import BF16, F16, F32
+from boltz_mlx_amd._lib import F16, F32
 from boltz_mlx_amd._lib import call as _call
 
 PRECISION = os.environ.get("BOLTZ_MLX_PRECISION", "fp32")
@@ -44,7 +44,8 @@ SIDE = " (side stream)"
 def start_timing() -> None:
     """Record a start/end torch.cuda.Event pair on the current stream around every bzpf launch from now on; launches
     issued on another stream than the current one at this call are keyed `name + SIDE` (their intervals overlap the
-    main stream's and include the wait for free compute units)."""
+    main stream's and include the wait for free compute units). Launches that boltz_mlx_amd.autograd makes in its
+    backward passes are not recorded."""
     global _TIMING, _TIMING_STREAM
     _TIMING = {}
     _TIMING_STREAM = torch.cuda.current_stream()
@@ -60,16 +61,28 @@ def stop_timing() -> dict:
     return {name: [a.elapsed_time(b) for a, b in pairs] for name, pairs in t.items()}
 
 
-def call(name: str, *args) -> None:
+# The C entry point behind each function of the torch binding (csrc/bzpf_torch.cpp)
+_BINDING = {"layer_norm": "bzpf_layernorm", "layer_norm_bwd": "bzpf_layernorm_bwd", "dropout": "bzpf_dropout",
+            "dropout_add_ln": "bzpf_dropout_add_ln", "dropout_add_ln_bwd": "bzpf_dropout_add_ln_bwd",
+            "grad_layer_norm": "bzpf_layernorm", "grad_dropout": "bzpf_dropout",
+            "grad_dropout_add_ln": "bzpf_dropout_add_ln"}
+
+
+def call(name: str, *args):
+    """A C entry point (device pointers and sizes), or a function of the torch binding (tensors; returns its outputs)."""
     if _TIMING is None:
-        _call(name, *args)
-        return
+        if name in _BINDING:
+            return getattr(_lib._train or _lib.train(), name)(*args)
+        return _call(name, *args)
     a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     a.record()
-    _call(name, *args)
+    out = getattr(_lib.train(), name)(*args) if name in _BINDING else _call(name, *args)
     b.record()
-    key = name if torch.cuda.current_stream() == _TIMING_STREAM else name + SIDE
+    key = _BINDING.get(name, name)
+    if torch.cuda.current_stream() != _TIMING_STREAM:
+        key += SIDE
     _TIMING.setdefault(key, []).append((a, b))
+    return out
 
 
 def set_precision(mode: str) -> None:
@@ -94,17 +107,6 @@ def _dt(t: torch.Tensor) -> int:
     if t.dtype == torch.float16:
         return F16
     raise TypeError(f"unsupported dtype {t.dtype}")
-
-
-_TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-
-
-def _dt3(dtype: torch.dtype) -> int:
-    """The type code of the entry points that take bf16 as well (LayerNorm and the training operators)."""
-    dt = _TYPES.get(dtype)
-    if dt is None:
-        raise TypeError(f"unsupported dtype {dtype}")
-    return dt
 
 
 # The current stream's handle without the Stream object (6 us of a launch's 20 on the host), where torch has these two.
@@ -219,75 +221,16 @@ def f32c(t: torch.Tensor) -> torch.Tensor:
 def layer_norm(x: torch.Tensor, weight, bias, eps: float = 1e-5, out_dtype=torch.float32) -> torch.Tensor:
     """LayerNorm over the last axis (boltz_mlx/kernels.py:482-507), 8 to 8192 channels, fp32 / fp16 / bf16 (not fp16 with
     bf16). weight and bias may be None. Its gradients: layer_norm_bwd, or boltz_mlx_amd.autograd.layer_norm."""
-    x = x.contiguous()
-    _dev(x)
-    rows, D = _row_shape("layer_norm", x)
-    w, b = _affine("layer_norm", x, weight), _affine("layer_norm", x, bias)
-    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    with _on(x):
-        call("bzpf_layernorm", _p(x), _dt3(x.dtype), _p(w), _p(b), float(eps), _p(y), _dt3(out_dtype), rows, D, _stream())
-    return y
+    w = None if weight is None else f32c(weight)
+    b = None if bias is None else f32c(bias)
+    return call("layer_norm", x, w, b, eps, out_dtype)
 
 
 def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight, eps: float = 1e-5, need_weight: bool = True,
                    need_bias: bool = True):
     """The gradients of layer_norm(x, weight, bias, eps) for the output's gradient dy: (dx in x's type, dweight, dbias in
     fp32; None where not needed). The row statistics are formed again from x."""
-    dy, x = dy.contiguous(), x.contiguous()
-    _dev(dy, x)
-    _alike("layer_norm_bwd", x, dy)
-    rows, D = _row_shape("layer_norm_bwd", x)
-    w = _affine("layer_norm_bwd", x, weight)
-    dx = torch.empty_like(x)
-    with _on(x):
-        dw, db, ws, nws = _param_grads(x, rows, D, need_weight, need_bias)
-        if rows:
-            call("bzpf_layernorm_bwd", _p(dy), _dt3(dy.dtype), _p(x), _dt3(x.dtype), _p(w), float(eps), _p(dx), _p(dw),
-                 _p(db), _p(ws), nws, rows, D, _stream())
-    return dx, dw, db
-
-
-def _param_grads(x: torch.Tensor, rows: int, D: int, need_weight: bool, need_bias: bool):
-    """(dweight, dbias, workspace, its bytes) for a backward pass over x's rows; zeros where there are no rows."""
-    make = torch.empty if rows else torch.zeros
-    dw = make((D,), dtype=torch.float32, device=x.device) if need_weight else None
-    db = make((D,), dtype=torch.float32, device=x.device) if need_bias else None
-    n = int((_lib._lib or _lib.load()).bzpf_layernorm_bwd_ws(rows, D)) if need_weight or need_bias else 0
-    ws = torch.empty((n // 4,), dtype=torch.float32, device=x.device) if n > 0 else None
-    return dw, db, ws, n
-
-
-def _affine(name: str, x: torch.Tensor, t):
-    """A LayerNorm's weight or bias in fp32, contiguous, checked against x (None stays)."""
-    if t is None:
-        return None
-    if t.dim() != 1 or t.shape[0] != x.shape[-1] or t.device != x.device:
-        raise ValueError(f"{name}: weight and bias must be [{x.shape[-1]}] tensors on {x.device}")
-    return f32c(t)
-
-
-def _row_shape(name: str, x: torch.Tensor) -> tuple:
-    """(rows, D) of a tensor taken as rows of its last axis."""
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"{name}: need rows of channels, got {tuple(x.shape)}")
-    return x.shape[:-1].numel(), x.shape[-1]
-
-
-def _alike(name: str, x: torch.Tensor, *ts) -> None:
-    for t in ts:
-        if t.shape != x.shape or t.device != x.device:
-            raise ValueError(f"{name}: need tensors of one shape on one device, got {tuple(x.shape)} on {x.device} and "
-                             f"{tuple(t.shape)} on {t.device}")
-
-
-_NO_SWITCH = contextlib.nullcontext()
-
-
-def _on(t: torch.Tensor):
-    """A context in which t's device is the current one, and so _stream() a stream of t's device."""
-    if not t.is_cuda or (_device is not None and t.device.index == _device()):
-        return _NO_SWITCH
-    return torch.cuda.device(t.device)
+    return call("layer_norm_bwd", dy, x, weight, eps, need_weight, need_bias)
 
 
 def dropout_rng(seed: int, offset: int = 0, device="cuda") -> torch.Tensor:
@@ -300,22 +243,10 @@ def dropout_rng(seed: int, offset: int = 0, device="cuda") -> torch.Tensor:
 _SHARED = {None: 0, "row": 1, "column": 2}
 
 
-def _drop_args(name: str, x: torch.Tensor, p: float, rng, site: int, shared) -> tuple:
-    """(p, rng, site, shared, I, J) for the C entry points, checked against x ([.., I, J, D] where draws are shared)."""
-    if not 0.0 <= p <= 1.0:
-        raise ValueError(f"{name}: p must lie in [0, 1], got {p}")
+def _shared(name: str, shared) -> int:
     if shared not in _SHARED:
         raise ValueError(f"{name}: shared must be None, 'row' or 'column', got {shared!r}")
-    if not 0 <= site < 65536:
-        raise ValueError(f"{name}: site must lie in [0, 65535], got {site}")
-    if p > 0 and (rng is None or rng.dtype != torch.int64 or rng.shape != (2,) or not rng.is_contiguous()
-                  or rng.device != x.device):
-        raise ValueError(f"{name}: rng must be an int64 tensor (seed, offset) on {x.device} (dropout_rng)")
-    if shared is not None and x.dim() < 3:
-        raise ValueError(f"{name}: draws are shared over the rows or columns of a [.., I, J, D] tensor, got "
-                         f"{tuple(x.shape)}")
-    I, J = (x.shape[-3], x.shape[-2]) if shared is not None else (1, 1)
-    return float(p), _p(rng) if p > 0 else None, int(site), _SHARED[shared], I, J
+    return _SHARED[shared]
 
 
 def dropout(x: torch.Tensor, p: float, rng, site: int = 0, shared=None, out_dtype=None) -> torch.Tensor:
@@ -323,15 +254,7 @@ def dropout(x: torch.Tensor, p: float, rng, site: int = 0, shared=None, out_dtyp
     probability p and the rest scaled by 1 / (1 - p). The draws are Philox4x32-10 words of (rng, site, place): no mask is
     stored, and the same call on the output's gradient is the backward pass. A dropped element is 0 whatever x holds.
     rng: dropout_rng(..) (may be None for p = 0). Differentiable form: boltz_mlx_amd.autograd.dropout."""
-    x = x.contiguous()
-    _dev(x)
-    args = _drop_args("dropout", x, p, rng, site, shared)
-    y = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
-    D = x.shape[-1] if x.dim() else 1
-    if x.numel():
-        with _on(x):
-            call("bzpf_dropout", _p(x), _dt3(x.dtype), *args, _p(y), _dt3(y.dtype), x.numel() // D, D, _stream())
-    return y
+    return call("dropout", x, p, rng, site, _shared("dropout", shared), out_dtype)
 
 
 def dropout_add_ln(z: torch.Tensor, y: torch.Tensor, weight, bias, eps: float, p: float, rng, site: int = 0, shared=None,
@@ -339,20 +262,7 @@ def dropout_add_ln(z: torch.Tensor, y: torch.Tensor, weight, bias, eps: float, p
     """(z + dropout(y), LayerNorm of that) for the fp32 residual stream z [.., D] and y of its shape: the training form of
     add_ln, out of place. out_dtype: the LayerNorm output's type (default y's); dropout's arguments as in dropout().
     Differentiable form: boltz_mlx_amd.autograd.dropout_add_ln."""
-    z, y = z.contiguous(), y.contiguous()
-    _dev(z, y)
-    _alike("dropout_add_ln", z, y)
-    if z.dtype != torch.float32:
-        raise ValueError("dropout_add_ln: z must be fp32")
-    args = _drop_args("dropout_add_ln", z, p, rng, site, shared)
-    rows, D = _row_shape("dropout_add_ln", z)
-    w, b = _affine("dropout_add_ln", z, weight), _affine("dropout_add_ln", z, bias)
-    z_new = torch.empty_like(z)
-    ln = torch.empty(z.shape, dtype=out_dtype or y.dtype, device=z.device)
-    with _on(z):
-        call("bzpf_dropout_add_ln", _p(z), _p(y), _dt3(y.dtype), *args, _p(w), _p(b), float(eps), _p(z_new), _p(ln),
-             _dt3(ln.dtype), rows, D, _stream())
-    return z_new, ln
+    return call("dropout_add_ln", z, y, weight, bias, eps, p, rng, site, _shared("dropout_add_ln", shared), out_dtype)
 
 
 def dropout_add_ln_bwd(dz_new, dln: torch.Tensor, z_new: torch.Tensor, weight, eps: float, p: float, rng, site: int = 0,
@@ -360,23 +270,8 @@ def dropout_add_ln_bwd(dz_new, dln: torch.Tensor, z_new: torch.Tensor, weight, e
     """The gradients of dropout_add_ln for those of its outputs, dz_new (fp32, or None for zero) and dln, at its output
     z_new and with the call's p, rng, site and shared: (dz fp32, dy in y_dtype (default dln's), dweight, dbias in fp32;
     None where not needed)."""
-    dln, z_new = dln.contiguous(), z_new.contiguous()
-    dz_new = None if dz_new is None else dz_new.contiguous()
-    _dev(dln, z_new, dz_new)
-    _alike("dropout_add_ln_bwd", z_new, dln, *(() if dz_new is None else (dz_new,)))
-    if z_new.dtype != torch.float32 or (dz_new is not None and dz_new.dtype != torch.float32):
-        raise ValueError("dropout_add_ln_bwd: z_new and dz_new must be fp32")
-    args = _drop_args("dropout_add_ln_bwd", z_new, p, rng, site, shared)
-    rows, D = _row_shape("dropout_add_ln_bwd", z_new)
-    w = _affine("dropout_add_ln_bwd", z_new, weight)
-    dz = torch.empty_like(z_new)
-    dy = torch.empty(z_new.shape, dtype=y_dtype or dln.dtype, device=z_new.device)
-    with _on(z_new):
-        dw, db, ws, nws = _param_grads(z_new, rows, D, need_weight, need_bias)
-        if rows:
-            call("bzpf_dropout_add_ln_bwd", _p(dz_new), _p(dln), _dt3(dln.dtype), _p(z_new), _p(w), float(eps), *args,
-                 _p(dz), _p(dy), _dt3(dy.dtype), _p(dw), _p(db), _p(ws), nws, rows, D, _stream())
-    return dz, dy, dw, db
+    return call("dropout_add_ln_bwd", dz_new, dln, z_new, weight, eps, p, rng, site,
+                _shared("dropout_add_ln_bwd", shared), y_dtype, need_weight, need_bias)
 
 
 def count_nonfinite(*tensors: torch.Tensor) -> torch.Tensor:

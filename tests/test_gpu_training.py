@@ -69,14 +69,14 @@ def row_terms(x, eps=1e-5):
     return c * rstd, rstd, U * (16 * np.abs(x).max(-1, keepdims=True) * rstd + 14)
 
 
-def ln_tol(x, w, b):
-    xh, _, E = row_terms(x)
+def ln_tol(x, w, b, eps=1e-5):
+    xh, _, E = row_terms(x, eps)
     w = 1.0 if w is None else w
     return np.abs(w) * (1 + np.abs(xh)) * E + 2 * U * (np.abs(xh * w) + (0 if b is None else np.abs(b)))
 
 
-def dx_tol(dy, x, w):
-    xh, rstd, E = row_terms(x)
+def dx_tol(dy, x, w, eps=1e-5):
+    xh, rstd, E = row_terms(x, eps)
     G = np.abs(dy if w is None else dy * w).max(-1, keepdims=True)
     return rstd * G * (1 + np.abs(xh)) * (6 * E + 60 * U)
 
@@ -170,6 +170,21 @@ def test_layer_norm_hard_rows():
     tw, tb = dw_tol(df, xf)
     close(dw, rw, tw)
     close(db, rb, tb)
+
+
+def test_layer_norm_tiny_and_huge_rows():
+    """Variances that are denormal in fp32 (eps 0) and squares near its largest value. A square of s errs by half a denormal
+    step, 2^-150, and so does the mean of the squares: 2^-149 / s^2 of the variance at most, half of that of rstd and xh."""
+    w, b = params(1, 130)
+    for scale in (1e-19, 1e-20, 1e17):
+        x, dy = rand(2, 20, 130, scale=scale), rand(3, 20, 130)
+        y, (dx, _, _) = K().layer_norm(x, w, b, 0.0), K().layer_norm_bwd(dy, x, w, 0.0)
+        xr, dr, wr = np64(x), np64(dy), np64(w)
+        xh, rstd, _ = row_terms(xr, 0.0)
+        rel = 2.0 ** -149 / xr.var(-1, keepdims=True)
+        close(y, T.ln(xr, wr, np64(b), 0.0), ln_tol(xr, wr, np64(b), 0.0) + rel * np.abs(xh * wr))
+        G = np.abs(dr * wr).max(-1, keepdims=True)
+        close(dx, T.ln_grads(dr, xr, wr, 0.0)[0], dx_tol(dr, xr, wr, 0.0) + 4 * rel * rstd * G * (1 + np.abs(xh)))
 
 
 @pytest.mark.parametrize("D", [64, 77, 128, 384, 2056, 8191])
@@ -433,6 +448,44 @@ def test_autograd_needs_and_types():
     a, c = drop.add_ln(z, y, ln, rng)
     assert torch.equal(a, z + y.float())
     close(ln.with_grad(z), np64(ln(z)), 0 * np64(z))
+
+
+def test_half_parameters():
+    """Parameters that are not fp32 are converted for the call and live until its launch."""
+    x, z, y, g = acts(1, 50, 96, F32), acts(2, 50, 96, F32), rand(3, 50, 96), rand(4, 50, 96)
+    for dt in (F16, BF16):
+        w, b = (t.to(dt) for t in params(5, 96))
+        wf, bf = w.float(), b.float()
+        assert torch.equal(K().layer_norm(x, w, b), K().layer_norm(x, wf, bf))
+        for got, want in ((K().layer_norm_bwd(g, x, w), K().layer_norm_bwd(g, x, wf)),
+                          (K().dropout_add_ln(z, y, w, b, 1e-5, 0.0, None), K().dropout_add_ln(z, y, wf, bf, 1e-5, 0.0, None)),
+                          (K().dropout_add_ln_bwd(g, y, z, w[::1], 1e-5, 0.0, None),
+                           K().dropout_add_ln_bwd(g, y, z, wf, 1e-5, 0.0, None))):
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
+    strided = torch.stack([wf, wf + 1], 1)[:, 0]
+    assert torch.equal(K().layer_norm_bwd(g, x, strided)[0], K().layer_norm_bwd(g, x, wf)[0])
+
+
+def test_gradients_of_gradients_are_refused():
+    from boltz_mlx_amd import autograd as A
+
+    x, w = rand(1, 4, 32).requires_grad_(), rand(2, 32).requires_grad_()
+    for out in (A.layer_norm(x, w), A.dropout(x, 0.5, K().dropout_rng(1)), A.dropout_add_ln(x, x, w)[1]):
+        with pytest.raises(RuntimeError, match="gradients of gradients"):
+            torch.autograd.grad(out.sum(), x, create_graph=True)
+
+
+def test_launch_times_are_recorded():
+    x, w, rng = rand(1, 40, 64), rand(2, 64), K().dropout_rng(1)
+    K().start_timing()
+    K().layer_norm(x, w, w)
+    K().layer_norm_bwd(x, x, w)
+    K().dropout(x, 0.5, rng)
+    zn, _ = K().dropout_add_ln(x, x, w, w, 1e-5, 0.5, rng)
+    K().dropout_add_ln_bwd(x, x, zn, w, 1e-5, 0.5, rng)
+    times = K().stop_timing()
+    assert set(times) == {"bzpf_layernorm", "bzpf_layernorm_bwd", "bzpf_dropout", "bzpf_dropout_add_ln",
+                          "bzpf_dropout_add_ln_bwd"} and all(len(v) == 1 for v in times.values())
 
 
 # -------------------------------------------------------------------------------------------------- streams and graphs

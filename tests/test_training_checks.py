@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from boltz_mlx_amd import _lib
+from boltz_mlx_amd import autograd as A
 from boltz_mlx_amd import kernels as K
 
 HOST = ctypes.create_string_buffer(4096)
@@ -98,71 +99,76 @@ def test_workspace_sizes():
         assert n > 0 and n % (8 * D) == 0 and n // (8 * D) <= 1024  # whole [2][D] of fp32, at most 1024 workgroups
 
 
-@pytest.fixture
-def host(monkeypatch):
-    """The wrappers' own checks without a device: nothing may reach a launch."""
-    monkeypatch.setattr(K, "_dev", lambda *ts: None)
-    monkeypatch.setattr(K, "_stream", lambda: 0)
-    calls = []
-    monkeypatch.setattr(K, "call", lambda *a: calls.append(a))
-    return calls
+def refused(kind, what, call):
+    with pytest.raises(kind, match=what):
+        call()
 
 
-def test_wrappers_refuse(host):
+def test_wrappers_refuse():
+    """What the wrappers say to each wrong argument (they look at devices last, so that this needs none)."""
     x, w, rng = torch.zeros(2, 3, 4, 16), torch.ones(16), torch.zeros(2, dtype=torch.int64)
-    bad = [
-        lambda: K.layer_norm(x, torch.ones(15), None), lambda: K.layer_norm(x, w, torch.ones(1, 16)),
-        lambda: K.layer_norm(torch.zeros(3, 0), None, None), lambda: K.layer_norm(torch.tensor(1.0), None, None),
-        lambda: K.layer_norm_bwd(x[0], x, w), lambda: K.layer_norm_bwd(x, x, torch.ones(17)),
-        lambda: K.dropout(x, 1.5, rng), lambda: K.dropout(x, -0.5, rng), lambda: K.dropout(x, float("nan"), rng),
-        lambda: K.dropout(x, 0.5, None), lambda: K.dropout(x, 0.5, rng.int()), lambda: K.dropout(x, 0.5, rng[:1]),
-        lambda: K.dropout(x, 0.5, rng, site=65536), lambda: K.dropout(x, 0.5, rng, shared="rows"),
-        lambda: K.dropout(x[0, 0], 0.5, rng, shared="row"),
-        lambda: K.dropout_add_ln(x.half(), x, w, w, 1e-5, 0.5, rng), lambda: K.dropout_add_ln(x, x[0], w, w, 1e-5, 0.5, rng),
-        lambda: K.dropout_add_ln(x, x, w[:3], w, 1e-5, 0.5, rng),
-        lambda: K.dropout_add_ln_bwd(x[0], x, x, w, 1e-5, 0.5, rng),
-        lambda: K.dropout_add_ln_bwd(x.half(), x, x, w, 1e-5, 0.5, rng),
-        lambda: K.dropout_add_ln_bwd(x, x, x.half(), w, 1e-5, 0.5, rng),
-    ]
-    for k, call in enumerate(bad):
-        with pytest.raises(ValueError):
-            call()
-            pytest.fail(f"call {k} was taken")
-    for call in (lambda: K.layer_norm(x.double(), w, w), lambda: K.dropout(x.long(), 0.5, rng),
-                 lambda: K.layer_norm_bwd(x, x.double(), w)):
-        with pytest.raises(TypeError):
-            call()
-    assert not host
+    shape, param, prob = "one shape on one device", "weight and bias must be", "p must lie"
+    state, width, fp32 = "rng must be an int64", "8 to 8192 channels", "must be fp32"
+    for what, call in [
+        (shape, lambda: K.layer_norm_bwd(x[0], x, w)), (param, lambda: K.layer_norm_bwd(x, x, torch.ones(17))),
+        ("one-dimensional", lambda: A.layer_norm(x, w[None])), (width, lambda: K.layer_norm_bwd(x[..., :7], x[..., :7], None)),
+        (width, lambda: K.layer_norm_bwd(torch.zeros(2, 8193), torch.zeros(2, 8193), None)),
+        ("rows of channels", lambda: K.layer_norm_bwd(torch.zeros(3, 0), torch.zeros(3, 0), None)),
+        ("rows of channels", lambda: K.layer_norm_bwd(torch.tensor(1.0), torch.tensor(1.0), None)),
+        (prob, lambda: K.dropout(x, 1.5, rng)), (prob, lambda: K.dropout(x, -0.5, rng)),
+        (prob, lambda: K.dropout(x, float("nan"), rng)), (state, lambda: K.dropout(x, 0.5, None)),
+        (state, lambda: K.dropout(x, 0.5, rng.int())), (state, lambda: K.dropout(x, 0.5, rng[:1])),
+        (state, lambda: K.dropout(x, 0.5, torch.zeros(4, dtype=torch.int64)[::2])),
+        ("site must lie", lambda: K.dropout(x, 0.5, rng, site=65536)), ("site must lie", lambda: K.dropout(x, 0.5, rng, -1)),
+        ("shared must be", lambda: K.dropout(x, 0.5, rng, shared="rows")),
+        ("rows or columns", lambda: K.dropout(x[0, 0], 0.5, rng, shared="row")),
+        (fp32, lambda: K.dropout_add_ln(x.half(), x, w, w, 1e-5, 0.5, rng)),
+        (shape, lambda: K.dropout_add_ln(x, x[0], w, w, 1e-5, 0.5, rng)),
+        (param, lambda: K.dropout_add_ln(x, x, w[:3], w, 1e-5, 0.5, rng)),
+        (param, lambda: K.dropout_add_ln(x, x, w, w[:3], 1e-5, 0.5, rng)),
+        ("shared must be", lambda: K.dropout_add_ln(x, x, w, w, 1e-5, 0.5, rng, 0, "both")),
+        (width, lambda: K.dropout_add_ln(x[..., :5], x[..., :5], None, None, 1e-5, 0.0, None)),
+        (shape, lambda: K.dropout_add_ln_bwd(x[0], x, x, w, 1e-5, 0.5, rng)),
+        (shape, lambda: K.dropout_add_ln_bwd(None, x[0], x, w, 1e-5, 0.5, rng)),
+        (fp32, lambda: K.dropout_add_ln_bwd(x.half(), x, x, w, 1e-5, 0.5, rng)),
+        (fp32, lambda: K.dropout_add_ln_bwd(x, x, x.half(), w, 1e-5, 0.5, rng)),
+        (shape, lambda: A.dropout_add_ln(x, x[0], w, w)), (prob, lambda: A.dropout(x, 2.0, rng)),
+        (param, lambda: A.layer_norm(x, w[:4])),
+    ]:
+        refused(ValueError, what, call)
+    for call in (lambda: K.layer_norm_bwd(x, x.double(), w), lambda: K.dropout(x.long(), 0.5, rng),
+                 lambda: K.dropout(x, 0.5, rng, out_dtype=torch.float64), lambda: A.layer_norm(x, w, w, out_dtype=torch.int8)):
+        refused(TypeError, "unsupported dtype", call)
+
+
+def test_layer_norm_refuses():
+    x, w = torch.zeros(3, 16), torch.ones(16)
+    refused(ValueError, "weight and bias", lambda: K.layer_norm(x, w[:15], None))
+    refused(ValueError, "weight and bias", lambda: K.layer_norm(x, w, w[:, None].expand(16, 2)))
+    refused(ValueError, "rows of channels", lambda: K.layer_norm(x[:, :0], None, None))
+    refused(ValueError, "rows of channels", lambda: K.layer_norm(x[0, 0], None, None))
+    refused(ValueError, "8 to 8192", lambda: K.layer_norm(x[:, :7], None, None))
+    refused(TypeError, "unsupported dtype", lambda: K.layer_norm(x, w, w, out_dtype=torch.float64))
 
 
 def test_cpu_tensors_are_refused():
     x, rng = torch.zeros(4, 16), torch.zeros(2, dtype=torch.int64)
     for call in (lambda: K.layer_norm_bwd(x, x, None), lambda: K.dropout(x, 0.5, rng),
                  lambda: K.dropout_add_ln(x, x, None, None, 1e-5, 0.0, None),
-                 lambda: K.dropout_add_ln_bwd(x, x, x, None, 1e-5, 0.0, None)):
-        with pytest.raises(ValueError):
-            call()
+                 lambda: K.dropout_add_ln_bwd(x, x, x, None, 1e-5, 0.0, None),
+                 lambda: A.layer_norm(x), lambda: A.dropout(x, 0.5, rng), lambda: A.dropout_add_ln(x, x)):
+        refused(ValueError, "ROCm device tensors", call)
 
 
-def test_converted_parameters_outlive_the_launch(host, monkeypatch):
-    """A weight that is not fp32 is converted for the call; its copy has to live until the launch is made."""
-    import weakref
+def test_a_missing_binding_is_an_error(monkeypatch):
+    import sys
 
-    copies, alive = [], []
+    import boltz_mlx_amd
 
-    def f32c(t):
-        c = t.float()
-        copies.append(weakref.ref(c))
-        return c
-
-    monkeypatch.setattr(K, "f32c", f32c)
-    monkeypatch.setattr(K, "call", lambda *a: alive.append([c() is not None for c in copies]))
-    x, w = torch.zeros(3, 16), torch.ones(16, dtype=torch.float16)
-    for call, n in ((lambda: K.layer_norm_bwd(x, x, w), 1), (lambda: K.dropout_add_ln(x, x, w, w, 1e-5, 0.0, None), 2),
-                    (lambda: K.dropout_add_ln_bwd(x, x, x, w, 1e-5, 0.0, None), 1)):
-        copies.clear(), alive.clear()
-        call()
-        assert alive == [[True] * n]
+    monkeypatch.setattr(_lib, "_train", None)
+    monkeypatch.setitem(sys.modules, "boltz_mlx_amd._train", None)
+    monkeypatch.delattr(boltz_mlx_amd, "_train", raising=False)
+    refused(_lib.BzpfError, "build it with", lambda: K.dropout(torch.zeros(3), 0.0, None))
 
 
 def test_modules():
