@@ -28,14 +28,16 @@ struct RowGrad {
 };
 
 // Workgroups of the backward pass: enough for four rows in each of their row places, but not fewer than one for each
-// compute unit while rows last, nor more than two (one past D = 2048): each writes its partial sums, which the second
-// kernel reads. Measured with 256 / 512 / 768 workgroups in bf16 (fp32): 1 M rows of 128 195 / 140 / 133 us (270 / 288 /
-// 287), 16000 of 1024 26 / 26 / 26 (41 / 41 / 43), 6000 of 2048 33 / 27 / 24 (33 / 33 / 34); 4096 of 4096 with 256 / 512
-// 30 / 30 (44 / 47), 2048 of 8192 31 / 43 (47 / 56).
+// compute unit while rows last (two up to D = 128, whose partial sums are small), nor more than two (one past D = 2048):
+// each writes its partial sums, which the second kernel reads. Measured with 256 / 512 / 768 workgroups in bf16 (fp32):
+// 1 M rows of 128 195 / 140 / 133 us (270 / 288 / 287), 16000 of 1024 26 / 26 / 26 (41 / 41 / 43), 6000 of 2048
+// 33 / 27 / 24 (33 / 33 / 34); 4096 of 4096 with 256 / 512 30 / 30 (44 / 47), 2048 of 8192 31 / 43 (47 / 56). At the lower
+// end, 256 / 512: 20667 rows of 80 9.8 / 9.4 (with a residual update 13.7 / 12.8), 2000 of 768 9.6 / 10.0 (12.5 / 15.8).
 static inline int64_t row_grad_blocks(int64_t rows, int D) {
   const int per = row_places(D);
-  const int64_t all = row_blocks(rows, per, 256), four = row_blocks(rows, 4 * per, D <= 2048 ? 512 : 256);
-  return all > four ? all : four;
+  const int64_t least = row_blocks(rows, per, D <= 128 ? 512 : 256);
+  const int64_t four = row_blocks(rows, 4 * per, D <= 2048 ? 512 : 256);
+  return least > four ? least : four;
 }
 
 // The sum of v over the 64 / L lanes of a wave that hold the same columns of different rows.
