@@ -2,7 +2,8 @@
 
 Every wrapper checks devices, dtypes, shapes and contiguity on the host, then calls the C entry point on torch's
 current HIP stream with raw device pointers. Outputs and intermediates are allocated here with torch (the C side
-never allocates). There is no CPU path: a CPU tensor or a missing library raises.
+never allocates). LayerNorm and the training operators (dropout, the residual update, the backward passes) do the same
+in the native torch binding. There is no CPU path: a CPU tensor or a missing library raises.
 
 Precision (mirrors the reference's BOLTZ_MLX_PRECISION, boltz_mlx/kernels.py:1212-1220): "fp32" keeps every
 operand in fp32 (the parity build); "f16" stores GEMM operands, LayerNorm outputs and intermediates in fp16 with

@@ -7,7 +7,8 @@
  * synchronises: the caller owns every buffer (inputs, outputs and intermediates) and the stream order.
  *
  * Storage types: BZPF_F32 (fp32) or BZPF_F16 (fp16 operands, fp32 accumulation / statistics / softmax); LayerNorm and
- * the training entry points take BZPF_BF16 too, but not fp16 and bf16 in one call. The pair
+ * the training entry points take BZPF_BF16 too, but not fp16 and bf16 in one call, and pointers aligned to their
+ * elements. The pair
  * representation z is always fp32 [N, N, 128] row-major. Pointers are 16-byte aligned; D = c_z = 128 for the
  * pair kernels.
  *
@@ -65,7 +66,8 @@ int bzpf_layernorm_bwd(const void* dy, int dy_dt, const void* x, int x_dt, const
  * so that distinct (seed, offset, site) draw apart. The word of element (r, c):
  *   shared = 0: word c % 4 of block n = r ceil(D / 4) + c / 4, a draw for each element;
  *   shared = 1: one draw for each row i of the [.., I, J, D] tensor (all j and c share it): g = r / J;
- *   shared = 2: one for each column j: g = r / (I J) * J + r % J; in both word g % 4 of block n = g / 4.
+ *   shared = 2: one for each column j: g = r / (I J) * J + r % J; in both word g % 4 of block n = g / 4, and fewer than
+ *   2^32 rows, a multiple of I J.
  * (The reference runs inference only; the two shared forms are the trunk's row- and
  * column-wise dropout.) */
 int bzpf_dropout(const void* x, int x_dt, double p, const int64_t* rng, int site, int shared, int64_t I, int64_t J,

@@ -466,6 +466,62 @@ def test_half_parameters():
     assert torch.equal(K().layer_norm_bwd(g, x, strided)[0], K().layer_norm_bwd(g, x, wf)[0])
 
 
+def test_autograd_layouts_and_repeats():
+    """Transposed inputs, expanded gradients, a single row, one graph walked twice, and a saved tensor changed in place."""
+    from boltz_mlx_amd import autograd as A
+
+    w, b = (t.requires_grad_() for t in params(1, 48))
+    base = rand(2, 48, 20).requires_grad_()
+    y = A.layer_norm(base.t(), w, b)
+    dx, dw, db = torch.autograd.grad(y.sum(), (base, w, b), retain_graph=True)
+    check_grads(dx.t(), dw, db, torch.ones(20, 48), base.t(), w)
+    again = torch.autograd.grad(y.sum(), (base, w, b))
+    assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), again))
+    with pytest.raises(RuntimeError):  # the graph is gone
+        torch.autograd.grad(y.sum(), base)
+    row = rand(3, 48).requires_grad_()
+    y = A.layer_norm(row, w, b)
+    assert y.shape == (48,)
+    (dr,) = torch.autograd.grad(y, row, base[:, 0].detach())
+    check_grads(dr[None], None, None, base[:, 0][None], row[None], w)
+    z = rand(4, 6, 48).requires_grad_()
+    zn, xn = A.dropout_add_ln(z, rand(5, 6, 48), w, b)
+    zn.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        xn.sum().backward()
+    x = rand(6, 30, 48).t().contiguous().t().requires_grad_()
+    rng = K().dropout_rng(4)
+    (g,) = torch.autograd.grad(A.dropout(x, 0.5, rng).sum(), x)
+    d = dropped_of(x, 0.5, rng)
+    assert np.array_equal(np64(g), np.where(d, 0.0, 2.0))
+
+
+def test_threads():
+    """Calls from several host threads at once, each on a stream of its own."""
+    import threading
+
+    xs = [acts(20 + k, 3000, 128, F32) for k in range(3)]
+    dy, w, rng = rand(1, 3000, 128), 1 + rand(2, 128, scale=0.1), K().dropout_rng(3)
+    ref = [K().layer_norm_bwd(dy, x, w) + (K().dropout(x, 0.3, rng, k),) for k, x in enumerate(xs)]
+    torch.cuda.synchronize()
+    got = [None] * 3
+
+    def work(k):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got[k] = K().layer_norm_bwd(dy, xs[k], w) + (K().dropout(xs[k], 0.3, rng, k),)
+        s.synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for g, r in zip(got, ref):
+        assert all(torch.equal(a, c) for a, c in zip(g, r))
+
+
 def test_gradients_of_gradients_are_refused():
     from boltz_mlx_amd import autograd as A
 
