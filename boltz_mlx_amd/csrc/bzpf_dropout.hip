@@ -77,13 +77,13 @@ hipError_t launch_dropout(const void* x, int x_dt, const Drop& drop, void* y, in
 // The update and the LayerNorm of it in one pass: z and y are read once, z_new and ln written once, the statistics are of
 // the values that z_new gets. 1 M rows of 128, fp16 y and ln: 246 us (6.2 TB/s); 160,000: 36 us; 20,667 of 77, fp32 y and
 // bf16 ln, a draw for each element: 8.1 us (2.8 TB/s).
-template <typename TY, typename TO, int L, int E>
+template <typename TY, typename TO, int L, int E, bool LINES>
 __global__ __launch_bounds__(row_threads(L)) void dropout_add_ln_k(
     const float* __restrict__ z, const TY* __restrict__ y, Drop drop, const float* __restrict__ w,
     const float* __restrict__ b, float eps, float* __restrict__ z_new, TO* __restrict__ ln, int64_t rows, int D) {
   __shared__ float red[2 * row_red(L)];
   constexpr int R = row_threads(L) / L, VE = 4, NV = E / VE;
-  const RowSpan<L, NV, VE> sp(threadIdx.x % L, D);
+  const RowSpan<L, NV, VE, LINES> sp(threadIdx.x % L, D);
   const int64_t per = (D + 3) / 4;
   Key key{};
   if (drop.mode != DROP_OFF) key = drop_key(drop);
@@ -113,12 +113,12 @@ hipError_t launch_dropout_add_ln(const float* z, const void* y, int y_dt, const 
                                  const float* b, float eps, float* z_new, void* ln, int ln_dt, int64_t rows, int D,
                                  hipStream_t st) {
   return with_types(y_dt, ln_dt, [&](auto ty, auto to) {
-    return with_row_layout(D, [&](auto lay) {
+    return with_row_layout<true>(D, [&](auto lay) {
       typedef decltype(lay) Lay;
       typedef std::remove_cv_t<std::remove_pointer_t<decltype(ty)>> TY;
       typedef std::remove_cv_t<std::remove_pointer_t<decltype(to)>> TO;
       constexpr int T = row_threads(Lay::L);
-      dropout_add_ln_k<TY, TO, Lay::L, Lay::E><<<row_blocks(rows, T / Lay::L, 1 << 20), T, 0, st>>>(
+      dropout_add_ln_k<TY, TO, Lay::L, Lay::E, Lay::LINES><<<row_blocks(rows, T / Lay::L, 1 << 20), T, 0, st>>>(
           z, static_cast<const TY*>(y), drop, w, b, eps, z_new, static_cast<TO*>(ln), rows, D);
       return hipGetLastError();
     });

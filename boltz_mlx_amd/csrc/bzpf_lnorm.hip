@@ -12,13 +12,13 @@ namespace bzpf {
 // Bound by memory: one read of x, one write of y, a row a group of L lanes; enough workgroups in flight hide the two sums
 // of a row. 1 M rows of 128, fp32 to bf16: 124 us (6.2 TB/s); 4099 of 1021 fp32: 6.3 us (5.3 TB/s); 2050 of 8192 bf16:
 // 13.3 us (5.1 TB/s).
-template <typename TX, typename TY, int L, int E>
+template <typename TX, typename TY, int L, int E, bool LINES>
 __global__ __launch_bounds__(row_threads(L)) void ln_rows_k(const TX* __restrict__ x, const float* __restrict__ w,
                                                             const float* __restrict__ b, float eps,
                                                             TY* __restrict__ y, int64_t rows, int D) {
   __shared__ float red[2 * row_red(L)];
   constexpr int R = row_threads(L) / L, VE = chunk_of<TX, TY>(), NV = E / VE;
-  const RowSpan<L, NV, VE> sp(threadIdx.x % L, D);
+  const RowSpan<L, NV, VE, LINES> sp(threadIdx.x % L, D);
   fv<VE> pw[NV], pb[NV];
   row_param(pw, sp, w, 1.f);
   row_param(pb, sp, b, 0.f);
@@ -35,12 +35,12 @@ __global__ __launch_bounds__(row_threads(L)) void ln_rows_k(const TX* __restrict
 hipError_t launch_layernorm_rows(const void* x, int x_dt, const float* w, const float* b, float eps, void* y, int y_dt,
                                  int64_t rows, int D, hipStream_t st) {
   return with_types(x_dt, y_dt, [&](auto tx, auto ty) {
-    return with_row_layout(D, [&](auto lay) {
+    return with_row_layout<false>(D, [&](auto lay) {
       typedef decltype(lay) Lay;
       typedef std::remove_cv_t<std::remove_pointer_t<decltype(tx)>> TX;
       typedef std::remove_cv_t<std::remove_pointer_t<decltype(ty)>> TY;
       constexpr int T = row_threads(Lay::L);
-      ln_rows_k<TX, TY, Lay::L, Lay::E><<<row_blocks(rows, T / Lay::L, 1 << 20), T, 0, st>>>(
+      ln_rows_k<TX, TY, Lay::L, Lay::E, Lay::LINES><<<row_blocks(rows, T / Lay::L, 1 << 20), T, 0, st>>>(
           static_cast<const TX*>(x), w, b, eps, static_cast<TY*>(y), rows, D);
       return hipGetLastError();
     });
@@ -89,7 +89,7 @@ hipError_t launch_row_grad_sum(const float* ws, int64_t blocks, int D, float* dw
 }
 
 int64_t row_grad_ws_bytes(int64_t rows, int D) {
-  const int64_t blocks = row_grad_blocks(rows, D);
+  const int64_t a = row_grad_blocks<false>(rows, D), b = row_grad_blocks<true>(rows, D), blocks = a > b ? a : b;
   return blocks > 1 ? blocks * 2 * D * (int64_t)sizeof(float) : 0;
 }
 

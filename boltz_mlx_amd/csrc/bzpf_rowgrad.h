@@ -33,8 +33,9 @@ struct RowGrad {
 // 1 M rows of 128 195 / 140 / 133 us (270 / 288 / 287), 16000 of 1024 26 / 26 / 26 (41 / 41 / 43), 6000 of 2048
 // 33 / 27 / 24 (33 / 33 / 34); 4096 of 4096 with 256 / 512 30 / 30 (44 / 47), 2048 of 8192 31 / 43 (47 / 56). At the lower
 // end, 256 / 512: 20667 rows of 80 9.8 / 9.4 (with a residual update 13.7 / 12.8), 2000 of 768 9.6 / 10.0 (12.5 / 15.8).
+template <bool RES>
 static inline int64_t row_grad_blocks(int64_t rows, int D) {
-  const int per = row_places(D);
+  const int per = row_places<RES>(D);
   const int64_t least = row_blocks(rows, per, D <= 128 ? 512 : 256);
   const int64_t four = row_blocks(rows, 4 * per, D <= 2048 ? 512 : 256);
   return least > four ? least : four;
@@ -59,26 +60,22 @@ __device__ __forceinline__ float column_sum(float v) {
   return v;
 }
 
-// sp.store of an fp32 chunk (two accesses where it has eight channels).
-template <int L, int NV>
-__device__ __forceinline__ void store_param(const RowSpan<L, NV, 4>& sp, int k, float* row, fv<4> v) {
-  sp.store(k, row, v);
-}
-template <int L, int NV>
-__device__ __forceinline__ void store_param(const RowSpan<L, NV, 8>& sp, int k, float* row, fv<8> v) {
+// The sums of a lane's own columns in chunk k, in fp32 (their chunk takes two accesses where it has eight channels).
+template <int L, int NV, int VE, bool LINES>
+__device__ __forceinline__ void store_param(const RowSpan<L, NV, VE, LINES>& sp, int k, float* row, fv<VE> v) {
   if (sp.whole(k) || sp.skip[k] == 0) {
-    store_chunk<4>(row + sp.at[k], fv<4>{v[0], v[1], v[2], v[3]});
-    store_chunk<4>(row + sp.at[k] + 4, fv<4>{v[4], v[5], v[6], v[7]});
+#pragma unroll
+    for (int j = 0; j < VE; j += 4) store_chunk<4>(row + sp.at[k] + j, fv<4>{v[j], v[j + 1], v[j + 2], v[j + 3]});
   } else {
 #pragma unroll
-    for (int e = 1; e < 8; e++)
+    for (int e = 1; e < VE; e++)
       if (e >= sp.skip[k]) row[sp.at[k] + e] = v[e];
   }
 }
 
 // The workgroup's sums over its rows of s (chunks as in sp) into out [D].
-template <int L, int NV, int VE>
-__device__ __forceinline__ void meet_columns(fv<VE> (&s)[NV], const RowSpan<L, NV, VE>& sp, int D, float* meet,
+template <int L, int NV, int VE, bool LINES>
+__device__ __forceinline__ void meet_columns(fv<VE> (&s)[NV], const RowSpan<L, NV, VE, LINES>& sp, int D, float* meet,
                                              float* out) {
   if constexpr (L > 64) {
 #pragma unroll
@@ -102,13 +99,13 @@ __device__ __forceinline__ void meet_columns(fv<VE> (&s)[NV], const RowSpan<L, N
 // the sums shows: 2000 of 768 bf16 6.2 us.
 // Four waves a SIMD (128 registers) with 8 channels a lane, two with 16: what the sums, the row and the next row's loads
 // need without spilling.
-template <bool RES, typename TX, typename TG, typename TY, int L, int E>
+template <bool RES, typename TX, typename TG, typename TY, int L, int E, bool LINES>
 __global__ __launch_bounds__(row_threads(L), E == 8 ? 4 : 2) void row_grad_k(RowGrad<TX, TG, TY> a) {
   constexpr int R = row_threads(L) / L, VE = RES ? 4 : chunk_of<TX, TG>(), NV = E / VE;
   __shared__ float red[4 * row_red(L)];
   __shared__ float meet[L <= 64 ? 4 * L * E : 1];
   const int D = a.D;
-  const RowSpan<L, NV, VE> sp(threadIdx.x % L, D);
+  const RowSpan<L, NV, VE, LINES> sp(threadIdx.x % L, D);
   const int64_t per = (D + 3) / 4;
   const float inv = 1.0f / D;
   Key key{};
@@ -185,10 +182,10 @@ __global__ __launch_bounds__(row_threads(L), E == 8 ? 4 : 2) void row_grad_k(Row
 
 template <bool RES, typename TX, typename TG, typename TY>
 static hipError_t launch_row_grad(const RowGrad<TX, TG, TY>& a, hipStream_t st) {
-  const unsigned blocks = (unsigned)row_grad_blocks(a.rows, a.D);
-  const hipError_t e = with_row_layout(a.D, [&](auto lay) {
+  const unsigned blocks = (unsigned)row_grad_blocks<RES>(a.rows, a.D);
+  const hipError_t e = with_row_layout<RES>(a.D, [&](auto lay) {
     typedef decltype(lay) Lay;
-    row_grad_k<RES, TX, TG, TY, Lay::L, Lay::E><<<blocks, row_threads(Lay::L), 0, st>>>(a);
+    row_grad_k<RES, TX, TG, TY, Lay::L, Lay::E, Lay::LINES><<<blocks, row_threads(Lay::L), 0, st>>>(a);
     return hipGetLastError();
   });
   if (e != hipSuccess || blocks == 1 || (!a.dw && !a.db)) return e;

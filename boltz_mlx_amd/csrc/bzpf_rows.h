@@ -40,12 +40,14 @@ __device__ __forceinline__ fv<VE> load_chunk(const T* p) {
 }
 // Outputs go out as non-temporal stores of whole lines: nothing of them waits in L2 for the write-back at the kernel's end.
 // Residual update of 20 M elements 42 us instead of 45 (5 M: 11.7, 14.2), LayerNorm backward 39 instead of 42 (13.6, 15.6),
-// dropout in fp16 22 instead of 24; at 128 M elements the gain is 2 to 4%.
-template <int VE, typename T>
+// dropout in fp16 22 instead of 24; at 128 M elements the gain is 2 to 4%. NT = false: ordinary stores (RowSpan::store).
+template <int VE, bool NT = true, typename T>
 __device__ __forceinline__ void store_chunk(T* p, fv<VE> v) {
   typedef typename Raw<T, VE>::V V;
   typedef typename Raw<T, VE>::U U;
-  __builtin_nontemporal_store(static_cast<U>(__builtin_convertvector(v, V)), reinterpret_cast<U*>(p));
+  const U u = __builtin_convertvector(v, V);
+  if constexpr (NT) __builtin_nontemporal_store(u, reinterpret_cast<U*>(p));
+  else *reinterpret_cast<U*>(p) = u;
 }
 
 __device__ __forceinline__ float sum_of(fv<4> v) { return (v[0] + v[1]) + (v[2] + v[3]); }
@@ -55,12 +57,12 @@ __device__ __forceinline__ float sum_of(fv<8> v) {
 
 // Where a lane's chunks lie: chunk k covers the columns at[k] .. at[k] + VE - 1. A chunk that would pass the row's end is
 // moved back to D - VE, and its first skip[k] elements belong to its neighbour (VE or more: the chunk lies wholly past
-// the end). Loads then need no branch; sums and stores leave the skipped elements out. The first half of a lane's chunks
-// is never moved (a layout serves widths past half of its own), none is where D fills the layout.
-template <int L, int NV, int VE>
+// the end). Loads then need no branch; sums leave the skipped elements out. The first half of a lane's chunks is never
+// moved (a layout serves widths past half of its own), none is where D fills the layout.
+template <int L, int NV, int VE, bool LINES>
 struct RowSpan {
   int at[NV], skip[NV];
-  bool full;
+  bool full, first;
   __device__ __forceinline__ RowSpan(int q, int D) {
 #pragma unroll
     for (int k = 0; k < NV; k++) {
@@ -69,6 +71,7 @@ struct RowSpan {
       skip[k] = c - at[k];
     }
     full = D == L * NV * VE;
+    first = q == 0;
   }
   static constexpr bool whole(int k) { return k < NV / 2; }
   // the sum of chunk k's own elements
@@ -79,10 +82,17 @@ struct RowSpan {
     }
     return sum_of(v);
   }
+  // Chunk k of a row to memory. A chunk that was moved back writes its skipped elements too: the neighbour, who forms them in
+  // the same chunk by the same instructions from the same values, writes the same bits (bf16 LayerNorm of 64 M elements at
+  // D = 77 2.6 -> 3.3 TB/s, 100 3.5 -> 4.9); a row's first lane has its neighbour's in another chunk and writes its own one
+  // by one.
+  // Not LINES: several rows lie in a wave and end inside a 64-byte line in fp32, which ordinary stores leave to L2 to join:
+  // residual update of 64 M elements at D = 77 3.5 -> 4.6 TB/s, 100 4.4 -> 5.2, 150 4.1 -> 5.0; from D = 257 on they lose
+  // (300: 5.1 -> 4.9), and so do chunks of 8 half channels (LayerNorm of 16 M, D = 77: 3.1, 2.4).
   template <typename T>
   __device__ __forceinline__ void store(int k, T* row, fv<VE> v) const {
-    if (whole(k) || skip[k] == 0) {
-      store_chunk<VE>(row + at[k], v);
+    if (whole(k) || skip[k] == 0 || (skip[k] < VE && !first)) {
+      store_chunk<VE, LINES || VE == 8>(row + at[k], v);
     } else if (skip[k] < VE) {
 #pragma unroll
       for (int e = 1; e < VE; e++)
@@ -135,8 +145,8 @@ constexpr int row_red(int L) { return L > 64 ? L / 64 : 1; }  // floats that one
 
 // A LayerNorm parameter at a lane's columns, or `none` where there is none: loaded before the rows, so that no load stands
 // between a row's sums and its use (the wait for it would also wait for the next row's loads, which were issued before).
-template <int L, int NV, int VE>
-__device__ __forceinline__ void row_param(fv<VE> (&v)[NV], const RowSpan<L, NV, VE>& sp, const float* p, float none) {
+template <int L, int NV, int VE, bool LINES>
+__device__ __forceinline__ void row_param(fv<VE> (&v)[NV], const RowSpan<L, NV, VE, LINES>& sp, const float* p, float none) {
 #pragma unroll
   for (int k = 0; k < NV; k++) {
     if (p) {
@@ -153,8 +163,8 @@ __device__ __forceinline__ void row_param(fv<VE> (&v)[NV], const RowSpan<L, NV, 
 
 // Centres the row in v and returns 1 / sqrt(var + eps), by two passes over the registers (mean, then the squared
 // deviations): both sums in fp32. Skipped elements are centred too and left out of the sums.
-template <int L, int NV, int VE>
-__device__ __forceinline__ float centre_row(fv<VE> (&v)[NV], const RowSpan<L, NV, VE>& sp, int D, float eps,
+template <int L, int NV, int VE, bool LINES>
+__device__ __forceinline__ float centre_row(fv<VE> (&v)[NV], const RowSpan<L, NV, VE, LINES>& sp, int D, float eps,
                                             float* red) {
   float s = 0.f;
 #pragma unroll
@@ -172,18 +182,28 @@ __device__ __forceinline__ float centre_row(fv<VE> (&v)[NV], const RowSpan<L, NV
   return __builtin_amdgcn_rsqf(tiny ? var * 0x1p100f : var) * (tiny ? 0x1p50f : 1.f);
 }
 
-// L lanes a row, E channels a lane (E / VE chunks).
-template <int L_, int E_>
+// L lanes a row, E channels a lane (E / VE chunks), LINES as in RowSpan::store.
+template <int L_, int E_, bool LINES_ = true>
 struct RowLayout {
   static constexpr int L = L_, E = E_;
+  static constexpr bool LINES = LINES_;
 };
 
-// Calls fn with the row layout of width D. One wave or less a row while 16 channels a lane hold it (no barrier then), whole
-// workgroups beyond. Measured on the backward pass of 16 M elements in bf16 (fp32): D = 1024 as 64 x 16 26 us (43), as
-// 256 x 8 39 (45); D = 2048 as 256 x 8 33 (42), as 64 x 32 (over 256 registers) 43 (57); D = 4096 as 256 x 16 30 (43), as
-// 512 x 8 32 (43); D = 8192 as 512 x 16 31 (48), as 1024 x 8 34 (51).
-template <typename Fn>
+// Calls fn with the row layout of width D. One wave or less a row while its registers hold it (no barrier then): 16 channels
+// a lane, 24 without a residual update, whose backward pass spills there (1030 channels of 64 M elements: LayerNorm backward
+// in bf16 2.0 -> 4.6 TB/s, with an update 3.6 -> 2.5). Whole workgroups beyond. Measured on the backward pass of 16 M
+// elements in bf16 (fp32): D = 1024 as 64 x 16 26 us (43), as 256 x 8 39 (45); D = 2048 as 256 x 8 33 (42), as 64 x 32 (over
+// 256 registers) 43 (57); D = 4096 as 256 x 16 30 (43), as 512 x 8 32 (43); D = 8192 as 512 x 16 31 (48), as 1024 x 8
+// 34 (51).
+template <bool RES, typename Fn>
 static inline auto with_row_layout(int D, Fn&& fn) {
+  if (D <= 256 && D % 16) {
+    if (D <= 16) return fn(RowLayout<2, 8, false>());
+    if (D <= 32) return fn(RowLayout<4, 8, false>());
+    if (D <= 64) return fn(RowLayout<8, 8, false>());
+    if (D <= 128) return fn(RowLayout<16, 8, false>());
+    return fn(RowLayout<32, 8, false>());
+  }
   if (D <= 16) return fn(RowLayout<2, 8>());
   if (D <= 32) return fn(RowLayout<4, 8>());
   if (D <= 64) return fn(RowLayout<8, 8>());
@@ -191,14 +211,18 @@ static inline auto with_row_layout(int D, Fn&& fn) {
   if (D <= 256) return fn(RowLayout<32, 8>());
   if (D <= 512) return fn(RowLayout<64, 8>());
   if (D <= 1024) return fn(RowLayout<64, 16>());
+  if constexpr (!RES) {
+    if (D <= 1536) return fn(RowLayout<64, 24>());
+  }
   if (D <= 2048) return fn(RowLayout<256, 8>());
   if (D <= 4096) return fn(RowLayout<256, 16>());
   return fn(RowLayout<512, 16>());
 }
 
 // Rows that a workgroup holds at once at width D.
+template <bool RES>
 static inline int row_places(int D) {
-  return with_row_layout(D, [](auto lay) { return row_threads(decltype(lay)::L) / decltype(lay)::L; });
+  return with_row_layout<RES>(D, [](auto lay) { return row_threads(decltype(lay)::L) / decltype(lay)::L; });
 }
 
 // Calls fn(a, b) with a null pointer of each of the two storage types: fp32, fp16, bf16, but not fp16 with bf16.
