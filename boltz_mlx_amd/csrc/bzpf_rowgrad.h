@@ -97,7 +97,7 @@ __device__ __forceinline__ void meet_columns(fv<VE> (&s)[NV], const RowSpan<L, N
 // Bound by memory where rows are many: 1 M rows of 128 fp32 with an fp16 gradient 213 us (6.0 TB/s), the residual update's
 // 357 us (5.7 TB/s), 2050 of 8192 bf16 20.5 us (5.7 TB/s with the partial sums). Where each lane has few rows the chain of
 // the sums shows: 2000 of 768 bf16 6.2 us.
-// Four waves a SIMD (128 registers) with 8 channels a lane, two with 16: what the sums, the row and the next row's loads
+// Four waves a SIMD (128 registers) with 8 channels a lane, two with 16 or 24: what the sums, the row and the next row's loads
 // need without spilling.
 template <bool RES, typename TX, typename TG, typename TY, int L, int E, bool LINES>
 __global__ __launch_bounds__(row_threads(L), E == 8 ? 4 : 2) void row_grad_k(RowGrad<TX, TG, TY> a) {
