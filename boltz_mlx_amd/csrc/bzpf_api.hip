@@ -33,6 +33,15 @@ bool dt_ok(int dt) { return dt == BZPF_F32 || dt == BZPF_F16; }
 bool dt3_ok(int dt) { return dt_ok(dt) || dt == BZPF_BF16; }
 bool pair_ok(int a, int b) { return dt3_ok(a) && dt3_ok(b) && (a == b || a == BZPF_F32 || b == BZPF_F32); }
 bool aligned_el(const void* p, int dt) { return (reinterpret_cast<uintptr_t>(p) & (dt == BZPF_F32 ? 3u : 1u)) == 0; }
+// Whether the n elements of an output share no byte with n of another tensor (null: none). `itself`: the output may be that
+// tensor, in its type, where the kernel has a whole row in registers before it writes it.
+bool apart(const void* out, int out_dt, const void* t, int t_dt, int64_t n, bool itself = false) {
+  const auto end = [n](const void* p, int dt) {
+    return reinterpret_cast<uintptr_t>(p) + (unsigned __int128)n * (dt == BZPF_F32 ? 4 : 2);
+  };
+  return t == nullptr || (itself && out == t && out_dt == t_dt) || end(out, out_dt) <= reinterpret_cast<uintptr_t>(t) ||
+         end(t, t_dt) <= reinterpret_cast<uintptr_t>(out);
+}
 bool width_ok(int64_t D) { return D >= bzpf::ROW_MIN_D && D <= bzpf::ROW_MAX_D; }
 hipStream_t S(void* s) { return static_cast<hipStream_t>(s); }
 
@@ -83,6 +92,8 @@ int bzpf_layernorm_bwd(const void* dy, int dy_dt, const void* x, int x_dt, const
   REQUIRE_EL(dx, x_dt);
   REQUIRE(aligned_el(w, BZPF_F32) && aligned_el(dw, BZPF_F32) && aligned_el(db, BZPF_F32) && aligned_el(ws, BZPF_F32),
           "bzpf_layernorm_bwd: w, dw, db or ws misaligned");
+  REQUIRE(apart(dx, x_dt, x, x_dt, rows * D, true) && apart(dx, x_dt, dy, dy_dt, rows * D, true),
+          "bzpf_layernorm_bwd: dx overlaps x or dy");
   const int64_t need = dw || db ? bzpf::row_grad_ws_bytes(rows, D) : 0;
   REQUIRE(need == 0 || (ws && ws_bytes >= need), "bzpf_layernorm_bwd: ws holds %lld bytes of %lld",
           (long long)(ws ? ws_bytes : 0), (long long)need);
@@ -126,6 +137,8 @@ int bzpf_dropout(const void* x, int x_dt, double p, const int64_t* rng, int site
   if (!make_drop("bzpf_dropout", p, rng, site, shared, rows, I, J, D, &d)) return BZPF_EINVAL;
   REQUIRE_EL(x, x_dt);
   REQUIRE_EL(y, y_dt);
+  // a row's last chunk reads columns that its neighbour writes too
+  REQUIRE(apart(y, y_dt, x, x_dt, rows * D), "bzpf_dropout: y overlaps x");
   return done(bzpf::launch_dropout(x, x_dt, d, y, y_dt, rows, D, S(stream)), "bzpf_dropout");
 }
 
@@ -143,6 +156,10 @@ int bzpf_dropout_add_ln(const float* z, const void* y, int y_dt, double p, const
   REQUIRE_EL(z_new, BZPF_F32);
   REQUIRE_EL(ln, ln_dt);
   REQUIRE(aligned_el(w, BZPF_F32) && aligned_el(b, BZPF_F32), "bzpf_dropout_add_ln: w or b misaligned");
+  const int64_t n = rows * D;
+  REQUIRE(apart(z_new, BZPF_F32, z, BZPF_F32, n) && apart(z_new, BZPF_F32, y, y_dt, n) &&
+              apart(z_new, BZPF_F32, ln, ln_dt, n) && apart(ln, ln_dt, z, BZPF_F32, n) && apart(ln, ln_dt, y, y_dt, n),
+          "bzpf_dropout_add_ln: z_new or ln overlaps another tensor");
   return done(bzpf::launch_dropout_add_ln(z, y, y_dt, d, w, b, eps, z_new, ln, ln_dt, rows, D, S(stream)),
               "bzpf_dropout_add_ln");
 }
@@ -163,6 +180,13 @@ int bzpf_dropout_add_ln_bwd(const float* dz_new, const void* dln, int ln_dt, con
   REQUIRE_EL(dy, y_dt);
   REQUIRE(aligned_el(w, BZPF_F32) && aligned_el(dw, BZPF_F32) && aligned_el(db, BZPF_F32) && aligned_el(ws, BZPF_F32),
           "bzpf_dropout_add_ln_bwd: w, dw, db or ws misaligned");
+  const int64_t n = rows * D;
+  const auto clear = [&](void* out, int dt) {
+    return apart(out, dt, dz_new, BZPF_F32, n, true) && apart(out, dt, dln, ln_dt, n, true) &&
+           apart(out, dt, z_new, BZPF_F32, n, true);
+  };
+  REQUIRE(clear(dz, BZPF_F32) && clear(dy, y_dt) && apart(dz, BZPF_F32, dy, y_dt, n),
+          "bzpf_dropout_add_ln_bwd: dz or dy overlaps another tensor");
   const int64_t need = dw || db ? bzpf::row_grad_ws_bytes(rows, D) : 0;
   REQUIRE(need == 0 || (ws && ws_bytes >= need), "bzpf_dropout_add_ln_bwd: ws holds %lld bytes of %lld",
           (long long)(ws ? ws_bytes : 0), (long long)need);

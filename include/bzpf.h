@@ -52,13 +52,14 @@ int bzpf_layernorm(const void* x, int x_dt, const float* w, const float* b, floa
  *   dx = rstd (g - mean(g) - xh mean(g xh)), g = dy w (x's type); dw = sum over rows of dy xh; db = sum over rows of dy.
  * dw / db (fp32 [D]) may each be NULL. ws: bzpf_layernorm_bwd_ws(rows, D) bytes for the workgroups' partial sums (0: none
  * needed; -1: a width or row count that is refused), of which ws_bytes are there; it may be NULL when dw and db are.
- * Sums in fp32 in a fixed order: equal inputs give equal bits. */
+ * dx may be x or dy itself, in its type, and overlaps neither otherwise. Sums in fp32 in a fixed order: equal inputs give
+ * equal bits. */
 int64_t bzpf_layernorm_bwd_ws(int64_t rows, int D);
 int bzpf_layernorm_bwd(const void* dy, int dy_dt, const void* x, int x_dt, const float* w, float eps, void* dx,
                        float* dw, float* db, float* ws, int64_t ws_bytes, int64_t rows, int D, void* stream);
 
 /* Dropout of x [rows, D] (any D >= 1): y = u < p ? 0 : x / (1 - p), p in [0, 1] to 2^-32; a dropped element is 0 whatever
- * x holds. The backward pass is the same call on dy. No mask is stored: u is a word of Philox4x32-10 (Salmon et al.,
+ * x holds. y must not overlap x. The backward pass is the same call on dy. No mask is stored: u is a word of Philox4x32-10 (Salmon et al.,
  * "Parallel random numbers: as easy as 1, 2, 3", 2011), a function of
  *   key      rng[0] (the seed), rng: two int64 on the device, read by the kernel (may be NULL when p = 0);
  *   counter  (n bits 0-31, n bits 32-47 | site << 16, rng[1] bits 0-31, rng[1] bits 32-63), 0 <= site < 65536,
@@ -74,15 +75,16 @@ int bzpf_dropout(const void* x, int x_dt, double p, const int64_t* rng, int site
 
 /* The residual update with dropout and the LayerNorm that follows (the training form of bzpf_add_ln):
  *   z_new = z + dropout(y);  ln = LN(z_new; w, b, eps)
- * over rows of D channels (8 <= D <= 8192); z and z_new fp32 (two buffers), y and ln of their types, dropout as in
- * bzpf_dropout. */
+ * over rows of D channels (8 <= D <= 8192); z and z_new fp32, y and ln of their types, dropout as in
+ * bzpf_dropout. z_new and ln overlap neither each other nor z or y. */
 int bzpf_dropout_add_ln(const float* z, const void* y, int y_dt, double p, const int64_t* rng, int site, int shared,
                         int64_t I, int64_t J, const float* w, const float* b, float eps, float* z_new, void* ln,
                         int ln_dt, int64_t rows, int D, void* stream);
 
 /* Its backward pass over rows >= 1: from the gradients dz_new (fp32; NULL: zero) and dln of the two outputs and z_new,
  *   dz = dz_new + (the LayerNorm's gradient of dln);  dy = dropout(dz), with the forward call's draws; dw, db and ws as in
- * bzpf_layernorm_bwd (the same workspace size). */
+ * bzpf_layernorm_bwd (the same workspace size). dz and dy may each be one of the three inputs itself, in its type, and
+ * overlap neither each other nor an input otherwise. */
 int bzpf_dropout_add_ln_bwd(const float* dz_new, const void* dln, int ln_dt, const float* z_new, const float* w,
                             float eps, double p, const int64_t* rng, int site, int shared, int64_t I, int64_t J,
                             float* dz, void* dy, int y_dt, float* dw, float* db, float* ws, int64_t ws_bytes,

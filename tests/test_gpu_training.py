@@ -664,3 +664,29 @@ def test_a_block_of_updates_trains():
     assert (xn.double().cpu() - x6).abs().max() <= 1e-5 * x6.abs().max()
     for g, w in zip(got, torch.autograd.grad((r, x6), ref_leaves, (gz.double().cpu(), gl.double().cpu()))):
         assert (g.double().cpu() - w).abs().max() <= 3e-5 * w.abs().max()
+
+
+# -------------------------------------------------------------------------------------------------- in place, from C
+
+@pytest.mark.parametrize("D", [9, 77, 128, 1021, 2055, 8191])
+def test_backward_passes_in_place(D):
+    """An output of a backward pass that is one of its inputs: the bits of the call with buffers of their own."""
+    from boltz_mlx_amd import _lib
+
+    rows, st = 700, torch.cuda.current_stream().cuda_stream
+    x, dy, dz_new, w = acts(1, rows, D, F32), rand(2, rows, D), rand(3, rows, D), 1 + rand(4, D, scale=0.1)
+    n = _lib.load().bzpf_layernorm_bwd_ws(rows, D)
+    ws, dw, db = torch.empty(n // 4 + 1, device="cuda"), torch.empty(D, device="cuda"), torch.empty(D, device="cuda")
+    tail = (dw.data_ptr(), db.data_ptr(), ws.data_ptr(), n, rows, D, st)
+    for k in range(2):
+        a, g = x.clone(), dy.clone()
+        out = (a, g)[k]
+        _lib.call("bzpf_layernorm_bwd", g.data_ptr(), 0, a.data_ptr(), 0, w.data_ptr(), 1e-5, out.data_ptr(), *tail)
+        assert all(torch.equal(p, q) for p, q in zip((out, dw, db), K().layer_norm_bwd(dy, x, w)))
+    rng = K().dropout_rng(7)
+    want = K().dropout_add_ln_bwd(dz_new, dy, x, w, 1e-5, 0.3, rng, 1)
+    for i, j in ((0, 1), (1, 2), (2, 0)):
+        t = [v.clone() for v in (dz_new, dy, x)]
+        _lib.call("bzpf_dropout_add_ln_bwd", t[0].data_ptr(), t[1].data_ptr(), 0, t[2].data_ptr(), w.data_ptr(), 1e-5, 0.3,
+                  rng.data_ptr(), 1, 0, 1, 1, t[i].data_ptr(), t[j].data_ptr(), 0, *tail)
+        assert all(torch.equal(p, q) for p, q in zip((t[i], t[j], dw, db), want))

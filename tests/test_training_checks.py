@@ -180,3 +180,36 @@ def test_modules():
     assert "0.25" in repr(d) and "row" in repr(d)
     with pytest.raises(ValueError):
         Dropout(1.5)
+
+
+# -------------------------------------------------------------------------------------------------- overlapping buffers
+
+def overlapping(code):
+    assert code == -1 and b"overlap" in _lib.load().bzpf_last_error()
+
+
+Q, R, S, V = P + 768, P + 1536, P + 2304, P + 3072  # tensors of 12 x 16 fp32, one behind the other
+
+
+@pytest.mark.parametrize("y, x_dt, y_dt", [(P, F32, F32), (P, F16, F16), (P, F32, BF16), (P + 764, F32, F32),
+                                           (P - 764, F32, F32), (P + 382, F16, F16)])
+def test_dropout_refuses_overlapping_buffers(y, x_dt, y_dt):
+    """In place, a row's last chunk may read what its neighbour has already dropped and scaled (12 rows of 16)."""
+    overlapping(drop(x=P, x_dt=x_dt, y=y, y_dt=y_dt))
+
+
+@pytest.mark.parametrize("change", [{"zn": P}, {"zn": Q}, {"zn": S}, {"ln": P}, {"ln": Q}, {"ln": R + 4}, {"zn": Q - 4},
+                                    {"ln": P, "ln_dt": F16}])
+def test_dropout_add_ln_refuses_overlapping_buffers(change):
+    overlapping(res(**{**dict(z=P, y=Q, zn=R, ln=S), **change}))
+
+
+@pytest.mark.parametrize("change", [{"dx": P + 4}, {"dx": Q + 764}, {"dx": P - 4}, {"dx": P, "x_dt": F16}])
+def test_layernorm_bwd_refuses_overlapping_buffers(change):
+    overlapping(ln_bwd(**{**dict(dy=P, x=Q, dx=R, rows=12, D=16), **change}))
+
+
+@pytest.mark.parametrize("change", [{"dz": P + 4}, {"dz": Q - 4}, {"dz": V}, {"dy": R + 8}, {"dy": P, "y_dt": F16},
+                                    {"dz": R, "dy": R}])
+def test_dropout_add_ln_bwd_refuses_overlapping_buffers(change):
+    overlapping(res_bwd(**{**dict(dzn=P, dln=Q, zn=R, dz=S, dy=V), **change}))
