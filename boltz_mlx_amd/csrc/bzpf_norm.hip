@@ -27,6 +27,13 @@ template <> struct V4<half_t> {
   }
 };
 
+// Four values of a weight or bias, which may lie at any element (a slice of a larger tensor): the access is the same one
+// instruction as at a 16-byte boundary.
+__device__ __forceinline__ f4 load_param(const float* p) {
+  typedef float E __attribute__((ext_vector_type(4), aligned(4)));
+  return *reinterpret_cast<const E*>(p);
+}
+
 // Row index for the transposed-token option: a row r = i*N + j of a [N, N, D] tensor maps to j*N + i.
 __device__ __forceinline__ int64_t trow(int64_t r, int64_t N, int trans) {
   if (!trans) return r;
@@ -64,8 +71,8 @@ __global__ __launch_bounds__(256) void layernorm_kernel(const TI* __restrict__ x
   for (int i = 0; i < NV; i++) {
     const int c = 64 * i + 4 * lane;
     f4 o = (v[i] - mean) * rstd;
-    if (w) o *= *reinterpret_cast<const f4*>(w + c);
-    if (b) o += *reinterpret_cast<const f4*>(b + c);
+    if (w) o *= load_param(w + c);
+    if (b) o += load_param(b + c);
     V4<TO>::store(yr + c, o);
   }
 }
@@ -105,8 +112,8 @@ __global__ __launch_bounds__(256) void add_ln_kernel(float* __restrict__ z, cons
   for (int i = 0; i < NV; i++) {
     const int c = 64 * i + 4 * lane;
     f4 o = (v[i] - mean) * rstd;
-    if (w) o *= *reinterpret_cast<const f4*>(w + c);
-    if (b) o += *reinterpret_cast<const f4*>(b + c);
+    if (w) o *= load_param(w + c);
+    if (b) o += load_param(b + c);
     V4<TO>::store(orow + c, o);
   }
 }

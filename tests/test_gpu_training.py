@@ -666,6 +666,33 @@ def test_a_block_of_updates_trains():
         assert (g.double().cpu() - w).abs().max() <= 3e-5 * w.abs().max()
 
 
+# -------------------------------------------------------------------------------------------------- LayerNorm's two kernels
+
+@pytest.mark.parametrize("D", [64, 128, 384, 1024])
+def test_layer_norm_parameters_at_any_element(D):
+    """A weight and a bias that are slices at odd offsets, with x and y at whole boundaries: the bits of aligned ones."""
+    w, b = params(3, D)
+    for off in (1, 2, 3):
+        ws, bs = torch.zeros(D + 5, device="cuda"), torch.zeros(D + 5, device="cuda")
+        ws[off:off + D], bs[5 - off:5 - off + D] = w, b
+        wo, bo = ws[off:off + D], bs[5 - off:5 - off + D]
+        for tx, ty in ((F32, F32), (F32, F16), (F16, F16), (BF16, BF16)):
+            x = acts(D, 37, D, tx)
+            assert torch.equal(K().layer_norm(x, wo, bo, out_dtype=ty), K().layer_norm(x, w, b, out_dtype=ty))
+    z, y = rand(1, 9, 9, 128), rand(2, 9, 9, 128)
+
+    class LN:
+        eps = 1e-5
+
+    def add_ln(w, b):
+        LN.weight, LN.bias = w, b
+        return K().add_ln(z.clone(), y, LN, out_dtype=F32)
+
+    w, b = params(5, 128)
+    ws, bs = torch.cat([w[:1], w]), torch.cat([b[:3], b])
+    assert torch.equal(add_ln(ws[1:], bs[3:]), add_ln(w, b))
+
+
 # -------------------------------------------------------------------------------------------------- in place, from C
 
 @pytest.mark.parametrize("D", [9, 77, 128, 1021, 2055, 8191])
