@@ -73,7 +73,7 @@ int bzpf_layernorm(const void* x, int x_dt, const float* w, const float* b, floa
   REQUIRE(aligned_el(w, BZPF_F32) && aligned_el(b, BZPF_F32), "bzpf_layernorm: w or b misaligned");
   // the widths, types and alignments that the first kernel serves keep its sums' order, and so their bits
   const bool narrow = D % 64 == 0 && (D / 64 <= 6 || D / 64 == 8 || D / 64 == 12 || D / 64 == 16);
-  if (narrow && dt_ok(x_dt) && dt_ok(y_dt) && aligned16(x) && aligned16(y))
+  if (narrow && rows <= bzpf::LN16_MAX_ROWS && dt_ok(x_dt) && dt_ok(y_dt) && aligned16(x) && aligned16(y))
     return done(bzpf::launch_layernorm(x, x_dt, w, b, eps, y, y_dt, rows, D, S(stream)), "bzpf_layernorm");
   return done(bzpf::launch_layernorm_rows(x, x_dt, w, b, eps, y, y_dt, rows, D, S(stream)), "bzpf_layernorm");
 }

@@ -8,6 +8,9 @@ namespace bzpf {
 
 enum { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2 };
 
+// LayerNorm over the first widths and types (bzpf_norm.hip): 16 threads a row and no row loop, so that the launch's 2^32
+// threads bound its rows.
+constexpr int64_t LN16_MAX_ROWS = 16 * (((int64_t)1 << 24) - 1);
 hipError_t launch_layernorm(const void* x, int x_dt, const float* w, const float* b, float eps, void* y, int y_dt,
                             int64_t rows, int D, hipStream_t st);
 hipError_t launch_add_ln(float* z, const void* y, int y_dt, float scale, int trans_y, const float* w, const float* b,

@@ -136,6 +136,7 @@ static hipError_t ln_dispatch(const void* x, const float* w, const float* b, flo
 
 hipError_t launch_layernorm(const void* x, int x_dt, const float* w, const float* b, float eps, void* y, int y_dt,
                             int64_t rows, int D, hipStream_t st) {
+  if (rows > LN16_MAX_ROWS) return hipErrorInvalidValue;
   if (x_dt == DT_F32 && y_dt == DT_F32) return ln_dispatch<float, float>(x, w, b, eps, y, rows, D, st);
   if (x_dt == DT_F32 && y_dt == DT_F16) return ln_dispatch<float, half_t>(x, w, b, eps, y, rows, D, st);
   if (x_dt == DT_F16 && y_dt == DT_F32) return ln_dispatch<half_t, float>(x, w, b, eps, y, rows, D, st);

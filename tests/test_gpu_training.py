@@ -693,6 +693,17 @@ def test_layer_norm_parameters_at_any_element(D):
     assert torch.equal(add_ln(ws[1:], bs[3:]), add_ln(w, b))
 
 
+def test_layer_norm_past_one_launch():
+    """More rows than the kernel of the earlier widths can launch threads for (16 a row, 2^32 in all)."""
+    rows, D = 2 ** 28 + 5, 64
+    x, (w, b) = torch.zeros(rows, D, dtype=F16, device="cuda"), params(3, D)
+    x[:1000], x[-1000:] = acts(1, 1000, D, F16), acts(2, 1000, D, F16)
+    y = K().layer_norm(x, w, b, out_dtype=F16)
+    for part in (slice(0, 1000), slice(rows - 1000, rows)):
+        close(y[part], T.ln(np64(x[part]), np64(w), np64(b)), ln_tol(np64(x[part]), np64(w), np64(b)))
+    assert torch.equal(y[1000:-1000:4099], b.half().expand(y[1000:-1000:4099].shape))
+
+
 # -------------------------------------------------------------------------------------------------- in place, from C
 
 @pytest.mark.parametrize("D", [9, 77, 128, 1021, 2055, 8191])
