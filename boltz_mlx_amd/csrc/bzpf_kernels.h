@@ -23,6 +23,7 @@ hipError_t launch_layernorm_rows(const void* x, int x_dt, const float* w, const 
 int64_t row_grad_ws_bytes(int64_t rows, int D);
 hipError_t launch_layernorm_bwd(const void* dy, int dy_dt, const void* x, int x_dt, const float* w, float eps, void* dx,
                                 float* dw, float* db, float* ws, int64_t rows, int D, hipStream_t st);
+constexpr int ROW_GRAD_BLOCKS = 512;  // workgroups of a backward pass at most: what the kernel that adds their sums reads
 hipError_t launch_row_grad_sum(const float* ws, int64_t blocks, int D, float* dw, float* db, hipStream_t st);
 // How a call drops: a draw u < `last` + 1 = round(p 2^32) drops its element (p = 1 fits so; p = 0 is DROP_OFF), the rest
 // is scaled by 1 / (1 - p). rng: (seed, offset) on the device, read by the kernel, so that a replayed graph draws anew

@@ -58,7 +58,7 @@ hipError_t launch_layernorm_bwd(const void* dy, int dy_dt, const void* x, int x_
   });
 }
 
-// Sums of the workgroups' partial [2][D] (dw, then db) over `blocks` <= 512 workgroups. A workgroup takes 32 columns (whole
+// Sums of the workgroups' partial [2][D] (dw, then db) over `blocks` <= ROW_GRAD_BLOCKS workgroups. A workgroup takes 32 columns (whole
 // lines of the partial sums; 16 took 8.3 us instead of 5.1 at 256 x 16384 columns): 32 threads a column each add every
 // 32nd partial sum, all loads in flight at once, then the 32 meet in a fixed order.
 __global__ __launch_bounds__(1024) void row_grad_sum_k(const float* __restrict__ ws, int blocks, int D,
@@ -66,12 +66,13 @@ __global__ __launch_bounds__(1024) void row_grad_sum_k(const float* __restrict__
   __shared__ float part[32][33];
   const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int col = min((int)blockIdx.x * 32 + c, 2 * D - 1);
-  float v[16];
+  constexpr int V = ROW_GRAD_BLOCKS / 32;
+  float v[V];
 #pragma unroll
-  for (int i = 0; i < 16; i++) v[i] = g + 32 * i < blocks ? ws[(int64_t)(g + 32 * i) * 2 * D + col] : 0.f;
+  for (int i = 0; i < V; i++) v[i] = g + 32 * i < blocks ? ws[(int64_t)(g + 32 * i) * 2 * D + col] : 0.f;
   float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; i++) s += v[i];
+  for (int i = 0; i < V; i++) s += v[i];
   part[g][c] = s;
   __syncthreads();
   if (threadIdx.x < 32 && blockIdx.x * 32 + c < 2 * D) {
@@ -84,6 +85,7 @@ __global__ __launch_bounds__(1024) void row_grad_sum_k(const float* __restrict__
 }
 
 hipError_t launch_row_grad_sum(const float* ws, int64_t blocks, int D, float* dw, float* db, hipStream_t st) {
+  if (blocks > ROW_GRAD_BLOCKS) return hipErrorInvalidValue;
   row_grad_sum_k<<<(unsigned)((2 * D + 31) / 32), 1024, 0, st>>>(ws, (int)blocks, D, dw, db);
   return hipGetLastError();
 }

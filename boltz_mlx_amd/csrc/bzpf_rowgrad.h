@@ -36,8 +36,8 @@ struct RowGrad {
 template <bool RES>
 static inline int64_t row_grad_blocks(int64_t rows, int D) {
   const int per = row_places<RES>(D);
-  const int64_t least = row_blocks(rows, per, D <= 128 ? 512 : 256);
-  const int64_t four = row_blocks(rows, 4 * per, D <= 2048 ? 512 : 256);
+  const int64_t least = row_blocks(rows, per, D <= 128 ? ROW_GRAD_BLOCKS : ROW_GRAD_BLOCKS / 2);
+  const int64_t four = row_blocks(rows, 4 * per, D <= 2048 ? ROW_GRAD_BLOCKS : ROW_GRAD_BLOCKS / 2);
   return least > four ? least : four;
 }
 

@@ -182,6 +182,14 @@ def test_modules():
         Dropout(1.5)
 
 
+def test_workspaces_hold_what_the_sum_reads():
+    """The kernel that adds the workgroups' partial sums reads those of 512 workgroups at most."""
+    ws = _lib.load().bzpf_layernorm_bwd_ws
+    for D in (8, 16, 64, 77, 128, 129, 384, 1024, 1025, 1536, 1537, 2048, 2049, 4097, 8192):
+        for rows in (300, 5000, 10 ** 5, 10 ** 6, 2 ** 33, 2 ** 45):
+            assert ws(rows, D) // (8 * D) <= 512
+
+
 # -------------------------------------------------------------------------------------------------- overlapping buffers
 
 def overlapping(code):
