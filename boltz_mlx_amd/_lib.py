@@ -103,6 +103,11 @@ def load(path: str | None = None):
     return lib
 
 
+def address(name: str) -> int:
+    """Where an entry point of the loaded library lies (for the torch binding)."""
+    return C.cast(getattr(load(), name), C.c_void_p).value
+
+
 def call(name: str, *args) -> None:
     """Call an entry point; a non-zero status raises BzpfError with the library's message."""
     rc = getattr(_lib or load(), name)(*args)
@@ -118,7 +123,7 @@ def train():
     """The torch binding of the training operators (boltz_mlx_amd/_train.so). Raises if it has not been built."""
     global _train
     if _train is None:
-        load()  # torch's HIP runtime and the library that it calls
+        load()  # torch's HIP runtime; the binding takes its entry points from this library
         try:
             from boltz_mlx_amd import _train as module
         except ImportError as e:

@@ -85,11 +85,10 @@ def _compile(src: str) -> str:
 
 
 def _link(out: str, objs: list[str], *libs: str) -> None:
-    """A shared object at `out`, against torch's libraries; it finds those and its neighbours where they are now."""
+    """A shared object at `out`, against torch's libraries, which it finds where they are now."""
     tlib = torch_lib_dir()
-    r = subprocess.run(["g++", "-shared", "-fPIC", *objs, "-o", out + ".tmp", f"-L{HERE}", f"-L{tlib}",
-                        "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}", *(f"-l:{lib}" for lib in libs)],
-                       capture_output=True, text=True)
+    r = subprocess.run(["g++", "-shared", "-fPIC", *objs, "-o", out + ".tmp", f"-L{tlib}", f"-Wl,-rpath,{tlib}",
+                        *(f"-l:{lib}" for lib in libs)], capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link of {os.path.basename(out)} failed:\n{r.stderr}")
     os.replace(out + ".tmp", out)
@@ -104,8 +103,7 @@ def build(verbose: bool = True) -> str:
     # Link against the HIP runtime that torch loads (torch/lib/libamdhip64.so), so that the library and torch
     # share one runtime instance (and one device context) in the process.
     _link(LIB, objs, "libamdhip64.so")
-    _link(TRAIN, [train], "libbzpf.so", "libtorch_python.so", "libtorch.so", "libtorch_cpu.so", "libc10_hip.so", "libc10.so",
-          "libamdhip64.so")
+    _link(TRAIN, [train], "libtorch_python.so", "libtorch.so", "libtorch_cpu.so", "libc10_hip.so", "libc10.so", "libamdhip64.so")
     if verbose:
         print(f"built {LIB} and {os.path.basename(TRAIN)} from {len(srcs)} sources")
     return LIB

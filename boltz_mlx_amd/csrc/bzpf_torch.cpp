@@ -1,5 +1,6 @@
 // torch binding of the training operators (boltz_mlx_amd/_train.so): argument checks, outputs and workspaces from torch's
-// allocator, torch's current stream, and the autograd nodes. Launches go through the C entry points of include/bzpf.h.
+// allocator, torch's current stream, and the autograd nodes. Launches go through the C entry points of include/bzpf.h, in
+// the library that the rest of the package calls.
 //
 // Native because a training step is bound by the host where its tensors are small: torch runs backward passes on a
 // thread of its own, where the same code in Python takes twice its time (a LayerNorm step at 400 x 384 112 us with
@@ -37,7 +38,17 @@ struct OnDevice {
   }
 };
 
-void check(int rc, const char* name) { TORCH_CHECK(rc == BZPF_OK, name, " failed (", rc, "): ", bzpf_last_error()); }
+// The entry points, in the library that boltz_mlx_amd._lib has loaded: this module links none, so that a process holds one
+// copy, whichever it is. Set when the module is imported, before any call.
+#define BZPF_ENTRIES(X)                                                                                       \
+  X(last_error) X(layernorm) X(layernorm_bwd_ws) X(layernorm_bwd) X(dropout) X(dropout_add_ln) X(dropout_add_ln_bwd)
+struct {
+#define X(f) decltype(&::bzpf_##f) f;
+  BZPF_ENTRIES(X)
+#undef X
+} lib;
+
+void check(int rc, const char* name) { TORCH_CHECK(rc == BZPF_OK, name, " failed (", rc, "): ", lib.last_error()); }
 
 template <typename... Ts>
 void on_gpu(const char* name, const Ts&... ts) {
@@ -114,7 +125,7 @@ struct ParamGrads {
     if (need_w) dw = make();
     if (need_b) db = make();
     if (!need_w && !need_b) return;
-    ws_bytes = bzpf_layernorm_bwd_ws(r.rows, (int)r.D);
+    ws_bytes = lib.layernorm_bwd_ws(r.rows, (int)r.D);
     if (ws_bytes > 0) ws = at::empty({ws_bytes / 4}, opt);
   }
 };
@@ -127,7 +138,7 @@ Tensor layer_norm(const Tensor& x_, const Tensor& weight, const Tensor& bias, do
   on_gpu(name, x_);
   const OnDevice dev(x_);
   const Tensor x = x_.contiguous(), y = at::empty(x.sizes(), x.options().dtype(to));
-  check(bzpf_layernorm(in(x), xt, f32(w), f32(b), (float)eps, out(y), yt, r.rows, D, dev.stream), "bzpf_layernorm");
+  check(lib.layernorm(in(x), xt, f32(w), f32(b), (float)eps, out(y), yt, r.rows, D, dev.stream), "bzpf_layernorm");
   return y;
 }
 
@@ -143,7 +154,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& dy_, const Tenso
   const Tensor dy = dy_.contiguous(), x = x_.contiguous(), dx = at::empty(x.sizes(), x.options());
   const ParamGrads g(x, r, need_weight, need_bias);
   if (r.rows)
-    check(bzpf_layernorm_bwd(in(dy), gt, in(x), xt, f32(w), (float)eps, out(dx), f32_out(g.dw), f32_out(g.db),
+    check(lib.layernorm_bwd(in(dy), gt, in(x), xt, f32(w), (float)eps, out(dx), f32_out(g.dw), f32_out(g.db),
                              f32_out(g.ws), g.ws_bytes, r.rows, D, dev.stream),
           "bzpf_layernorm_bwd");
   return {dx, g.dw, g.db};
@@ -158,7 +169,7 @@ Tensor dropout(const Tensor& x_, const Drop& d, const Tensor& rng, at::ScalarTyp
   const Tensor x = x_.contiguous(), y = at::empty(x.sizes(), x.options().dtype(to));
   const int64_t n = x.numel(), D = x.dim() ? x.size(-1) : 1;
   if (n)
-    check(bzpf_dropout(in(x), xt, d.p, a.rng, (int)d.site, (int)d.shared, a.I, a.J, out(y), yt, n / D, D, dev.stream),
+    check(lib.dropout(in(x), xt, d.p, a.rng, (int)d.site, (int)d.shared, a.I, a.J, out(y), yt, n / D, D, dev.stream),
           "bzpf_dropout");
   return y;
 }
@@ -176,7 +187,7 @@ std::tuple<Tensor, Tensor> dropout_add_ln(const Tensor& z_, const Tensor& y_, co
   const OnDevice dev(z_);
   const Tensor z = z_.contiguous(), y = y_.contiguous(), z_new = at::empty(z.sizes(), z.options());
   const Tensor ln = at::empty(z.sizes(), z.options().dtype(to));
-  check(bzpf_dropout_add_ln(f32(z), in(y), yt, d.p, a.rng, (int)d.site, (int)d.shared, a.I, a.J, f32(w), f32(b),
+  check(lib.dropout_add_ln(f32(z), in(y), yt, d.p, a.rng, (int)d.site, (int)d.shared, a.I, a.J, f32(w), f32(b),
                             (float)eps, f32_out(z_new), out(ln), lt, r.rows, D, dev.stream),
         "bzpf_dropout_add_ln");
   return {z_new, ln};
@@ -205,7 +216,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> dropout_add_ln_bwd(const Tensor& dz_n
   const Tensor dy = at::empty(z_new.sizes(), z_new.options().dtype(y_type));
   const ParamGrads g(z_new, r, need_weight, need_bias);
   if (r.rows)
-    check(bzpf_dropout_add_ln_bwd(f32(dz_new), in(dln), lt, f32(z_new), f32(w), (float)eps, d.p, a.rng, (int)d.site,
+    check(lib.dropout_add_ln_bwd(f32(dz_new), in(dln), lt, f32(z_new), f32(w), (float)eps, d.p, a.rng, (int)d.site,
                                   (int)d.shared, a.I, a.J, f32_out(dz), out(dy), yt, f32_out(g.dw), f32_out(g.db),
                                   f32_out(g.ws), g.ws_bytes, r.rows, D, dev.stream),
           "bzpf_dropout_add_ln_bwd");
@@ -320,6 +331,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   namespace py = pybind11;
   typedef py::call_guard<py::gil_scoped_release> NoGil;
   typedef std::optional<at::ScalarType> Type;
+
+  const py::object address = py::module_::import("boltz_mlx_amd._lib").attr("address");
+#define X(f) lib.f = reinterpret_cast<decltype(lib.f)>(address("bzpf_" #f).cast<uintptr_t>());
+  BZPF_ENTRIES(X)
+#undef X
 
   m.def("layer_norm", [](const Tensor& x, Opt w, Opt b, double eps, at::ScalarType to) {
     return layer_norm(x, get(w), get(b), eps, to);

@@ -221,3 +221,30 @@ def test_layernorm_bwd_refuses_overlapping_buffers(change):
                                     {"dz": R, "dy": R}])
 def test_dropout_add_ln_bwd_refuses_overlapping_buffers(change):
     overlapping(res_bwd(**{**dict(dzn=P, dln=Q, zn=R, dz=S, dy=V), **change}))
+
+
+# -------------------------------------------------------------------------------------------------- the binding
+
+def python(code, *args):
+    """The output of a program in a process of its own (what it loads stays out of this one)."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code, *args], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
+    return r.stdout
+
+
+def test_binding_calls_the_loaded_library(tmp_path):
+    """With a library loaded from elsewhere, the torch binding calls that one, and the package's own is not in the process."""
+    import shutil
+
+    other = tmp_path / "other.so"
+    shutil.copy(_lib.LIB_PATH, other)
+    out = python("import sys; from boltz_mlx_amd import _lib; _lib.load(sys.argv[1]); _lib.train(); "
+                 "print(*sorted({w for w in open('/proc/self/maps').read().split() if w.startswith('/')}), sep='\\n')",
+                 str(other)).splitlines()
+    assert str(other) in out and any(w.endswith("/_train.so") for w in out)
+    assert not any(w.endswith("/libbzpf.so") for w in out)
