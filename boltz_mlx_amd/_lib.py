@@ -11,7 +11,7 @@ import os
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libbzpf.so")
 
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 
 vp, i32, i64, f32, f64 = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_double
 
@@ -127,7 +127,22 @@ def train():
         try:
             from boltz_mlx_amd import _train as module
         except ImportError as e:
-            raise BzpfError("boltz_mlx_amd/_train.so is missing or does not load: build it with "
+            raise BzpfError(f"boltz_mlx_amd/_train.so is missing or does not load ({e}): build it with "
                             "`python -c 'import __graft_entry__ as g; g.build()'`") from e
         _train = module
     return _train
+
+
+_no_train = False
+
+
+def has_train() -> bool:
+    """Whether the binding is there; looked for once, so that a program that runs without it pays nothing for that."""
+    global _no_train
+    if _train is None and not _no_train:
+        load()
+        try:
+            train()
+        except BzpfError:
+            _no_train = True
+    return _train is not None

@@ -64,7 +64,7 @@ def torch_flags() -> list[str]:
     dirs = (inc, os.path.join(inc, "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"],
             os.path.join(rocm, "include"))
     return ["-O2", "-fPIC", "-std=c++17", "-Wall", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__=1",
-            "-DTORCH_API_INCLUDE_EXTENSION_H", "-DTORCH_EXTENSION_NAME=_train",
+            "-DTORCH_API_INCLUDE_EXTENSION_H", "-DTORCH_EXTENSION_NAME=_train", f'-DBZPF_TORCH="{torch.__version__}"',
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
             *(x for d in dirs for x in ("-isystem", d))]
 

@@ -11,6 +11,7 @@
 
 #include <c10/hip/HIPStream.h>
 
+#include <string>
 #include <tuple>
 
 #include "bzpf.h"
@@ -332,6 +333,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   typedef py::call_guard<py::gil_scoped_release> NoGil;
   typedef std::optional<at::ScalarType> Type;
 
+  const std::string torch_here = py::str(py::module_::import("torch").attr("__version__"));
+  if (torch_here != BZPF_TORCH) throw py::import_error("built with torch " BZPF_TORCH ", this is " + torch_here);
   const py::object address = py::module_::import("boltz_mlx_amd._lib").attr("address");
 #define X(f) lib.f = reinterpret_cast<decltype(lib.f)>(address("bzpf_" #f).cast<uintptr_t>());
   BZPF_ENTRIES(X)

@@ -3,7 +3,7 @@
 Every wrapper checks devices, dtypes, shapes and contiguity on the host, then calls the C entry point on torch's
 current HIP stream with raw device pointers. Outputs and intermediates are allocated here with torch (the C side
 never allocates). LayerNorm and the training operators (dropout, the residual update, the backward passes) do the same
-in the native torch binding. There is no CPU path: a CPU tensor or a missing library raises.
+in the native torch binding; LayerNorm does without it where it is not built. There is no CPU path: a CPU tensor or a missing library raises.
 
 Precision (mirrors the reference's BOLTZ_MLX_PRECISION, boltz_mlx/kernels.py:1212-1220): "fp32" keeps every
 operand in fp32 (the parity build); "f16" stores GEMM operands, LayerNorm outputs and intermediates in fp16 with
@@ -23,7 +23,7 @@ from typing import NamedTuple
 import torch
 
 from boltz_mlx_amd import _lib
-from boltz_mlx_amd._lib import F16, F32
+from boltz_mlx_amd._lib import BF16, F16, F32
 from boltz_mlx_amd._lib import call as _call
 
 PRECISION = os.environ.get("BOLTZ_MLX_PRECISION", "fp32")
@@ -224,7 +224,34 @@ def layer_norm(x: torch.Tensor, weight, bias, eps: float = 1e-5, out_dtype=torch
     bf16). weight and bias may be None. Its gradients: layer_norm_bwd, or boltz_mlx_amd.autograd.layer_norm."""
     w = None if weight is None else f32c(weight)
     b = None if bias is None else f32c(bias)
+    if _lib._train is None and not _lib.has_train():
+        return _layer_norm_c(x, w, b, eps, out_dtype)
     return call("layer_norm", x, w, b, eps, out_dtype)
+
+
+_DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+
+def _layer_norm_c(x: torch.Tensor, w, b, eps: float, out_dtype) -> torch.Tensor:
+    """layer_norm through the C ABI, with the torch binding's checks (the binding halves the call's time on the host)."""
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"layer_norm: need rows of channels, got {list(x.shape)}")
+    D = x.shape[-1]
+    if not 8 <= D <= 8192:
+        raise ValueError(f"layer_norm: rows of 8 to 8192 channels, got {D}")
+    for t in (x.dtype, out_dtype):
+        if t not in _DTYPES:
+            raise TypeError(f"unsupported dtype {t}")
+    if any(p is not None and (p.numel() != D or p.device != x.device) for p in (w, b)):
+        raise ValueError(f"layer_norm: weight and bias must be [{D}] tensors on {x.device}")
+    if not x.is_cuda:
+        raise ValueError("layer_norm: need ROCm device tensors")
+    with torch.cuda.device(x.device):
+        x = x.contiguous()
+        y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+        call("bzpf_layernorm", _p(x), _DTYPES[x.dtype], _p(w), _p(b), float(eps), _p(y), _DTYPES[out_dtype],
+             x.numel() // D, D, _stream())
+    return y
 
 
 def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight, eps: float = 1e-5, need_weight: bool = True,

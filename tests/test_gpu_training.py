@@ -693,6 +693,29 @@ def test_layer_norm_parameters_at_any_element(D):
     assert torch.equal(add_ln(ws[1:], bs[3:]), add_ln(w, b))
 
 
+def test_layer_norm_without_the_binding(monkeypatch):
+    """Where the torch binding is not built, LayerNorm goes through the C ABI: the same bits, on the caller's stream."""
+    from boltz_mlx_amd import _lib
+
+    cases = []
+    for k, (tx, ty) in enumerate(TYPES):
+        for D in (77, 128, 384, 2055):
+            x, (w, b) = acts(k, 33, D, tx), params(D, D)
+            cases.append((x, w, b, ty))
+            cases.append((x.t().contiguous().t(), w.half(), None, ty))
+    want = [K().layer_norm(x, w, b, 1e-5, out_dtype=ty) for x, w, b, ty in cases]
+    torch.cuda.synchronize()
+    assert _lib._train is not None
+    monkeypatch.setattr(_lib, "_train", None)
+    monkeypatch.setattr(_lib, "_no_train", True)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        got = [K().layer_norm(x, w, b, 1e-5, out_dtype=ty) for x, w, b, ty in cases]
+        assert K().layer_norm(cases[0][0][:0], None, None).shape == (0, 77)
+    torch.cuda.synchronize()
+    for a, c, (_, _, _, ty) in zip(got, want, cases):
+        assert a.dtype == ty and torch.equal(a, c)
+
+
 def test_layer_norm_past_one_launch():
     """More rows than the kernel of the earlier widths can launch threads for (16 a row, 2^32 in all)."""
     rows, D = 2 ** 28 + 5, 64

@@ -248,3 +248,36 @@ def test_binding_calls_the_loaded_library(tmp_path):
                  str(other)).splitlines()
     assert str(other) in out and any(w.endswith("/_train.so") for w in out)
     assert not any(w.endswith("/libbzpf.so") for w in out)
+
+
+def test_layer_norm_needs_no_binding(monkeypatch):
+    """Inference calls LayerNorm everywhere, and runs where the torch binding is not built: the same checks, through the C
+    ABI (its results: tests/test_gpu_training.py)."""
+    import sys
+
+    import boltz_mlx_amd
+
+    monkeypatch.setattr(_lib, "_train", None)
+    monkeypatch.setattr(_lib, "_no_train", False)
+    monkeypatch.setitem(sys.modules, "boltz_mlx_amd._train", None)
+    monkeypatch.delattr(boltz_mlx_amd, "_train", raising=False)
+    test_layer_norm_refuses()
+    refused(TypeError, "unsupported dtype", lambda: K.layer_norm(torch.zeros(3, 16).double(), None, None))
+    refused(ValueError, "ROCm device tensors", lambda: K.layer_norm(torch.zeros(3, 16), torch.ones(16), None))
+    assert _lib._no_train
+
+
+def test_binding_of_another_torch_is_refused():
+    """A binding built with another torch does not load: the training operators say so, LayerNorm does without it."""
+    out = python("""
+import torch
+torch.__version__ = "1.2.3"
+from boltz_mlx_amd import _lib, kernels as K
+for call in (lambda: K.layer_norm(torch.zeros(3, 16), None, None), lambda: K.dropout(torch.zeros(3), 0.0, None)):
+    try:
+        call()
+    except (ValueError, _lib.BzpfError) as e:
+        print(e)
+""").splitlines()
+    assert out[0] == "layer_norm: need ROCm device tensors"
+    assert "this is 1.2.3" in out[1] and "build it with" in out[1]
