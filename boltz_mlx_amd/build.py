@@ -96,16 +96,21 @@ def _link(out: str, objs: list[str], *libs: str) -> None:
 
 def build(verbose: bool = True) -> str:
     os.makedirs(BUILD, exist_ok=True)
-    binding = os.path.join(CSRC, "bzpf_torch.cpp")
-    srcs = [binding, *sources()]  # the binding first: torch's headers take the longest
-    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
-        train, *objs = ex.map(_compile, srcs)
+    srcs = sources()
+    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
+        binding = ex.submit(_compile, os.path.join(CSRC, "bzpf_torch.cpp"))  # first: torch's headers take the longest
+        objs = list(ex.map(_compile, srcs))
     # Link against the HIP runtime that torch loads (torch/lib/libamdhip64.so), so that the library and torch
     # share one runtime instance (and one device context) in the process.
     _link(LIB, objs, "libamdhip64.so")
-    _link(TRAIN, [train], "libtorch_python.so", "libtorch.so", "libtorch_cpu.so", "libc10_hip.so", "libc10.so", "libamdhip64.so")
+    # The library stands before the binding's result is asked for: inference needs it alone. A binding of earlier sources
+    # goes where there is no new one.
+    if binding.exception() is not None and os.path.exists(TRAIN):
+        os.remove(TRAIN)
+    _link(TRAIN, [binding.result()], "libtorch_python.so", "libtorch.so", "libtorch_cpu.so", "libc10_hip.so", "libc10.so",
+          "libamdhip64.so")
     if verbose:
-        print(f"built {LIB} and {os.path.basename(TRAIN)} from {len(srcs)} sources")
+        print(f"built {LIB} and {os.path.basename(TRAIN)} from {len(srcs) + 1} sources")
     return LIB
 
 

@@ -281,3 +281,22 @@ for call in (lambda: K.layer_norm(torch.zeros(3, 16), None, None), lambda: K.dro
 """).splitlines()
     assert out[0] == "layer_norm: need ROCm device tensors"
     assert "this is 1.2.3" in out[1] and "build it with" in out[1]
+
+
+def test_a_binding_that_does_not_compile_leaves_the_library(monkeypatch, tmp_path):
+    """Where torch's headers cannot be compiled, the build says so, with libbzpf.so linked (inference needs no more) and no
+    binding of earlier sources left beside it."""
+    from boltz_mlx_amd import build as B
+
+    def compile_(src):
+        if src.endswith(".cpp"):
+            raise RuntimeError("no headers")
+        return src
+
+    linked, old = [], tmp_path / "old.so"
+    old.touch()
+    monkeypatch.setattr(B, "TRAIN", str(old))
+    monkeypatch.setattr(B, "_compile", compile_)
+    monkeypatch.setattr(B, "_link", lambda out, objs, *libs: linked.append((out, list(objs))))
+    refused(RuntimeError, "no headers", lambda: B.build(verbose=False))
+    assert linked == [(B.LIB, B.sources())] and not old.exists()
