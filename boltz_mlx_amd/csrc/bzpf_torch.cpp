@@ -11,6 +11,7 @@
 
 #include <c10/hip/HIPStream.h>
 
+#include <stdexcept>
 #include <string>
 #include <tuple>
 
@@ -49,7 +50,13 @@ struct {
 #undef X
 } lib;
 
-void check(int rc, const char* name) { TORCH_CHECK(rc == BZPF_OK, name, " failed (", rc, "): ", lib.last_error()); }
+// An entry point's refusal or failure: boltz_mlx_amd._lib.BzpfError in Python, as from every other call of the package.
+struct Failure : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+void check(int rc, const char* name) {
+  if (rc != BZPF_OK) throw Failure(c10::str(name, " failed (", rc, "): ", lib.last_error()));
+}
 
 template <typename... Ts>
 void on_gpu(const char* name, const Ts&... ts) {
@@ -335,6 +342,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
 
   const std::string torch_here = py::str(py::module_::import("torch").attr("__version__"));
   if (torch_here != BZPF_TORCH) throw py::import_error("built with torch " BZPF_TORCH ", this is " + torch_here);
+  py::register_local_exception_translator([](std::exception_ptr p) {
+    try {
+      if (p) std::rethrow_exception(p);
+    } catch (const Failure& e) {
+      PyErr_SetString(py::module_::import("boltz_mlx_amd._lib").attr("BzpfError").ptr(), e.what());
+    }
+  });
   const py::object address = py::module_::import("boltz_mlx_amd._lib").attr("address");
 #define X(f) lib.f = reinterpret_cast<decltype(lib.f)>(address("bzpf_" #f).cast<uintptr_t>());
   BZPF_ENTRIES(X)

@@ -531,6 +531,26 @@ def test_gradients_of_gradients_are_refused():
             torch.autograd.grad(out.sum(), x, create_graph=True)
 
 
+def test_entry_points_refusals_are_the_packages_error(monkeypatch):
+    """What a C entry point refuses raises BzpfError, through the torch binding as everywhere else."""
+    from boltz_mlx_amd import _lib
+    from boltz_mlx_amd import autograd as A
+
+    x, rng = rand(1, 6, 32, dtype=F16), K().dropout_rng(1)
+    calls = [lambda: K().layer_norm(x, None, None, out_dtype=BF16), lambda: K().layer_norm_bwd(x, x.bfloat16(), None),
+             lambda: K().dropout(x, 0.5, rng, out_dtype=BF16),
+             lambda: K().dropout_add_ln(x.float(), x, None, None, 1e-5, 0.5, rng, out_dtype=BF16),
+             lambda: K().dropout_add_ln_bwd(None, x, x.float(), None, 1e-5, 0.5, rng, y_dtype=BF16),
+             lambda: A.layer_norm(x.requires_grad_(), out_dtype=BF16)]
+    for call in calls:
+        with pytest.raises(_lib.BzpfError, match="failed .-1.: bzpf_.*bad dtype"):
+            call()
+    monkeypatch.setattr(_lib, "_train", None)
+    monkeypatch.setattr(_lib, "_no_train", True)
+    with pytest.raises(_lib.BzpfError, match="bad dtype"):
+        calls[0]()
+
+
 def test_launch_times_are_recorded():
     x, w, rng = rand(1, 40, 64), rand(2, 64), K().dropout_rng(1)
     K().start_timing()
