@@ -1,9 +1,11 @@
 """torch-facing wrappers of the bzpf C ABI, plus the precision policy of the pair path.
 
-Every wrapper checks devices, dtypes, shapes and contiguity on the host, then calls the C entry point on torch's
-current HIP stream with raw device pointers. Outputs and intermediates are allocated here with torch (the C side
-never allocates). LayerNorm and the training operators (dropout, the residual update, the backward passes) do the same
-in the native torch binding; LayerNorm does without it where it is not built. There is no CPU path: a CPU tensor or a missing library raises.
+Every wrapper checks devices, dtypes, shapes and contiguity on the host, then calls the C entry point on torch's current
+HIP stream with raw device pointers; one that writes a tensor of the caller's counts its version up, as torch's in-place
+operations do, so that a graph which has saved it raises instead of using the new values. Outputs and intermediates are
+allocated here with torch (the C side never allocates). LayerNorm and the training operators (dropout, the residual
+update, the backward passes) do the same in the native torch binding; LayerNorm does without it where it is not built.
+There is no CPU path: a CPU tensor or a missing library raises.
 
 Precision (mirrors the reference's BOLTZ_MLX_PRECISION, boltz_mlx/kernels.py:1212-1220): "fp32" keeps every
 operand in fp32 (the parity build); "f16" stores GEMM operands, LayerNorm outputs and intermediates in fp16 with
@@ -21,6 +23,7 @@ import threading
 from typing import NamedTuple
 
 import torch
+from torch.autograd.graph import increment_version as _written  # a kernel wrote its tensor: autograd has to see that
 
 from boltz_mlx_amd import _lib
 from boltz_mlx_amd._lib import BF16, F16, F32
@@ -330,6 +333,7 @@ def add_ln(z: torch.Tensor, y: torch.Tensor, ln=None, scale: float = 1.0, trans_
         w, b, eps = f32c(ln.weight), f32c(ln.bias), ln.eps
     call("bzpf_add_ln", _p(z), _p(y), _dt(y), float(scale), int(trans_y), _p(w), _p(b), float(eps), _p(out),
          _dt(out) if out is not None else F32, int(trans_out), N, D, _stream())
+    _written(z)
     return out
 
 
@@ -376,6 +380,7 @@ def trimul_tail64(o, norm_out, eps_out: float, w_po, xn, w_go, z, accumulate: bo
     ow, ob = f32c(norm_out.weight), f32c(norm_out.bias)
     call("bzpf_trimul_tail64", _p(o), _p(ow), _p(ob), float(eps_out), _p(w_po),
          _p(xn), _p(w_go), _p(z), int(accumulate), _p(nw), _p(nb), float(neps), _p(nxt), _dt(xn), N, ld, _stream())
+    _written(z)
     return nxt
 
 
@@ -406,6 +411,7 @@ def linear_resid_ln64(x, w, trans: bool, z, accumulate: bool, next_ln=None, N: i
         nw, nb, neps = f32c(next_ln.weight), f32c(next_ln.bias), next_ln.eps
     call("bzpf_linear_resid_ln64", _p(x), _p(w), int(trans), _p(z), int(accumulate), _p(nw), _p(nb), float(neps),
          _p(nxt), _dt(x), N, _stream())
+    _written(z)
     return nxt
 
 
@@ -552,6 +558,7 @@ def trimul_tail(o, norm_out, eps_out: float, w_po, xn, w_go, z, accumulate: bool
     call("bzpf_trimul_tail", _p(o), _p(ow), _p(ob), float(eps_out), _p(w_po),
          _p(xn), _p(w_go), _p(z), int(accumulate), _p(nw), _p(nb), float(neps), _p(nxt), _dt(xn), N, ld, D,
          _stream())
+    _written(z)
     return nxt
 
 
@@ -631,6 +638,7 @@ def linear_resid_ln(x, w, trans: bool, z, accumulate: bool, next_ln=None, N: int
         nw, nb, neps = f32c(next_ln.weight), f32c(next_ln.bias), next_ln.eps
     call("bzpf_linear_resid_ln", _p(x), _p(w), int(trans), _p(z), int(accumulate), _p(nw), _p(nb), float(neps),
          _p(nxt), _dt(x), N, D, _stream())
+    _written(z)
     return nxt
 
 
@@ -652,6 +660,7 @@ def transition(xn, w12, w3, z, accumulate: bool, next_ln=None, pair_bias=None):
     if pair_bias is None:
         call("bzpf_transition", _p(xn), _p(w12), _p(w3), _p(z), int(accumulate), _p(nw), _p(nb), float(neps),
              _p(nxt), _dt(xn), rows, D, hidden, _stream())
+        _written(z)
         return nxt
     ln, w = pair_bias
     _dev(w)
@@ -664,6 +673,7 @@ def transition(xn, w12, w3, z, accumulate: bool, next_ln=None, pair_bias=None):
     call("bzpf_transition_pb", _p(xn), _p(w12), _p(w3), _p(z), int(accumulate), _p(nw), _p(nb), float(neps),
          _p(nxt), _p(w), _p(lw), _p(lb), float(ln.eps), _p(bias), H, _dt(xn), rows, D, hidden,
          _stream())
+    _written(z)
     return nxt, bias
 
 
@@ -698,6 +708,7 @@ def attn_out_transition(o, w_o, trans: bool, z, ln, w12, w3, next_ln=None, pair_
     call("bzpf_attn_out_transition", _p(o), _p(w_o), int(trans), _p(lw), _p(lb),
          float(ln.eps), _p(w12), _p(w3), _p(z), _p(nw), _p(nb), float(neps), _p(nxt), _p(pw), _p(plw), _p(plb),
          float(peps), _p(bias), H, _dt(o), N, D, hidden, _stream())
+    _written(z)
     return nxt if pair_bias is None else (nxt, bias)
 
 
@@ -714,6 +725,7 @@ def linear(x, w, bias=None, out=None, out_dtype=None, accumulate: bool = False) 
     _dev(out)
     b = None if bias is None else f32c(bias)
     call("bzpf_linear", _p(x), _p(w), _p(b), _p(out), _dt(x), _dt(out), rows, K, M, int(accumulate), _stream())
+    _written(out)
     return out
 
 
@@ -730,6 +742,7 @@ def linear_residual(x, w, res: torch.Tensor, out: torch.Tensor, bias=None) -> to
         raise ValueError("linear_residual: shape/dtype mismatch")
     b = None if bias is None else f32c(bias)
     call("bzpf_linear_residual", _p(x), _p(w), _p(b), _p(res), res.stride(0), _p(out), _dt(x), rows, K, M, _stream())
+    _written(out)
     return out
 
 
@@ -748,6 +761,7 @@ def linear_gated(x, w, gate: torch.Tensor, out: torch.Tensor, bias=None) -> torc
     b = None if bias is None else f32c(bias)
     call("bzpf_linear_gated", _p(x), _p(w), _p(b), _p(gate), gate.stride(0), gate.shape[0], _p(out), _dt(x), rows,
          K, M, _stream())
+    _written(out)
     return out
 
 
@@ -864,6 +878,7 @@ def seq_attention_packed(qkvg, bias, mask, inf: float, H: int, out=None, multipl
     call("bzpf_seq_attention_batched", base, base + HD * es, base + 2 * HD * es, base + 3 * HD * es, HD4, N * HD4,
          _p(b4), H * N * N, int(multiplicity), _p(m2), N, float(inf), _p(out), HD, N * HD, _dt(qkvg), _dt(b4), S, N,
          H, hd, _stream())
+    _written(out)
     return out
 
 
@@ -945,6 +960,7 @@ def transition64_f16(x: torch.Tensor, ln, w12: torch.Tensor, w3: torch.Tensor) -
     lw, lb = f32c(ln.weight), f32c(ln.bias)
     call("bzpf_transition64_f16", _p(x), _p(lw), _p(lb), float(ln.eps), _p(w12), _p(w3),
          rows, H, _stream())
+    _written(x)
 
 
 def ln_linear_f32(x: torch.Tensor, ln, w: torch.Tensor) -> torch.Tensor:

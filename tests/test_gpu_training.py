@@ -496,6 +496,27 @@ def test_autograd_layouts_and_repeats():
     assert np.array_equal(np64(g), np.where(d, 0.0, 2.0))
 
 
+def test_a_saved_tensor_changed_by_the_packages_own_kernels():
+    """The inference wrappers write through device pointers: a backward pass whose saved tensor one of them has changed
+    raises, as after torch's own in-place operations."""
+    from boltz_mlx_amd import autograd as A
+
+    class LN:
+        weight, bias, eps = torch.ones(128, device="cuda"), torch.zeros(128, device="cuda"), 1e-5
+
+    w, b = (t.requires_grad_() for t in params(1, 128))
+    z, y = rand(2, 6, 6, 128), rand(3, 6, 6, 128)
+    outs = [A.layer_norm(z, w, b)]
+    zn, xn = A.dropout_add_ln(y, z, w, b)
+    outs.append(xn)
+    K().add_ln(z, y, LN)
+    K().transition(rand(4, 36, 128), rand(5, 512, 128), rand(6, 128, 256), zn.detach(), True)
+    K().linear(rand(7, 36, 128), rand(8, 128, 128), out=zn.detach().view(36, 128), accumulate=True)
+    for out in outs:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out.sum(), w)
+
+
 def test_threads():
     """Calls from several host threads at once, each on a stream of its own."""
     import threading

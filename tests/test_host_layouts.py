@@ -124,6 +124,52 @@ def test_converted_parameters_outlive_the_launch(monkeypatch, name):
     assert len(calls) == 1 and len(copies) >= 2 and all(calls[0])
 
 
+def _writing_calls():
+    """{wrapper: (the caller's tensor that it writes, the call)}."""
+    from boltz_mlx_amd import kernels as K
+
+    N, h = 3, torch.float16
+    ld = K.row_pitch(N)
+    z, z64, x64 = torch.zeros(N, N, 128), torch.zeros(N, N, 64), torch.zeros(N * N, 64)
+    o, xn, w, w12, w3 = (torch.zeros(*s, dtype=h) for s in ((128, N, ld), (N * N, 128), (128, 128), (512, 128), (128, 256)))
+    xn64, w64 = xn[:, :64].contiguous(), torch.zeros(64, 64, dtype=h)
+    ln, ln64, pw = _HalfLN(128), _HalfLN(64), torch.zeros(4, 128, dtype=h)
+    out, out16 = torch.zeros(N * N, 128), torch.zeros(N, 128, dtype=h)
+    qkvg, bias, mask = torch.zeros(N, 512, dtype=h), torch.zeros(4, N, N), torch.zeros(N)
+    return {
+        "add_ln": (z, lambda: K.add_ln(z, z, ln)),
+        "trimul_tail": (z, lambda: K.trimul_tail(o, ln, 1e-5, w, xn, w, z, True, ln, N)),
+        "trimul_tail64": (z64, lambda: K.trimul_tail64(o[:64], ln64, 1e-5, w64, xn64, w64, z64, True, ln64, N)),
+        "linear_resid_ln": (z, lambda: K.linear_resid_ln(xn, w, False, z, True, ln, N)),
+        "linear_resid_ln64": (z64, lambda: K.linear_resid_ln64(xn, w[:64], False, z64, True, ln64, N)),
+        "transition": (z, lambda: K.transition(xn, w12, w3, z, True, ln)),
+        "transition, pair bias": (z, lambda: K.transition(xn, w12, w3, z, True, ln, (ln, pw))),
+        "attn_out_transition": (z, lambda: K.attn_out_transition(xn, w, True, z, ln, w12, w3, ln)),
+        "transition64_f16": (x64, lambda: K.transition64_f16(x64, ln64, w12[:, :64].contiguous(), w3[:64])),
+        "linear": (out, lambda: K.linear(xn, w, out=out, accumulate=True)),
+        "seq_attention_packed": (out16, lambda: K.seq_attention_packed(qkvg, bias, mask, 1e9, 4, out=out16)),
+    }
+
+
+@pytest.mark.parametrize("name", _writing_calls())
+def test_written_tensors_count_up(monkeypatch, name):
+    """A wrapper that writes a tensor of its caller's counts its version up: autograd sees the kernel's write."""
+    from boltz_mlx_amd import kernels as K
+
+    monkeypatch.setattr(K, "_dev", lambda *ts: None)
+    monkeypatch.setattr(K, "_stream", lambda: 0)
+    monkeypatch.setattr(K, "call", lambda *args: None)
+    t, call = _writing_calls()[name]
+    before = t._version
+    call()
+    assert t._version == before + 1
+    with torch.no_grad():
+        call()
+    with torch.inference_mode():
+        call()
+    assert t._version == before + 3
+
+
 class _DeviceMask(torch.Tensor):
     """A CPU tensor that says it is on the GPU, so that what a scope shares can be followed without one."""
 
