@@ -707,6 +707,18 @@ def test_a_block_of_updates_trains():
         assert (g.double().cpu() - w).abs().max() <= 3e-5 * w.abs().max()
 
 
+# -------------------------------------------------------------------------------------------------- more of dropout's ends
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_no_dropout_keeps_every_bit(dtype):
+    x = rand(3, 20, 6, 51, dtype=dtype)
+    x[::2, ::3, ::7], x[1::2, ::3, ::5], x[0, 0, :2] = float("inf"), float("nan"), -0.0
+    bits = torch.int32 if dtype == F32 else torch.int16
+    for p in (0.0, 2.0 ** -34):  # the second rounds to no draw at all
+        for shared in (None, "row", "column"):
+            assert torch.equal(K().dropout(x, p, K().dropout_rng(1), 2, shared).view(bits), x.view(bits))
+
+
 # -------------------------------------------------------------------------------------------------- LayerNorm's two kernels
 
 @pytest.mark.parametrize("D", [64, 128, 384, 1024])
@@ -732,6 +744,42 @@ def test_layer_norm_parameters_at_any_element(D):
     w, b = params(5, 128)
     ws, bs = torch.cat([w[:1], w]), torch.cat([b[:3], b])
     assert torch.equal(add_ln(ws[1:], bs[3:]), add_ln(w, b))
+
+
+# The widths and types that LayerNorm served before it took every width: SHA-256 of the outputs (fp32 and fp16 in, fp32 and
+# fp16 out, in that order) of the library as it was then, for the inputs below.
+EARLIER = {
+    64: "eaba80f696e4beb0",
+    128: "6511081e6816421d",
+    192: "f6c8ad3a965efa8e",
+    256: "93d555ca95c6be38",
+    320: "c882499ddb6a75fe",
+    384: "6fae8af8104e92a7",
+    512: "cb0af66ac15ca896",
+    768: "d27715d0c777c274",
+    1024: "6d5eb8b9f369ed98",
+}
+
+
+def earlier_digest(layer_norm, D):
+    """Inputs from integers alone, so that they are the same anywhere."""
+    import hashlib
+
+    r, c = np.arange(131, dtype=np.int64)[:, None], np.arange(D, dtype=np.int64)
+    x = ((r * D + c) * 2654435761 % 2 ** 32) / 2.0 ** 29 - 4 + r % 7
+    w, b = 1 + (c * 40503 % 65536 - 32768) / 2.0 ** 18, (c * 30011 % 65536 - 32768) / 2.0 ** 16
+    x, w, b = (torch.tensor(v, dtype=F32, device="cuda") for v in (x, w, b))
+    digest = hashlib.sha256()
+    for tx in (F32, F16):
+        for ty in (F32, F16):
+            for args in ((w, b), (None, None)):
+                digest.update(layer_norm(x.to(tx), *args, 1e-5, out_dtype=ty).cpu().numpy().tobytes())
+    return digest.hexdigest()[:16]
+
+
+@pytest.mark.parametrize("D", EARLIER)
+def test_earlier_widths_keep_their_bits(D):
+    assert earlier_digest(K().layer_norm, D) == EARLIER[D]
 
 
 def test_layer_norm_without_the_binding(monkeypatch):
