@@ -719,6 +719,79 @@ def test_no_dropout_keeps_every_bit(dtype):
             assert torch.equal(K().dropout(x, p, K().dropout_rng(1), 2, shared).view(bits), x.view(bits))
 
 
+# -------------------------------------------------------------------------------------------------- more sizes past 32 bits
+
+BIG = (1025, 1024, 2048)  # 2^31 + 2^21 elements; more rows than a forward launch has workgroups, which turn once more
+
+
+def big(seed, dtype):
+    """Rows of a tensor of size BIG: 1024 of them, repeated, and others in the last 80."""
+    rows, D = BIG[0] * BIG[1], BIG[2]
+    x = acts(seed, 1024, D, dtype).repeat(BIG[0], 1)
+    x[rows - 80:] = acts(seed + 5, 80, D, dtype)
+    return x
+
+
+def check_param_sums(dw, db, dy, x):
+    """dw and db against sums in float64 on the device, a slice of rows at a time, with dw_tol's tolerance."""
+    depth = len(x) // 256 + 128
+    rw, rb, tw, tb = (torch.zeros(x.shape[1], dtype=torch.float64, device="cuda") for _ in range(4))
+    for i in range(0, len(x), 2 ** 15):
+        xs, g = x[i:i + 2 ** 15].double(), dy[i:i + 2 ** 15].double()
+        c = xs - xs.mean(-1, keepdim=True)
+        rstd = 1 / ((c * c).mean(-1, keepdim=True) + 1e-5).sqrt()
+        xh, E = c * rstd, U * (16 * xs.abs().amax(-1, keepdim=True) * rstd + 14)
+        rw += (g * xh).sum(0)
+        rb += g.sum(0)
+        tw += (g.abs() * (1 + xh.abs()) * E).sum(0) + depth * U * (g * xh).abs().sum(0)
+        tb += depth * U * g.abs().sum(0)
+    close(dw, np64(rw), np64(tw))
+    close(db, np64(rb), np64(tb))
+
+
+def test_layer_norm_gradients_past_32_bits():
+    x, dy, w = big(1, F16), big(11, F16), params(2, BIG[2])[0]
+    dx, dw, db = K().layer_norm_bwd(dy, x, w)
+    tail = [np64(t[-1200:]) for t in (dy, x)]
+    close(dx[-1200:], T.ln_grads(*tail, np64(w))[0], dx_tol(*tail, np64(w)))
+    check_param_sums(dw, db, dy, x)
+
+
+@pytest.mark.parametrize("shared", [None, "row", "column"])
+def test_residual_update_past_32_bits(shared):
+    """The residual update and its backward pass: the last rows' values, draws and gradients, and the sums over all rows."""
+    rows, D = BIG[0] * BIG[1], BIG[2]
+    z, y, (w, b), rng, p = big(1, F32), big(21, F16), params(2, D), K().dropout_rng(2 ** 33 + 7, 5), 0.25
+    zn, xn = K().dropout_add_ln(z.view(BIG), y.view(BIG), w, b, 1e-5, p, rng, 6, shared)
+    zn, xn = zn.view(rows, D), xn.view(rows, D)
+    n = 1200
+    d = T.dropped(BIG, p, 2 ** 33 + 7, 5, 6, shared, first_row=rows - n, rows=n)
+    zt, yt, znt, xnt = (np64(t[-n:]) for t in (z, y, zn, xn))
+    close(zn[-n:], zt + T.dropout(yt, p, d), 3 * U * np.abs(yt) / (1 - p))
+    close(xn[-n:], T.ln(znt, np64(w), np64(b)), ln_tol(znt, np64(w), np64(b)))
+    dz, dy, dw, db = K().dropout_add_ln_bwd(z.view(BIG), xn.view(BIG), zn.view(BIG), w, 1e-5, p, rng, 6, shared)
+    rz, ry, _, _ = T.residual_grads(zt, xnt, znt, p, d, np64(w))
+    tol = dx_tol(xnt, znt, np64(w)) + 2 * U * np.abs(rz)
+    close(dz.view(rows, D)[-n:], rz, tol)
+    got = dy.view(rows, D)[-n:]
+    assert (np64(got)[d] == 0).all()
+    close(got, ry, (tol + 2 * U * np.abs(rz)) / (1 - p))
+    check_param_sums(dw, db, xn, zn)
+
+
+@pytest.mark.parametrize("shared", [None, "row", "column"])
+def test_dropout_of_odd_rows_past_32_bits(shared):
+    shape, rng, p = (1026, 1025, 2047), K().dropout_rng(9, 2 ** 40), 0.5
+    rows, D = shape[0] * shape[1], shape[2]
+    x = acts(3, 1025, D, F16).repeat(shape[0], 1)
+    x[x == 0] = 1
+    y = K().dropout(x.view(shape), p, rng, 8, shared).view(rows, D)
+    n = 1200
+    d = T.dropped(shape, p, 9, 2 ** 40, 8, shared, first_row=rows - n, rows=n)
+    assert np.array_equal(np64(y[-n:]) == 0, d)
+    close(y[-n:], T.dropout(np64(x[-n:]), p, d), 2 * U * np.abs(np64(x[-n:])) / (1 - p))
+
+
 # -------------------------------------------------------------------------------------------------- LayerNorm's two kernels
 
 @pytest.mark.parametrize("D", [64, 128, 384, 1024])
