@@ -3,8 +3,8 @@
 boltz_mlx_amd.layers run inference only, as the reference does; layers.norm and layers.dropout offer these functions.)
 
 Once differentiable: a backward pass with create_graph raises. What a function saves is its input (the residual update:
-its output z_new), the weight and the generator's state; changing one of them in place before the backward pass raises
-torch's error, so advance the generator (rng[1] += 1) after the step's backward pass.
+its output z_new), the weight and the generator's state; changing one of them in place before the backward pass, with torch
+or with a wrapper of boltz_mlx_amd.kernels that writes its argument, raises torch's error there, so advance the generator (rng[1] += 1) after the step's backward pass.
 
 To capture a step into a HIP graph, run no eager backward pass over the same leaves whose graph is still alive, and take
 the gradients inside the capture with torch.autograd.grad (or call the *_bwd functions of boltz_mlx_amd.kernels).

@@ -8,8 +8,8 @@
  *
  * Storage types: BZPF_F32 (fp32) or BZPF_F16 (fp16 operands, fp32 accumulation / statistics / softmax); LayerNorm and
  * the training entry points take BZPF_BF16 too, but not fp16 and bf16 in one call, and pointers aligned to their
- * elements. The pair representation z is always fp32 [N, N, 128] row-major. Other pointers are 16-byte aligned;
- * D = c_z = 128 for the pair kernels.
+ * elements; their outputs are buffers of their own where an entry point does not say otherwise. The pair representation
+ * z is always fp32 [N, N, 128] row-major. Other pointers are 16-byte aligned; D = c_z = 128 for the pair kernels.
  *
  * Each entry point replaces a kernel wrapper of the reference (paths relative to the reference checkout,
  * jackryan225/boltz-mlx), which launched MSL source through mx.fast.metal_kernel (boltz_mlx/kernels.py:315-324).
