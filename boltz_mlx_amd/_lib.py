@@ -27,6 +27,18 @@ SIGNATURES = {
     "bzpf_dropout_add_ln": [vp, vp, i32, f64, vp, i32, i32, i64, i64, vp, vp, f32, vp, vp, i32, i64, i32, vp],
     "bzpf_dropout_add_ln_bwd": [vp, vp, i32, vp, vp, f32, f64, vp, i32, i32, i64, i64, vp, vp, i32, vp, vp, vp, i64, i64,
                                 i32, vp],
+    "bzpf_rel_bias": [vp, vp, i64, i32, i32, vp, vp, vp, vp, i32, i64, i64, vp, vp, i32, i64, i32, i64, i64, vp],
+    "bzpf_rel_bias_bwd_ws": [i64, i32, i64, i64, i32],
+    "bzpf_rel_bias_bwd": [vp, i32, vp, i64, i32, i32, vp, vp, vp, vp, i32, i64, i64, vp, vp, i64, i64, i32, i64, i64, vp],
+    "bzpf_qk_norm_rope": [vp, i64, vp, i64, i32, vp, vp, f32, vp, i32, i64, f64, i32, i32, vp, vp, i32, i64, i32, i32, i32, vp],
+    "bzpf_qk_norm_rope_bwd_ws": [i32],
+    "bzpf_qk_norm_rope_bwd": [vp, vp, i32, vp, i64, vp, i64, i32, vp, vp, f32, vp, i32, i64, f64, i32, i32, vp, vp, vp, vp, vp,
+                              i64, i64, i32, i32, i32, vp],
+    "bzpf_attention": [vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i64,
+                       i64, vp],
+    "bzpf_attention_bwd_ws": [i32, i32, i32, i32, i64, i64, i32],
+    "bzpf_attention_bwd": [vp, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp,
+                           vp, vp, i64, i32, i32, i32, i32, i64, i64, vp],
     "bzpf_add_ln": [vp, vp, i32, f32, i32, vp, vp, f32, vp, i32, i32, i64, i32, vp],
     "bzpf_count_nonfinite": [vp, i32, i64, vp, vp],
     "bzpf_linear_gated": [vp, vp, vp, vp, i64, i64, vp, i32, i64, i32, i32, vp],
@@ -71,7 +83,8 @@ SIGNATURES = {
     "bzpf_pair_bias": [vp, vp, vp, f32, vp, vp, i32, i64, i32, i32, vp],
 }
 _RESTYPES = {"bzpf_version": C.c_char_p, "bzpf_last_error": C.c_char_p, "bzpf_row_pitch": i64,
-             "bzpf_pwa_wsplit_bytes": i64, "bzpf_layernorm_bwd_ws": i64}
+             "bzpf_pwa_wsplit_bytes": i64, "bzpf_layernorm_bwd_ws": i64, "bzpf_rel_bias_bwd_ws": i64,
+             "bzpf_qk_norm_rope_bwd_ws": i64, "bzpf_attention_bwd_ws": i64}
 
 _lib = None
 

@@ -49,6 +49,10 @@ def sources() -> list[str]:
     return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hip"))
 
 
+def binding_sources() -> list[str]:
+    return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cpp"))
+
+
 # Per-source additions. The fp16 attention core is VALU-bound; without NaN semantics its fmaxf reductions over MFMA
 # results need no canonicalising v_max_f32 per logit (its inputs are finite or -inf by construction).
 FILE_FLAGS = {"bzpf_triattn_mfma.hip": ["-fno-honor-nans"]}
@@ -96,21 +100,23 @@ def _link(out: str, objs: list[str], *libs: str) -> None:
 
 def build(verbose: bool = True) -> str:
     os.makedirs(BUILD, exist_ok=True)
-    srcs = sources()
-    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
-        binding = ex.submit(_compile, os.path.join(CSRC, "bzpf_torch.cpp"))  # first: torch's headers take the longest
-        objs = list(ex.map(_compile, srcs))
+    srcs, bsrcs = sources(), binding_sources()
+    with cf.ThreadPoolExecutor(max_workers=8) as ex:
+        binding = [ex.submit(_compile, src) for src in bsrcs]  # first: torch's headers take long
+        # the sources with the most kernels first
+        objs = dict(zip(big_first := sorted(srcs, key=os.path.getsize, reverse=True), ex.map(_compile, big_first)))
+        objs = [objs[src] for src in srcs]
     # Link against the HIP runtime that torch loads (torch/lib/libamdhip64.so), so that the library and torch
     # share one runtime instance (and one device context) in the process.
     _link(LIB, objs, "libamdhip64.so")
     # The library stands before the binding's result is asked for: inference needs it alone. A binding of earlier sources
     # goes where there is no new one.
-    if binding.exception() is not None and os.path.exists(TRAIN):
+    if any(b.exception() is not None for b in binding) and os.path.exists(TRAIN):
         os.remove(TRAIN)
-    _link(TRAIN, [binding.result()], "libtorch_python.so", "libtorch.so", "libtorch_cpu.so", "libc10_hip.so", "libc10.so",
+    _link(TRAIN, [b.result() for b in binding], "libtorch_python.so", "libtorch.so", "libtorch_cpu.so", "libc10_hip.so", "libc10.so",
           "libamdhip64.so")
     if verbose:
-        print(f"built {LIB} and {os.path.basename(TRAIN)} from {len(srcs) + 1} sources")
+        print(f"built {LIB} and {os.path.basename(TRAIN)} from {len(srcs) + len(bsrcs)} sources")
     return LIB
 
 

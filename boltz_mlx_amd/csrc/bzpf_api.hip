@@ -4,12 +4,17 @@
 #include <cstdio>
 
 #include "bzpf.h"
+#include "bzpf_api.h"
 #include "bzpf_kernels.h"
 #include "bzpf_layout.h"
 
 namespace {
 
 thread_local char g_err[512] = "";
+
+}  // namespace
+
+namespace bzpf_api {
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -27,12 +32,12 @@ int done(hipError_t e, const char* what) {
   return fail(BZPF_ELAUNCH, "%s: %s", what, hipGetErrorString(e));
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-bool dt_ok(int dt) { return dt == BZPF_F32 || dt == BZPF_F16; }
-// The training entry points: bf16 too, but not fp16 and bf16 in one call; pointers at element alignment.
-bool dt3_ok(int dt) { return dt_ok(dt) || dt == BZPF_BF16; }
-bool pair_ok(int a, int b) { return dt3_ok(a) && dt3_ok(b) && (a == b || a == BZPF_F32 || b == BZPF_F32); }
-bool aligned_el(const void* p, int dt) { return (reinterpret_cast<uintptr_t>(p) & (dt == BZPF_F32 ? 3u : 1u)) == 0; }
+}  // namespace bzpf_api
+
+namespace {
+
+using namespace bzpf_api;
+
 // Whether the n elements of an output share no byte with n of another tensor (null: none). `itself`: the output may be that
 // tensor, in its type, where the kernel has a whole row in registers before it writes it.
 bool apart(const void* out, int out_dt, const void* t, int t_dt, int64_t n, bool itself = false) {
@@ -43,16 +48,8 @@ bool apart(const void* out, int out_dt, const void* t, int t_dt, int64_t n, bool
          end(t, t_dt) <= reinterpret_cast<uintptr_t>(out);
 }
 bool width_ok(int64_t D) { return D >= bzpf::ROW_MIN_D && D <= bzpf::ROW_MAX_D; }
-hipStream_t S(void* s) { return static_cast<hipStream_t>(s); }
 
 }  // namespace
-
-#define REQUIRE(cond, ...) \
-  do {                     \
-    if (!(cond)) return fail(BZPF_EINVAL, __VA_ARGS__); \
-  } while (0)
-#define REQUIRE_EL(p, dt) REQUIRE((p) != nullptr && aligned_el(p, dt), "%s: %s must be non-null and aligned to its elements", __func__, #p)
-#define REQUIRE_PTR(p) REQUIRE((p) != nullptr && aligned16(p), "%s: %s must be a non-null 16-byte aligned pointer", __func__, #p)
 
 extern "C" {
 

@@ -163,4 +163,61 @@ hipError_t launch_triattn_pack(const void* P, int trans, float q_scale, float b_
 hipError_t launch_pair_bias(const float* z, const float* lnw, const float* lnb, float eps, const void* w, void* out,
                             int dt, int64_t rows, int H, hipStream_t st);
 
+// The learned position bias by buckets (bzpf_relbias.hip): positions and groups [N] and [M] of each batch element, `batch_*`
+// elements apart (0: shared).
+struct RelBias {
+  const float* table;   // [count][H]
+  const uint8_t* lut;   // [span]: the bucket of distance lo + i
+  int64_t lo;
+  int span, count, H;
+  const void *pos_q, *pos_k, *group_q, *group_k;  // groups: null for one
+  bool wide;                                      // 64-bit integers
+  int64_t batch_q, batch_k, N, M;
+};
+hipError_t launch_rel_bias(const RelBias& a, const void* add, void* out, int dt, int64_t B, hipStream_t st);
+int64_t rel_bias_bwd_ws_bytes(int64_t B, int H, int64_t N, int64_t M, int count);
+hipError_t launch_rel_bias_bwd(const RelBias& a, const void* dy, int dt, float* dtable, float* ws, int64_t B, hipStream_t st);
+
+// Norms of queries [0] and keys [1] with the position rotation (bzpf_qknorm.hip).
+constexpr int QK_MAX_C = 256;
+struct QKNorm {
+  const void* x[2];
+  int64_t ld[2];      // row pitch of x
+  const float* w[2];  // [C] or null
+  void* y[2];         // outputs [rows][H C]; in the backward pass their gradients, read
+  void* dx[2];
+  int H[2];
+  int C, rot;
+  bool inter, wide;
+  const void* pos;    // [pos_rows], row r at pos[r % pos_rows]; null: no rotation
+  int64_t pos_rows, rows;
+  double log2_base;
+  float eps;
+  float* ws;          // partial weight gradients [workgroups][2][C]; null: none wanted
+  int L, hp, sub;     // set by the launch
+};
+hipError_t launch_qk_norm(const QKNorm& a, int x_dt, int y_dt, hipStream_t st);
+int64_t qk_norm_ws_bytes(int C);
+hipError_t launch_qk_norm_bwd(const QKNorm& a, int x_dt, int dy_dt, float* dwq, float* dwk, hipStream_t st);
+
+// The sequence attention's training form (bzpf_attn_fwd.hip, bzpf_attn_bwd.hip). q [S][N], k and v [S][M], g [S][N]: rows of
+// pitch ld*, samples s* elements apart; the rest contiguous.
+struct Attn {
+  const void *q, *k, *v, *g, *bias;  // g, bias: may be null
+  const float* mask;                 // [S][M] or null
+  int64_t ldq, ldk, ldv, ldg, sq, sk, sv, sg, N, M;
+  int S, H, C, mult, dt, bias_dt;
+  float scale;
+  void* out;     // [S][N][H C]
+  float* stats;  // [S][H][N][2]: a row's largest logit and the sum of exp(logit - that)
+  const void* dout;
+  void *dq, *dk, *dv, *dg, *dbias;
+  float* delta;  // [S][H][N]
+  void* dO;      // [S][N][H C]: sigmoid(g) dout
+  void* dO_lo;   // what rounding to a half type has left of it
+};
+hipError_t launch_attention(const Attn& a, hipStream_t st);
+int64_t attention_bwd_ws_bytes(int dt, int64_t S, int64_t N, int H, int C, bool gate);
+hipError_t launch_attention_bwd(Attn a, void* ws, hipStream_t st);
+
 }  // namespace bzpf

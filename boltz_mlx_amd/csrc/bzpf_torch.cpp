@@ -1,67 +1,21 @@
-// torch binding of the training operators (boltz_mlx_amd/_train.so): argument checks, outputs and workspaces from torch's
-// allocator, torch's current stream, and the autograd nodes. Launches go through the C entry points of include/bzpf.h, in
-// the library that the rest of the package calls.
+// torch binding of the training operators (boltz_mlx_amd/_train.so; the attention's are in bzpf_torch_attn.cpp): argument
+// checks, outputs and workspaces from torch's allocator, torch's current stream, and the autograd nodes. Launches go through
+// the C entry points of include/bzpf.h, in the library that the rest of the package calls.
 //
 // Native because a training step is bound by the host where its tensors are small: torch runs backward passes on a
 // thread of its own, where the same code in Python takes twice its time (a LayerNorm step at 400 x 384 112 us with
 // Python autograd functions; of it the kernels take 12 us, torch's own engine some 45 us).
 //
 // Arguments are checked before devices, so that what a call would refuse can be seen without a GPU.
-#include <torch/extension.h>
+#include "bzpf_torch.h"
 
-#include <c10/hip/HIPStream.h>
-
-#include <stdexcept>
-#include <string>
-#include <tuple>
-
-#include "bzpf.h"
+namespace bzpf_torch {
+Entries lib;
+}
 
 namespace {
 
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-typedef const std::optional<Tensor>& Opt;  // None: an undefined tensor
-Tensor get(Opt o) { return o.value_or(Tensor()); }
-
-int type_code(at::ScalarType t) {
-  TORCH_CHECK_TYPE(t == at::kFloat || t == at::kHalf || t == at::kBFloat16, "unsupported dtype ", t);
-  return t == at::kFloat ? BZPF_F32 : t == at::kHalf ? BZPF_F16 : BZPF_BF16;
-}
-int type_code(const Tensor& t) { return type_code(t.scalar_type()); }
-
-// The calling thread's device is t's for the scope, and so the current stream one of t's device.
-struct OnDevice {
-  c10::OptionalDeviceGuard guard;
-  void* stream;
-  explicit OnDevice(const Tensor& t) : guard(t.device()) {
-    stream = c10::hip::getCurrentHIPStream(t.device().index()).stream();
-  }
-};
-
-// The entry points, in the library that boltz_mlx_amd._lib has loaded: this module links none, so that a process holds one
-// copy, whichever it is. Set when the module is imported, before any call.
-#define BZPF_ENTRIES(X)                                                                                       \
-  X(last_error) X(layernorm) X(layernorm_bwd_ws) X(layernorm_bwd) X(dropout) X(dropout_add_ln) X(dropout_add_ln_bwd)
-struct {
-#define X(f) decltype(&::bzpf_##f) f;
-  BZPF_ENTRIES(X)
-#undef X
-} lib;
-
-// An entry point's refusal or failure: boltz_mlx_amd._lib.BzpfError in Python, as from every other call of the package.
-struct Failure : std::runtime_error {
-  using std::runtime_error::runtime_error;
-};
-void check(int rc, const char* name) {
-  if (rc != BZPF_OK) throw Failure(c10::str(name, " failed (", rc, "): ", lib.last_error()));
-}
-
-template <typename... Ts>
-void on_gpu(const char* name, const Ts&... ts) {
-  TORCH_CHECK_VALUE((... && (!ts.defined() || ts.is_cuda())), name, ": need ROCm device tensors");
-}
+using namespace bzpf_torch;
 
 struct Rows {
   int64_t rows, D;
@@ -95,11 +49,6 @@ Tensor param(const char* name, const Tensor& x, const Tensor& p) {
                     "] tensors on ", x.device());
   return p.scalar_type() == at::kFloat && p.is_contiguous() ? p : p.detach().to(at::kFloat).contiguous();
 }
-const float* f32(const Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
-float* f32_out(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
-const void* in(const Tensor& t) { return t.const_data_ptr(); }
-void* out(const Tensor& t) { return t.data_ptr(); }
-
 struct Drop {
   double p;
   int64_t site, shared;  // 0: a draw for each element, 1: for each row, 2: for each column of [.., I, J, D]
@@ -232,14 +181,6 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> dropout_add_ln_bwd(const Tensor& dz_n
 }
 
 // ------------------------------------------------------------------------------------------------ autograd
-
-// Backward passes are not differentiable: a call that asks for their graph is refused rather than given none.
-void once(const char* name) {
-  TORCH_CHECK(!at::GradMode::is_enabled(), name, ": gradients of gradients are not provided (create_graph)");
-}
-int64_t type_of(const Tensor& t) { return static_cast<int64_t>(t.defined() ? t.scalar_type() : at::kFloat); }
-// A parameter's gradient in its type.
-Tensor as(const Tensor& g, int64_t type) { return g.defined() ? g.to(static_cast<at::ScalarType>(type)) : g; }
 
 // The weight and bias of a node: which of them are there (a node's inputs are counted over those that are), and the bias's
 // type. `before`: the node's inputs before them.
@@ -384,4 +325,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         DropoutAddLNNode::apply(z, y, w, b, eps, p, rng, site, shared, to.value_or(y.scalar_type()));
     return std::make_tuple(o[0], o[1]);
   }, NoGil());
+  bind_attention(m);
 }

@@ -4,7 +4,7 @@ Every wrapper checks devices, dtypes, shapes and contiguity on the host, then ca
 HIP stream with raw device pointers; one that writes a tensor of the caller's counts its version up, as torch's in-place
 operations do, so that a graph which has saved it raises instead of using the new values. Outputs and intermediates are
 allocated here with torch (the C side never allocates). LayerNorm and the training operators (dropout, the residual
-update, the backward passes) do the same in the native torch binding; LayerNorm does without it where it is not built.
+update, the attention's training form, the backward passes) do the same in the native torch binding; LayerNorm does without it where it is not built.
 There is no CPU path: a CPU tensor or a missing library raises.
 
 Precision (mirrors the reference's BOLTZ_MLX_PRECISION, boltz_mlx/kernels.py:1212-1220): "fp32" keeps every
@@ -69,7 +69,10 @@ def stop_timing() -> dict:
 _BINDING = {"layer_norm": "bzpf_layernorm", "layer_norm_bwd": "bzpf_layernorm_bwd", "dropout": "bzpf_dropout",
             "dropout_add_ln": "bzpf_dropout_add_ln", "dropout_add_ln_bwd": "bzpf_dropout_add_ln_bwd",
             "grad_layer_norm": "bzpf_layernorm", "grad_dropout": "bzpf_dropout",
-            "grad_dropout_add_ln": "bzpf_dropout_add_ln"}
+            "grad_dropout_add_ln": "bzpf_dropout_add_ln", "rel_bias": "bzpf_rel_bias", "rel_bias_bwd": "bzpf_rel_bias_bwd",
+            "grad_rel_bias": "bzpf_rel_bias", "qk_norm_rope": "bzpf_qk_norm_rope", "qk_norm_rope_bwd": "bzpf_qk_norm_rope_bwd",
+            "grad_qk_norm_rope": "bzpf_qk_norm_rope", "attention": "bzpf_attention", "attention_bwd": "bzpf_attention_bwd",
+            "grad_attention": "bzpf_attention"}
 
 
 def call(name: str, *args):
@@ -303,6 +306,93 @@ def dropout_add_ln_bwd(dz_new, dln: torch.Tensor, z_new: torch.Tensor, weight, e
     None where not needed)."""
     return call("dropout_add_ln_bwd", dz_new, dln, z_new, weight, eps, p, rng, site,
                 _shared("dropout_add_ln_bwd", shared), y_dtype, need_weight, need_bias)
+
+
+class RelBuckets(NamedTuple):
+    """The buckets of a relative position bias (rel_buckets makes it): the bucket of distance lo + i is lut[i], of distances
+    past its ends that of the end; the last of the `count` buckets is for pairs of different groups where `other`."""
+
+    lut: torch.Tensor
+    lo: int
+    count: int
+    other: bool
+
+
+def rel_buckets(edges, other: bool = False, device="cuda") -> RelBuckets:
+    """Buckets between the integers `edges` (rising): a distance pos_q - pos_k lies in the bucket with the number of edges at
+    or below it, so that clipped_edges(32) gives each distance from -32 to 32 its own and those beyond the last ones; one more
+    bucket for pairs of different groups (chains) where `other`. At most 256 buckets, edges at most 16384 apart."""
+    edges = [int(e) for e in edges]
+    if any(b <= a for a, b in zip(edges, edges[1:])):
+        raise ValueError("rel_buckets: edges must rise")
+    count = len(edges) + 1 + bool(other)
+    lo, hi = (edges[0] - 1, edges[-1]) if edges else (0, 0)
+    if count > 256 or hi - lo >= 16384:
+        raise ValueError(f"rel_buckets: at most 256 buckets over 16384 distances, got {count} over {hi - lo + 1}")
+    lut, k = [], 0
+    for d in range(lo, hi + 1):
+        k += k < len(edges) and edges[k] <= d
+        lut.append(k)
+    return RelBuckets(torch.tensor(lut, dtype=torch.uint8, device=device), lo, count, bool(other))
+
+
+def clipped_edges(reach: int) -> list:
+    """Edges of 2 * reach + 1 buckets: one for each distance from -reach to reach, those beyond in the last ones."""
+    return list(range(1 - reach, reach + 1))
+
+
+def rel_bias(table: torch.Tensor, buckets: RelBuckets, pos_q, pos_k=None, group_q=None, group_k=None, add=None,
+             out_dtype=None) -> torch.Tensor:
+    """The learned relative position bias [H, N, M]: table[bucket of pos_q[i] - pos_k[j]][h], plus `add` (a pair bias of the
+    output's shape and type) where given. table [buckets.count, H]; pos_q [N] and pos_k [M] (default: pos_q's) int32 or int64,
+    or [B, N] and [B, M] for a batch ([B, H, N, M]; a one-dimensional one is shared); group_q and group_k of their shapes say
+    which chain a token is in (they count where the buckets have one for other groups). out_dtype: default add's type, else
+    the table's. Its gradient: rel_bias_bwd, or boltz_mlx_amd.autograd.rel_bias. The positions' absolute values stay below
+    2^62."""
+    return call("rel_bias", table, *buckets, pos_q, pos_k, group_q, group_k, add, out_dtype)
+
+
+def rel_bias_bwd(dbias: torch.Tensor, buckets: RelBuckets, pos_q, pos_k=None, group_q=None, group_k=None) -> torch.Tensor:
+    """The table's gradient [buckets.count, H] (fp32) for the bias's (add's gradient is dbias itself)."""
+    return call("rel_bias_bwd", dbias, *buckets, pos_q, pos_k, group_q, group_k)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, w_q, w_k, H: int, pos=None, eps: float = 1e-5, base: float = 10000.0,
+                 rotary=None, interleaved: bool = False, out_dtype=None):
+    """Queries q [.., H * C] and keys k [.., Hk * C] (views of a fused projection's rows as they are) with each head divided by
+    the root of its mean square (plus eps) and scaled by w_q / w_k [C] (None: ones), then rotated by its token's position: pair
+    p of the first `rotary` channels (default all C) by pos * base^(-2p / rotary); its channels are p and p + rotary / 2, or 2p
+    and 2p + 1 where `interleaved`. pos: int32 or int64 for each row, or for each of the last ones ([N]); None: no rotation.
+    C even, up to 256; fp32 / fp16 / bf16 in and out (not fp16 with bf16). Returns (q, k), contiguous, in out_dtype (default
+    q's). Their gradients: qk_norm_rope_bwd, or boltz_mlx_amd.autograd.qk_norm_rope."""
+    return call("qk_norm_rope", q, k, w_q, w_k, H, pos, eps, base, rotary, interleaved, out_dtype)
+
+
+def qk_norm_rope_bwd(dqn: torch.Tensor, dkn: torch.Tensor, q: torch.Tensor, k: torch.Tensor, w_q, w_k, H: int, pos=None,
+                     eps: float = 1e-5, base: float = 10000.0, rotary=None, interleaved: bool = False,
+                     need_weights: bool = True):
+    """The gradients of qk_norm_rope for those of its outputs: (dq, dk in q's type, dw_q, dw_k in fp32; None where not
+    needed)."""
+    return call("qk_norm_rope_bwd", dqn, dkn, q, k, w_q, w_k, H, pos, eps, base, rotary, interleaved, need_weights)
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, H: int, g=None, bias=None, mask=None,
+              multiplicity: int = 1):
+    """seq_attention's training form, for any lengths: (out, stats) with out = sigmoid(g) * softmax(q k^T / sqrt(C) + bias) v
+    over the keys with mask != 0 (over all of them in a sample that has none; a row whose logits are all -inf gives 0), and
+    stats, what attention_bwd needs: fp32 [(S,) H, N, 2], each row's largest logit and the sum of exp(logit - that).
+    q, g [(S,) N, H * C] and k, v [(S,) M, H * C] (views of a fused projection's rows as they are), fp32, fp16 or bf16, C a
+    multiple of 8 up to 128; bias [(S / multiplicity,) H, N, M] of q's type (or fp16 / bf16 with fp32 q), shared by consecutive
+    groups of `multiplicity` samples; mask fp32 [(S,) M]; g, bias and mask may be None. Differentiable form:
+    boltz_mlx_amd.autograd.attention."""
+    return call("attention", q, k, v, H, g, bias, mask, multiplicity)
+
+
+def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, H: int, out: torch.Tensor,
+                  stats: torch.Tensor, g=None, bias=None, mask=None, multiplicity: int = 1, need_bias: bool = True):
+    """The gradients of attention at its output and stats: (dq, dk, dv, dg in q's type, dbias in the bias's, summed over the
+    samples that share it); dg and dbias None where there is none."""
+    return call("attention_bwd", dout, q, k, v, H, out, stats, g, bias, mask, multiplicity, need_bias)
 
 
 def count_nonfinite(*tensors: torch.Tensor) -> torch.Tensor:

@@ -17,6 +17,7 @@ from typing import Optional
 
 import torch
 
+from boltz_mlx_amd import autograd as A
 from boltz_mlx_amd import kernels as K
 from boltz_mlx_amd.layers.norm import LayerNorm
 
@@ -93,6 +94,41 @@ class AttentionPairBias(torch.nn.Module):
             self.fused(s[b].float().contiguous(), k_in[b].float().contiguous(), bias, mask[b], out[b],
                        accumulate=False)
         return out
+
+    def with_grad(self, s: torch.Tensor, z: Optional[torch.Tensor], mask: torch.Tensor, k_in: Optional[torch.Tensor] = None,
+                  multiplicity: int = 1, pair_bias: Optional[torch.Tensor] = None, qk_norm=None, rel_bias=None, pos=None,
+                  chain=None) -> torch.Tensor:
+        """The update [B, N, c_s] with gradients for s, k_in, z or pair_bias, and the parameters, in s's type (fp32, fp16 or
+        bf16; forward() carries none): torch's products around the attention kernels. Arguments as in forward(); k_in: s by
+        default; z [B / multiplicity, N, M, c_z], or pair_bias [B / multiplicity, H, N, M], or neither. qk_norm and rel_bias
+        (QKNorm and RelativeBias of layers.positions) add the tokens' positions pos and chains chain ([N] or [B, N]; the
+        samples of a group share its first one's bias): queries and keys are the same tokens then."""
+        linear, t = torch.nn.functional.linear, s.dtype
+        B, N, _ = s.shape
+        projs = (self.proj_q, self.proj_k, self.proj_v, self.proj_g)
+        if k_in is None or k_in is s:
+            x = linear(s, torch.cat([p.weight for p in projs]).to(t))
+            q, k, v, g = x.chunk(4, -1)
+            q = q + self.proj_q.bias.to(t)
+        else:
+            q, g = linear(s, self.proj_q.weight.to(t), self.proj_q.bias.to(t)), linear(s, self.proj_g.weight.to(t))
+            k, v = (linear(k_in.to(t), p.weight.to(t)) for p in (self.proj_k, self.proj_v))
+        bias = pair_bias
+        if bias is None and z is not None:
+            if self.compute_pair_bias:
+                z = linear(self.proj_z[0].with_grad(z, out_dtype=t), self.proj_z[1].weight.to(t))
+            bias = z.permute(0, 3, 1, 2)
+        bias = None if bias is None else bias.to(t)
+        if qk_norm is not None:
+            q, k = qk_norm(q, k, pos)
+        if rel_bias is not None:
+            share = pos if pos.dim() == 1 else pos[::multiplicity]
+            chains = chain if chain is None or chain.dim() == 1 else chain[::multiplicity]
+            bias = rel_bias(share, chains, add=bias, out_dtype=t)
+            if bias.dim() == 3:
+                bias = bias.expand(B // multiplicity, -1, -1, -1)
+        o = A.attention(q, k, v, self.num_heads, g=g, bias=bias, mask=mask.to(torch.float32), multiplicity=multiplicity)
+        return linear(o, self.proj_o.weight.to(t))
 
     def fused(self, s: torch.Tensor, k_in: torch.Tensor, bias: torch.Tensor, mask: torch.Tensor, out: torch.Tensor,
               accumulate: bool = True) -> None:

@@ -389,6 +389,69 @@ int bzpf_pwa_avg(const void* wp, int64_t ldw, const float* v, int64_t ldv, const
 int bzpf_pair_bias(const float* z, const float* ln_w, const float* ln_b, float eps, const void* w, void* out, int dt,
                    int64_t rows, int D, int H, void* stream);
 
+/* ---- The sequence attention's training form. Pointers at element alignment, fp32 / fp16 / bf16; outputs are buffers of their
+ * own (an overlap with another argument is refused). The reference has none of these: it runs inference only, and its
+ * attention takes no positions (boltz_mlx/layers/attentionv2.py:59-83). ---- */
+
+/* A learned relative position bias by buckets: out[b][h][i][j] = table[k][h] (+ add[b][h][i][j]) in dt, for table fp32
+ * [count][H] and add (or NULL) of out's type and shape [B][H][N][M]. k is the bucket of the pair's distance d = pos_q[i] -
+ * pos_k[j]: lut[d - lo], lut[0] below and lut[span - 1] above (lut uint8 [span] on the device, not falling, entries below
+ * count); where groups are given, pairs of different groups lie in bucket count - 1. pos_q / group_q [N], pos_k / group_k
+ * [M], int64 where wide, else int32, of absolute value below 2^62; batch element b's start b * batch_q (b * batch_k) elements
+ * on (0: shared). 1 <= count <= 256, 1 <= span <= 16384. */
+int bzpf_rel_bias(const float* table, const unsigned char* lut, int64_t lo, int span, int count, const void* pos_q,
+                  const void* pos_k, const void* group_q, const void* group_k, int wide, int64_t batch_q, int64_t batch_k,
+                  const void* add, void* out, int dt, int64_t B, int H, int64_t N, int64_t M, void* stream);
+
+/* The table's gradient: dtable [count][H] fp32, the sums of dout [B][H][N][M] (dt) over each bucket's pairs (add's gradient is
+ * dout itself). ws: bzpf_rel_bias_bwd_ws bytes (-1 for bad sizes). Sums are formed in a fixed order. */
+int64_t bzpf_rel_bias_bwd_ws(int64_t B, int H, int64_t N, int64_t M, int count);
+int bzpf_rel_bias_bwd(const void* dout, int dt, const unsigned char* lut, int64_t lo, int span, int count, const void* pos_q,
+                      const void* pos_k, const void* group_q, const void* group_k, int wide, int64_t batch_q,
+                      int64_t batch_k, float* dtable, float* ws, int64_t ws_bytes, int64_t B, int H, int64_t N, int64_t M,
+                      void* stream);
+
+/* Norms of queries and keys for each head with the position rotation: for each of `rows` tokens and each head of C channels
+ *   y = R(pos) (w * x / sqrt(mean(x^2) + eps))
+ * for q (H heads, w_q) and k (Hk heads, w_k; w fp32 [C] or NULL for ones), rows of pitch ldq / ldk in x_dt, outputs
+ * [rows][H C] and [rows][Hk C] in y_dt (not fp16 with bf16). R turns pair p of the first `rotary` channels by pos *
+ * base^(-2p / rotary); its channels are p and p + rotary / 2, or 2p and 2p + 1 where interleaved. Row r's position is pos[r %
+ * pos_rows] (int64 where wide, else int32); pos NULL: no rotation. C even, 2 to 256, rotary even, 0 to C. */
+int bzpf_qk_norm_rope(const void* q, int64_t ldq, const void* k, int64_t ldk, int x_dt, const float* w_q, const float* w_k,
+                      float eps, const void* pos, int wide, int64_t pos_rows, double base, int rotary, int interleaved,
+                      void* qn, void* kn, int y_dt, int64_t rows, int H, int Hk, int C, void* stream);
+
+/* Its gradients for those of its outputs, dqn and dkn ([rows][H C], [rows][Hk C] in y_dt): dq and dk (contiguous, x_dt), and
+ * dw_q, dw_k fp32 [C] (NULL where not wanted). ws: bzpf_qk_norm_rope_bwd_ws(C) bytes where a weight's gradient is wanted. */
+int64_t bzpf_qk_norm_rope_bwd_ws(int C);
+int bzpf_qk_norm_rope_bwd(const void* dqn, const void* dkn, int y_dt, const void* q, int64_t ldq, const void* k, int64_t ldk,
+                          int x_dt, const float* w_q, const float* w_k, float eps, const void* pos, int wide,
+                          int64_t pos_rows, double base, int rotary, int interleaved, void* dq, void* dk, float* dw_q,
+                          float* dw_k, float* ws, int64_t ws_bytes, int64_t rows, int H, int Hk, int C, void* stream);
+
+/* Sequence attention with the statistics that its backward pass needs, for S samples:
+ *   x[h][i][j] = q_i . k_j / sqrt(C) + bias[h][i][j] over the keys with mask[j] != 0 (all of them where the sample has none);
+ *   out[i][h C + c] = sigmoid(g[i][h C + c]) * sum_j softmax_j(x)[j] v[j][h C + c]   (0 for a row whose logits are all -inf).
+ * q, g [S][N] and k, v [S][M] are rows of H heads of C channels (C a multiple of 8, 8 to 128) of pitch ld*, samples s*
+ * elements apart, in dt; g NULL: no gate. bias (or NULL) [S / mult][H][N][M] in bias_dt (dt, or fp16 / bf16 with fp32
+ * operands), shared by consecutive groups of mult samples; mask (or NULL) fp32 [S][M]. out [S][N][H C] in dt; stats fp32
+ * [S][H][N][2]: a row's largest logit and the sum of exp(logit - that). What bzpf_seq_attention_batched computes, for any N
+ * and M, in bf16 too. */
+int bzpf_attention(const void* q, int64_t ldq, int64_t sq, const void* k, int64_t ldk, int64_t sk, const void* v, int64_t ldv,
+                   int64_t sv, const void* g, int64_t ldg, int64_t sg, const void* bias, int bias_dt, int mult,
+                   const float* mask, void* out, float* stats, int dt, int S, int H, int C, int64_t N, int64_t M,
+                   void* stream);
+
+/* Its gradients for dout [S][N][H C] (dt, contiguous) at its output and statistics: dq, dk, dv, dg contiguous in dt (dg NULL
+ * where g is), dbias in bias_dt (NULL where not wanted), summed over the samples that share it. ws: bzpf_attention_bwd_ws
+ * bytes (gate: g is given), 16-byte aligned. No atomics: equal inputs give equal bits. */
+int64_t bzpf_attention_bwd_ws(int dt, int S, int H, int C, int64_t N, int64_t M, int gate);
+int bzpf_attention_bwd(const void* dout, const void* q, int64_t ldq, int64_t sq, const void* k, int64_t ldk, int64_t sk,
+                       const void* v, int64_t ldv, int64_t sv, const void* g, int64_t ldg, int64_t sg, const void* bias,
+                       int bias_dt, int mult, const float* mask, const void* out, const float* stats, void* dq, void* dk,
+                       void* dv, void* dg, void* dbias, void* ws, int64_t ws_bytes, int dt, int S, int H, int C, int64_t N,
+                       int64_t M, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
