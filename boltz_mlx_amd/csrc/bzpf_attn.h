@@ -5,6 +5,8 @@
 // k in the same order, so that the sum over the step is the same). An accumulator holds D[8 (i / 4) + 4 (lane / 32) + i % 4]
 // [lane % 32], i = 0..15, which is the fragment layout of the next product's second operand with its k in the order
 // 16 s + {4 hl .. 4 hl + 3, 8 + 4 hl .. 8 + 4 hl + 3}: probabilities never leave their lanes.
+// Where the keys are an accumulator's rows (forward, dq), a tile's LDS rows hold them in the order that gives a lane's i-th
+// element key 16 hl + i: a lane's 16 biases are then neighbours in memory.
 #pragma once
 
 #include <type_traits>
@@ -16,6 +18,82 @@
 namespace bzpf {
 
 constexpr float LOG2E = 1.4426950408889634f;
+
+// A row's exponentials are 2^(x by - at) for by = log2 e and at = top by rounded: one instruction before the exponential. What
+// the rounding of at is worth, 2^-off(), is put right once for a row. From 2^100 on two logits are equal or 2^76 apart, and
+// by = 2^-64 says as much without overflow: a row whose logits are all the type's lowest value is a softmax over equals. A row
+// without logits (top = -inf) has at = 0 and exponentials of 0.
+struct Exponent {
+  float by, at;
+  __device__ __forceinline__ Exponent() {}
+  __device__ __forceinline__ explicit Exponent(float top) {
+    by = __builtin_fabsf(top) > 0x1p100f ? 0x1p-64f : LOG2E;
+    at = top == -INFINITY ? 0.f : top * by;
+  }
+  __device__ __forceinline__ float of(float x) const { return __builtin_amdgcn_exp2f(fmaf(x, by, -at)); }
+  __device__ __forceinline__ float off(float top) const { return top == -INFINITY ? 0.f : fmaf(top, by, -at); }
+};
+
+// How a launch's waves work (attn_form chooses): in the wide form the four waves of a workgroup hold 32 rows each and share
+// tiles of the other side's rows, in two buffers; in the split form they hold the same 32 rows, each with every fourth block
+// of the other side and tiles of its own (no barrier: a wave's LDS accesses keep their order), and meet at the end.
+template <typename T, bool SPLIT>
+struct Form {
+  static constexpr int NW = SPLIT ? 1 : 4, GROUPS = SPLIT ? 4 : 1, NTH = 64 * NW, ROWS = 32 * NW;
+  static constexpr int BR = SPLIT || sizeof(T) == 4 ? 32 : 64, BUFS = SPLIT ? 1 : 2;
+  // Between a tile's writes and its reads. Two buffers: the other one's readers passed the barrier before, this one's next
+  // writer passes the next one.
+  static __device__ __forceinline__ void sync() {
+    if constexpr (SPLIT) order();
+    else __syncthreads();
+  }
+  // Between a tile's reads and its next writes.
+  static __device__ __forceinline__ void again() {
+    if constexpr (SPLIT) order();
+  }
+  static __device__ __forceinline__ void order() {  // of a wave's own LDS accesses: the compiler is to keep it
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+};
+
+// Split where 128-row workgroups would not give two to each compute unit; heads past 96 channels have the wide form alone
+// (their split form needs more registers than there are).
+constexpr int SPLIT_STEPS = 6;
+static inline bool attn_split(int64_t rows, const Attn& a) {
+  return a.C <= 16 * SPLIT_STEPS && (rows + 127) / 128 * a.S * a.H < 512;
+}
+// Calls fn(true_type) or fn(false_type) for it.
+template <int KS, typename Fn>
+static inline hipError_t with_split(int64_t rows, const Attn& a, Fn&& fn) {
+  if constexpr (KS <= SPLIT_STEPS) {
+    if (attn_split(rows, a)) return fn(std::true_type());
+  }
+  return fn(std::false_type());
+}
+
+// The sum over the four waves of a split workgroup of what each has in acc[NT] (a 32 x 32 tile each), for the accumulator rows
+// 8 w .. 8 w + 7 of wave w: its part of the result, 4 elements for each of the tiles. `scale`: each wave's factor for its own.
+template <int NT>
+__device__ __forceinline__ void meet4(const f16x (&acc)[NT], f4* lds, int wave, int l, float scale, f4 (&out)[NT]) {
+  __syncthreads();  // the area's last readers are done
+#pragma unroll
+  for (int tt = 0; tt < NT; tt++)
+#pragma unroll
+    for (int qq = 0; qq < 4; qq++) {
+      f4 v;
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = acc[tt][4 * qq + e] * scale;
+      lds[((wave * NT + tt) * 4 + qq) * 64 + l] = v;
+    }
+  __syncthreads();
+#pragma unroll
+  for (int tt = 0; tt < NT; tt++) {
+    const f4* const p = lds + (tt * 4 + wave) * 64 + l;
+    out[tt] = (p[0] + p[NT * 256]) + (p[2 * NT * 256] + p[3 * NT * 256]);
+  }
+}
 
 template <typename T> struct Frag { typedef T V __attribute__((ext_vector_type(8))); };
 template <typename T> using frag = typename Frag<T>::V;
@@ -73,6 +151,15 @@ __device__ __forceinline__ frag<T> col_frag(const T* tile, int row0, int tt) {
   return f;
 }
 
+constexpr __host__ __device__ uint64_t all_rows(int n) { return n >= 64 ? ~0ull : (1ull << n) - 1; }
+
+// p and a 32-bit byte offset: with a wave-uniform p both are operands of the load itself.
+template <typename T>
+__device__ __forceinline__ T* at_byte(T* p, uint32_t bytes) {
+  typedef std::conditional_t<std::is_const_v<T>, const char, char> B;
+  return reinterpret_cast<T*>(reinterpret_cast<B*>(p) + bytes);
+}
+
 // 8 elements of a row in memory, at element alignment.
 template <typename T>
 __device__ __forceinline__ frag<T> load8(const T* p) {
@@ -83,41 +170,164 @@ __device__ __forceinline__ frag<T> load8(const T* p) {
 // BR rows of a [rows][C] operand on their way from memory to a tile: loads are issued by load() and end in store(), a block
 // of work later. Rows past the end are read at the last one and stored as zeros, as are those that `keep` leaves out
 // (bit r: row r), so that nothing of theirs, infinite or NaN, meets a zero probability; so are the channels past C.
-template <typename T, int KS, int BR, int NTH>
+// Addresses are a wave's own base and a lane's 32-bit byte offset (one instruction's own operands): row pitches are below 2^23.
+// KEYS: rows in the order of an accumulator's rows, as above.
+template <typename T, int KS, int BR, int NTH, bool KEYS>
 struct Stage {
   static constexpr int TOTAL = BR * 2 * KS, NV = (TOTAL + NTH - 1) / NTH;
   frag<T> r[NV];
-  __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t row0, int64_t rows, int C) {
+  // base: the first row; left: rows from it on (at least one); t: the thread's number among NTH
+  __device__ __forceinline__ void load(const T* base, uint32_t ld, int64_t left, int C, int t) {
+    const int last = left < BR ? (int)left - 1 : BR - 1;
 #pragma unroll
     for (int n = 0; n < NV; n++) {
-      const int e = threadIdx.x + NTH * n, c = 8 * (e % (2 * KS));
-      const int64_t row = min(row0 + min(e / (2 * KS), BR - 1), rows - 1);
-      r[n] = load8(base + row * ld + (c < C ? c : 0));
+      const int e = t + NTH * n, c = 8 * (e % (2 * KS));
+      r[n] = load8(at_byte(base, ((uint32_t)min(e / (2 * KS), last) * ld + (c < C ? c : 0)) * (uint32_t)sizeof(T)));
     }
   }
-  __device__ __forceinline__ void store(T* tile, uint64_t keep, int C) const {
+  __device__ __forceinline__ void store(T* tile, uint64_t keep, int C, int t) const {
 #pragma unroll
     for (int n = 0; n < NV; n++) {
-      const int e = threadIdx.x + NTH * n, row = e / (2 * KS), c = 8 * (e % (2 * KS));
+      const int e = t + NTH * n, row = e / (2 * KS), c = 8 * (e % (2 * KS));
       if (TOTAL % NTH && e >= TOTAL) break;
-      const bool on = c < C && (keep >> row & 1);
-      *reinterpret_cast<frag<T>*>(tile + row * TILE_LD<T, KS> + c) = on ? r[n] : frag<T>{};
+      const bool on = c < C && (keep == all_rows(BR) || (keep >> row & 1));
+      const int at = KEYS ? (row & ~31) + 8 * (row >> 2 & 3) + 4 * (row >> 4 & 1) + (row & 3) : row;
+      *reinterpret_cast<frag<T>*>(tile + at * TILE_LD<T, KS> + c) = on ? r[n] : frag<T>{};
     }
   }
 };
 
-// Four consecutive bias elements of a row, of which n (4 and more: all) exist.
+typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+
+// 16 bytes of a row, of which the first n elements (a whole chunk: any n past it) exist; the others are zero.
 template <typename BT>
-struct Bias4 {
-  typedef BT V __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u4 load_part(const BT* p, int64_t n) {
+  constexpr int E = 16 / (int)sizeof(BT);
+  typedef BT V __attribute__((ext_vector_type(E)));
   V v;
-  __device__ __forceinline__ void load(const BT* p) {
-    typedef BT U __attribute__((ext_vector_type(4), aligned(sizeof(BT))));
-    v = *reinterpret_cast<const U*>(p);
-  }
-  __device__ __forceinline__ void load(const BT* p, int64_t n) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) v[e] = e < n ? p[e] : (BT)0.f;
+  for (int e = 0; e < E; e++) v[e] = e < n ? p[e] : (BT)0.f;
+  return __builtin_bit_cast(u4, v);
+}
+template <typename BT>
+__device__ __forceinline__ u4 load_all(const BT* p) {
+  typedef BT U __attribute__((ext_vector_type(16 / sizeof(BT)), aligned(sizeof(BT))));
+  return __builtin_bit_cast(u4, *reinterpret_cast<const U*>(p));
+}
+
+// The biases of a wave's 32 rows against BK keys, on their way through LDS: from memory in whole rows (a lane for each row
+// would take 32 lines an instruction: 220 us instead of XX for 4096 x 4096 and 16 heads), to the lanes that own the rows.
+// 16-byte pieces lie at places that keep the lanes' reads of one column on different banks.
+template <typename BT, int BK>
+struct BiasRows {
+  static constexpr int CPR = BK * (int)sizeof(BT) / 16, NV = 32 * CPR / 64, E = 16 / (int)sizeof(BT), BYTES = 32 * CPR * 16;
+  u4 r[NV];
+  static __device__ __forceinline__ int place(int row, int c) {
+    return row * CPR + (CPR == 8 ? c ^ (row & 7) : c ^ (row >> 1 & 3));
+  }
+  // base: the wave's first row, at the first key; rows: those of the 32 that exist (at least one); left: keys from there on
+  __device__ __forceinline__ void load(const BT* base, int rows, int64_t M, int64_t left) {
+    const int l = threadIdx.x & 63;
+#pragma unroll
+    for (int n = 0; n < NV; n++) {
+      const int id = l + 64 * n, c = id % CPR;
+      const BT* const p = at_byte(base, ((uint32_t)min(id / CPR, rows - 1) * (uint32_t)M + c * E) * (uint32_t)sizeof(BT));
+      r[n] = left >= BK ? load_all(p) : load_part(p, left - c * E);
+    }
+  }
+  __device__ __forceinline__ void store(u4* lds) const {
+    const int l = threadIdx.x & 63;
+#pragma unroll
+    for (int n = 0; n < NV; n++) lds[place((l + 64 * n) / CPR, (l + 64 * n) % CPR)] = r[n];
+  }
+  // The lane's 16 of tile kt.
+  static __device__ __forceinline__ f16x get(const u4* lds, int kt) {
+    typedef BT V __attribute__((ext_vector_type(E)));
+    const int l = threadIdx.x & 63;
+    f16x x;
+#pragma unroll
+    for (int p = 0; p < 16 / E; p++) {
+      const V v = __builtin_bit_cast(V, lds[place(l & 31, (32 * kt + 16 * (l >> 5)) / E + p)]);
+#pragma unroll
+      for (int e = 0; e < E; e++) x[p * E + e] = (float)v[e];
+    }
+    return x;
+  }
+};
+
+// A 32 x 32 tile of half-type biases whose columns are the lanes (dk and dv), through LDS as above and out of it with the
+// transposing reads; and the tile of their gradients, the other way.
+template <typename BT>
+struct BiasTile {
+  static constexpr int BYTES = 2048;
+  u4 r[2];
+  __device__ __forceinline__ void load(const BT* base, int rows, int64_t M, int64_t left) {
+    const int l = threadIdx.x & 63, c = 8 * (l & 3);
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+      const BT* const p = at_byte(base, ((uint32_t)min((l >> 2) + 16 * n, rows - 1) * (uint32_t)M + c) * 2u);
+      r[n] = left >= 32 ? load_all(p) : load_part(p, left - c);
+    }
+  }
+  __device__ __forceinline__ void store(u4* lds) const {
+    const int l = threadIdx.x & 63;
+    lds[l] = r[0];
+    lds[64 + l] = r[1];
+  }
+  // The lane's elements of rows 8 qq + 4 hl .. + 3.
+  static __device__ __forceinline__ f4 get(const u4* lds, int qq) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef BT V __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4* lds4;
+    const int l = threadIdx.x & 63;
+    const BT* const p = reinterpret_cast<const BT*>(lds) + (8 * qq + 4 * (l >> 5) + ((l & 15) >> 2)) * 32 + 16 * ((l >> 4) & 1) + 4 * (l & 3);
+    return __builtin_convertvector(__builtin_bit_cast(V, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p)), f4);
+  }
+  static __device__ __forceinline__ void put(u4* lds, int i, float x) {
+    const int l = threadIdx.x & 63;
+    reinterpret_cast<BT*>(lds)[(8 * (i >> 2) + 4 * (l >> 5) + (i & 3)) * 32 + (l & 31)] = (BT)x;
+  }
+  // The tile to memory: `rows` of its rows, `left` of its columns.
+  static __device__ __forceinline__ void write(const u4* lds, BT* base, int rows, int64_t M, int64_t left) {
+    typedef BT V __attribute__((ext_vector_type(8)));
+    typedef BT U __attribute__((ext_vector_type(8), aligned(sizeof(BT))));
+    const int l = threadIdx.x & 63, c = 8 * (l & 3);
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+      const int row = (l >> 2) + 16 * n;
+      if (row >= rows) continue;
+      BT* const p = at_byte(base, ((uint32_t)row * (uint32_t)M + c) * 2u);
+      const V x = __builtin_bit_cast(V, lds[64 * n + l]);
+      if (left >= 32) {
+        *reinterpret_cast<U*>(p) = x;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (c + e < left) p[e] = x[e];
+      }
+    }
+  }
+};
+
+// Rows of an fp32 matrix tile whose columns are a wave's lanes, a row an instruction: the tile is a buffer, the row's offset the
+// instruction's scalar one, so that an access costs no address arithmetic. Past the buffer's end loads give 0 and stores drop.
+struct Columns {
+  __amdgpu_buffer_rsrc_t rsrc;
+  uint32_t pitch;  // bytes
+  // base: the tile's first row; rows: those of it that exist
+  __device__ __forceinline__ Columns(const float* base, int rows, int64_t M)
+      : rsrc(__builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)(rows * M * 4), 0x00020000)), pitch((uint32_t)M * 4) {}
+  // lane: byte offset of the lane's first row and column; r: the row from there; whole: every row of the tile exists (else the
+  // row has to be in the lane's offset, which the range check covers: 16 of them, not to be kept over a loop)
+  __device__ __forceinline__ float get(uint32_t lane, int r, bool whole) const {
+    if (!whole) asm volatile("" : "+v"(lane));
+    return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, whole ? (int)lane : (int)(lane + r * pitch),
+                                                                whole ? (int)(r * pitch) : 0, 0));
+  }
+  __device__ __forceinline__ void put(uint32_t lane, int r, bool whole, float x) const {
+    if (!whole) asm volatile("" : "+v"(lane));
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), rsrc, whole ? (int)lane : (int)(lane + r * pitch),
+                                          whole ? (int)(r * pitch) : 0, 0);
   }
 };
 
@@ -132,11 +342,10 @@ __device__ __forceinline__ float both_sum(float v) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-// Whether the mask leaves the sample a key: one without keys runs without its mask.
-template <int NTH>
+// Whether the mask leaves the sample a key (256 threads): one without keys runs without its mask.
 __device__ __forceinline__ bool any_key(const float* mask, int64_t M) {
   if (!mask) return true;
-  for (int64_t k = 0; k < M; k += NTH) {
+  for (int64_t k = 0; k < M; k += 256) {
     const int64_t at = k + threadIdx.x;
     if (__syncthreads_or(at < M && mask[at] != 0.0f)) return true;
   }
@@ -158,13 +367,10 @@ __device__ __forceinline__ bool unit_of(const Attn& a, int64_t blocks, int64_t p
   return true;
 }
 
-constexpr uint64_t all_rows(int n) { return n >= 64 ? ~0ull : (1ull << n) - 1; }
-
 // Calls fn(T, BT, KS) with the types of q and of the bias and the number of 16-channel steps.
 template <typename Fn>
 static inline hipError_t with_attn(const Attn& a, Fn&& fn) {
   const auto steps = [&](auto t, auto b) {
-    if (a.C <= 16) return fn(t, b, std::integral_constant<int, 1>());
     if (a.C <= 32) return fn(t, b, std::integral_constant<int, 2>());
     if (a.C <= 48) return fn(t, b, std::integral_constant<int, 3>());
     if (a.C <= 64) return fn(t, b, std::integral_constant<int, 4>());

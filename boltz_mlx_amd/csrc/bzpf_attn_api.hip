@@ -212,6 +212,8 @@ int bzpf_qk_norm_rope_bwd(const void* dqn, const void* dkn, int y_dt, const void
 
 namespace {
 
+constexpr int64_t ATT_LEN = 1 << 22, ATT_PITCH = 1 << 23;  // what the kernels' 32-bit offsets within a block hold
+
 int make_attn(const char* who, const void* q, int64_t ldq, int64_t sq, const void* k, int64_t ldk, int64_t sk, const void* v,
               int64_t ldv, int64_t sv, const void* g, int64_t ldg, int64_t sg, const void* bias, int bias_dt, int mult,
               const float* mask, const void* out, const float* stats, int dt, int S, int H, int C, int64_t N, int64_t M,
@@ -222,17 +224,16 @@ int make_attn(const char* who, const void* q, int64_t ldq, int64_t sq, const voi
   REQUIRE(C >= 8 && C <= 128 && C % 8 == 0, "%s: heads of 8 to 128 channels, a multiple of 8 (C=%d)", who, C);
   REQUIRE(S >= 1 && H >= 1 && H <= 65535 && mult >= 1 && S % mult == 0, "%s: bad sample or head counts (S=%d H=%d mult=%d)",
           who, S, H, mult);
-  REQUIRE(N >= 1 && M >= 1 && N <= INT32_MAX && M <= INT32_MAX && product(S, H, N, M) >= 0 && product(S, N > M ? N : M, H, 4 * C) >= 0,
-          "%s: bad sizes (N=%lld M=%lld)", who, (long long)N, (long long)M);
+  REQUIRE(N >= 1 && M >= 1 && N <= ATT_LEN && M <= ATT_LEN && product(S, H, N, M) >= 0 && product(S, N > M ? N : M, H, 4 * C) >= 0,
+          "%s: 1 to 2^22 queries and keys (N=%lld M=%lld)", who, (long long)N, (long long)M);
   REQUIRE(q && k && v && out && stats, "%s: NULL pointer", who);
   for (const void* p : {q, k, v, g, out}) REQUIRE(aligned_el(p, dt), "%s: a tensor is misaligned", who);
   REQUIRE(aligned_el(bias, bias_dt) && aligned_el(mask, BZPF_F32) && aligned_el(stats, BZPF_F32), "%s: a tensor is misaligned", who);
   const int64_t w = (int64_t)H * C;
   REQUIRE((N == 1 || (ldq >= w && (!g || ldg >= w))) && (M == 1 || (ldk >= w && ldv >= w)), "%s: row pitches below a row's width", who);
+  for (int64_t l : {w, ldq, ldk, ldv, ldg}) REQUIRE(l >= 0 && l < ATT_PITCH, "%s: rows of fewer than 2^23 elements", who);
   REQUIRE(sq >= 0 && sk >= 0 && sv >= 0 && sg >= 0, "%s: negative sample strides", who);
   for (int64_t s : {sq, sk, sv, sg}) REQUIRE(product(S, s, 4, 1) >= 0, "%s: bad strides", who);
-  for (int64_t l : {ldq, ldg}) REQUIRE(l >= 0 && product(N, l, 4, 1) >= 0, "%s: bad strides", who);
-  for (int64_t l : {ldk, ldv}) REQUIRE(l >= 0 && product(M, l, 4, 1) >= 0, "%s: bad strides", who);
   *a = bzpf::Attn{};
   a->q = q, a->k = k, a->v = v, a->g = g, a->bias = bias, a->mask = mask;
   a->ldq = ldq, a->ldk = ldk, a->ldv = ldv, a->ldg = ldg, a->sq = sq, a->sk = sk, a->sv = sv, a->sg = sg;
@@ -263,7 +264,7 @@ int bzpf_attention(const void* q, int64_t ldq, int64_t sq, const void* k, int64_
 }
 
 int64_t bzpf_attention_bwd_ws(int dt, int S_, int H, int C, int64_t N, int64_t M, int gate) {
-  if (!dt3_ok(dt) || S_ < 1 || H < 1 || H > 65535 || C < 8 || C > 128 || C % 8 || N < 1 || N > INT32_MAX || M < 1 || M > INT32_MAX ||
+  if (!dt3_ok(dt) || S_ < 1 || H < 1 || H > 65535 || C < 8 || C > 128 || C % 8 || N < 1 || N > ATT_LEN || M < 1 || M > ATT_LEN ||
       product(S_, N > M ? N : M, H, 4 * C) < 0)
     return -1;
   return bzpf::attention_bwd_ws_bytes(dt, S_, N, H, C, gate != 0);

@@ -54,41 +54,51 @@ __global__ __launch_bounds__(256) void attn_rows_k(Attn a, int L) {
   if (on && l == 0) a.delta[(smp * a.H + h) * a.N + row - smp * a.N] = d;
 }
 
-// A row's maximum (0 for a row without logits, whose probabilities are exp(-inf)) and the sum's reciprocal (0 for it).
+// What a row's probabilities and their gradients need: p = 2^(x by - at) inv.
 struct RowStat {
-  float top, inv, delta;
+  Exponent ex;
+  float inv, delta;
   __device__ __forceinline__ RowStat(const Attn& a, int64_t row) {
-    const float m = a.stats[2 * row], s = a.stats[2 * row + 1];
-    top = m == -INFINITY ? 0.f : m;
-    inv = s == 0.f ? 0.f : 1.0f / s;
+    const float top = a.stats[2 * row], sum = a.stats[2 * row + 1];
+    ex = Exponent(top);
+    inv = sum == 0.f ? 0.f : __builtin_amdgcn_exp2f(-ex.off(top)) / sum;
     delta = a.delta[row];
   }
 };
 
 // dq: a wave holds 32 queries as the columns of S^T, as the forward pass does. The sum's reciprocal is a row's own, so that it
 // scales dq at the end and ds is rounded before it. TWO: dO has a second part.
-template <typename T, typename BT, int KS, int NW, bool TWO>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_dq_k(Attn a, int64_t per_xcd) {
-  constexpr int BK = sizeof(T) == 2 ? 64 : 32, KT = BK / 32, NT = (KS + 1) / 2, NTH = 64 * NW, WQ = 32 * NW;
-  __shared__ LDS_ALIGN T Kt[2][BK * TILE_LD<T, KS>];
-  __shared__ LDS_ALIGN T Vt[2][BK * TILE_LD<T, KS>];
-  const int64_t qblocks = (a.N + WQ - 1) / WQ;
+template <typename T, typename BT, int KS, bool SPLIT, bool TWO>
+__global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_dq_k(Attn a, int64_t per_xcd) {
+  typedef Form<T, SPLIT> F;
+  constexpr int BK = F::BR, KT = BK / 32, NT = (KS + 1) / 2, TILE = BK * TILE_LD<T, KS>;
+  constexpr int TILES = F::GROUPS * F::BUFS * 2 * TILE * (int)sizeof(T), MEET = SPLIT ? 4 * NT * 4096 : 0;
+  constexpr bool MEND = sizeof(T) == 2;
+  __shared__ LDS_ALIGN char lds[TILES > MEET ? TILES : MEET];
+  __shared__ LDS_ALIGN char bias_lds[4 * BiasRows<BT, BK>::BYTES];
+  const int64_t qblocks = (a.N + F::ROWS - 1) / F::ROWS;
   Unit un;
   if (!unit_of(a, qblocks, per_xcd, &un)) return;  // whole workgroup
-  const int t = threadIdx.x, l = t & 63, hl = l >> 5;
-  const int64_t j = un.block * WQ + 32 * (t >> 6) + (l & 31), jc = min(j, a.N - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, hl = l >> 5;
+  const int t = SPLIT ? l : threadIdx.x, group = SPLIT ? wave : 0;
+  T* const Kt = reinterpret_cast<T*>(lds) + group * F::BUFS * 2 * TILE;
+  T* const Vt = Kt + F::BUFS * TILE;
+  const int64_t j0 = un.block * F::ROWS, j = j0 + (SPLIT ? 0 : 32 * wave) + (l & 31), jc = min(j, a.N - 1);
   const int hc = un.h * a.C;
   const T* const q = static_cast<const T*>(a.q) + un.smp * a.sq + jc * a.ldq + hc;
   const T* const k = static_cast<const T*>(a.k) + un.smp * a.sk + hc;
   const T* const v = static_cast<const T*>(a.v) + un.smp * a.sv + hc;
-  const T* const dO = static_cast<const T*>(a.dO) + (un.smp * a.N + jc) * a.H * a.C + hc;
-  const BT* const bias = a.bias ? static_cast<const BT*>(a.bias) + (((int64_t)(un.smp / a.mult) * a.H + un.h) * a.N + jc) * a.M : nullptr;
+  const int64_t orow = (un.smp * a.N + jc) * a.H * a.C + hc;
+  const T* const dO = static_cast<const T*>(a.dO) + orow;
+  const T* const dO_lo = TWO ? static_cast<const T*>(a.dO_lo) + orow : nullptr;
+  const int64_t b0 = min(j0 + (SPLIT ? 0 : 32 * wave), a.N - 1);  // the wave's first row
+  const BT* const bias = a.bias ? static_cast<const BT*>(a.bias) + (((int64_t)(un.smp / a.mult) * a.H + un.h) * a.N + b0) * a.M : nullptr;
+  const int brows = (int)min(a.N - b0, (int64_t)32);
+  u4* const Bt = reinterpret_cast<u4*>(bias_lds + wave * BiasRows<BT, BK>::BYTES);
   const float* mask = a.mask ? a.mask + un.smp * a.M : nullptr;
-  if (!any_key<NTH>(mask, a.M)) mask = nullptr;
-  const T* const dO_lo = TWO ? static_cast<const T*>(a.dO_lo) + (un.smp * a.N + jc) * a.H * a.C + hc : nullptr;
+  if (!any_key(mask, a.M)) mask = nullptr;
   const int64_t srow = ((int64_t)un.smp * a.H + un.h) * a.N + jc;
   const RowStat rs(a, srow);
-  constexpr bool MEND = sizeof(T) == 2;
 
   frag<T> qf[KS], df[KS], dl[TWO ? KS : 1];
 #pragma unroll
@@ -106,121 +116,154 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void at
     if constexpr (MEND) pk[tt] = f16x{};
   }
 
-  Stage<T, KS, BK, NTH> ks, vs;
-  Bias4<BT> bs[KT][4];
+  Stage<T, KS, BK, F::NTH, true> ks, vs;
+  BiasRows<BT, BK> bs;
   float mk = 1.f;
   const auto fetch = [&](int64_t k0) {
-    ks.load(k, a.ldk, k0, a.M, a.C);
-    vs.load(v, a.ldv, k0, a.M, a.C);
+    ks.load(k + k0 * a.ldk, (uint32_t)a.ldk, a.M - k0, a.C, t);
+    vs.load(v + k0 * a.ldv, (uint32_t)a.ldv, a.M - k0, a.C, t);
     if (mask) mk = mask[min(k0 + l, a.M - 1)];
   };
   const auto fetch_bias = [&](int64_t k0) {
-    if (!bias) return;
-#pragma unroll
-    for (int kt = 0; kt < KT; kt++)
-#pragma unroll
-      for (int qq = 0; qq < 4; qq++) {
-        const int64_t at = k0 + 32 * kt + 8 * qq + 4 * hl;
-        if (k0 + BK <= a.M) bs[kt][qq].load(bias + at);
-        else bs[kt][qq].load(bias + at, a.M - at);
-      }
+    if (bias) bs.load(bias + k0, brows, a.M, a.M - k0);
   };
-  fetch(0);
-  fetch_bias(0);
-  for (int64_t k0 = 0; k0 < a.M; k0 += BK) {
-    const int buf = (int)(k0 / BK & 1);
+  constexpr int STEP = F::GROUPS * BK;
+  int64_t k0 = group * BK;
+  if (k0 < a.M) {
+    fetch(k0);
+    fetch_bias(k0);
+  }
+  for (int buf = 0; k0 < a.M; k0 += STEP, buf = (buf + 1) % F::BUFS) {
     const uint64_t keep = __ballot(k0 + l < a.M && l < BK && mk != 0.f);
-    ks.store(Kt[buf], keep, a.C);
-    vs.store(Vt[buf], keep, a.C);
-    __syncthreads();  // as in the forward pass
-    const bool more = k0 + BK < a.M;
-    if (more) fetch(k0 + BK);
+    T* const Kb = Kt + buf * TILE;
+    T* const Vb = Vt + buf * TILE;
+    ks.store(Kb, keep, a.C, t);
+    vs.store(Vb, keep, a.C, t);
+    if (bias) bs.store(Bt);
+    F::sync();
+    const bool more = k0 + STEP < a.M;
+    if (more) {
+      fetch(k0 + STEP);
+      fetch_bias(k0 + STEP);
+    }
 #pragma unroll
     for (int kt = 0; kt < KT; kt++) {
       f16x x = f16x{}, dp = f16x{};
 #pragma unroll
       for (int m = 0; m < KS; m++) {
-        x = mma(row_frag<T, KS>(Kt[buf], 32 * kt + (l & 31), m), qf[m], x);
-        const frag<T> vm = row_frag<T, KS>(Vt[buf], 32 * kt + (l & 31), m);
+        x = mma(row_frag<T, KS>(Kb, 32 * kt + (l & 31), m), qf[m], x);
+        const frag<T> vm = row_frag<T, KS>(Vb, 32 * kt + (l & 31), m);
         dp = mma(vm, df[m], dp);
         if constexpr (TWO) dp = mma(vm, dl[m], dp);
       }
-      if (bias) {
-#pragma unroll
-        for (int i = 0; i < 16; i++) x[i] = fmaf(x[i], a.scale, (float)bs[kt][i >> 2].v[i & 3]);
-      } else {
-        x *= a.scale;
-      }
-      const uint32_t w = (uint32_t)(keep >> (32 * kt)) >> (4 * hl);
+      f16x b = f16x{};
+      if (bias) b = BiasRows<BT, BK>::get(Bt, kt);
 #pragma unroll
       for (int i = 0; i < 16; i++) {
-        const bool on = keep == all_rows(BK) || (w >> (8 * (i >> 2) + (i & 3)) & 1);
-        x[i] = on ? __builtin_amdgcn_exp2f((x[i] - rs.top) * LOG2E) : 0.f;
-        dp[i] = on ? x[i] * (dp[i] - rs.delta) : 0.f;
-        if constexpr (MEND) off += dp[i];
+        x[i] = rs.ex.of(fmaf(x[i], a.scale, b[i]));
+        dp[i] = x[i] * (dp[i] - rs.delta);
+      }
+      if (keep != all_rows(BK)) {
+        const uint32_t w = (uint32_t)(keep >> (32 * kt)) >> (16 * hl);
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const bool on = w >> i & 1;
+          x[i] = on ? x[i] : 0.f;
+          dp[i] = on ? dp[i] : 0.f;
+        }
+      }
+      if constexpr (MEND) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) off += dp[i];
       }
 #pragma unroll
       for (int s = 0; s < 2; s++) {
         const frag<T> d = as_frag<T>(dp, s), p = as_frag<T>(x, s);
 #pragma unroll
         for (int tt = 0; tt < NT; tt++) {
-          const frag<T> kf = col_frag<T, KS>(Kt[buf], 32 * kt + 16 * s, tt);
+          const frag<T> kf = col_frag<T, KS>(Kb, 32 * kt + 16 * s, tt);
           dq[tt] = mma(kf, d, dq[tt]);
           if constexpr (MEND) pk[tt] = mma(kf, p, pk[tt]);
         }
       }
     }
-    if (more) fetch_bias(k0 + BK);
+    F::again();
+    if constexpr (!SPLIT) F::order();  // the biases are the wave's own
   }
   if constexpr (MEND) {
-    off = both_sum(off) * rs.inv;
+    off = both_sum(off);
+    if constexpr (SPLIT) {
+      float* const sums = reinterpret_cast<float*>(lds);
+      __syncthreads();
+      sums[threadIdx.x] = off;
+      __syncthreads();
+      off = (sums[l] + sums[64 + l]) + (sums[128 + l] + sums[192 + l]);
+    }
+    off *= rs.inv;
 #pragma unroll
     for (int tt = 0; tt < NT; tt++) dq[tt] -= off * pk[tt];
-    if (j < a.N && hl == 0) a.delta[srow] = rs.delta + off;  // this lane's row alone: no other reads it in this kernel
+    // no other workgroup reads this row's, and this one's waves have what they need
+    if (j < a.N && hl == 0 && (!SPLIT || wave == 0)) a.delta[srow] = rs.delta + off;
   }
-  if (j >= a.N) return;
-  const float by = rs.inv * a.scale;
-  T* const out = static_cast<T*>(a.dq) + (un.smp * a.N + j) * a.H * a.C + hc;
+  T* const out = static_cast<T*>(a.dq) + orow;
+  const auto put = [&](int tt, int qq, f4 r) {
+    const int c = 32 * tt + 8 * qq + 4 * hl;
+    if (c >= a.C) return;
+    r *= rs.inv * a.scale;
+    store_chunk<4, false>(out + c, fv<4>{r[0], r[1], r[2], r[3]});
+  };
+  if constexpr (SPLIT) {
+    f4 r[NT];
+    meet4<NT>(dq, reinterpret_cast<f4*>(lds), wave, l, 1.f, r);
+    if (j >= a.N) return;
 #pragma unroll
-  for (int tt = 0; tt < NT; tt++)
+    for (int tt = 0; tt < NT; tt++) put(tt, wave, r[tt]);
+  } else {
+    if (j >= a.N) return;
 #pragma unroll
-    for (int qq = 0; qq < 4; qq++) {
-      const int c = 32 * tt + 8 * qq + 4 * hl;
-      if (c >= a.C) continue;
-      fv<4> r;
+    for (int tt = 0; tt < NT; tt++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) r[e] = dq[tt][4 * qq + e] * by;
-      store_chunk<4, false>(out + c, r);
-    }
+      for (int qq = 0; qq < 4; qq++) put(tt, qq, f4{dq[tt][4 * qq], dq[tt][4 * qq + 1], dq[tt][4 * qq + 2], dq[tt][4 * qq + 3]});
+  }
 }
 
 // dk and dv (and dbias): a wave holds 32 keys as the columns of S = Q K^T, so that dk^T = q^T ds and dv^T = dO^T p take p and
 // ds from their lanes; the queries' statistics come from LDS, four rows a read.
-template <typename T, typename BT, int KS, int NW, bool TWO>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_dkv_k(Attn a, int64_t per_xcd) {
-  constexpr int BQ = sizeof(T) == 2 ? 64 : 32, QT = BQ / 32, NT = (KS + 1) / 2, NTH = 64 * NW, WK = 32 * NW;
-  static_assert(BQ <= NTH, "a thread a row of statistics");
-  __shared__ LDS_ALIGN T Qt[2][BQ * TILE_LD<T, KS>];
-  __shared__ LDS_ALIGN T Dt[2][BQ * TILE_LD<T, KS>];
-  __shared__ LDS_ALIGN T Lt[TWO ? 2 : 1][TWO ? BQ * TILE_LD<T, KS> : 8];
-  __shared__ LDS_ALIGN float St[2][3][BQ];
-  const int64_t kblocks = (a.M + WK - 1) / WK;
+template <typename T, typename BT, int KS, bool SPLIT, bool TWO>
+__global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_dkv_k(Attn a, int64_t per_xcd) {
+  typedef Form<T, SPLIT> F;
+  constexpr int BQ = F::BR, QT = BQ / 32, NT = (KS + 1) / 2, TILE = BQ * TILE_LD<T, KS>, PARTS = TWO ? 3 : 2;
+  constexpr int TILES = F::GROUPS * F::BUFS * PARTS * TILE * (int)sizeof(T), MEET = SPLIT ? 4 * NT * 4096 : 0;
+  __shared__ LDS_ALIGN char lds[TILES > MEET ? TILES : MEET];
+  __shared__ LDS_ALIGN float St[F::GROUPS][F::BUFS][4][BQ];
+  __shared__ int Big[F::GROUPS][F::BUFS];
+  __shared__ LDS_ALIGN char bias_lds[sizeof(BT) == 2 ? 4 * BiasTile<half_t>::BYTES : 16];
+  static_assert(BQ <= F::NTH, "a thread a row of statistics");
+  const int64_t kblocks = (a.M + F::ROWS - 1) / F::ROWS;
   Unit un;
   if (!unit_of(a, kblocks, per_xcd, &un)) return;  // whole workgroup
-  const int t = threadIdx.x, l = t & 63, hl = l >> 5;
-  const int64_t key = un.block * WK + 32 * (t >> 6) + (l & 31), kc = min(key, a.M - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, hl = l >> 5;
+  const int t = SPLIT ? l : threadIdx.x, group = SPLIT ? wave : 0;
+  T* const Qt = reinterpret_cast<T*>(lds) + group * F::BUFS * PARTS * TILE;
+  T* const Dt = Qt + F::BUFS * TILE;
+  T* const Lt = Dt + F::BUFS * TILE;
+  const int64_t first = un.block * F::ROWS + (SPLIT ? 0 : 32 * wave), key0 = min(first, a.M - 1);  // the wave's first key
+  const int64_t key = first + (l & 31), kc = min(key, a.M - 1);
+  u4* const Bt = reinterpret_cast<u4*>(bias_lds + wave * BiasTile<half_t>::BYTES);
   const int hc = un.h * a.C;
+  const int64_t pitch = (int64_t)a.H * a.C, osmp = un.smp * a.N * pitch + hc;
   const T* const q = static_cast<const T*>(a.q) + un.smp * a.sq + hc;
-  const T* const dO = static_cast<const T*>(a.dO) + un.smp * a.N * a.H * a.C + hc;
-  const T* const dO_lo = TWO ? static_cast<const T*>(a.dO_lo) + un.smp * a.N * a.H * a.C + hc : nullptr;
+  const T* const dO = static_cast<const T*>(a.dO) + osmp;
+  const T* const dO_lo = TWO ? static_cast<const T*>(a.dO_lo) + osmp : nullptr;
   const T* const k = static_cast<const T*>(a.k) + un.smp * a.sk + kc * a.ldk + hc;
   const T* const v = static_cast<const T*>(a.v) + un.smp * a.sv + kc * a.ldv + hc;
   const int64_t plane = ((int64_t)(un.smp / a.mult) * a.H + un.h) * a.N * a.M;
-  const BT* const bias = a.bias ? static_cast<const BT*>(a.bias) + plane + kc : nullptr;
-  BT* const db = a.dbias && a.mult == 1 ? static_cast<BT*>(a.dbias) + plane + kc : nullptr;
+  const BT* const bias = a.bias ? static_cast<const BT*>(a.bias) + plane : nullptr;
+  BT* const db = a.dbias && a.mult == 1 ? static_cast<BT*>(a.dbias) + plane : nullptr;
+  const uint32_t boff = (4 * hl * (uint32_t)a.M + (uint32_t)kc) * (uint32_t)sizeof(BT);  // a lane's first row of a tile, its key
   const int64_t srow = ((int64_t)un.smp * a.H + un.h) * a.N;
   const float* mask = a.mask ? a.mask + un.smp * a.M : nullptr;
-  if (!any_key<NTH>(mask, a.M)) mask = nullptr;
+  if (!any_key(mask, a.M)) mask = nullptr;
   const bool on = key < a.M && (!mask || mask[kc] != 0.f);
 
   frag<T> kf[KS], vf[KS];
@@ -234,71 +277,114 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void at
 #pragma unroll
   for (int tt = 0; tt < NT; tt++) dk[tt] = dv[tt] = f16x{};
 
-  Stage<T, KS, BQ, NTH> qs, ds, ls;
-  BT bs[QT][16];
-  float st[3];
+  Stage<T, KS, BQ, F::NTH, false> qs, ds, ls;
+  constexpr bool HALF = sizeof(BT) == 2;
+  BiasTile<std::conditional_t<HALF, BT, half_t>> bt;  // the next tile's biases
+  float bs[HALF ? 1 : 16] = {};                       // fp32: a row's 32 keys a half wave and instruction
+  float st[4];
   const auto fetch = [&](int64_t q0) {
-    qs.load(q, a.ldq, q0, a.N, a.C);
-    ds.load(dO, (int64_t)a.H * a.C, q0, a.N, a.C);
-    if constexpr (TWO) ls.load(dO_lo, (int64_t)a.H * a.C, q0, a.N, a.C);
+    qs.load(q + q0 * a.ldq, (uint32_t)a.ldq, a.N - q0, a.C, t);
+    ds.load(dO + q0 * pitch, (uint32_t)pitch, a.N - q0, a.C, t);
+    if constexpr (TWO) ls.load(dO_lo + q0 * pitch, (uint32_t)pitch, a.N - q0, a.C, t);
     if (t < BQ) {
       const RowStat r(a, srow + min(q0 + t, a.N - 1));
-      const bool in = q0 + t < a.N;  // past the end: exp(y - inf) = 0
-      st[0] = in ? r.top : INFINITY;
+      const bool in = q0 + t < a.N;  // past the end: 2^(y by - inf) = 0
+      st[0] = in ? r.ex.at : INFINITY;
       st[1] = in ? r.inv : 0.f;
       st[2] = in ? r.delta : 0.f;
+      st[3] = r.ex.by;
     }
   };
-  const auto fetch_bias = [&](int64_t q0) {
-    if (!bias) return;
+  const auto fetch_bias = [&](int64_t r0) {
+    if (!bias || r0 >= a.N) return;
+    const int n = (int)min(a.N - r0, (int64_t)32);
+    if constexpr (HALF) {
+      bt.load(bias + r0 * a.M + key0, n, a.M, a.M - key0);
+    } else {
+      const Columns at(bias + r0 * a.M, n, a.M);
 #pragma unroll
-    for (int qt = 0; qt < QT; qt++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) bs[qt][i] = bias[min(q0 + 32 * qt + 8 * (i >> 2) + 4 * hl + (i & 3), a.N - 1) * a.M];
+      for (int i = 0; i < 16; i++) bs[i] = at.get(boff, 8 * (i >> 2) + (i & 3), n == 32);
+    }
   };
-  fetch(0);
-  fetch_bias(0);
-  for (int64_t q0 = 0; q0 < a.N; q0 += BQ) {
-    const int buf = (int)(q0 / BQ & 1);
+  constexpr int STEP = F::GROUPS * BQ;
+  int64_t q0 = group * BQ;
+  if (q0 < a.N) fetch(q0);
+  fetch_bias(q0);
+  for (int buf = 0; q0 < a.N; q0 += STEP, buf = (buf + 1) % F::BUFS) {
     const uint64_t rows = all_rows((int)min(a.N - q0, (int64_t)BQ));
-    qs.store(Qt[buf], rows, a.C);
-    ds.store(Dt[buf], rows, a.C);
-    if constexpr (TWO) ls.store(Lt[buf], rows, a.C);
-    if (t < BQ)
+    T* const Qb = Qt + buf * TILE;
+    T* const Db = Dt + buf * TILE;
+    T* const Lb = Lt + buf * TILE;
+    float(*const Sb)[BQ] = St[group][buf];
+    qs.store(Qb, rows, a.C, t);
+    ds.store(Db, rows, a.C, t);
+    if constexpr (TWO) ls.store(Lb, rows, a.C, t);
+    if (t < BQ) {
 #pragma unroll
-      for (int i = 0; i < 3; i++) St[buf][i][t] = st[i];
-    __syncthreads();  // as in the forward pass
-    const bool more = q0 + BQ < a.N;
-    if (more) fetch(q0 + BQ);
+      for (int i = 0; i < 4; i++) Sb[i][t] = st[i];
+      Big[group][buf] = __any(st[3] != LOG2E);
+    }
+    F::sync();
+    const bool big = __builtin_amdgcn_readfirstlane(Big[group][buf]);  // a row with an exponent of its own (Exponent)
+    if (q0 + STEP < a.N) fetch(q0 + STEP);
 #pragma unroll
     for (int qt = 0; qt < QT; qt++) {
+      const int64_t r0 = q0 + 32 * qt;
+      if (r0 >= a.N) break;
+      const int64_t next = qt + 1 < QT ? r0 + 32 : q0 + STEP;
+      if constexpr (HALF) {
+        if (bias) bt.store(Bt);
+        F::order();
+        fetch_bias(next);
+      }
       f16x x = f16x{}, dp = f16x{};
 #pragma unroll
       for (int m = 0; m < KS; m++) {
-        x = mma(row_frag<T, KS>(Qt[buf], 32 * qt + (l & 31), m), kf[m], x);
-        dp = mma(row_frag<T, KS>(Dt[buf], 32 * qt + (l & 31), m), vf[m], dp);
-        if constexpr (TWO) dp = mma(row_frag<T, KS>(Lt[buf], 32 * qt + (l & 31), m), vf[m], dp);
+        x = mma(row_frag<T, KS>(Qb, 32 * qt + (l & 31), m), kf[m], x);
+        dp = mma(row_frag<T, KS>(Db, 32 * qt + (l & 31), m), vf[m], dp);
+        if constexpr (TWO) dp = mma(row_frag<T, KS>(Lb, 32 * qt + (l & 31), m), vf[m], dp);
       }
+      // A key that takes no part has what it has in its own column alone, which ends as zeros.
+      const auto probs = [&](auto any) {
 #pragma unroll
-      for (int qq = 0; qq < 4; qq++) {
-        const int r = 32 * qt + 8 * qq + 4 * hl;
-        const f4 top = *reinterpret_cast<const f4*>(&St[buf][0][r]);
-        const f4 inv = *reinterpret_cast<const f4*>(&St[buf][1][r]);
-        const f4 delta = *reinterpret_cast<const f4*>(&St[buf][2][r]);
+        for (int qq = 0; qq < 4; qq++) {
+          const int r = 32 * qt + 8 * qq + 4 * hl;
+          const f4 at = *reinterpret_cast<const f4*>(&Sb[0][r]);
+          const f4 inv = *reinterpret_cast<const f4*>(&Sb[1][r]);
+          const f4 delta = *reinterpret_cast<const f4*>(&Sb[2][r]);
+          f4 by = f4{LOG2E, LOG2E, LOG2E, LOG2E}, b = f4{};
+          if constexpr (any()) by = *reinterpret_cast<const f4*>(&Sb[3][r]);
+          if constexpr (HALF) {
+            if (bias) b = decltype(bt)::get(Bt, qq);
+          } else {
+            b = f4{bs[4 * qq], bs[4 * qq + 1], bs[4 * qq + 2], bs[4 * qq + 3]};
+          }
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int i = 4 * qq + e;
-          const float y = bias ? fmaf(x[i], a.scale, (float)bs[qt][i]) : x[i] * a.scale;
-          const float p = on ? __builtin_amdgcn_exp2f((y - top[e]) * LOG2E) * inv[e] : 0.f;
-          x[i] = p;
-          dp[i] = on ? p * (dp[i] - delta[e]) : 0.f;
+          for (int e = 0; e < 4; e++) {
+            const int i = 4 * qq + e;
+            x[i] = __builtin_amdgcn_exp2f(fmaf(fmaf(x[i], a.scale, b[e]), by[e], -at[e])) * inv[e];
+            dp[i] = x[i] * (dp[i] - delta[e]);
+          }
+          __builtin_amdgcn_sched_barrier(0);  // sixteen rows' statistics at once would not fit in the registers
         }
-      }
-      if (db && key < a.M) {
+      };
+      if (big) probs(std::true_type());
+      else probs(std::false_type());
+      if constexpr (!HALF) fetch_bias(next);
+      if (db) {
+        const int n = (int)min(a.N - r0, (int64_t)32);
+        if constexpr (HALF) {
+          F::order();
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int64_t r = q0 + 32 * qt + 8 * (i >> 2) + 4 * hl + (i & 3);
-          if (r < a.N) db[r * a.M] = (BT)dp[i];
+          for (int i = 0; i < 16; i++) decltype(bt)::put(Bt, i, on ? dp[i] : 0.f);
+          F::order();
+          decltype(bt)::write(Bt, db + r0 * a.M + key0, n, a.M, a.M - first);
+          F::order();
+        } else if (key < a.M) {
+          const Columns at(db + r0 * a.M, n, a.M);
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            at.put(boff, 8 * (i >> 2) + (i & 3), n == 32, on ? dp[i] : 0.f);
         }
       }
 #pragma unroll
@@ -306,28 +392,37 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void at
         const frag<T> p = as_frag<T>(x, s), d = as_frag<T>(dp, s);
 #pragma unroll
         for (int tt = 0; tt < NT; tt++) {
-          dv[tt] = mma(col_frag<T, KS>(Dt[buf], 32 * qt + 16 * s, tt), p, dv[tt]);
-          if constexpr (TWO) dv[tt] = mma(col_frag<T, KS>(Lt[buf], 32 * qt + 16 * s, tt), p, dv[tt]);
-          dk[tt] = mma(col_frag<T, KS>(Qt[buf], 32 * qt + 16 * s, tt), d, dk[tt]);
+          dv[tt] = mma(col_frag<T, KS>(Db, 32 * qt + 16 * s, tt), p, dv[tt]);
+          if constexpr (TWO) dv[tt] = mma(col_frag<T, KS>(Lb, 32 * qt + 16 * s, tt), p, dv[tt]);
+          dk[tt] = mma(col_frag<T, KS>(Qb, 32 * qt + 16 * s, tt), d, dk[tt]);
         }
       }
     }
-    if (more) fetch_bias(q0 + BQ);
+    F::again();
   }
-  if (key >= a.M) return;
-  const int64_t at = (un.smp * a.M + key) * a.H * a.C + hc;
+  const int64_t at = (un.smp * a.M + kc) * pitch + hc;
+  const auto put = [&](void* to, int tt, int qq, f4 r, float by) {
+    const int c = 32 * tt + 8 * qq + 4 * hl;
+    if (!on) r = f4{};
+    if (key < a.M && c < a.C) store_chunk<4, false>(static_cast<T*>(to) + at + c, fv<4>{r[0] * by, r[1] * by, r[2] * by, r[3] * by});
+  };
+  if constexpr (SPLIT) {
+    f4 r[NT];
+    meet4<NT>(dk, reinterpret_cast<f4*>(lds), wave, l, 1.f, r);
 #pragma unroll
-  for (int tt = 0; tt < NT; tt++)
+    for (int tt = 0; tt < NT; tt++) put(a.dk, tt, wave, r[tt], a.scale);
+    meet4<NT>(dv, reinterpret_cast<f4*>(lds), wave, l, 1.f, r);
 #pragma unroll
-    for (int qq = 0; qq < 4; qq++) {
-      const int c = 32 * tt + 8 * qq + 4 * hl;
-      if (c >= a.C) continue;
-      fv<4> rk, rv;
+    for (int tt = 0; tt < NT; tt++) put(a.dv, tt, wave, r[tt], 1.f);
+  } else {
 #pragma unroll
-      for (int e = 0; e < 4; e++) rk[e] = dk[tt][4 * qq + e] * a.scale, rv[e] = dv[tt][4 * qq + e];
-      store_chunk<4, false>(static_cast<T*>(a.dk) + at + c, rk);
-      store_chunk<4, false>(static_cast<T*>(a.dv) + at + c, rv);
-    }
+    for (int tt = 0; tt < NT; tt++)
+#pragma unroll
+      for (int qq = 0; qq < 4; qq++) {
+        put(a.dk, tt, qq, f4{dk[tt][4 * qq], dk[tt][4 * qq + 1], dk[tt][4 * qq + 2], dk[tt][4 * qq + 3]}, a.scale);
+        put(a.dv, tt, qq, f4{dv[tt][4 * qq], dv[tt][4 * qq + 1], dv[tt][4 * qq + 2], dv[tt][4 * qq + 3]}, 1.f);
+      }
+  }
 }
 
 // dbias of a bias that `mult` samples share: a wave sums ds of one 32 x 32 tile over them in registers. Operands come
@@ -341,9 +436,12 @@ __global__ __launch_bounds__(256, 1) void attn_dbias_k(Attn a, int64_t tiles_k, 
   const int h = (int)(bh % a.H), hc = h * a.C;
   const int64_t b = bh / a.H, j = 32 * qt + (l & 31), jc = min(j, a.N - 1), kc = min(32 * kt + (l & 31), a.M - 1);
   const int64_t k4 = 32 * kt + 4 * hl, row = (bh * a.N + jc) * a.M;
-  Bias4<BT> bs[4];
+  f16x bias;
 #pragma unroll
-  for (int qq = 0; qq < 4; qq++) bs[qq].load(static_cast<const BT*>(a.bias) + row + k4 + 8 * qq, a.M - k4 - 8 * qq);
+  for (int i = 0; i < 16; i++) {
+    const int64_t at = k4 + 8 * (i >> 2) + (i & 3);
+    bias[i] = at < a.M ? (float)(static_cast<const BT*>(a.bias) + row)[at] : 0.f;
+  }
   f16x sum = f16x{};
   for (int64_t smp = b * a.mult; smp < (b + 1) * a.mult; smp++) {
     const T* const q = static_cast<const T*>(a.q) + smp * a.sq + jc * a.ldq + hc;
@@ -377,8 +475,8 @@ __global__ __launch_bounds__(256, 1) void attn_dbias_k(Attn a, int64_t tiles_k, 
     }
 #pragma unroll
     for (int i = 0; i < 16; i++) {
-      const float y = fmaf(x[i], a.scale, (float)bs[i >> 2].v[i & 3]);
-      const float d = __builtin_amdgcn_exp2f((y - rs.top) * LOG2E) * rs.inv * (dp[i] - rs.delta);
+      const float y = fmaf(x[i], a.scale, bias[i]);
+      const float d = rs.ex.of(y) * rs.inv * (dp[i] - rs.delta);
       sum[i] += keep >> (8 * (i >> 2) + (i & 3)) & 1 ? d : 0.f;
     }
   }
@@ -425,30 +523,33 @@ hipError_t launch_attention_bwd(Attn a, void* ws, hipStream_t st) {
     attn_rows_k<T><<<(unsigned)wgs, 256, 0, st>>>(a, L);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const auto go = [&](auto nw, auto two) {
-      constexpr int NW = decltype(nw)::value;
+    const auto blocks = [&](int64_t n, int rows) { return ((n + rows - 1) / rows * a.S * a.H + 7) / 8; };  // for each XCD
+    const auto go = [&](auto two) {
       constexpr bool TWO = decltype(two)::value;
-      const int64_t uq = (a.N + 32 * NW - 1) / (32 * NW) * a.S * a.H, pq = (uq + 7) / 8;
-      const int64_t uk = (a.M + 32 * NW - 1) / (32 * NW) * a.S * a.H, pk = (uk + 7) / 8;
-      const int64_t tk = (a.M + 31) / 32, tiles = tk * ((a.N + 31) / 32) * a.H * (a.S / a.mult);
-      if (8 * pq > INT32_MAX || 8 * pk > INT32_MAX || (tiles + 3) / 4 > INT32_MAX) return hipErrorInvalidValue;
-      attn_dq_k<T, BT, KS, NW, TWO><<<(unsigned)(8 * pq), 64 * NW, 0, st>>>(a, pq);
-      hipError_t e = hipGetLastError();
-      if (e != hipSuccess) return e;
-      attn_dkv_k<T, BT, KS, NW, TWO><<<(unsigned)(8 * pk), 64 * NW, 0, st>>>(a, pk);
-      e = hipGetLastError();
+      const auto dq = [&](auto split) {
+        const int64_t per = blocks(a.N, Form<T, decltype(split)::value>::ROWS);
+        if (8 * per > INT32_MAX) return hipErrorInvalidValue;
+        attn_dq_k<T, BT, KS, decltype(split)::value, TWO><<<(unsigned)(8 * per), 256, 0, st>>>(a, per);
+        return hipGetLastError();
+      };
+      const auto dkv = [&](auto split) {
+        const int64_t per = blocks(a.M, Form<T, decltype(split)::value>::ROWS);
+        if (8 * per > INT32_MAX) return hipErrorInvalidValue;
+        attn_dkv_k<T, BT, KS, decltype(split)::value, TWO><<<(unsigned)(8 * per), 256, 0, st>>>(a, per);
+        return hipGetLastError();
+      };
+      hipError_t e = with_split<KS>(a.N, a, dq);
+      if (e == hipSuccess) e = with_split<KS>(a.M, a, dkv);
       if (e != hipSuccess || !a.dbias || a.mult == 1) return e;
+      const int64_t tk = (a.M + 31) / 32, tiles = tk * ((a.N + 31) / 32) * a.H * (a.S / a.mult);
+      if ((tiles + 3) / 4 > INT32_MAX) return hipErrorInvalidValue;
       attn_dbias_k<T, BT, KS, TWO><<<(unsigned)((tiles + 3) / 4), 256, 0, st>>>(a, tk, tiles);
       return hipGetLastError();
     };
-    const int64_t n = a.N < a.M ? a.N : a.M;
-    const bool few = (n + 127) / 128 * a.S * a.H < 512;
-    typedef std::integral_constant<int, 2> Two;
-    typedef std::integral_constant<int, 4> Four;
     if constexpr (sizeof(T) == 2) {
-      if (a.g) return few ? go(Two(), std::true_type()) : go(Four(), std::true_type());
+      if (a.g) return go(std::true_type());
     }
-    return few ? go(Two(), std::false_type()) : go(Four(), std::false_type());
+    return go(std::false_type());
   });
 }
 

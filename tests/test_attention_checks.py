@@ -97,8 +97,8 @@ ATT = dict(q=AT[0], ldq=48, sq=240, k=AT[1], ldk=48, sk=336, v=AT[2], ldv=48, sv
     {"q": None}, {"k": None}, {"v": None}, {"out": None}, {"stats": None}, {"q": AT[0] + 1}, {"k": AT[1] + 1}, {"v": AT[2] + 1},
     {"g": AT[3] + 1}, {"bias": AT[4] + 1}, {"mask": AT[5] + 2}, {"out": AT[6] + 1}, {"stats": AT[7] + 2}, {"dt": 3}, {"bias_dt": F32},
     {"bias_dt": BF16}, {"dt": F32, "bias_dt": 7}, {"C": 0}, {"C": 12}, {"C": 136}, {"H": 0}, {"S": 0}, {"mult": 0}, {"mult": 3}, {"N": 0},
-    {"M": 0}, {"N": -1}, {"N": 2 ** 31}, {"M": 2 ** 31}, {"ldq": 47}, {"ldk": 40}, {"ldv": 0}, {"ldg": 1}, {"sq": -1}, {"sv": -8},
-    {"sk": 2 ** 62}, {"ldk": 2 ** 60}, {"out": AT[0]}, {"out": AT[1] + 600}, {"out": AT[4]}, {"stats": AT[6]}, {"stats": AT[5]},
+    {"M": 0}, {"N": -1}, {"N": 2 ** 22 + 1}, {"M": 2 ** 22 + 1}, {"ldq": 47}, {"ldk": 40}, {"ldv": 0}, {"ldg": 1}, {"sq": -1}, {"sv": -8},
+    {"sk": 2 ** 62}, {"ldk": 2 ** 23}, {"ldg": 2 ** 60}, {"out": AT[0]}, {"out": AT[1] + 600}, {"out": AT[4]}, {"stats": AT[6]}, {"stats": AT[5]},
     {"out": AT[3] + 900},
 ])
 def test_attention_refuses(change):
