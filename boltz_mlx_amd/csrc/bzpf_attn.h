@@ -255,79 +255,33 @@ struct BiasRows {
   }
 };
 
-// A 32 x 32 tile of half-type biases whose columns are the lanes (dk and dv), through LDS as above and out of it with the
-// transposing reads; and the tile of their gradients, the other way.
-template <typename BT>
-struct BiasTile {
-  static constexpr int BYTES = 2048;
-  u4 r[2];
-  __device__ __forceinline__ void load(const BT* base, int rows, int64_t M, int64_t left) {
-    const int l = threadIdx.x & 63, c = 8 * (l & 3);
-#pragma unroll
-    for (int n = 0; n < 2; n++) {
-      const BT* const p = at_byte(base, ((uint32_t)min((l >> 2) + 16 * n, rows - 1) * (uint32_t)M + c) * 2u);
-      r[n] = left >= 32 ? load_all(p) : load_part(p, left - c);
-    }
-  }
-  __device__ __forceinline__ void store(u4* lds) const {
-    const int l = threadIdx.x & 63;
-    lds[l] = r[0];
-    lds[64 + l] = r[1];
-  }
-  // The lane's elements of rows 8 qq + 4 hl .. + 3.
-  static __device__ __forceinline__ f4 get(const u4* lds, int qq) {
-    typedef short s4 __attribute__((ext_vector_type(4)));
-    typedef BT V __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) s4* lds4;
-    const int l = threadIdx.x & 63;
-    const BT* const p = reinterpret_cast<const BT*>(lds) + (8 * qq + 4 * (l >> 5) + ((l & 15) >> 2)) * 32 + 16 * ((l >> 4) & 1) + 4 * (l & 3);
-    return __builtin_convertvector(__builtin_bit_cast(V, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p)), f4);
-  }
-  static __device__ __forceinline__ void put(u4* lds, int i, float x) {
-    const int l = threadIdx.x & 63;
-    reinterpret_cast<BT*>(lds)[(8 * (i >> 2) + 4 * (l >> 5) + (i & 3)) * 32 + (l & 31)] = (BT)x;
-  }
-  // The tile to memory: `rows` of its rows, `left` of its columns.
-  static __device__ __forceinline__ void write(const u4* lds, BT* base, int rows, int64_t M, int64_t left) {
-    typedef BT V __attribute__((ext_vector_type(8)));
-    typedef BT U __attribute__((ext_vector_type(8), aligned(sizeof(BT))));
-    const int l = threadIdx.x & 63, c = 8 * (l & 3);
-#pragma unroll
-    for (int n = 0; n < 2; n++) {
-      const int row = (l >> 2) + 16 * n;
-      if (row >= rows) continue;
-      BT* const p = at_byte(base, ((uint32_t)row * (uint32_t)M + c) * 2u);
-      const V x = __builtin_bit_cast(V, lds[64 * n + l]);
-      if (left >= 32) {
-        *reinterpret_cast<U*>(p) = x;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (c + e < left) p[e] = x[e];
-      }
-    }
-  }
-};
-
-// Rows of an fp32 matrix tile whose columns are a wave's lanes, a row an instruction: the tile is a buffer, the row's offset the
+// Rows of a matrix tile whose columns are a wave's lanes, a row an instruction: the tile is a buffer, the row's offset the
 // instruction's scalar one, so that an access costs no address arithmetic. Past the buffer's end loads give 0 and stores drop.
+template <typename BT>
 struct Columns {
   __amdgpu_buffer_rsrc_t rsrc;
   uint32_t pitch;  // bytes
   // base: the tile's first row; rows: those of it that exist
-  __device__ __forceinline__ Columns(const float* base, int rows, int64_t M)
-      : rsrc(__builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)(rows * M * 4), 0x00020000)), pitch((uint32_t)M * 4) {}
+  __device__ __forceinline__ Columns(const BT* base, int rows, int64_t M)
+      : rsrc(__builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)(rows * M * (int64_t)sizeof(BT)), 0x00020000)),
+        pitch((uint32_t)M * (uint32_t)sizeof(BT)) {}
   // lane: byte offset of the lane's first row and column; r: the row from there; whole: every row of the tile exists (else the
   // row has to be in the lane's offset, which the range check covers: 16 of them, not to be kept over a loop)
-  __device__ __forceinline__ float get(uint32_t lane, int r, bool whole) const {
+  __device__ __forceinline__ BT get(uint32_t lane, int r, bool whole) const {
     if (!whole) asm volatile("" : "+v"(lane));
-    return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc, whole ? (int)lane : (int)(lane + r * pitch),
-                                                                whole ? (int)(r * pitch) : 0, 0));
+    const int v = whole ? (int)lane : (int)(lane + r * pitch), s = whole ? (int)(r * pitch) : 0;
+    if constexpr (sizeof(BT) == 2)
+      return __builtin_bit_cast(BT, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rsrc, v, s, 0));
+    else
+      return __builtin_bit_cast(BT, (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rsrc, v, s, 0));
   }
   __device__ __forceinline__ void put(uint32_t lane, int r, bool whole, float x) const {
     if (!whole) asm volatile("" : "+v"(lane));
-    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), rsrc, whole ? (int)lane : (int)(lane + r * pitch),
-                                          whole ? (int)(r * pitch) : 0, 0);
+    const int v = whole ? (int)lane : (int)(lane + r * pitch), s = whole ? (int)(r * pitch) : 0;
+    if constexpr (sizeof(BT) == 2)
+      __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (BT)x), rsrc, v, s, 0);
+    else
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, (BT)x), rsrc, v, s, 0);
   }
 };
 
@@ -358,12 +312,13 @@ struct Unit {
   int64_t block;
   int smp, h;
 };
-__device__ __forceinline__ bool unit_of(const Attn& a, int64_t blocks, int64_t per_xcd, Unit* u) {
-  const int64_t n = (int64_t)(blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
-  if (n >= blocks * a.S * a.H) return false;
-  u->block = n % blocks;
-  u->smp = (int)(n / blocks % a.S);
-  u->h = (int)(n / blocks / a.S);
+__device__ __forceinline__ bool unit_of(const Attn& a, int64_t blocks, int64_t per_xcd, Unit* u) {  // all below 2^31
+  const uint32_t n = blockIdx.x % 8 * (uint32_t)per_xcd + blockIdx.x / 8, per_head = (uint32_t)blocks * (uint32_t)a.S;
+  u->h = (int)(n / per_head);
+  if (u->h >= a.H) return false;
+  const uint32_t rest = n - (uint32_t)u->h * per_head;
+  u->smp = (int)(rest / (uint32_t)blocks);
+  u->block = rest - (uint32_t)u->smp * (uint32_t)blocks;
   return true;
 }
 

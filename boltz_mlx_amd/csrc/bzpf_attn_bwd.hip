@@ -17,7 +17,8 @@ namespace bzpf {
 
 namespace {
 
-// delta [S][H][N], and with a gate dO (two parts in half types) and dg. L lanes a head, 8 channels each.
+// What the other kernels need of a row (p = 2^(x by - at) inv), [S][H][N], and with a gate dO (two parts in half types) and
+// dg. L lanes a head, 8 channels each.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_rows_k(Attn a, int L) {
   const int l = threadIdx.x % L, heads = 256 / L;
@@ -51,18 +52,21 @@ __global__ __launch_bounds__(256) void attn_rows_k(Attn a, int L) {
     }
   }
   for (int o = 1; o < L; o *= 2) d += __shfl_xor(d, o);
-  if (on && l == 0) a.delta[(smp * a.H + h) * a.N + row - smp * a.N] = d;
+  if (on && l == 0) {
+    const int64_t to = (smp * a.H + h) * a.N + row - smp * a.N;
+    const float top = a.stats[2 * to], sum = a.stats[2 * to + 1];
+    const Exponent ex(top);
+    static_cast<f4*>(a.rows)[to] = f4{ex.at, sum == 0.f ? 0.f : __builtin_amdgcn_exp2f(-ex.off(top)) / sum, d, ex.by};
+  }
 }
 
-// What a row's probabilities and their gradients need: p = 2^(x by - at) inv.
+// A row as attn_rows_k left it.
 struct RowStat {
   Exponent ex;
   float inv, delta;
   __device__ __forceinline__ RowStat(const Attn& a, int64_t row) {
-    const float top = a.stats[2 * row], sum = a.stats[2 * row + 1];
-    ex = Exponent(top);
-    inv = sum == 0.f ? 0.f : __builtin_amdgcn_exp2f(-ex.off(top)) / sum;
-    delta = a.delta[row];
+    const f4 v = static_cast<const f4*>(a.rows)[row];
+    ex.at = v[0], ex.by = v[3], inv = v[1], delta = v[2];
   }
 };
 
@@ -203,7 +207,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
 #pragma unroll
     for (int tt = 0; tt < NT; tt++) dq[tt] -= off * pk[tt];
     // no other workgroup reads this row's, and this one's waves have what they need
-    if (j < a.N && hl == 0 && (!SPLIT || wave == 0)) a.delta[srow] = rs.delta + off;
+    if (j < a.N && hl == 0 && (!SPLIT || wave == 0)) static_cast<float*>(a.rows)[4 * srow + 2] = rs.delta + off;
   }
   T* const out = static_cast<T*>(a.dq) + orow;
   const auto put = [&](int tt, int qq, f4 r) {
@@ -237,7 +241,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
   __shared__ LDS_ALIGN char lds[TILES > MEET ? TILES : MEET];
   __shared__ LDS_ALIGN float St[F::GROUPS][F::BUFS][4][BQ];
   __shared__ int Big[F::GROUPS][F::BUFS];
-  __shared__ LDS_ALIGN char bias_lds[sizeof(BT) == 2 ? 4 * BiasTile<half_t>::BYTES : 16];
   static_assert(BQ <= F::NTH, "a thread a row of statistics");
   const int64_t kblocks = (a.M + F::ROWS - 1) / F::ROWS;
   Unit un;
@@ -247,9 +250,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
   T* const Qt = reinterpret_cast<T*>(lds) + group * F::BUFS * PARTS * TILE;
   T* const Dt = Qt + F::BUFS * TILE;
   T* const Lt = Dt + F::BUFS * TILE;
-  const int64_t first = un.block * F::ROWS + (SPLIT ? 0 : 32 * wave), key0 = min(first, a.M - 1);  // the wave's first key
-  const int64_t key = first + (l & 31), kc = min(key, a.M - 1);
-  u4* const Bt = reinterpret_cast<u4*>(bias_lds + wave * BiasTile<half_t>::BYTES);
+  const int64_t key = un.block * F::ROWS + (SPLIT ? 0 : 32 * wave) + (l & 31), kc = min(key, a.M - 1);
   const int hc = un.h * a.C;
   const int64_t pitch = (int64_t)a.H * a.C, osmp = un.smp * a.N * pitch + hc;
   const T* const q = static_cast<const T*>(a.q) + un.smp * a.sq + hc;
@@ -278,32 +279,27 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
   for (int tt = 0; tt < NT; tt++) dk[tt] = dv[tt] = f16x{};
 
   Stage<T, KS, BQ, F::NTH, false> qs, ds, ls;
-  constexpr bool HALF = sizeof(BT) == 2;
-  BiasTile<std::conditional_t<HALF, BT, half_t>> bt;  // the next tile's biases
-  float bs[HALF ? 1 : 16] = {};                       // fp32: a row's 32 keys a half wave and instruction
-  float st[4];
+  BT bs[16] = {};  // the next tile's biases, a row's 32 keys a half wave and instruction; zero where there are none
+  f4 st;
   const auto fetch = [&](int64_t q0) {
     qs.load(q + q0 * a.ldq, (uint32_t)a.ldq, a.N - q0, a.C, t);
     ds.load(dO + q0 * pitch, (uint32_t)pitch, a.N - q0, a.C, t);
     if constexpr (TWO) ls.load(dO_lo + q0 * pitch, (uint32_t)pitch, a.N - q0, a.C, t);
     if (t < BQ) {
-      const RowStat r(a, srow + min(q0 + t, a.N - 1));
-      const bool in = q0 + t < a.N;  // past the end: 2^(y by - inf) = 0
-      st[0] = in ? r.ex.at : INFINITY;
-      st[1] = in ? r.inv : 0.f;
-      st[2] = in ? r.delta : 0.f;
-      st[3] = r.ex.by;
+      st = static_cast<const f4*>(a.rows)[srow + min(q0 + t, a.N - 1)];
+      if (q0 + t >= a.N) st = f4{INFINITY, 0.f, 0.f, LOG2E};  // past the end: 2^(y by - inf) = 0
     }
   };
   const auto fetch_bias = [&](int64_t r0) {
     if (!bias || r0 >= a.N) return;
     const int n = (int)min(a.N - r0, (int64_t)32);
-    if constexpr (HALF) {
-      bt.load(bias + r0 * a.M + key0, n, a.M, a.M - key0);
-    } else {
-      const Columns at(bias + r0 * a.M, n, a.M);
+    const Columns<BT> at(bias + r0 * a.M, n, a.M);
+    if (n == 32) {
 #pragma unroll
-      for (int i = 0; i < 16; i++) bs[i] = at.get(boff, 8 * (i >> 2) + (i & 3), n == 32);
+      for (int i = 0; i < 16; i++) bs[i] = at.get(boff, 8 * (i >> 2) + (i & 3), true);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; i++) bs[i] = at.get(boff, 8 * (i >> 2) + (i & 3), false);
     }
   };
   constexpr int STEP = F::GROUPS * BQ;
@@ -332,11 +328,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
       const int64_t r0 = q0 + 32 * qt;
       if (r0 >= a.N) break;
       const int64_t next = qt + 1 < QT ? r0 + 32 : q0 + STEP;
-      if constexpr (HALF) {
-        if (bias) bt.store(Bt);
-        F::order();
-        fetch_bias(next);
-      }
       f16x x = f16x{}, dp = f16x{};
 #pragma unroll
       for (int m = 0; m < KS; m++) {
@@ -352,17 +343,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
           const f4 at = *reinterpret_cast<const f4*>(&Sb[0][r]);
           const f4 inv = *reinterpret_cast<const f4*>(&Sb[1][r]);
           const f4 delta = *reinterpret_cast<const f4*>(&Sb[2][r]);
-          f4 by = f4{LOG2E, LOG2E, LOG2E, LOG2E}, b = f4{};
+          f4 by = f4{LOG2E, LOG2E, LOG2E, LOG2E};
           if constexpr (any()) by = *reinterpret_cast<const f4*>(&Sb[3][r]);
-          if constexpr (HALF) {
-            if (bias) b = decltype(bt)::get(Bt, qq);
-          } else {
-            b = f4{bs[4 * qq], bs[4 * qq + 1], bs[4 * qq + 2], bs[4 * qq + 3]};
-          }
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const int i = 4 * qq + e;
-            x[i] = __builtin_amdgcn_exp2f(fmaf(fmaf(x[i], a.scale, b[e]), by[e], -at[e])) * inv[e];
+            x[i] = __builtin_amdgcn_exp2f(fmaf(fmaf(x[i], a.scale, (float)bs[i]), by[e], -at[e])) * inv[e];
             dp[i] = x[i] * (dp[i] - delta[e]);
           }
           __builtin_amdgcn_sched_barrier(0);  // sixteen rows' statistics at once would not fit in the registers
@@ -370,21 +356,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
       };
       if (big) probs(std::true_type());
       else probs(std::false_type());
-      if constexpr (!HALF) fetch_bias(next);
-      if (db) {
-        const int n = (int)min(a.N - r0, (int64_t)32);
-        if constexpr (HALF) {
-          F::order();
+      fetch_bias(next);
+      if (db && key < a.M) {
+        const Columns<BT> at(db + r0 * a.M, (int)min(a.N - r0, (int64_t)32), a.M);
+        if (r0 + 32 <= a.N) {
 #pragma unroll
-          for (int i = 0; i < 16; i++) decltype(bt)::put(Bt, i, on ? dp[i] : 0.f);
-          F::order();
-          decltype(bt)::write(Bt, db + r0 * a.M + key0, n, a.M, a.M - first);
-          F::order();
-        } else if (key < a.M) {
-          const Columns at(db + r0 * a.M, n, a.M);
+          for (int i = 0; i < 16; i++) at.put(boff, 8 * (i >> 2) + (i & 3), true, on ? dp[i] : 0.f);
+        } else {
 #pragma unroll
-          for (int i = 0; i < 16; i++)
-            at.put(boff, 8 * (i >> 2) + (i & 3), n == 32, on ? dp[i] : 0.f);
+          for (int i = 0; i < 16; i++) at.put(boff, 8 * (i >> 2) + (i & 3), false, on ? dp[i] : 0.f);
         }
       }
 #pragma unroll
@@ -497,19 +477,19 @@ __global__ __launch_bounds__(256, 1) void attn_dbias_k(Attn a, int64_t tiles_k, 
 
 }  // namespace
 
-// The workspace: delta, then dO (in half types its second part after it) where there is a gate.
-static int64_t delta_bytes(int64_t rows) { return (rows * 4 + 15) / 16 * 16; }
+// The workspace: what each row needs, then dO (in half types its second part after it) where there is a gate.
+static int64_t stat_bytes(int64_t rows) { return rows * 16; }
 static int64_t part_bytes(int dt, int64_t rows, int C) { return rows * C * (dt == DT_F32 ? 4 : 2); }
 
 int64_t attention_bwd_ws_bytes(int dt, int64_t S, int64_t N, int H, int C, bool gate) {
   const int64_t rows = S * N * H;
-  return delta_bytes(rows) + (gate ? part_bytes(dt, rows, C) * (dt == DT_F32 ? 1 : 2) : 0);
+  return stat_bytes(rows) + (gate ? part_bytes(dt, rows, C) * (dt == DT_F32 ? 1 : 2) : 0);
 }
 
 hipError_t launch_attention_bwd(Attn a, void* ws, hipStream_t st) {
   const int64_t rows = (int64_t)a.S * a.N * a.H;
-  a.delta = static_cast<float*>(ws);
-  char* const parts = static_cast<char*>(ws) + delta_bytes(rows);
+  a.rows = ws;
+  char* const parts = static_cast<char*>(ws) + stat_bytes(rows);
   a.dO = a.g ? parts : const_cast<void*>(a.dout);
   a.dO_lo = parts + part_bytes(a.dt, rows, a.C);
   return with_attn(a, [&](auto t, auto b, auto ks) {

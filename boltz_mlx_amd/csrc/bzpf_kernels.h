@@ -212,7 +212,7 @@ struct Attn {
   float* stats;  // [S][H][N][2]: a row's largest logit and the sum of exp(logit - that)
   const void* dout;
   void *dq, *dk, *dv, *dg, *dbias;
-  float* delta;  // [S][H][N]
+  void* rows;    // [S][H][N] of four floats (attn_rows_k)
   void* dO;      // [S][N][H C]: sigmoid(g) dout
   void* dO_lo;   // what rounding to a half type has left of it
 };
