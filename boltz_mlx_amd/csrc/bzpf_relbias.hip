@@ -4,8 +4,10 @@
 // bucket(d) = lut[clamp(d - lo, 0, span - 1)], not falling with d; pairs of different groups (chains) take the last one.
 //
 // Both are bound by memory: the bias is written once (the pair bias read once), its gradient read once. A thread owns a
-// chunk of 16 bytes of a row. As buckets do not fall with the distance, the two ends of a chunk's positions say whether the
-// whole chunk lies in one bucket (most do: those beyond the reach, or in another chain); then one look-up serves it.
+// chunk of 16 bytes of a row. As buckets do not fall with the distance, the ends of a chunk's positions say whether it lies
+// beyond the first or the last edge (most do, or are of another chain): then one number serves the whole chunk.
+#include <type_traits>
+
 #include "bzpf_common.h"
 #include "bzpf_kernels.h"
 #include "bzpf_rows.h"
@@ -14,54 +16,114 @@ namespace bzpf {
 
 namespace {
 
-// A position or group number, 32 or 64 bits wide.
+// A position or group number, 32 or 64 bits wide. Both are two loads of 32 bits, the second of the same ones where there are
+// no others: a branch would end in a wait for each number, one after the other (table's gradient at 16 x 2000 x 2000 in
+// bfloat16 58 us so, 96 us with a branch).
+template <typename P>
+__device__ __forceinline__ int64_t number(P p, bool wide, int64_t i) {
+  const int64_t at = i << wide;
+  const uint32_t lo = p[at], hi = p[at + wide];
+  return (int64_t)((uint64_t)(wide ? hi : (uint32_t)((int32_t)lo >> 31)) << 32 | lo);
+}
 __device__ __forceinline__ int64_t whole(const void* p, bool wide, int64_t i) {
-  return wide ? static_cast<const int64_t*>(p)[i] : (int64_t) static_cast<const int32_t*>(p)[i];
+  return number(static_cast<const uint32_t*>(p), wide, i);
+}
+// At a place that is the same in every lane: scalar loads.
+__device__ __forceinline__ int64_t scalar(const void* p, bool wide, int64_t i) {
+  return number((const __attribute__((address_space(4))) uint32_t*)p, wide, i);
 }
 
-// A chunk of V keys: their positions, the ends of these, and the keys' group where they share one.
+// V of them from place i on, of which there are at least n (the last one stands in for the rest). In vectors, the branch around
+// all of them: two loads a number, each lane's a line of its own, took 22 us instead of 12 for the bias of 400 x 400.
+template <int V>
+__device__ __forceinline__ void numbers(const void* p, bool wide, int64_t i, int64_t n, int64_t (&to)[V]) {
+  typedef int64_t W __attribute__((ext_vector_type(2), aligned(8)));
+  typedef int32_t D __attribute__((ext_vector_type(4), aligned(4)));
+  if (n < V) {
+#pragma unroll 1
+    for (int e = 0; e < V; e++) {
+      const int64_t x = whole(p, wide, i + (e < n ? e : n - 1));
+#pragma unroll
+      for (int k = 0; k < V; k++) to[k] = k == e ? x : to[k];
+    }
+  } else if (wide) {
+    const W* const q = reinterpret_cast<const W*>(static_cast<const int64_t*>(p) + i);
+#pragma unroll
+    for (int e = 0; e < V; e++) to[e] = q[e / 2][e % 2];
+  } else {
+    const D* const q = reinterpret_cast<const D*>(static_cast<const int32_t*>(p) + i);
+#pragma unroll
+    for (int e = 0; e < V; e++) to[e] = q[e / 4][e % 4];
+  }
+}
+
+// Where a chunk of keys lies for a query: in one bucket (the first, the last, other groups') or in several.
+enum { FIRST, LAST, OTHER, MIXED };
+
+// A chunk of V keys: their positions from the first one's on in 32 bits, and their groups, one up to `cut` and another from
+// there on. `rare`: positions that do not fit, or more groups; such a chunk's keys are looked at one by one in memory.
 template <int V>
 struct Keys {
-  int64_t pos[V], least, most, group;
-  bool one_group;
-  __device__ __forceinline__ void load(const RelBias& a, int64_t at, int n) {
-    one_group = true;
-    group = a.group_k ? whole(a.group_k, a.wide, at) : 0;
+  int rel[V], least, most, cut;
+  int64_t base, group0, group1, at;
+  bool rare;
+  __device__ __forceinline__ void load(const RelBias& a, int64_t at_, int n) {
+    at = at_, rare = false, cut = V, least = most = 0;
+    int64_t pos[V], group[V];
+    numbers(a.pos_k, a.wide, at, n, pos);
+    if (a.group_k) numbers(a.group_k, a.wide, at, n, group);
+    base = pos[0];
+    if (a.group_k) group0 = group[0], group1 = group[V - 1];
 #pragma unroll
     for (int e = 0; e < V; e++) {
-      const int64_t j = at + (e < n ? e : 0);
-      pos[e] = whole(a.pos_k, a.wide, j);
-      least = e == 0 || pos[e] < least ? pos[e] : least;
-      most = e == 0 || pos[e] > most ? pos[e] : most;
-      if (a.group_k) one_group &= whole(a.group_k, a.wide, j) == group;
+      const int64_t d = pos[e] - base;
+      rare |= d >= FAR || d <= -FAR;
+      rel[e] = (int)d;
+      least = min(least, rel[e]);
+      most = max(most, rel[e]);
+      if (a.group_k) {
+        if (cut == V && group[e] != group0) cut = e;
+        rare |= e >= cut && group[e] != group1;
+      }
     }
+  }
+  static constexpr int64_t FAR = 1 << 29;
+};
+
+// A query against a chunk.
+template <int V>
+struct Query {
+  int from, kind;  // distance - lo of the chunk's first key, at most 2^30 either way
+  bool same0, same1;
+  __device__ __forceinline__ Query(const RelBias& a, const Keys<V>& k, int64_t pos, int64_t group) {
+    const int64_t d = pos - a.lo - k.base;
+    from = (int)(d < -2 * Keys<V>::FAR ? -2 * Keys<V>::FAR : d > 2 * Keys<V>::FAR ? 2 * Keys<V>::FAR : d);
+    same0 = !a.group_k || group == k.group0;
+    same1 = k.cut == V ? same0 : group == k.group1;
+    kind = !same0 && !same1 ? OTHER : !same0 || !same1 ? MIXED : from - k.least <= 0 ? FIRST : from - k.most >= a.span - 1 ? LAST : MIXED;
+    if (k.rare) kind = MIXED;
+  }
+  // The keys' buckets, of a chunk that is not rare.
+  __device__ __forceinline__ void buckets(const RelBias& a, const uint8_t* lut, const Keys<V>& k, int (&at)[V]) const {
+#pragma unroll
+    for (int e = 0; e < V; e++) at[e] = lut[min(max(from - k.rel[e], 0), a.span - 1)];
+    if (a.group_k) {
+      const unsigned first = (1u << k.cut) - 1, same = (same0 ? first : 0u) | (same1 ? ~first : 0u);
+#pragma unroll
+      for (int e = 0; e < V; e++) at[e] = same >> e & 1 ? at[e] : a.count - 1;
+    }
+  }
+  // The bucket of a chunk that lies in one.
+  __device__ __forceinline__ int one(const RelBias& a, const uint8_t* lut) const {
+    return kind == OTHER ? a.count - 1 : lut[kind == FIRST ? 0 : a.span - 1];
   }
 };
 
-__device__ __forceinline__ int bucket_of(const RelBias& a, const uint8_t* lut, int64_t d) {
-  d -= a.lo;
+// The bucket of query i and key j from memory.
+__device__ __forceinline__ int bucket_of(const RelBias& a, const uint8_t* lut, int64_t i, int64_t j) {
+  if (a.group_q && whole(a.group_q, a.wide, i) != whole(a.group_k, a.wide, j)) return a.count - 1;
+  const int64_t d = whole(a.pos_q, a.wide, i) - a.lo - whole(a.pos_k, a.wide, j);
   return lut[d < 0 ? 0 : d >= a.span ? a.span - 1 : (int)d];
-}
-
-// The buckets of a query at `pos` of `group` against the chunk: in at[], or in at[0] alone where they are one (returned).
-template <int V>
-__device__ __forceinline__ bool buckets(const RelBias& a, const uint8_t* lut, const Keys<V>& k, int64_t pos, int64_t group,
-                                        int64_t key0, int n, int (&at)[V]) {
-  if (k.one_group) {
-    at[0] = bucket_of(a, lut, pos - k.most);
-    const bool one = at[0] == bucket_of(a, lut, pos - k.least);
-    if (a.group_q && group != k.group) {
-      at[0] = a.count - 1;
-      return true;
-    }
-    if (one) return true;
-  }
-#pragma unroll
-  for (int e = 0; e < V; e++) {
-    at[e] = bucket_of(a, lut, pos - k.pos[e]);
-    if (!k.one_group && whole(a.group_k, a.wide, key0 + (e < n ? e : 0)) != group) at[e] = a.count - 1;
-  }
-  return false;
 }
 
 // The batch element's own positions and groups.
@@ -91,7 +153,8 @@ __global__ __launch_bounds__(256) void rel_bias_k(RelBias a, const T* __restrict
   extern __shared__ float tab[];
   const int h0 = blockIdx.y * heads, nh = min(heads, a.H - h0), t = threadIdx.x;
   uint8_t* const lut = reinterpret_cast<uint8_t*>(tab + heads * a.count);
-  for (int e = t; e < nh * a.count; e += 256) tab[e] = a.table[(int64_t)(e % a.count) * a.H + h0 + e / a.count];
+  for (int h = t >> 6; h < nh; h += 4)
+    for (int k = t & 63; k < a.count; k += 64) tab[h * a.count + k] = a.table[(int64_t)k * a.H + h0 + h];
   for (int e = t; e < a.span; e += 256) lut[e] = a.lut[e];
   __syncthreads();
   const int64_t b = blockIdx.z;
@@ -102,111 +165,311 @@ __global__ __launch_bounds__(256) void rel_bias_k(RelBias a, const T* __restrict
     const int64_t j0 = min(c * V, a.M - n);  // the last chunk is moved back: its neighbour's keys get the same values
     Keys<V> keys;
     keys.load(a, j0, n);
-    for (int64_t i = (int64_t)blockIdx.x * rows_per + t / L; i < r1; i += 256 / L) {
-      int at[V];
-      const bool one = buckets(a, lut, keys, whole(a.pos_q, a.wide, i), a.group_q ? whole(a.group_q, a.wide, i) : 0, j0, n, at);
-      const int64_t plane = a.N * a.M, base = ((b * a.H + h0) * a.N + i) * a.M + j0;
-      if (n < V) {
-        for (int h = 0; h < nh; h++)
-#pragma unroll
-          for (int e = 0; e < V - 1; e++)
-            if (e < n) {
-              const float v = tab[h * a.count + (one ? at[0] : at[e])];
-              out[base + h * plane + e] = (T)(add ? v + (float)add[base + h * plane + e] : v);
-            }
+    const int64_t plane = a.N * a.M;
+    int64_t i = (int64_t)blockIdx.x * rows_per + t / L;
+    const auto pos_of = [&](int64_t i) { return whole(a.pos_q, a.wide, min(i, a.N - 1)); };
+    const auto group_of = [&](int64_t i) { return a.group_q ? whole(a.group_q, a.wide, min(i, a.N - 1)) : 0; };
+    int64_t pos = pos_of(i), group = group_of(i);
+    for (; i < r1; i += 256 / L) {
+      const Query<V> q(a, keys, pos, group);
+      pos = pos_of(i + 256 / L), group = group_of(i + 256 / L);  // the next row's, on their way
+      const int64_t base = ((b * a.H + h0) * a.N + i) * a.M + j0;
+      if (keys.rare || n < V) {
+#pragma unroll 1
+        for (int e = 0; e < n; e++) {
+          const int k = bucket_of(a, lut, i, j0 + e);
+#pragma unroll 1
+          for (int h = 0; h < nh; h++) {
+            const int64_t to = base + h * plane + e;
+            out[to] = (T)(add ? tab[h * a.count + k] + (float)add[to] : tab[h * a.count + k]);
+          }
+        }
         continue;
       }
-      if (!one) {
-        for (int h = 0; h < nh; h++) {
-          fv<V> v;
-#pragma unroll
-          for (int e = 0; e < V; e++) v[e] = tab[h * a.count + at[e]];
-          if (add) v += load_chunk<V>(add + base + h * plane);
-          store_chunk<V, false>(out + base + h * plane, v);
-        }
+      int at[V];
+      if (q.kind == MIXED) {
+        q.buckets(a, lut, keys, at);
       } else {
-        for (int h = 0; h < nh; h++) {
-          fv<V> v = fv<V>{} + tab[h * a.count + at[0]];
-          if (add) v += load_chunk<V>(add + base + h * plane);
-          store_chunk<V, false>(out + base + h * plane, v);
+        const int one = q.one(a, lut);
+#pragma unroll
+        for (int e = 0; e < V; e++) at[e] = one;
+      }
+      const bool all_one = __all(q.kind != MIXED);
+#pragma unroll 1
+      for (int h = 0; h < nh; h += 4) {  // four heads' pair biases on their way at once
+        Raw<T, V> r[4];
+        if (add) {
+#pragma unroll
+          for (int u = 0; u < 4; u++) r[u].load(add + base + min(h + u, nh - 1) * plane);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          if (h + u >= nh) break;
+          const float* const row = tab + (h + u) * a.count;
+          fv<V> v;
+          if (all_one) {
+            v = fv<V>{} + row[at[0]];
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; e++) v[e] = row[at[e]];
+          }
+          if (add) v += r[u].get();
+          store_chunk<V, false>(out + base + (h + u) * plane, v);
         }
       }
     }
   }
 }
 
-constexpr int GT = 128;  // threads of a gradient workgroup, each with a column of sums of its own in LDS
+// The gradient as products with one-hot rows on the matrix cores: a wave takes 32 keys of a row at a time for 16 heads, the
+// heads' 32 values as a 32 x 16 operand and, for every 16 buckets that the pairs reach, a 16 x 32 one whose rows say which
+// pairs lie in a bucket: 16 x 16 sums in fp32. Adding into LDS, a column a thread, took 104 us for 16 x 2000 x 2000 bf16 (an LDS
+// addition of a wave's 64 lanes costs about 100 cycles there). Half types are their own operand, fp32 goes as three bf16
+// parts, which hold its 24 bits. Rows whose 32 pairs lie in one bucket (beyond the first or last edge, in another chain: most)
+// are added up without a product. A value that is not finite spoils its head's sums.
+template <typename T> struct OneHot;
+template <> struct OneHot<half_t> {
+  typedef half_t P;
+  static constexpr uint32_t ONE = 0x3C00u;
+  static constexpr int PARTS = 1;
+};
+template <> struct OneHot<bf16_t> {
+  typedef bf16_t P;
+  static constexpr uint32_t ONE = 0x3F80u;
+  static constexpr int PARTS = 1;
+};
+template <> struct OneHot<float> {
+  typedef bf16_t P;
+  static constexpr uint32_t ONE = 0x3F80u;
+  static constexpr int PARTS = 3;
+};
+typedef half_t h8 __attribute__((ext_vector_type(8)));
+typedef bf16_t b8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ f4 mma16(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f4 mma16(b8 a, b8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-// A thread adds its elements into its own column [bucket][thread] of LDS (ds_add_f32 without contention, so that the order
-// of a column's additions is the program's: equal inputs give equal bits), and keeps the sum of the bucket it is in a
-// register while successive chunks stay in one. grid (row blocks, heads, batch).
-template <typename T>
-__global__ __launch_bounds__(GT) void rel_bias_bwd_k(RelBias a, const T* __restrict__ dy, float* __restrict__ part,
-                                                     int64_t step, int rows_per) {
-  constexpr int V = CHUNK<T>, U = 4;
-  extern __shared__ float sums[];
-  const int t = threadIdx.x;
-  uint8_t* const lut = reinterpret_cast<uint8_t*>(sums + a.count * GT);
-  for (int k = 0; k < a.count; k++) sums[k * GT + t] = 0.f;
-  for (int e = t; e < a.span; e += GT) lut[e] = a.lut[e];
-  __syncthreads();
-  const int64_t b = blockIdx.z;
-  const int h = blockIdx.y;
+constexpr int64_t BOUND = (int64_t)1 << 30;  // distances past it are all alike (edges are at most 2^14 apart)
+__device__ __forceinline__ int bounded(int64_t d) { return (int)(d < -BOUND ? -BOUND : d > BOUND ? BOUND : d); }
+
+constexpr int GK = 8;  // keys of a lane: a product's k = 8 (lane / 16) .. + 7
+
+// A wave's 32 keys, each lane's 8 neighbours: their distances from the first key in 32 bits. Past the end a lane's keys are
+// moved back to the last 8, and the first `skip` of them are its neighbours' (there are at least 8).
+struct KeyTile {
+  int rel[GK];
+  int64_t base, group;
+  int least, most;
+  bool one_group, rare;  // rare: positions that 32 bits do not hold
+  unsigned other;        // the lane's keys that are not of `group`
+  int64_t j;             // the lane's first key
+  int skip;
+  __device__ __forceinline__ void load(const RelBias& a, int64_t j0) {
+    const int64_t want = j0 + GK * ((threadIdx.x & 63) >> 4);
+    j = min(want, max(a.M - GK, (int64_t)0));
+    skip = (int)min(want - j, (int64_t)GK);
+    base = scalar(a.pos_k, a.wide, j0);
+    group = a.group_k ? scalar(a.group_k, a.wide, j0) : 0;
+    bool far = false;
+    other = 0;
+    int lo = 0, hi = 0;
+    int64_t pos[GK], groups[GK];
+    numbers(a.pos_k, a.wide, j, a.M, pos);
+    if (a.group_k) numbers(a.group_k, a.wide, j, a.M, groups);
+#pragma unroll
+    for (int e = 0; e < GK; e++) {
+      const int64_t d = pos[e] - base;
+      far |= d < -BOUND / 2 || d > BOUND / 2;
+      rel[e] = (int)d;
+      lo = min(lo, rel[e]);
+      hi = max(hi, rel[e]);
+      if (a.group_k && groups[e] != group) other |= 1u << e;
+    }
+    for (int o = 16; o < 64; o *= 2) lo = min(lo, __shfl_xor(lo, o)), hi = max(hi, __shfl_xor(hi, o));
+    least = __builtin_amdgcn_readfirstlane(lo);
+    most = __builtin_amdgcn_readfirstlane(hi);
+    one_group = !__any(other != 0);
+    rare = __any(far);
+  }
+};
+
+// grid (blocks of 128 keys, row blocks, batch times groups of 16 heads); partial sums [row block, key block, batch][H][count].
+// BT: groups of 16 buckets.
+template <typename T, int BT>
+__global__ __launch_bounds__(256) void rel_bias_bwd_k(RelBias a, const T* __restrict__ dy, float* __restrict__ part, int rows_per) {
+  typedef OneHot<T> OH;
+  typedef typename OH::P P;
+  typedef P P8 __attribute__((ext_vector_type(8)));
+  typedef T TV __attribute__((ext_vector_type(GK)));
+  typedef T TU __attribute__((ext_vector_type(GK), aligned(sizeof(T))));
+  __shared__ float meet[16][16 * BT + 1];
+  const int l = threadIdx.x & 63, c = l & 15, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hg = (a.H + 15) / 16;
+  const int64_t b = blockIdx.z / hg;
+  const int h0 = 16 * (int)(blockIdx.z % hg), h = min(h0 + c, a.H - 1);
   a = of_batch(a, b);
-  const int64_t chunks = (a.M + V - 1) / V, r1 = min(a.N, ((int64_t)blockIdx.x + 1) * rows_per);
-  const int L = row_lanes(chunks, GT), n = a.M < V ? (int)a.M : V;
-  float* const mine = sums + t;
-  float run = 0.f;
-  int cur = 0;
-  for (int64_t c = t % L; c < chunks; c += L) {
-    const int64_t j0 = min(c * V, a.M - n);
-    const int skip = (int)(c * V - j0);  // elements that the neighbour has
-    Keys<V> keys;
-    keys.load(a, j0, n);
-    const T* const col = dy + ((b * a.H + h) * a.N) * a.M + j0;
-    const int stride = GT / L;
-    for (int64_t i = (int64_t)blockIdx.x * rows_per + t / L; i < r1; i += (int64_t)U * stride) {
-      Raw<T, V> raw[U];
-      int64_t pos[U], group[U];
+  for (int e = threadIdx.x; e < 16 * (16 * BT + 1); e += 256) (&meet[0][0])[e] = 0.f;
+  // The lane's buckets, 16 t + c: distances (from lo) `from` .. from + width - 1. The look-up table does not fall: bucket k's
+  // distances start where its entries reach k.
+  __shared__ int start[257];
+  for (int i = 1 + threadIdx.x; i < a.span; i += 256)
+    for (int k = a.lut[i - 1] + 1; k <= a.lut[i]; k++) start[k] = i;
+  __syncthreads();
+  int from[BT];
+  uint32_t width[BT];
+  const int first = a.lut[0], last = a.lut[a.span - 1];
+  // The distance of a pair of different groups: none that a pair has, or one of the last bucket where that is theirs too.
+  const int others = last == a.count - 1 ? (int)BOUND : INT32_MIN;
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        const int64_t r = min(i + (int64_t)u * stride, r1 - 1);
-        if (n == V) raw[u].load(col + r * a.M);
-        else
+  for (int t = 0; t < BT; t++) {
+    const int k = 16 * t + c;
+    const bool in = k >= first && k <= last;
+    const int64_t at = in && k > first ? start[k] : -BOUND * 2 + 1, end = in && k < last ? start[k + 1] : BOUND * 2;
+    from[t] = in ? (int)at : 0;
+    width[t] = in ? (uint32_t)(end - at) : 0u;
+    if (a.group_k && k == a.count - 1 && k != last) from[t] = others, width[t] = 1;
+  }
+  // The distances of buckets 16 t .. 16 t + 15, and whether the pairs of different groups are theirs: a product for them is
+  // left out where the 32 pairs are none of theirs.
+  int low[BT], high[BT];
 #pragma unroll
-          for (int e = 0; e < V; e++) raw[u].v[e] = e < n ? col[r * a.M + e] : (T)0.f;
-        pos[u] = whole(a.pos_q, a.wide, r);
-        group[u] = a.group_q ? whole(a.group_q, a.wide, r) : 0;
-      }
+  for (int t = 0; t < BT; t++) {
+    const int k0 = 16 * t, k1 = 16 * t + 16;
+    low[t] = k0 > last ? INT32_MAX : __builtin_amdgcn_readfirstlane(k0 <= first ? INT32_MIN : start[k0]);
+    high[t] = k1 <= first ? INT32_MIN : __builtin_amdgcn_readfirstlane(k1 > last ? INT32_MAX : start[k1]);
+  }
+
+  f4 acc[BT];
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        if (i + (int64_t)u * stride >= r1) break;
-        fv<V> v = raw[u].get();
-#pragma unroll
-        for (int e = 0; e < V; e++) v[e] = e >= skip ? v[e] : 0.f;
-        int at[V];
-        if (buckets(a, lut, keys, pos[u], group[u], j0, n, at)) {
-          if (at[0] != cur) {
-            atomicAdd(mine + cur * GT, run);
-            run = 0.f;
-            cur = at[0];
-          }
-          run += sum_of(v);
+  for (int t = 0; t < BT; t++) acc[t] = f4{};
+  float run[3] = {0.f, 0.f, 0.f};  // the lane's head, of rows in one bucket
+  const int64_t r0 = (int64_t)blockIdx.y * rows_per, r1 = min(a.N, r0 + rows_per);
+  const int64_t j0 = (int64_t)blockIdx.x * 16 * GK + 4 * GK * wave;
+  if (j0 < a.M) {
+    KeyTile keys;
+    keys.load(a, j0);
+    const bool whole_tile = j0 + 4 * GK <= a.M, short_rows = a.M < GK, on = h0 + c < a.H;
+    const T* const col = dy + ((b * a.H + h) * a.N) * a.M + keys.j;
+    struct Row {  // the lane's values, the query's position and group
+      TV v;
+      int64_t pos, group;
+    };
+    const auto fetch = [&](int64_t i) {
+      Row f;
+      const int64_t r = min(i, r1 - 1);
+      f.pos = scalar(a.pos_q, a.wide, r);
+      f.group = a.group_q ? scalar(a.group_q, a.wide, r) : 0;
+      const T* const p = col + r * a.M;
+      f.v = TV{};
+      if (on) {
+        if (!short_rows) {
+          f.v = *reinterpret_cast<const TU*>(p);
         } else {
 #pragma unroll
-          for (int e = 0; e < V; e++)
-            if (e >= skip && e < n) atomicAdd(mine + at[e] * GT, v[e]);
+          for (int e = 0; e < GK - 1; e++)
+            if (e < a.M) f.v[e] = p[e];
         }
       }
+      return f;
+    };
+    const auto work = [&](TV v, int64_t pos, int64_t group) {
+      if (!whole_tile) {
+#pragma unroll
+        for (int e = 0; e < GK; e++) v[e] = e >= keys.skip ? v[e] : (T)0.f;
+      }
+      const int at = bounded(pos - a.lo - keys.base);
+      const bool same = !a.group_k || group == keys.group;
+      const int kind = keys.rare || !keys.one_group ? MIXED : !same ? OTHER : at - keys.least <= 0 ? FIRST
+                       : at - keys.most >= a.span - 1 ? LAST : MIXED;
+      if (kind != MIXED) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < GK; e += 2) s += (float)v[e] + (float)v[e + 1];
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+          if (kind == k) run[k] += s;
+        return;
+      }
+      int d[GK];
+#pragma unroll
+      for (int e = 0; e < GK; e++) d[e] = at - keys.rel[e];
+      if (keys.rare) {
+#pragma unroll
+        for (int e = 0; e < GK; e++) d[e] = bounded(pos - a.lo - whole(a.pos_k, a.wide, min(keys.j + e, a.M - 1)));
+      }
+      if (!keys.one_group || !same) {
+        unsigned other = keys.other;
+        if (!same) {
+          other = 0;
+#pragma unroll
+          for (int e = 0; e < GK; e++) other |= (whole(a.group_k, a.wide, min(keys.j + e, a.M - 1)) != group) << e;
+        }
+#pragma unroll
+        for (int e = 0; e < GK; e++) d[e] = other >> e & 1 ? others : d[e];
+      }
+      P8 x[GK / 8][OH::PARTS];
+#pragma unroll
+      for (int e = 0; e < GK; e++) {
+        P8* const to = x[e / 8];
+        if constexpr (OH::PARTS == 1) {
+          to[0][e % 8] = v[e];
+        } else {
+          const float hi = (float)(P)v[e], mid = (float)(P)(v[e] - hi);
+          to[0][e % 8] = (P)hi;
+          to[1][e % 8] = (P)mid;
+          to[2][e % 8] = (P)(v[e] - hi - mid);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < BT; t++) {
+        const bool reached = at - keys.least >= low[t] && at - keys.most < high[t];
+        if (BT > 2 && !reached && !keys.rare && ((same && keys.one_group) || t != (a.count - 1) / 16)) continue;
+        typedef uint32_t W4 __attribute__((ext_vector_type(4)));
+        W4 w[GK / 8];
+#pragma unroll
+        for (int e = 0; e < GK; e += 2) {
+          const bool p = (uint32_t)d[e] - (uint32_t)from[t] < width[t], q = (uint32_t)d[e + 1] - (uint32_t)from[t] < width[t];
+          w[e / 8][e % 8 / 2] = (p ? OH::ONE : 0u) | (q ? OH::ONE << 16 : 0u);
+        }
+#pragma unroll
+        for (int k = 0; k < GK / 8; k++)
+#pragma unroll
+          for (int p = 0; p < OH::PARTS; p++) acc[t] = mma16(__builtin_bit_cast(P8, w[k]), x[k][p], acc[t]);
+      }
+    };
+    // Five rows in flight, and the loop's body once: the kernel's code would not fit the instruction cache unrolled (45 KB;
+    // most workgroups run a part of it once).
+    Row f[5];
+#pragma unroll
+    for (int u = 0; u < 5; u++) f[u] = fetch(r0 + u);
+#pragma unroll 1
+    for (int64_t i = r0; i < r1; i++) {
+      const Row now = f[0];
+#pragma unroll
+      for (int u = 0; u < 4; u++) f[u] = f[u + 1];
+      f[4] = fetch(i + 5);
+      work(now.v, now.pos, now.group);
     }
   }
-  atomicAdd(mine + cur * GT, run);
-  __syncthreads();
-  float* const to = part + ((b * gridDim.x + blockIdx.x) * a.H + h) * step;
-  for (int k = t >> 6; k < a.count; k += GT / 64) {
-    const float s = row_sum<64>(sums[k * GT + (t & 63)] + sums[k * GT + 64 + (t & 63)], nullptr);
-    if ((t & 63) == 0) to[k] = s;
+  // The workgroup's sums: a wave at a time, in their order. acc[t][i] is bucket 16 t + 4 (lane / 16) + i of head h0 + c.
+#pragma unroll
+  for (int k = 0; k < 3; k++) run[k] = xgroups_sum(run[k]);
+  for (int w = 0; w < 4; w++) {
+    if (w == wave) {
+#pragma unroll
+      for (int t = 0; t < BT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) meet[c][16 * t + 4 * (l >> 4) + i] += acc[t][i];
+      if (l < 16) {
+        meet[c][first] += run[FIRST];
+        meet[c][last] += run[LAST];
+        meet[c][a.count - 1] += run[OTHER];
+      }
+    }
+    __syncthreads();
   }
+  float* const to = part + (((b * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * a.H + h0) * a.count;
+  const int heads = min(16, a.H - h0);
+  for (int e = threadIdx.x; e < heads * a.count; e += 256) to[e] = meet[e / a.count][e % a.count];
 }
 
 // dtable[k][h] from the partial sums [blocks][H][count], in a fixed order: 16 waves a workgroup each add every 16th, a lane
@@ -227,13 +490,10 @@ __global__ __launch_bounds__(1024) void rel_bias_sum_k(const float* __restrict__
   dtable[(int64_t)k * H + h] = s;
 }
 
-// Row blocks of a (batch element, head)'s gradient: about eight workgroups a compute unit over all of them, and at least
-// four chunks for each thread.
+// Row blocks of the gradient: about three workgroups a compute unit over key blocks, heads and batch, and at least 8 rows each.
 int64_t grad_blocks(int64_t B, int H, int64_t N, int64_t M) {
-  const int64_t want = (2048 + B * H - 1) / (B * H), most = (N * ((M + 7) / 8) + 4 * GT - 1) / (4 * GT);
-  int64_t n = want < most ? want : most;
-  if (n > N) n = N;
-  return n < 1 ? 1 : n;
+  const int64_t others = B * ((H + 15) / 16) * ((M + 16 * GK - 1) / (16 * GK)), want = (768 + others - 1) / others, most = (N + 7) / 8;
+  return want < most ? want : most;
 }
 
 template <typename Fn>
@@ -266,24 +526,26 @@ hipError_t launch_rel_bias(const RelBias& a, const void* add, void* out, int dt,
 }
 
 int64_t rel_bias_bwd_ws_bytes(int64_t B, int H, int64_t N, int64_t M, int count) {
-  return B * grad_blocks(B, H, N, M) * H * count * (int64_t)sizeof(float);
+  return B * grad_blocks(B, H, N, M) * ((M + 16 * GK - 1) / (16 * GK)) * H * count * (int64_t)sizeof(float);
 }
 
 hipError_t launch_rel_bias_bwd(const RelBias& a, const void* dy, int dt, float* dtable, float* ws, int64_t B,
                                hipStream_t st) {
-  const int64_t nb = grad_blocks(B, a.H, a.N, a.M), per = (a.N + nb - 1) / nb;
+  const int64_t nb = grad_blocks(B, a.H, a.N, a.M), per = (a.N + nb - 1) / nb, kb = (a.M + 16 * GK - 1) / (16 * GK), bh = B * ((a.H + 15) / 16);
+  if (nb > 65535 || bh > 65535) return hipErrorInvalidValue;
   const hipError_t e = with_type(dt, [&](auto t) {
     typedef decltype(t) T;
-    const size_t lds = (size_t)a.count * GT * 4 + (size_t)(a.span + 3) / 4 * 4;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&rel_bias_bwd_k<T>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    if (e != hipSuccess) return e;
-    rel_bias_bwd_k<T><<<dim3((unsigned)nb, (unsigned)a.H, (unsigned)B), GT, lds, st>>>(a, static_cast<const T*>(dy), ws,
-                                                                                    a.count, (int)per);
-    return hipGetLastError();
+    const auto go = [&](auto bt) {
+      rel_bias_bwd_k<T, decltype(bt)::value><<<dim3((unsigned)kb, (unsigned)nb, (unsigned)bh), 256, 0, st>>>(
+          a, static_cast<const T*>(dy), ws, (int)per);
+      return hipGetLastError();
+    };
+    if (a.count <= 32) return go(std::integral_constant<int, 2>());
+    if (a.count <= 80) return go(std::integral_constant<int, 5>());
+    return go(std::integral_constant<int, 16>());
   });
   if (e != hipSuccess) return e;
-  rel_bias_sum_k<<<dim3((unsigned)((a.count + 63) / 64), (unsigned)a.H), 1024, 0, st>>>(ws, B * nb, a.H, a.count, dtable);
+  rel_bias_sum_k<<<dim3((unsigned)((a.count + 63) / 64), (unsigned)a.H), 1024, 0, st>>>(ws, B * nb * kb, a.H, a.count, dtable);
   return hipGetLastError();
 }
 

@@ -3,8 +3,8 @@ the attention and its gradients) against the float64 oracle.
 
 Tolerances, from the kernels' arithmetic: u = 2^-24 is fp32's half step, h the half step of a half type (fp16 2^-11, bf16
 2^-8; 0 in fp32). Bounds are sums over the terms' sizes, first order.
-Position bias: one addition in fp32, one rounding. Its gradient: a sum whose terms pass at most as many additions as one
-thread makes (its share of the rows and chunks) and 40 more (the chunk, the wave, the partial sums).
+Position bias: one addition in fp32, one rounding. Its gradient: a sum whose terms pass at most as many additions as a wave
+makes for its rows, and those of the waves and of the partial sums.
 Norms: a sum of C <= 256 squares passes at most 22 additions, halved by the root: xh errs by 16u; an angle by 4u (its turns'
 rounding) and the 2^-52 of its turns, its sine and cosine by 2u more. y: 32u of the pair's sizes. dx, with G the pair's sizes
 of dy: g errs by 10u G, the mean of w g xh by 60u of the mean of the sizes: rstd u (32 |w| G + 96 |xh| mean(|w| G |xh|)).
@@ -79,12 +79,11 @@ def positions(seed, *shape, chains=1):
 
 
 def grad_depth(B, H, N, M):
-    """Additions that a thread makes at most: the launch's row blocks, the rows and chunks of one of its 128 threads."""
-    blocks = max(1, min(-(-2048 // (B * H)), -(-(N * -(-M // 8)) // 512), N))
-    chunks, lanes = -(-M // 4), 1
-    while lanes < 128 and lanes < chunks:
-        lanes *= 2
-    return -(-(-(-N // blocks)) // (128 // lanes)) * -(-chunks // lanes) * 8 + 40 + blocks * B // 16
+    """Additions that a term passes at most: those of its wave's rows (32 pairs and three parts in a product at most), of the
+    four waves, and of the partial sums, 16 at a time."""
+    others = B * -(-H // 16) * -(-M // 128)
+    blocks = min(-(-768 // others), -(-N // 8))
+    return 97 * -(-N // blocks) + 4 + B * blocks * -(-M // 128) // 16 + 16
 
 
 BIASES = [
