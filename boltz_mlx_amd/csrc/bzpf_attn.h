@@ -199,15 +199,16 @@ struct Stage {
 
 typedef unsigned int u4 __attribute__((ext_vector_type(4)));
 
-// 16 bytes of a row, of which the first n elements (a whole chunk: any n past it) exist; the others are zero.
+// 16 bytes of elements without the first s of them (0 <= s < 16 / sizeof(BT); zeros come in behind).
 template <typename BT>
-__device__ __forceinline__ u4 load_part(const BT* p, int64_t n) {
-  constexpr int E = 16 / (int)sizeof(BT);
-  typedef BT V __attribute__((ext_vector_type(E)));
-  V v;
-#pragma unroll
-  for (int e = 0; e < E; e++) v[e] = e < n ? p[e] : (BT)0.f;
-  return __builtin_bit_cast(u4, v);
+__device__ __forceinline__ u4 without(u4 v, int s) {
+  if constexpr (sizeof(BT) == 2) {
+    if (s & 1) v = u4{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+    s >>= 1;
+  }
+  if (s & 1) v = u4{v[1], v[2], v[3], 0u};
+  if (s & 2) v = u4{v[2], v[3], 0u, 0u};
+  return v;
 }
 template <typename BT>
 __device__ __forceinline__ u4 load_all(const BT* p) {
@@ -216,7 +217,7 @@ __device__ __forceinline__ u4 load_all(const BT* p) {
 }
 
 // The biases of a wave's 32 rows against BK keys, on their way through LDS: from memory in whole rows (a lane for each row
-// would take 32 lines an instruction: 220 us instead of XX for 4096 x 4096 and 16 heads), to the lanes that own the rows.
+// would take 32 lines an instruction: forward pass of 2 x 16 x 2000 x 2000 bfloat16 227 us instead of 171), to the lanes that own the rows.
 // 16-byte pieces lie at places that keep the lanes' reads of one column on different banks.
 template <typename BT, int BK>
 struct BiasRows {
@@ -225,20 +226,50 @@ struct BiasRows {
   static __device__ __forceinline__ int place(int row, int c) {
     return row * CPR + (CPR == 8 ? c ^ (row & 7) : c ^ (row >> 1 & 3));
   }
-  // base: the wave's first row, at the first key; rows: those of the 32 that exist (at least one); left: keys from there on
-  __device__ __forceinline__ void load(const BT* base, int rows, int64_t M, int64_t left) {
-    const int l = threadIdx.x & 63;
+  // base: the wave's first row; rows: those of the 32 that exist (at least one); from key k0 on. A piece that the row's end cuts
+  // is read where it ends with the row, and put right in store() (an element at a time took 1.2 to 1.5 times as long for the
+  // whole kernel at 400 and 2000 keys).
+  __device__ __forceinline__ void load(const BT* base, int rows, int M, int k0) {
+    const int l = threadIdx.x & 63, last = M - k0 - E;
+    if (M < E) {
+      load_short(base, rows, M);
+      return;
+    }
 #pragma unroll
     for (int n = 0; n < NV; n++) {
-      const int id = l + 64 * n, c = id % CPR;
-      const BT* const p = at_byte(base, ((uint32_t)min(id / CPR, rows - 1) * (uint32_t)M + c * E) * (uint32_t)sizeof(BT));
-      r[n] = left >= BK ? load_all(p) : load_part(p, left - c * E);
+      const int id = l + 64 * n;
+      r[n] = load_all(at_byte(base, (uint32_t)(min(id / CPR, rows - 1) * M + k0 + min(id % CPR * E, last)) * (uint32_t)sizeof(BT)));
     }
   }
-  __device__ __forceinline__ void store(u4* lds) const {
+  // Rows of fewer elements than a piece has: one by one, from the first on.
+  __device__ __forceinline__ void load_short(const BT* base, int rows, int M) {
+    typedef BT V __attribute__((ext_vector_type(E)));
     const int l = threadIdx.x & 63;
+    V v[NV] = {};
+#pragma unroll 1
+    for (int e = M - 1; e >= 0; e--) {
 #pragma unroll
-    for (int n = 0; n < NV; n++) lds[place((l + 64 * n) / CPR, (l + 64 * n) % CPR)] = r[n];
+      for (int n = 0; n < NV; n++) {
+        const BT x = base[min((l + 64 * n) / CPR, rows - 1) * M + e];
+        V w;
+        w[0] = x;
+#pragma unroll
+        for (int i = 1; i < E; i++) w[i] = v[n][i - 1];
+        v[n] = w;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NV; n++) r[n] = __builtin_bit_cast(u4, v[n]);
+  }
+  __device__ __forceinline__ void store(u4* lds, int M, int k0) const {
+    const int l = threadIdx.x & 63, last = M - k0 - E;
+#pragma unroll
+    for (int n = 0; n < NV; n++) {
+      const int c = (l + 64 * n) % CPR;
+      u4 v = r[n];
+      if (last < BK - E && M >= E) v = without<BT>(v, max(c * E - last, 0) & (E - 1));  // a piece past the end: no matter what
+      lds[place((l + 64 * n) / CPR, c)] = v;
+    }
   }
   // The lane's 16 of tile kt.
   static __device__ __forceinline__ f16x get(const u4* lds, int kt) {

@@ -64,10 +64,7 @@ __global__ __launch_bounds__(256) void attn_rows_k(Attn a, int L) {
 struct RowStat {
   Exponent ex;
   float inv, delta;
-  __device__ __forceinline__ RowStat(const Attn& a, int64_t row) {
-    const f4 v = static_cast<const f4*>(a.rows)[row];
-    ex.at = v[0], ex.by = v[3], inv = v[1], delta = v[2];
-  }
+  __device__ __forceinline__ explicit RowStat(f4 v) { ex.at = v[0], ex.by = v[3], inv = v[1], delta = v[2]; }
 };
 
 // dq: a wave holds 32 queries as the columns of S^T, as the forward pass does. The sum's reciprocal is a row's own, so that it
@@ -102,18 +99,25 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
   const float* mask = a.mask ? a.mask + un.smp * a.M : nullptr;
   if (!any_key(mask, a.M)) mask = nullptr;
   const int64_t srow = ((int64_t)un.smp * a.H + un.h) * a.N + jc;
-  const RowStat rs(a, srow);
+  const RowStat rs(static_cast<const f4*>(a.rows)[srow]);
 
-  frag<T> qf[KS], df[KS], dl[TWO ? KS : 1];
+  // dO's second part waits in LDS in the wide form (in registers it had 64 channels spill: XX us instead of XX).
+  constexpr bool ASIDE = TWO && !SPLIT;
+  __shared__ frag<T> aside[ASIDE ? 4 * KS * 64 : 1];
+  frag<T> qf[KS], df[KS], dl[TWO && !ASIDE ? KS : 1];
 #pragma unroll
   for (int m = 0; m < KS; m++) {
     const bool in = 16 * m + 8 * hl < a.C;
     qf[m] = in ? load8(q + 16 * m + 8 * hl) : frag<T>{};
     df[m] = in ? load8(dO + 16 * m + 8 * hl) : frag<T>{};
-    if constexpr (TWO) dl[m] = in ? load8(dO_lo + 16 * m + 8 * hl) : frag<T>{};
+    if constexpr (TWO) {
+      const frag<T> f = in ? load8(dO_lo + 16 * m + 8 * hl) : frag<T>{};
+      if constexpr (ASIDE) aside[(wave * KS + m) * 64 + l] = f;  // read by the lane that wrote it
+      else dl[m] = f;
+    }
   }
   f16x dq[NT], pk[MEND ? NT : 1];
-  float off = 0.f;  // the row's sum of ds
+  float off = 0.f, taken = 0.f;  // the row's sums of ds and of what its products take for it
 #pragma unroll
   for (int tt = 0; tt < NT; tt++) {
     dq[tt] = f16x{};
@@ -129,7 +133,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
     if (mask) mk = mask[min(k0 + l, a.M - 1)];
   };
   const auto fetch_bias = [&](int64_t k0) {
-    if (bias) bs.load(bias + k0, brows, a.M, a.M - k0);
+    if (bias) bs.load(bias, brows, (int)a.M, (int)k0);
   };
   constexpr int STEP = F::GROUPS * BK;
   int64_t k0 = group * BK;
@@ -143,7 +147,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
     T* const Vb = Vt + buf * TILE;
     ks.store(Kb, keep, a.C, t);
     vs.store(Vb, keep, a.C, t);
-    if (bias) bs.store(Bt);
+    if (bias) bs.store(Bt, (int)a.M, (int)k0);
     F::sync();
     const bool more = k0 + STEP < a.M;
     if (more) {
@@ -158,7 +162,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
         x = mma(row_frag<T, KS>(Kb, 32 * kt + (l & 31), m), qf[m], x);
         const frag<T> vm = row_frag<T, KS>(Vb, 32 * kt + (l & 31), m);
         dp = mma(vm, df[m], dp);
-        if constexpr (TWO) dp = mma(vm, dl[m], dp);
+        if constexpr (ASIDE) dp = mma(vm, aside[(wave * KS + m) * 64 + l], dp);
+        else if constexpr (TWO) dp = mma(vm, dl[m], dp);
       }
       f16x b = f16x{};
       if (bias) b = BiasRows<BT, BK>::get(Bt, kt);
@@ -176,13 +181,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
           dp[i] = on ? dp[i] : 0.f;
         }
       }
-      if constexpr (MEND) {
-#pragma unroll
-        for (int i = 0; i < 16; i++) off += dp[i];
-      }
 #pragma unroll
       for (int s = 0; s < 2; s++) {
         const frag<T> d = as_frag<T>(dp, s), p = as_frag<T>(x, s);
+        if constexpr (MEND) {
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            off += dp[8 * s + e];
+            taken += (float)d[e];
+          }
+        }
 #pragma unroll
         for (int tt = 0; tt < NT; tt++) {
           const frag<T> kf = col_frag<T, KS>(Kb, 32 * kt + 16 * s, tt);
@@ -195,17 +203,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
     if constexpr (!SPLIT) F::order();  // the biases are the wave's own
   }
   if constexpr (MEND) {
-    off = both_sum(off);
+    off = both_sum(off), taken = both_sum(taken);
     if constexpr (SPLIT) {
       float* const sums = reinterpret_cast<float*>(lds);
       __syncthreads();
       sums[threadIdx.x] = off;
+      sums[256 + threadIdx.x] = taken;
       __syncthreads();
       off = (sums[l] + sums[64 + l]) + (sums[128 + l] + sums[192 + l]);
+      taken = (sums[256 + l] + sums[320 + l]) + (sums[384 + l] + sums[448 + l]);
     }
-    off *= rs.inv;
+    off *= rs.inv, taken *= rs.inv;
 #pragma unroll
-    for (int tt = 0; tt < NT; tt++) dq[tt] -= off * pk[tt];
+    for (int tt = 0; tt < NT; tt++) dq[tt] -= taken * pk[tt];
     // no other workgroup reads this row's, and this one's waves have what they need
     if (j < a.N && hl == 0 && (!SPLIT || wave == 0)) static_cast<float*>(a.rows)[4 * srow + 2] = rs.delta + off;
   }
@@ -405,72 +415,98 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
   }
 }
 
-// dbias of a bias that `mult` samples share: a wave sums ds of one 32 x 32 tile over them in registers. Operands come
-// from L2, where the samples' rows lie.
+// dbias of a bias that `mult` samples share: a wave sums ds of one 32 x 32 tile over them in registers, the workgroup's four a
+// 64 x 64 one whose rows of q, dO, k and v go through LDS, the next sample's on their way meanwhile.
 template <typename T, typename BT, int KS, bool TWO>
-__global__ __launch_bounds__(256, 1) void attn_dbias_k(Attn a, int64_t tiles_k, int64_t tiles) {
-  const int l = threadIdx.x & 63, hl = l >> 5;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= tiles) return;  // whole wave; no barriers
-  const int64_t kt = w % tiles_k, tiles_q = (a.N + 31) / 32, qt = w / tiles_k % tiles_q, bh = w / tiles_k / tiles_q;
-  const int h = (int)(bh % a.H), hc = h * a.C;
-  const int64_t b = bh / a.H, j = 32 * qt + (l & 31), jc = min(j, a.N - 1), kc = min(32 * kt + (l & 31), a.M - 1);
-  const int64_t k4 = 32 * kt + 4 * hl, row = (bh * a.N + jc) * a.M;
-  f16x bias;
-#pragma unroll
-  for (int i = 0; i < 16; i++) {
-    const int64_t at = k4 + 8 * (i >> 2) + (i & 3);
-    bias[i] = at < a.M ? (float)(static_cast<const BT*>(a.bias) + row)[at] : 0.f;
+__global__ __launch_bounds__(256, 1) void attn_dbias_k(Attn a, uint32_t tiles_k, uint32_t tiles_q) {
+  constexpr int TILE = 64 * TILE_LD<T, KS>;
+  __shared__ LDS_ALIGN T tiles[(TWO ? 5 : 4) * TILE];
+  __shared__ LDS_ALIGN char bias_lds[4 * BiasRows<BT, 32>::BYTES];
+  T* const Qt = tiles;
+  T* const Dt = Qt + TILE;
+  T* const Kt = Dt + TILE;
+  T* const Vt = Kt + TILE;
+  T* const Lt = Vt + TILE;
+  const int t = threadIdx.x, l = t & 63, hl = l >> 5, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const uint32_t per_head = tiles_k * tiles_q, bh = blockIdx.x / per_head, rest = blockIdx.x - bh * per_head;
+  const int64_t q0 = 64 * (int64_t)(rest / tiles_k), k0 = 64 * (int64_t)(rest % tiles_k);
+  const int h = (int)(bh % (uint32_t)a.H), b = (int)(bh / (uint32_t)a.H), hc = h * a.C;
+  const int qw = 32 * (wave & 1), kw = 32 * (wave >> 1);  // the wave's tile
+  const int64_t j = q0 + qw + (l & 31), jc = min(j, a.N - 1), first = k0 + kw + 16 * hl;  // the lane's query and first key
+  const int64_t pitch = (int64_t)a.H * a.C;
+  Stage<T, KS, 64, 256, false> qs, ds, ls;
+  Stage<T, KS, 64, 256, true> ks, vs;
+  float mk = 1.f;
+  f4 rows;
+  const auto fetch = [&](int64_t smp) {
+    const int64_t out = (smp * a.N + q0) * pitch + hc;
+    qs.load(static_cast<const T*>(a.q) + smp * a.sq + q0 * a.ldq + hc, (uint32_t)a.ldq, a.N - q0, a.C, t);
+    ds.load(static_cast<const T*>(a.dO) + out, (uint32_t)pitch, a.N - q0, a.C, t);
+    if constexpr (TWO) ls.load(static_cast<const T*>(a.dO_lo) + out, (uint32_t)pitch, a.N - q0, a.C, t);
+    ks.load(static_cast<const T*>(a.k) + smp * a.sk + k0 * a.ldk + hc, (uint32_t)a.ldk, a.M - k0, a.C, t);
+    vs.load(static_cast<const T*>(a.v) + smp * a.sv + k0 * a.ldv + hc, (uint32_t)a.ldv, a.M - k0, a.C, t);
+    rows = static_cast<const f4*>(a.rows)[(smp * a.H + h) * a.N + jc];
+    if (a.mask) mk = a.mask[smp * a.M + min(k0 + l, a.M - 1)];
+  };
+  const int64_t s0 = (int64_t)b * a.mult, s1 = s0 + a.mult;
+  fetch(s0);
+  f16x bias, sum = f16x{};
+  {
+    const int64_t r0 = min(q0 + qw, a.N - 1), c0 = min(k0 + kw, a.M - 1);
+    BiasRows<BT, 32> bs;
+    u4* const Bt = reinterpret_cast<u4*>(bias_lds + wave * BiasRows<BT, 32>::BYTES);
+    bs.load(static_cast<const BT*>(a.bias) + ((int64_t)bh * a.N + r0) * a.M, (int)min(a.N - r0, (int64_t)32), (int)a.M, (int)c0);
+    bs.store(Bt, (int)a.M, (int)c0);
+    Form<T, true>::order();
+    bias = BiasRows<BT, 32>::get(Bt, 0);
   }
-  f16x sum = f16x{};
-  for (int64_t smp = b * a.mult; smp < (b + 1) * a.mult; smp++) {
-    const T* const q = static_cast<const T*>(a.q) + smp * a.sq + jc * a.ldq + hc;
-    const T* const dO = static_cast<const T*>(a.dO) + (smp * a.N + jc) * a.H * a.C + hc;
-    const T* const dO_lo = TWO ? static_cast<const T*>(a.dO_lo) + (smp * a.N + jc) * a.H * a.C + hc : nullptr;
-    const T* const k = static_cast<const T*>(a.k) + smp * a.sk + kc * a.ldk + hc;
-    const T* const v = static_cast<const T*>(a.v) + smp * a.sv + kc * a.ldv + hc;
-    bool on = true;
-    if (a.mask) {
-      const float* const mask = a.mask + smp * a.M;
-      on = mask[kc] != 0.f;
-      if (!__any(on)) {  // none of this tile's keys: does the sample have one at all?
-        bool found = false;
-        for (int64_t i = l; i < a.M && !found; i += 64) found = mask[i] != 0.f;
-        on = !__any(found);
-        if (!on) continue;
-      }
+  for (int64_t smp = s0; smp < s1; smp++) {
+    uint64_t keep = __ballot(k0 + l < a.M && mk != 0.f);
+    if (!keep) {  // none of these keys: does the sample have one at all?
+      bool found = false;
+      for (int64_t i = l; i < a.M && !__any(found); i += 64) found = a.mask[smp * a.M + i] != 0.f;
+      if (!__any(found)) keep = __ballot(k0 + l < a.M);
     }
-    const uint32_t keep = (uint32_t)__ballot(on) >> (4 * hl);
-    const RowStat rs(a, (smp * a.H + h) * a.N + jc);
+    const uint64_t live = all_rows((int)min(a.N - q0, (int64_t)64));
+    __syncthreads();  // the tiles' readers are done
+    qs.store(Qt, live, a.C, t);
+    ds.store(Dt, live, a.C, t);
+    if constexpr (TWO) ls.store(Lt, live, a.C, t);
+    ks.store(Kt, keep, a.C, t);
+    vs.store(Vt, keep, a.C, t);
+    RowStat rs(rows);
+    __syncthreads();
+    if (smp + 1 < s1) fetch(smp + 1);
+    if (!keep) continue;  // the same in every wave
     f16x x = f16x{}, dp = f16x{};
 #pragma unroll
     for (int m = 0; m < KS; m++) {
-      const int c = 16 * m + 8 * hl;
-      const bool in = c < a.C;
-      const frag<T> z{};
-      x = mma(in && on ? load8(k + c) : z, in ? load8(q + c) : z, x);
-      const frag<T> vm = in && on ? load8(v + c) : z;
-      dp = mma(vm, in ? load8(dO + c) : z, dp);
-      if constexpr (TWO) dp = mma(vm, in ? load8(dO_lo + c) : z, dp);
+      x = mma(row_frag<T, KS>(Kt, kw + (l & 31), m), row_frag<T, KS>(Qt, qw + (l & 31), m), x);
+      const frag<T> vm = row_frag<T, KS>(Vt, kw + (l & 31), m);
+      dp = mma(vm, row_frag<T, KS>(Dt, qw + (l & 31), m), dp);
+      if constexpr (TWO) dp = mma(vm, row_frag<T, KS>(Lt, qw + (l & 31), m), dp);
     }
+    const uint32_t on = (uint32_t)(keep >> kw) >> (16 * hl);
 #pragma unroll
     for (int i = 0; i < 16; i++) {
-      const float y = fmaf(x[i], a.scale, bias[i]);
-      const float d = rs.ex.of(y) * rs.inv * (dp[i] - rs.delta);
-      sum[i] += keep >> (8 * (i >> 2) + (i & 3)) & 1 ? d : 0.f;
+      const float d = rs.ex.of(fmaf(x[i], a.scale, bias[i])) * rs.inv * (dp[i] - rs.delta);
+      sum[i] += on >> i & 1 ? d : 0.f;
     }
   }
-  if (j >= a.N) return;
-  BT* const out = static_cast<BT*>(a.dbias) + row;
+  if (j >= a.N || first >= a.M) return;
+  BT* const out = static_cast<BT*>(a.dbias) + ((int64_t)bh * a.N + j) * a.M + first;
+  constexpr int V = 16 / (int)sizeof(BT);
 #pragma unroll
-  for (int qq = 0; qq < 4; qq++) {
-    const int64_t at = k4 + 8 * qq;
-    if (at + 4 <= a.M) {
-      store_chunk<4, false>(out + at, fv<4>{sum[4 * qq], sum[4 * qq + 1], sum[4 * qq + 2], sum[4 * qq + 3]});
+  for (int c = 0; c < 16; c += V) {
+    if (first + c + V <= a.M) {
+      fv<V> y;
+#pragma unroll
+      for (int e = 0; e < V; e++) y[e] = sum[c + e];
+      store_chunk<V, false>(out + c, y);
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (at + e < a.M) out[at + e] = (BT)sum[4 * qq + e];
+      for (int e = 0; e < V; e++)
+        if (first + c + e < a.M) out[c + e] = (BT)sum[c + e];
     }
   }
 }
@@ -521,9 +557,9 @@ hipError_t launch_attention_bwd(Attn a, void* ws, hipStream_t st) {
       hipError_t e = with_split<KS>(a.N, a, dq);
       if (e == hipSuccess) e = with_split<KS>(a.M, a, dkv);
       if (e != hipSuccess || !a.dbias || a.mult == 1) return e;
-      const int64_t tk = (a.M + 31) / 32, tiles = tk * ((a.N + 31) / 32) * a.H * (a.S / a.mult);
-      if ((tiles + 3) / 4 > INT32_MAX) return hipErrorInvalidValue;
-      attn_dbias_k<T, BT, KS, TWO><<<(unsigned)((tiles + 3) / 4), 256, 0, st>>>(a, tk, tiles);
+      const int64_t tk = (a.M + 63) / 64, tq = (a.N + 63) / 64, tiles = tk * tq * a.H * (a.S / a.mult);
+      if (tiles > INT32_MAX) return hipErrorInvalidValue;
+      attn_dbias_k<T, BT, KS, TWO><<<(unsigned)tiles, 256, 0, st>>>(a, (uint32_t)tk, (uint32_t)tq);
       return hipGetLastError();
     };
     if constexpr (sizeof(T) == 2) {

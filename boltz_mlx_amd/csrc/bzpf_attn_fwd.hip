@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_f
     if (mask) mk = mask[min(k0 + l, a.M - 1)];
   };
   const auto fetch_bias = [&](int64_t k0) {
-    if (bias) bs.load(bias + k0, brows, a.M, a.M - k0);
+    if (bias) bs.load(bias, brows, (int)a.M, (int)k0);
   };
   constexpr int STEP = F::GROUPS * BK;
   int64_t k0 = group * BK;
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_f
     T* const Vb = Vt + buf * TILE;
     ks.store(Kb, keep, a.C, t);
     vs.store(Vb, keep, a.C, t);
-    if (bias) bs.store(Bt);
+    if (bias) bs.store(Bt, (int)a.M, (int)k0);
     F::sync();
     const bool more = k0 + STEP < a.M;
     if (more) {

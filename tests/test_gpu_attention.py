@@ -399,7 +399,10 @@ def tolerances(a, H, dtype, dout=None):
     raw = heads(np.abs(dout) * ((t_out + h * (np.abs(out) + t_out) + tiny) * 1.0), H).sum(-1, keepdims=True)
     scale = 1 / np.sqrt(C)
     low = tiny / total
-    t["q"] = scale * rows((eds + h * (np.abs(ds) + 2 * p * raw) + low * (1 + raw)) @ ak + U * M * ((np.abs(ds) + p * raw) @ ak))
+    # Half types take the rounded ds' own sum off dq: with e_j the rounding of ds_j, (sum of e_j ds_j) (sum of p k) on top of the
+    # (sum of e_j ds_j k_j) that the products have, together sum of e_j ds_j (k_j - sum of p k); raw's part of ds as there.
+    taken = (h * (np.abs(ds) + p * raw) + low * np.ones_like(ds)).sum(-1, keepdims=True) * np.abs(p @ heads(k, H)) * (1 + h)
+    t["q"] = scale * rows((eds + h * (np.abs(ds) + 2 * p * raw) + low * (1 + raw)) @ ak + U * M * ((np.abs(ds) + p * raw) @ ak) + taken)
     t["k"] = scale * rows((eds + h * np.abs(ds) + tiny).swapaxes(-1, -2) @ aq + U * N * (np.abs(ds).swapaxes(-1, -2) @ aq))
     t["v"] = rows((p * (Ep + h + U * N) + tiny).swapaxes(-1, -2) @ np.abs(d) + p.swapaxes(-1, -2) @ ed)
     if g is not None:
