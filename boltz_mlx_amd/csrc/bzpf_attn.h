@@ -306,13 +306,29 @@ struct Columns {
     else
       return __builtin_bit_cast(BT, (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rsrc, v, s, 0));
   }
-  __device__ __forceinline__ void put(uint32_t lane, int r, bool whole, float x) const {
+  // 16 values on their way to memory: those of half types in pairs, as conversions make them; zeros where not `on`.
+  struct Packed {
+    static constexpr int E = 4 / (int)sizeof(BT);
+    uint32_t w[16 / E];
+    __device__ __forceinline__ Packed(const f16x& x, bool on) {
+      typedef BT V __attribute__((ext_vector_type(E)));
+#pragma unroll
+      for (int i = 0; i < 16; i += E) {
+        V v;
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = (BT)x[i + e];
+        w[i / E] = on ? __builtin_bit_cast(uint32_t, v) : 0u;
+      }
+    }
+    __device__ __forceinline__ uint32_t operator[](int i) const { return w[i / E] >> (32 / E * (i % E) & 31); }
+  };
+  __device__ __forceinline__ void put(uint32_t lane, int r, bool whole, uint32_t x) const {
     if (!whole) asm volatile("" : "+v"(lane));
     const int v = whole ? (int)lane : (int)(lane + r * pitch), s = whole ? (int)(r * pitch) : 0;
     if constexpr (sizeof(BT) == 2)
-      __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (BT)x), rsrc, v, s, 0);
+      __builtin_amdgcn_raw_buffer_store_b16((uint16_t)x, rsrc, v, s, 0);
     else
-      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, (BT)x), rsrc, v, s, 0);
+      __builtin_amdgcn_raw_buffer_store_b32(x, rsrc, v, s, 0);
   }
 };
 

@@ -291,19 +291,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
   Stage<T, KS, BQ, F::NTH, false> qs, ds, ls;
   BT bs[16] = {};  // the next tile's biases, a row's 32 keys a half wave and instruction; zero where there are none
   f4 st;
+  // The loop's loads depend on no condition (past the end they repeat the last block): the waits after a branch that leaves
+  // some out would be for all loads in flight, the next block's among them.
   const auto fetch = [&](int64_t q0) {
+    q0 = min(q0, (a.N - 1) / BQ * BQ);
     qs.load(q + q0 * a.ldq, (uint32_t)a.ldq, a.N - q0, a.C, t);
     ds.load(dO + q0 * pitch, (uint32_t)pitch, a.N - q0, a.C, t);
     if constexpr (TWO) ls.load(dO_lo + q0 * pitch, (uint32_t)pitch, a.N - q0, a.C, t);
-    if (t < BQ) {
-      st = static_cast<const f4*>(a.rows)[srow + min(q0 + t, a.N - 1)];
-      if (q0 + t >= a.N) st = f4{INFINITY, 0.f, 0.f, LOG2E};  // past the end: 2^(y by - inf) = 0
-    }
+    st = static_cast<const f4*>(a.rows)[srow + min(q0 + t % BQ, a.N - 1)];
   };
   const auto fetch_bias = [&](int64_t r0) {
-    if (!bias || r0 >= a.N) return;
+    r0 = min(r0, (a.N - 1) / 32 * 32);
     const int n = (int)min(a.N - r0, (int64_t)32);
-    const Columns<BT> at(bias + r0 * a.M, n, a.M);
+    const Columns<BT> at(bias ? bias + r0 * a.M : nullptr, bias ? n : 0, a.M);
     if (n == 32) {
 #pragma unroll
       for (int i = 0; i < 16; i++) bs[i] = at.get(boff, 8 * (i >> 2) + (i & 3), true);
@@ -312,9 +312,23 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
       for (int i = 0; i < 16; i++) bs[i] = at.get(boff, 8 * (i >> 2) + (i & 3), false);
     }
   };
+  // A key that takes no part has zeros; lanes without a key write past every buffer's end.
+  const uint32_t to = key < a.M ? boff : 0x80000000u;
+  const auto put_bias = [&](int64_t r0, const f16x& x) {
+    const int n = (int)min(a.N - r0, (int64_t)32);
+    const Columns<BT> at(db + r0 * a.M, n, a.M);
+    const typename Columns<BT>::Packed v(x, on);
+    if (n == 32) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) at.put(to, 8 * (i >> 2) + (i & 3), true, v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; i++) at.put(to, 8 * (i >> 2) + (i & 3), false, v[i]);
+    }
+  };
   constexpr int STEP = F::GROUPS * BQ;
   int64_t q0 = group * BQ;
-  if (q0 < a.N) fetch(q0);
+  fetch(q0);
   fetch_bias(q0);
   for (int buf = 0; q0 < a.N; q0 += STEP, buf = (buf + 1) % F::BUFS) {
     const uint64_t rows = all_rows((int)min(a.N - q0, (int64_t)BQ));
@@ -326,13 +340,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
     ds.store(Db, rows, a.C, t);
     if constexpr (TWO) ls.store(Lb, rows, a.C, t);
     if (t < BQ) {
+      if (q0 + t >= a.N) st = f4{INFINITY, 0.f, 0.f, LOG2E};  // past the end: 2^(y by - inf) = 0
 #pragma unroll
       for (int i = 0; i < 4; i++) Sb[i][t] = st[i];
       Big[group][buf] = __any(st[3] != LOG2E);
     }
     F::sync();
     const bool big = __builtin_amdgcn_readfirstlane(Big[group][buf]);  // a row with an exponent of its own (Exponent)
-    if (q0 + STEP < a.N) fetch(q0 + STEP);
+    fetch(q0 + STEP);
 #pragma unroll
     for (int qt = 0; qt < QT; qt++) {
       const int64_t r0 = q0 + 32 * qt;
@@ -367,16 +382,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
       if (big) probs(std::true_type());
       else probs(std::false_type());
       fetch_bias(next);
-      if (db && key < a.M) {
-        const Columns<BT> at(db + r0 * a.M, (int)min(a.N - r0, (int64_t)32), a.M);
-        if (r0 + 32 <= a.N) {
-#pragma unroll
-          for (int i = 0; i < 16; i++) at.put(boff, 8 * (i >> 2) + (i & 3), true, on ? dp[i] : 0.f);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; i++) at.put(boff, 8 * (i >> 2) + (i & 3), false, on ? dp[i] : 0.f);
-        }
-      }
+      if (db) put_bias(r0, dp);
 #pragma unroll
       for (int s = 0; s < 2; s++) {
         const frag<T> p = as_frag<T>(x, s), d = as_frag<T>(dp, s);

@@ -94,15 +94,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_f
       x[kt] = s;
     }
     most = both_max(most);
-    if (__any(most > top)) {
-      const Exponent now(most);
-      const float by = __builtin_amdgcn_exp2f(fminf(ex.at - now.at, 0.f));  // a row without logits so far: 0 times anything
+    const Exponent now(most);
+    const float by = __builtin_amdgcn_exp2f(fminf(ex.at - now.at, 0.f));  // a row without logits so far: 0 times anything
 #pragma unroll
-      for (int tt = 0; tt < NT; tt++) o[tt] *= by;
-      sum *= by;
-      top = most;
-      ex = now;
-    }
+    for (int tt = 0; tt < NT; tt++) o[tt] *= by;
+    sum *= by;
+    top = most;
+    ex = now;
 #pragma unroll
     for (int kt = 0; kt < KT; kt++) {
 #pragma unroll
