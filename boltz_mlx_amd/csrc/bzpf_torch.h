@@ -71,7 +71,13 @@ inline void once(const char* name) {
 }
 inline int64_t type_of(const Tensor& t) { return static_cast<int64_t>(t.defined() ? t.scalar_type() : at::kFloat); }
 // A parameter's gradient in its type.
-inline Tensor as(const Tensor& g, int64_t type) { return g.defined() ? g.to(static_cast<at::ScalarType>(type)) : g; }
+inline Tensor as(const Tensor& g, int64_t type) {
+  return g.defined() && type_of(g) != type ? g.to(static_cast<at::ScalarType>(type)) : g;
+}
+// A parameter as the kernels read it (itself where it is so already: a call's host time counts beside kernels of a few us).
+inline Tensor param(const Tensor& w) {
+  return !w.defined() || (w.scalar_type() == at::kFloat && w.is_contiguous()) ? w : w.detach().to(at::kFloat).contiguous();
+}
 
 // Adds the functions of the sequence attention's training form to the module (bzpf_torch_attn.cpp).
 void bind_attention(pybind11::module_& m);

@@ -67,7 +67,7 @@ Tensor rel_bias(const Tensor& table, Rel r, const Tensor& add_, at::ScalarType t
   }
   on_gpu(name, table, r.pos_q);
   const OnDevice dev(table);
-  const Tensor w = table.detach().to(at::kFloat).contiguous(), add = add_.defined() ? add_.contiguous() : add_;
+  const Tensor w = param(table), add = add_.defined() ? add_.contiguous() : add_;
   const auto opt = table.options().dtype(to);
   const Tensor y = r.batched ? at::empty({r.B, H, r.N, r.M}, opt) : at::empty({H, r.N, r.M}, opt);
   if (y.numel())
@@ -174,7 +174,6 @@ struct QK {
       pos_rows = pos.numel();
       wide = pos.scalar_type() == at::kLong;
     }
-    const auto param = [](const Tensor& w) { return w.defined() ? w.detach().to(at::kFloat).contiguous() : w; };
     wq = param(wq_), wk = param(wk_);
   }
 };
