@@ -343,9 +343,8 @@ __device__ __forceinline__ float both_sum(float v) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-// Whether the mask leaves the sample a key (256 threads): one without keys runs without its mask.
+// Whether the mask leaves the sample a key (all 256 threads of the workgroup): one without keys runs without its mask.
 __device__ __forceinline__ bool any_key(const float* mask, int64_t M) {
-  if (!mask) return true;
   for (int64_t k = 0; k < M; k += 256) {
     const int64_t at = k + threadIdx.x;
     if (__syncthreads_or(at < M && mask[at] != 0.0f)) return true;

@@ -97,7 +97,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
   const int brows = (int)min(a.N - b0, (int64_t)32);
   u4* const Bt = reinterpret_cast<u4*>(bias_lds + wave * BiasRows<BT, BK>::BYTES);
   const float* mask = a.mask ? a.mask + un.smp * a.M : nullptr;
-  if (!any_key(mask, a.M)) mask = nullptr;
   const int64_t srow = ((int64_t)un.smp * a.H + un.h) * a.N + jc;
   const RowStat rs(static_cast<const f4*>(a.rows)[srow]);
 
@@ -141,8 +140,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
     fetch(k0);
     fetch_bias(k0);
   }
+  const bool masked = mask && any_key(mask, a.M);  // the first loads are on their way
   for (int buf = 0; k0 < a.M; k0 += STEP, buf = (buf + 1) % F::BUFS) {
-    const uint64_t keep = __ballot(k0 + l < a.M && l < BK && mk != 0.f);
+    const uint64_t keep = __ballot(k0 + l < a.M && l < BK && (!masked || mk != 0.f));
     T* const Kb = Kt + buf * TILE;
     T* const Vb = Vt + buf * TILE;
     ks.store(Kb, keep, a.C, t);
@@ -274,16 +274,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
   const uint32_t boff = (4 * hl * (uint32_t)a.M + (uint32_t)kc) * (uint32_t)sizeof(BT);  // a lane's first row of a tile, its key
   const int64_t srow = ((int64_t)un.smp * a.H + un.h) * a.N;
   const float* mask = a.mask ? a.mask + un.smp * a.M : nullptr;
-  if (!any_key(mask, a.M)) mask = nullptr;
-  const bool on = key < a.M && (!mask || mask[kc] != 0.f);
-
   frag<T> kf[KS], vf[KS];
 #pragma unroll
   for (int m = 0; m < KS; m++) {
-    const bool in = on && 16 * m + 8 * hl < a.C;
-    kf[m] = in ? load8(k + 16 * m + 8 * hl) : frag<T>{};
-    vf[m] = in ? load8(v + 16 * m + 8 * hl) : frag<T>{};
+    const int c = 16 * m + 8 * hl < a.C ? 16 * m + 8 * hl : 0;
+    kf[m] = load8(k + c);
+    vf[m] = load8(v + c);
   }
+  const float mk = mask ? mask[kc] : 1.f;
   f16x dk[NT], dv[NT];
 #pragma unroll
   for (int tt = 0; tt < NT; tt++) dk[tt] = dv[tt] = f16x{};
@@ -312,6 +310,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
       for (int i = 0; i < 16; i++) bs[i] = at.get(boff, 8 * (i >> 2) + (i & 3), false);
     }
   };
+  constexpr int STEP = F::GROUPS * BQ;
+  int64_t q0 = group * BQ;
+  fetch(q0);
+  fetch_bias(q0);
+  const bool masked = mask && any_key(mask, a.M);  // of the whole workgroup; the first loads are on their way
+  const bool on = key < a.M && (!masked || mk != 0.f);
+#pragma unroll
+  for (int m = 0; m < KS; m++) {
+    const bool in = on && 16 * m + 8 * hl < a.C;
+    kf[m] = in ? kf[m] : frag<T>{};
+    vf[m] = in ? vf[m] : frag<T>{};
+  }
   // A key that takes no part has zeros; lanes without a key write past every buffer's end.
   const uint32_t to = key < a.M ? boff : 0x80000000u;
   const auto put_bias = [&](int64_t r0, const f16x& x) {
@@ -326,10 +336,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
       for (int i = 0; i < 16; i++) at.put(to, 8 * (i >> 2) + (i & 3), false, v[i]);
     }
   };
-  constexpr int STEP = F::GROUPS * BQ;
-  int64_t q0 = group * BQ;
-  fetch(q0);
-  fetch_bias(q0);
   for (int buf = 0; q0 < a.N; q0 += STEP, buf = (buf + 1) % F::BUFS) {
     const uint64_t rows = all_rows((int)min(a.N - q0, (int64_t)BQ));
     T* const Qb = Qt + buf * TILE;

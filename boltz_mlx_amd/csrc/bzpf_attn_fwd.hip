@@ -32,7 +32,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_f
   const int brows = (int)min(a.N - b0, (int64_t)32);
   u4* const Bt = reinterpret_cast<u4*>(bias_lds + wave * BiasRows<BT, BK>::BYTES);
   const float* mask = a.mask ? a.mask + un.smp * a.M : nullptr;
-  if (!any_key(mask, a.M)) mask = nullptr;
 
   frag<T> qf[KS];
 #pragma unroll
@@ -60,8 +59,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_f
     fetch(k0);
     fetch_bias(k0);
   }
+  const bool masked = mask && any_key(mask, a.M);  // the first loads are on their way
   for (int buf = 0; k0 < a.M; k0 += STEP, buf = (buf + 1) % F::BUFS) {
-    const uint64_t keep = __ballot(k0 + l < a.M && l < BK && mk != 0.f);
+    const uint64_t keep = __ballot(k0 + l < a.M && l < BK && (!masked || mk != 0.f));
     T* const Kb = Kt + buf * TILE;
     T* const Vb = Vt + buf * TILE;
     ks.store(Kb, keep, a.C, t);
