@@ -34,8 +34,9 @@ SIGNATURES = {
     "bzpf_qk_norm_rope_bwd_ws": [i32],
     "bzpf_qk_norm_rope_bwd": [vp, vp, i32, vp, i64, vp, i64, i32, vp, vp, f32, vp, i32, i64, f64, i32, i32, vp, vp, vp, vp, vp,
                               i64, i64, i32, i32, i32, vp],
-    "bzpf_attention": [vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i64,
-                       i64, vp],
+    "bzpf_attention_ws": [i32, i32, i32, i64, i64],
+    "bzpf_attention": [vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i32, i32, vp, vp, vp, vp, i64, i32, i32, i32,
+                       i32, i64, i64, vp],
     "bzpf_attention_bwd_ws": [i32, i32, i32, i32, i64, i64, i32],
     "bzpf_attention_bwd": [vp, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp,
                            vp, vp, i64, i32, i32, i32, i32, i64, i64, vp],
@@ -84,7 +85,8 @@ SIGNATURES = {
 }
 _RESTYPES = {"bzpf_version": C.c_char_p, "bzpf_last_error": C.c_char_p, "bzpf_row_pitch": i64,
              "bzpf_pwa_wsplit_bytes": i64, "bzpf_layernorm_bwd_ws": i64, "bzpf_rel_bias_bwd_ws": i64,
-             "bzpf_qk_norm_rope_bwd_ws": i64, "bzpf_attention_bwd_ws": i64}
+             "bzpf_qk_norm_rope_bwd_ws": i64, "bzpf_attention_ws": i64,
+             "bzpf_attention_bwd_ws": i64}
 
 _lib = None
 

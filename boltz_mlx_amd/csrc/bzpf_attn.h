@@ -19,20 +19,40 @@ namespace bzpf {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-// A row's exponentials are 2^(x by - at) for by = log2 e and at = top by rounded: one instruction before the exponential. What
-// the rounding of at is worth, 2^-off(), is put right once for a row. From 2^100 on two logits are equal or 2^76 apart, and
-// by = 2^-64 says as much without overflow: a row whose logits are all the type's lowest value is a softmax over equals. A row
+// A row's exponentials are 2^(x log2 e - at) for at = top log2 e rounded: one instruction before the exponential. What the
+// rounding of at is worth, 2^off, is put right once for a row. Past 2^20 that would be too much for a half type's
+// probabilities (and from 2^30 on for any): such a row (`big`) has 2^((x - top) log2 e), two instructions, with by = 1 and
+// at = top; so a row whose logits are all the type's lowest value, or all one bar of any size, is a softmax over equals. A row
 // without logits (top = -inf) has at = 0 and exponentials of 0.
 struct Exponent {
-  float by, at;
+  float top, by, at;
   __device__ __forceinline__ Exponent() {}
-  __device__ __forceinline__ explicit Exponent(float top) {
-    by = __builtin_fabsf(top) > 0x1p100f ? 0x1p-64f : LOG2E;
-    at = top == -INFINITY ? 0.f : top * by;
+  __device__ __forceinline__ explicit Exponent(float t) : top(t) {
+    by = __builtin_fabsf(t) > 0x1p20f && t != -INFINITY ? 1.0f : LOG2E;
+    at = t == -INFINITY ? 0.f : t * by;
   }
-  __device__ __forceinline__ float of(float x) const { return __builtin_amdgcn_exp2f(fmaf(x, by, -at)); }
-  __device__ __forceinline__ float off(float top) const { return top == -INFINITY ? 0.f : fmaf(top, by, -at); }
+  __device__ __forceinline__ bool big() const { return by == 1.0f; }
+  __device__ __forceinline__ float of(float x) const {
+    const float z = fmaf(x, by, -at);
+    return __builtin_amdgcn_exp2f(big() ? z * LOG2E : z);
+  }
+  __device__ __forceinline__ float off() const { return top == -INFINITY ? 0.f : fmaf(top, by, -at); }
+  // What sums of an earlier maximum are worth at this one, which is no smaller (of a row without logits so far: nothing).
+  __device__ __forceinline__ float since(const Exponent& old) const {
+    return old.top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(fmaf(old.top - top, LOG2E, off() - old.off()));
+  }
 };
+
+// 16 logits' exponentials for a row a lane, where waves without big rows have one instruction each.
+__device__ __forceinline__ void exponentials(f16x& x, const Exponent& ex, bool some_big) {
+  if (some_big) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) x[i] = ex.big() ? (x[i] - ex.at) * LOG2E : x[i];
+  }
+  const float at = ex.big() ? 0.f : ex.at;
+#pragma unroll
+  for (int i = 0; i < 16; i++) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], ex.by, -at));
+}
 
 // How a launch's waves work (attn_form chooses): in the wide form the four waves of a workgroup hold 32 rows each and share
 // tiles of the other side's rows, in two buffers; in the split form they hold the same 32 rows, each with every fourth block

@@ -247,20 +247,30 @@ int make_attn(const char* who, const void* q, int64_t ldq, int64_t sq, const voi
 
 extern "C" {
 
+int64_t bzpf_attention_ws(int S_, int H, int C, int64_t N, int64_t M) {
+  if (S_ < 1 || H < 1 || H > 65535 || C < 8 || C > 128 || C % 8 || N < 1 || N > ATT_LEN || M < 1 || M > ATT_LEN) return -1;
+  bzpf::Attn a{};
+  a.S = S_, a.H = H, a.C = C, a.N = N, a.M = M;
+  return bzpf::attention_ws_bytes(a);
+}
+
 int bzpf_attention(const void* q, int64_t ldq, int64_t sq, const void* k, int64_t ldk, int64_t sk, const void* v, int64_t ldv,
                    int64_t sv, const void* g, int64_t ldg, int64_t sg, const void* bias, int bias_dt, int mult,
-                   const float* mask, void* out, float* stats, int dt, int S_, int H, int C, int64_t N, int64_t M,
-                   void* stream) {
+                   const float* mask, void* out, float* stats, void* ws, int64_t ws_bytes, int dt, int S_, int H, int C,
+                   int64_t N, int64_t M, void* stream) {
   bzpf::Attn a;
   const int rc = make_attn("bzpf_attention", q, ldq, sq, k, ldk, sk, v, ldv, sv, g, ldg, sg, bias, bias_dt, mult, mask, out,
                            stats, dt, S_, H, C, N, M, &a);
   if (rc != BZPF_OK) return rc;
   const int64_t w = (int64_t)H * C;
-  const Range outs[] = {{out, S_ * N * w * size_of(dt)}, {stats, (int64_t)S_ * H * N * 8}};
+  const int64_t need = bzpf::attention_ws_bytes(a);
+  REQUIRE(ws_bytes >= need && (ws || !need), "bzpf_attention: ws holds %lld bytes of %lld", (long long)(ws ? ws_bytes : 0), (long long)need);
+  REQUIRE(((uintptr_t)ws & 15) == 0, "bzpf_attention: ws must be 16-byte aligned");
+  const Range outs[] = {{out, S_ * N * w * size_of(dt)}, {stats, (int64_t)S_ * H * N * 8}, {ws, need}};
   const Range ins[] = {{q, extent(S_, sq, N, ldq, w, dt)}, {k, extent(S_, sk, M, ldk, w, dt)}, {v, extent(S_, sv, M, ldv, w, dt)},
                        {g, extent(S_, sg, N, ldg, w, dt)}, {bias, (int64_t)(S_ / mult) * H * N * M * size_of(bias_dt)}, {mask, S_ * M * 4}};
   REQUIRE(all_apart(outs, ins), "bzpf_attention: out or stats overlaps another tensor");
-  return done(bzpf::launch_attention(a, S(stream)), "bzpf_attention");
+  return done(bzpf::launch_attention(a, ws, S(stream)), "bzpf_attention");
 }
 
 int64_t bzpf_attention_bwd_ws(int dt, int S_, int H, int C, int64_t N, int64_t M, int gate) {

@@ -17,7 +17,7 @@ namespace bzpf {
 
 namespace {
 
-// What the other kernels need of a row (p = 2^(x by - at) inv), [S][H][N], and with a gate dO (two parts in half types) and
+// What the other kernels need of a row (p = Exponent(by, at).of(x) inv), [S][H][N], and with a gate dO (two parts in half types) and
 // dg. L lanes a head, 8 channels each.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_rows_k(Attn a, int L) {
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256) void attn_rows_k(Attn a, int L) {
     const int64_t to = (smp * a.H + h) * a.N + row - smp * a.N;
     const float top = a.stats[2 * to], sum = a.stats[2 * to + 1];
     const Exponent ex(top);
-    static_cast<f4*>(a.rows)[to] = f4{ex.at, sum == 0.f ? 0.f : __builtin_amdgcn_exp2f(-ex.off(top)) / sum, d, ex.by};
+    static_cast<f4*>(a.rows)[to] = f4{ex.at, sum == 0.f ? 0.f : __builtin_amdgcn_exp2f(-ex.off()) / sum, d, ex.by};
   }
 }
 
@@ -99,6 +99,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
   const float* mask = a.mask ? a.mask + un.smp * a.M : nullptr;
   const int64_t srow = ((int64_t)un.smp * a.H + un.h) * a.N + jc;
   const RowStat rs(static_cast<const f4*>(a.rows)[srow]);
+  const bool some_big = __any(rs.ex.big());
 
   // dO's second part waits in LDS in the wide form (in registers it had 64 channels spill: XX us instead of XX).
   constexpr bool ASIDE = TWO && !SPLIT;
@@ -168,10 +169,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
       f16x b = f16x{};
       if (bias) b = BiasRows<BT, BK>::get(Bt, kt);
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
-        x[i] = rs.ex.of(fmaf(x[i], a.scale, b[i]));
-        dp[i] = x[i] * (dp[i] - rs.delta);
-      }
+      for (int i = 0; i < 16; i++) x[i] = fmaf(x[i], a.scale, b[i]);
+      exponentials(x, rs.ex, some_big);
+#pragma unroll
+      for (int i = 0; i < 16; i++) dp[i] = x[i] * (dp[i] - rs.delta);
       if (keep != all_rows(BK)) {
         const uint32_t w = (uint32_t)(keep >> (32 * kt)) >> (16 * hl);
 #pragma unroll
@@ -352,7 +353,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
       Big[group][buf] = __any(st[3] != LOG2E);
     }
     F::sync();
-    const bool big = __builtin_amdgcn_readfirstlane(Big[group][buf]);  // a row with an exponent of its own (Exponent)
+    const bool big = __builtin_amdgcn_readfirstlane(Big[group][buf]);  // a big row (Exponent)
     fetch(q0 + STEP);
 #pragma unroll
     for (int qt = 0; qt < QT; qt++) {
@@ -379,7 +380,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const int i = 4 * qq + e;
-            x[i] = __builtin_amdgcn_exp2f(fmaf(fmaf(x[i], a.scale, (float)bs[i]), by[e], -at[e])) * inv[e];
+            float z = fmaf(fmaf(x[i], a.scale, (float)bs[i]), by[e], -at[e]);
+            if constexpr (any()) z = by[e] == 1.0f ? z * LOG2E : z;
+            x[i] = __builtin_amdgcn_exp2f(z) * inv[e];
             dp[i] = x[i] * (dp[i] - delta[e]);
           }
           __builtin_amdgcn_sched_barrier(0);  // sixteen rows' statistics at once would not fit in the registers

@@ -216,7 +216,8 @@ struct Attn {
   void* dO;      // [S][N][H C]: sigmoid(g) dout
   void* dO_lo;   // what rounding to a half type has left of it
 };
-hipError_t launch_attention(const Attn& a, hipStream_t st);
+int64_t attention_ws_bytes(const Attn& a);  // of S, N, M, H and C alone
+hipError_t launch_attention(const Attn& a, void* ws, hipStream_t st);
 int64_t attention_bwd_ws_bytes(int dt, int64_t S, int64_t N, int H, int C, bool gate);
 hipError_t launch_attention_bwd(Attn a, void* ws, hipStream_t st);
 

@@ -39,7 +39,7 @@ struct OnDevice {
 #define BZPF_ENTRIES(X)                                                                                                \
   X(last_error) X(layernorm) X(layernorm_bwd_ws) X(layernorm_bwd) X(dropout) X(dropout_add_ln) X(dropout_add_ln_bwd) \
   X(rel_bias) X(rel_bias_bwd_ws) X(rel_bias_bwd) X(qk_norm_rope) X(qk_norm_rope_bwd_ws) X(qk_norm_rope_bwd)            \
-  X(attention) X(attention_bwd_ws) X(attention_bwd)
+  X(attention_ws) X(attention) X(attention_bwd_ws) X(attention_bwd)
 struct Entries {
 #define X(f) decltype(&::bzpf_##f) f;
   BZPF_ENTRIES(X)

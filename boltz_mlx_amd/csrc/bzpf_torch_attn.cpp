@@ -309,8 +309,10 @@ std::tuple<Tensor, Tensor> attention(const Att& a) {
     stats.select(-1, 1).zero_();
     return {o, stats};
   }
+  const int64_t bytes = lib.attention_ws((int)a.S, (int)a.H, (int)a.C, a.N, a.M);
+  const Tensor ws = bytes > 0 ? at::empty({bytes}, a.q.options().dtype(at::kByte)) : Tensor();
   check(lib.attention(BZPF_ROWS(a.q), BZPF_ROWS(a.k), BZPF_ROWS(a.v), BZPF_ROWS(a.g), in(a.bias), a.bias_type(), (int)a.mult,
-                      f32(a.mask), out(o), f32_out(stats), type_code(a.q), (int)a.S, (int)a.H, (int)a.C, a.N, a.M, dev.stream),
+                      f32(a.mask), out(o), f32_out(stats), out(ws), bytes, type_code(a.q), (int)a.S, (int)a.H, (int)a.C, a.N, a.M, dev.stream),
         "bzpf_attention");
   return {o, stats};
 }

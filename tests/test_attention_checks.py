@@ -90,7 +90,7 @@ def test_qk_norm_rope_bwd_refuses(change):
 
 
 ATT = dict(q=AT[0], ldq=48, sq=240, k=AT[1], ldk=48, sk=336, v=AT[2], ldv=48, sv=336, g=AT[3], ldg=48, sg=240, bias=AT[4], bias_dt=F16,
-           mult=2, mask=AT[5], out=AT[6], stats=AT[7], dt=F16, S=2, H=3, C=16, N=5, M=7, stream=None)
+           mult=2, mask=AT[5], out=AT[6], stats=AT[7], ws=None, ws_bytes=0, dt=F16, S=2, H=3, C=16, N=5, M=7, stream=None)
 
 
 @pytest.mark.parametrize("change", [
@@ -99,10 +99,20 @@ ATT = dict(q=AT[0], ldq=48, sq=240, k=AT[1], ldk=48, sk=336, v=AT[2], ldv=48, sv
     {"bias_dt": BF16}, {"dt": F32, "bias_dt": 7}, {"C": 0}, {"C": 12}, {"C": 136}, {"H": 0}, {"S": 0}, {"mult": 0}, {"mult": 3}, {"N": 0},
     {"M": 0}, {"N": -1}, {"N": 2 ** 22 + 1}, {"M": 2 ** 22 + 1}, {"ldq": 47}, {"ldk": 40}, {"ldv": 0}, {"ldg": 1}, {"sq": -1}, {"sv": -8},
     {"sk": 2 ** 62}, {"ldk": 2 ** 23}, {"ldg": 2 ** 60}, {"out": AT[0]}, {"out": AT[1] + 600}, {"out": AT[4]}, {"stats": AT[6]}, {"stats": AT[5]},
-    {"out": AT[3] + 900},
+    {"out": AT[3] + 900}, {"ws": AT[8] + 8}, {"ws_bytes": -1},
 ])
 def test_attention_refuses(change):
     assert rc("bzpf_attention", ATT, change) == -1
+
+
+@pytest.mark.parametrize("ws, size, what", [(None, 1 << 40, "ws holds 0"), (1 << 40, 1000, "ws holds 1000"),
+                                            ((1 << 40) + 4, 1 << 40, "16-byte"), (1 << 44, 1 << 40, "overlaps")])
+def test_attention_refuses_workspaces(ws, size, what):
+    """One query against a long axis, whose parts meet in the workspace."""
+    few = dict(q=1 << 41, k=1 << 42, sk=0, v=1 << 43, sv=0, g=None, bias=None, mult=1, mask=None, out=1 << 44, stats=1 << 45, S=1, N=1, M=50001)
+    assert _lib.load().bzpf_attention_ws(1, 3, 16, 1, 50001) > 1000
+    assert rc("bzpf_attention", ATT, dict(few, ws=ws, ws_bytes=size)) == -1
+    assert what in _lib.load().bzpf_last_error().decode()
 
 
 ATT_BWD = dict(dout=AT[8], q=AT[0], ldq=48, sq=240, k=AT[1], ldk=48, sk=336, v=AT[2], ldv=48, sv=336, g=AT[3], ldg=48, sg=240,
@@ -125,6 +135,9 @@ def test_workspace_sizes():
     assert lib.bzpf_attention_bwd_ws(F32, 2, 3, 16, 5, 7, 1) >= 2 * 3 * 5 * 4 + 2 * 3 * 5 * 16 * 4
     for bad in ((3, 2, 3, 16, 5, 7, 0), (F32, 0, 3, 16, 5, 7, 0), (F32, 2, 3, 12, 5, 7, 0), (F32, 2, 3, 16, 0, 7, 0), (F32, 2, 3, 136, 5, 7, 1)):
         assert lib.bzpf_attention_bwd_ws(*bad) == -1
+    assert lib.bzpf_attention_ws(2, 3, 16, 5, 10000) == lib.bzpf_attention_ws(1, 1, 16, 1, 1) == 0 < lib.bzpf_attention_ws(1, 1, 128, 2, 1 << 22)
+    for bad in ((0, 3, 16, 5, 7), (2, 0, 16, 5, 7), (2, 3, 20, 5, 7), (2, 3, 16, 0, 7), (2, 3, 16, 5, (1 << 22) + 1)):
+        assert lib.bzpf_attention_ws(*bad) == -1
     assert lib.bzpf_rel_bias_bwd_ws(1, 16, 400, 400, 66) > 0 and lib.bzpf_qk_norm_rope_bwd_ws(24) > 0
     assert lib.bzpf_rel_bias_bwd_ws(1, 16, 400, 400, 0) == lib.bzpf_rel_bias_bwd_ws(0, 1, 1, 1, 1) == -1
     assert lib.bzpf_qk_norm_rope_bwd_ws(25) == lib.bzpf_qk_norm_rope_bwd_ws(258) == -1

@@ -470,6 +470,66 @@ def test_attention_half_bias_with_fp32(bias):
     check(inputs(3, 2, 1, 2, 32, 33, 64, F32, bias, False, "holes"), 2)
 
 
+@pytest.mark.parametrize("S, mult, H, C, N, M, dtype", [
+    (1, 1, 16, 24, 1, 400, F32), (2, 2, 3, 64, 1, 5000, F32), (1, 1, 2, 128, 3, 2050, BF16), (3, 1, 1, 8, 4, 1025, F16),
+    (1, 1, 1, 40, 2, 30011, BF16), (65, 5, 16, 32, 1, 257, F16), (2, 1, 4, 96, 4, 1, F32), (1, 1, 5, 72, 2, 4096, F16),
+])
+def test_attention_few_queries(S, mult, H, C, N, M, dtype):
+    """One to four queries: keys by groups of lanes, a long axis split over workgroups."""
+    for n, (bias, gate, mask) in enumerate([("same", True, "tail"), (None, False, None), ("same", False, "holes")]):
+        check(inputs(10 * n + C, S, mult, H, C, N, M, dtype, bias, gate, mask), H, backward=M < 3000)
+
+
+@pytest.mark.parametrize("N", [1, 40])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_bars_of_different_sizes(N, dtype):
+    """Rows that the bias bars altogether, with the type's lowest value in some places and -1e30 in others: a softmax over
+    the latter's keys, in whatever order they come."""
+    H, C, M = 2, 16, 700
+    a = inputs(8, 1, 1, H, C, N, M, dtype, mask=None)
+    low = torch.finfo(dtype).min
+    for bars in ((low, -1e30), (-1e30, low)):
+        a["bias"].fill_(low)
+        a["bias"][..., 300:310] = -1e30
+        if bars[0] != low:
+            a["bias"][..., 300:310] = low
+            a["bias"][..., :20] = -1e30
+        at = (a["bias"][0, 0, 0] > -2e30).nonzero()[:, 0]
+        o, stats = call(a, H)
+        v = heads(np64(a["v"]), H)[:, :, at.cpu().numpy()]
+        want = rows(np.broadcast_to(v.mean(2, keepdims=True), (1, H, N, C))) / (1 + np.exp(-np64(a["g"])))
+        close(o, want, (STEP[dtype] + 64 * U) * np.abs(v).mean())
+        assert (stats[..., 1] == len(at)).all() and (stats[..., 0] > -1.1e30).all()
+
+
+@pytest.mark.parametrize("N, M", [(1, 300), (40, 300), (300, 40)])
+@pytest.mark.parametrize("base", [9e5, -1.04e6, 1.0485775e6, 3e7, -1e9, -1e10, 4e12, -1e15, -1e30, 1.3e30, 3e38])
+def test_attention_logits_far_from_zero(N, M, base):
+    """Logits (the biases alone: q is 0) that are a large number and small steps from it, as far as fp32 has them: the softmax
+    of the steps, forward and backward. p errs by u (2 |x - top| + 8 + M), and no step is past 100."""
+    H, C = 2, 16
+    for dtype, bias in ((F32, F32), (F32, BF16)):
+        a = inputs(12, 1, 1, H, C, N, M, dtype, bias=bias, mask=None)
+        a["q"].zero_()
+        step = torch.randint(0, 9, a["bias"].shape, generator=torch.Generator().manual_seed(5)).cuda()
+        a["bias"] = (torch.tensor(base, dtype=F32, device="cuda") - step).to(bias)
+        o, stats = call(a, H)
+        dout = rand(7, *o.shape, scale=0.1)
+        d = call_bwd(dout, a, H, o, stats)
+        want, wstats, _ = T.attention(*(np64(a[n]) for n in ("q", "k", "v")), H, np64(a["g"]), np64(a["bias"]), None, 1)
+        grads = T.attention_grads(np64(dout), *(np64(a[n]) for n in ("q", "k", "v")), H, np64(a["g"]), np64(a["bias"]), None, 1)
+        e = U * (2 * 8 + 8 + M)
+        assert np.array_equal(np64(stats)[..., 0], wstats[..., 0])
+        close(stats[..., 1], wstats[..., 1], e * wstats[..., 1])
+        big = np.abs(np64(a["v"])).max()
+        close(o, want, 4 * e * big)
+        # dp of sizes up to C |dO| |v|, delta the same; sums over N or M of them with |k|
+        size = C * np.abs(np64(dout)).max() * big * np.abs(np64(a["k"])).max()
+        for n in ("q", "v", "bias"):
+            close(d[n], grads[n], 8 * e * size * (N if n == "v" else 1))
+        assert (d["k"] == 0).all()
+
+
 def test_attention_is_seq_attention():
     """The inference kernels' result for the same inputs (their tolerance: both against the oracle's bound)."""
     N, H, C = 64, 4, 32
