@@ -94,6 +94,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_f
       x[kt] = s;
     }
     most = both_max(most);
+    // Without a branch: around the accumulators the compiler copies them all (4096 x 4096, 16 heads of 64 channels bf16 163 us
+    // so, 186 us with one; a base that follows the maximum only where that is e^4 past it gains nothing).
     const Exponent now(most);
     const float by = now.since(ex);
 #pragma unroll
