@@ -17,8 +17,8 @@ namespace bzpf {
 namespace {
 
 // A position or group number, 32 or 64 bits wide. Both are two loads of 32 bits, the second of the same ones where there are
-// no others: a branch would end in a wait for each number, one after the other (table's gradient at 16 x 2000 x 2000 in
-// bfloat16 58 us so, 96 us with a branch).
+// no others: a branch would end in a wait for each number, one after the other (table's gradient of 16 x 2000 x 2000 in
+// bfloat16 with one row in flight 58 us so, 96 us with a branch).
 template <typename P>
 __device__ __forceinline__ int64_t number(P p, bool wide, int64_t i) {
   const int64_t at = i << wide;
@@ -226,7 +226,9 @@ __global__ __launch_bounds__(256) void rel_bias_k(RelBias a, const T* __restrict
 // pairs lie in a bucket: 16 x 16 sums in fp32. Adding into LDS, a column a thread, took 104 us for 16 x 2000 x 2000 bf16 (an LDS
 // addition of a wave's 64 lanes costs about 100 cycles there). Half types are their own operand, fp32 goes as three bf16
 // parts, which hold its 24 bits. Rows whose 32 pairs lie in one bucket (beyond the first or last edge, in another chain: most)
-// are added up without a product. A value that is not finite spoils its head's sums.
+// are added up without a product, and a product is left out where none of its 16 buckets is reached. A value that is not
+// finite spoils its head's sums. 16 x 2000 x 2000 bf16, logarithmic buckets to 512: 37 us (3.4 TB/s); 2 x 16 x 400 x 400 fp16, three
+// chains: 14 us, which is the latency of eight rows behind the keys' and the look-up table's.
 template <typename T> struct OneHot;
 template <> struct OneHot<half_t> {
   typedef half_t P;
@@ -253,14 +255,13 @@ __device__ __forceinline__ int bounded(int64_t d) { return (int)(d < -BOUND ? -B
 
 constexpr int GK = 8;  // keys of a lane: a product's k = 8 (lane / 16) .. + 7
 
-// A wave's 32 keys, each lane's 8 neighbours: their distances from the first key in 32 bits. Past the end a lane's keys are
-// moved back to the last 8, and the first `skip` of them are its neighbours' (there are at least 8).
+// A wave's 32 keys, each lane's 8 neighbours: their distances from the first key and their groups, in 32 bits. Past the end a
+// lane's keys are moved back to the last 8, and the first `skip` of them are its neighbours' (there are at least 8).
 struct KeyTile {
-  int rel[GK];
-  int64_t base, group;
-  int least, most;
-  bool one_group, rare;  // rare: positions that 32 bits do not hold
-  unsigned other;        // the lane's keys that are not of `group`
+  int rel[GK], group[GK];
+  int64_t base;
+  int least, most, first_group;
+  bool one_group, rare;  // rare: positions or groups that 32 bits do not hold
   int64_t j;             // the lane's first key
   int skip;
   __device__ __forceinline__ void load(const RelBias& a, int64_t j0) {
@@ -268,26 +269,26 @@ struct KeyTile {
     j = min(want, max(a.M - GK, (int64_t)0));
     skip = (int)min(want - j, (int64_t)GK);
     base = scalar(a.pos_k, a.wide, j0);
-    group = a.group_k ? scalar(a.group_k, a.wide, j0) : 0;
-    bool far = false;
-    other = 0;
-    int lo = 0, hi = 0;
-    int64_t pos[GK], groups[GK];
+    int64_t pos[GK], groups[GK] = {};
     numbers(a.pos_k, a.wide, j, a.M, pos);
     if (a.group_k) numbers(a.group_k, a.wide, j, a.M, groups);
+    bool far = false, other = false;
+    int lo = 0, hi = 0;
+    first_group = __builtin_amdgcn_readfirstlane((int)groups[0]);
 #pragma unroll
     for (int e = 0; e < GK; e++) {
       const int64_t d = pos[e] - base;
-      far |= d < -BOUND / 2 || d > BOUND / 2;
       rel[e] = (int)d;
+      group[e] = (int)groups[e];
+      far |= d < -BOUND / 2 || d > BOUND / 2 || group[e] != groups[e];
       lo = min(lo, rel[e]);
       hi = max(hi, rel[e]);
-      if (a.group_k && groups[e] != group) other |= 1u << e;
+      other |= group[e] != first_group;
     }
     for (int o = 16; o < 64; o *= 2) lo = min(lo, __shfl_xor(lo, o)), hi = max(hi, __shfl_xor(hi, o));
     least = __builtin_amdgcn_readfirstlane(lo);
     most = __builtin_amdgcn_readfirstlane(hi);
-    one_group = !__any(other != 0);
+    one_group = !__any(other);
     rare = __any(far);
   }
 };
@@ -328,16 +329,6 @@ __global__ __launch_bounds__(256) void rel_bias_bwd_k(RelBias a, const T* __rest
     width[t] = in ? (uint32_t)(end - at) : 0u;
     if (a.group_k && k == a.count - 1 && k != last) from[t] = others, width[t] = 1;
   }
-  // The distances of buckets 16 t .. 16 t + 15, and whether the pairs of different groups are theirs: a product for them is
-  // left out where the 32 pairs are none of theirs.
-  int low[BT], high[BT];
-#pragma unroll
-  for (int t = 0; t < BT; t++) {
-    const int k0 = 16 * t, k1 = 16 * t + 16;
-    low[t] = k0 > last ? INT32_MAX : __builtin_amdgcn_readfirstlane(k0 <= first ? INT32_MIN : start[k0]);
-    high[t] = k1 <= first ? INT32_MIN : __builtin_amdgcn_readfirstlane(k1 > last ? INT32_MAX : start[k1]);
-  }
-
   f4 acc[BT];
 #pragma unroll
   for (int t = 0; t < BT; t++) acc[t] = f4{};
@@ -347,107 +338,123 @@ __global__ __launch_bounds__(256) void rel_bias_bwd_k(RelBias a, const T* __rest
   if (j0 < a.M) {
     KeyTile keys;
     keys.load(a, j0);
-    const bool whole_tile = j0 + 4 * GK <= a.M, short_rows = a.M < GK, on = h0 + c < a.H;
+    // lanes past the last head have its values too, in sums of their own that go nowhere
     const T* const col = dy + ((b * a.H + h) * a.N) * a.M + keys.j;
-    struct Row {  // the lane's values, the query's position and group
-      TV v;
-      int64_t pos, group;
-    };
-    const auto fetch = [&](int64_t i) {
-      Row f;
-      const int64_t r = min(i, r1 - 1);
-      f.pos = scalar(a.pos_q, a.wide, r);
-      f.group = a.group_q ? scalar(a.group_q, a.wide, r) : 0;
-      const T* const p = col + r * a.M;
-      f.v = TV{};
-      if (on) {
-        if (!short_rows) {
-          f.v = *reinterpret_cast<const TU*>(p);
-        } else {
-#pragma unroll
-          for (int e = 0; e < GK - 1; e++)
-            if (e < a.M) f.v[e] = p[e];
-        }
-      }
-      return f;
-    };
-    const auto work = [&](TV v, int64_t pos, int64_t group) {
-      if (!whole_tile) {
-#pragma unroll
-        for (int e = 0; e < GK; e++) v[e] = e >= keys.skip ? v[e] : (T)0.f;
-      }
-      const int at = bounded(pos - a.lo - keys.base);
-      const bool same = !a.group_k || group == keys.group;
-      const int kind = keys.rare || !keys.one_group ? MIXED : !same ? OTHER : at - keys.least <= 0 ? FIRST
-                       : at - keys.most >= a.span - 1 ? LAST : MIXED;
-      if (kind != MIXED) {
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < GK; e += 2) s += (float)v[e] + (float)v[e + 1];
-#pragma unroll
-        for (int k = 0; k < 3; k++)
-          if (kind == k) run[k] += s;
-        return;
-      }
-      int d[GK];
-#pragma unroll
-      for (int e = 0; e < GK; e++) d[e] = at - keys.rel[e];
-      if (keys.rare) {
-#pragma unroll
-        for (int e = 0; e < GK; e++) d[e] = bounded(pos - a.lo - whole(a.pos_k, a.wide, min(keys.j + e, a.M - 1)));
-      }
-      if (!keys.one_group || !same) {
-        unsigned other = keys.other;
-        if (!same) {
-          other = 0;
-#pragma unroll
-          for (int e = 0; e < GK; e++) other |= (whole(a.group_k, a.wide, min(keys.j + e, a.M - 1)) != group) << e;
-        }
-#pragma unroll
-        for (int e = 0; e < GK; e++) d[e] = other >> e & 1 ? others : d[e];
-      }
-      P8 x[GK / 8][OH::PARTS];
+    // 32 pairs of a row in several buckets, at distances d: a product for each 16 buckets of `reached`.
+    const auto products = [&](const TV& v, const int (&d)[GK], uint32_t reached) {
+      P8 x[OH::PARTS];
 #pragma unroll
       for (int e = 0; e < GK; e++) {
-        P8* const to = x[e / 8];
         if constexpr (OH::PARTS == 1) {
-          to[0][e % 8] = v[e];
+          x[0][e] = v[e];
         } else {
           const float hi = (float)(P)v[e], mid = (float)(P)(v[e] - hi);
-          to[0][e % 8] = (P)hi;
-          to[1][e % 8] = (P)mid;
-          to[2][e % 8] = (P)(v[e] - hi - mid);
+          x[0][e] = (P)hi;
+          x[1][e] = (P)mid;
+          x[2][e] = (P)(v[e] - hi - mid);
         }
       }
 #pragma unroll
       for (int t = 0; t < BT; t++) {
-        const bool reached = at - keys.least >= low[t] && at - keys.most < high[t];
-        if (BT > 2 && !reached && !keys.rare && ((same && keys.one_group) || t != (a.count - 1) / 16)) continue;
+        if (BT > 2 && !(reached >> t & 1)) continue;
         typedef uint32_t W4 __attribute__((ext_vector_type(4)));
-        W4 w[GK / 8];
+        W4 w;
 #pragma unroll
         for (int e = 0; e < GK; e += 2) {
           const bool p = (uint32_t)d[e] - (uint32_t)from[t] < width[t], q = (uint32_t)d[e + 1] - (uint32_t)from[t] < width[t];
-          w[e / 8][e % 8 / 2] = (p ? OH::ONE : 0u) | (q ? OH::ONE << 16 : 0u);
+          w[e / 2] = (p ? OH::ONE : 0u) | (q ? OH::ONE << 16 : 0u);
         }
 #pragma unroll
-        for (int k = 0; k < GK / 8; k++)
-#pragma unroll
-          for (int p = 0; p < OH::PARTS; p++) acc[t] = mma16(__builtin_bit_cast(P8, w[k]), x[k][p], acc[t]);
+        for (int p = 0; p < OH::PARTS; p++) acc[t] = mma16(__builtin_bit_cast(P8, w), x[p], acc[t]);
       }
     };
-    // Five rows in flight, and the loop's body once: the kernel's code would not fit the instruction cache unrolled (45 KB;
-    // most workgroups run a part of it once).
-    Row f[5];
+    const auto sum_up = [&](const TV& v, int k) {  // 32 pairs in one bucket
+      float s = 0.f;
 #pragma unroll
-    for (int u = 0; u < 5; u++) f[u] = fetch(r0 + u);
+      for (int e = 0; e < GK; e += 2) s += (float)v[e] + (float)v[e + 1];
+      if (k == FIRST) run[FIRST] += s;
+      else if (k == LAST) run[LAST] += s;
+      else run[OTHER] += s;
+    };
+    if (a.M >= GK && !keys.rare) {
+      // 64 rows' distances, kinds and reached buckets at once, a lane a row; then row by row, some rows' values on their way.
+      constexpr int U = BT > 5 ? 2 : 4;
+      const bool whole_tile = j0 + 4 * GK <= a.M;
+      const auto fetch = [&](int64_t i) { return *reinterpret_cast<const TU*>(col + min(i, r1 - 1) * a.M); };
+      TU f[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) f[u] = fetch(r0 + u);
+      for (int64_t c0 = r0; c0 < r1; c0 += 64) {
+        const int64_t r = min(c0 + l, r1 - 1);
+        const int at = bounded(whole(a.pos_q, a.wide, r) - a.lo - keys.base), n = (int)min(r1 - c0, (int64_t)64);
+        const int64_t group = a.group_q ? whole(a.group_q, a.wide, r) : 0;
+        const bool alien = group != (int)group, same = group == keys.first_group;  // alien: no key's group
+        const bool low = same && at - keys.least <= 0, high = same && !low && at - keys.most >= a.span - 1;
+        uint32_t reached = 0;
+        if constexpr (BT > 2) {
+#pragma unroll
+          for (int t = 0; t < BT; t++) {
+            const int k0 = 16 * t, k1 = 16 * t + 16;
+            const bool from = k0 <= last && (k0 <= first || at - keys.least >= start[k0]);
+            reached |= (uint32_t)(from && k1 > first && (k1 > last || at - keys.most < start[k1])) << t;
+          }
+        }
+        if (!keys.one_group) reached |= 1u << (a.count - 1) / 16;
+        const uint64_t firsts = __ballot(low), lasts = __ballot(high), aliens = __ballot(alien);
+        const uint64_t ones = keys.one_group ? firsts | lasts | __ballot(!same) : aliens;
+        for (int i0 = 0; i0 < n; i0 += U) {
+#pragma unroll
+          for (int u = 0; u < U; u++) {
+            TV v = f[u];
+            f[u] = fetch(c0 + i0 + u + U);
+            const int i = i0 + u;
+            if (i >= n) continue;
+            if (!whole_tile) {
+#pragma unroll
+              for (int e = 0; e < GK; e++) v[e] = e >= keys.skip ? v[e] : (T)0.f;
+            }
+            if (ones >> i & 1) {
+              sum_up(v, keys.one_group && firsts >> i & 1 ? FIRST : keys.one_group && lasts >> i & 1 ? LAST : OTHER);
+            } else {
+              const int row = __builtin_amdgcn_readlane(at, i);
+              int d[GK];
+#pragma unroll
+              for (int e = 0; e < GK; e++) d[e] = row - keys.rel[e];
+              if (!keys.one_group) {
+                const int g = __builtin_amdgcn_readlane((int)group, i);
+#pragma unroll
+                for (int e = 0; e < GK; e++) d[e] = keys.group[e] == g ? d[e] : others;
+              }
+              products(v, d, __builtin_amdgcn_readlane(reached, i));
+            }
+          }
+        }
+      }
+    } else {
+      // Fewer than 8 keys, or such as 32 bits do not hold: one row after the other, all buckets.
 #pragma unroll 1
-    for (int64_t i = r0; i < r1; i++) {
-      const Row now = f[0];
+      for (int64_t i = r0; i < r1; i++) {
+        const int64_t pos = scalar(a.pos_q, a.wide, i), group = a.group_q ? scalar(a.group_q, a.wide, i) : 0;
+        const T* const p = col + i * a.M;
+        TV v = TV{};
+        if (a.M >= GK) {
+          v = *reinterpret_cast<const TU*>(p);
+        } else {
 #pragma unroll
-      for (int u = 0; u < 4; u++) f[u] = f[u + 1];
-      f[4] = fetch(i + 5);
-      work(now.v, now.pos, now.group);
+          for (int e = 0; e < GK - 1; e++)
+            if (e < a.M) v[e] = p[e];
+        }
+#pragma unroll
+        for (int e = 0; e < GK; e++) v[e] = e >= keys.skip ? v[e] : (T)0.f;
+        int d[GK];
+#pragma unroll
+        for (int e = 0; e < GK; e++) {
+          const int64_t j = min(keys.j + e, a.M - 1);
+          const bool other = a.group_k && whole(a.group_k, a.wide, j) != group;
+          d[e] = other ? others : bounded(pos - a.lo - whole(a.pos_k, a.wide, j));
+        }
+        products(v, d, ~0u);
+      }
     }
   }
   // The workgroup's sums: a wave at a time, in their order. acc[t][i] is bucket 16 t + 4 (lane / 16) + i of head h0 + c.

@@ -124,6 +124,32 @@ def test_rel_bias(B, H, N, M, edges, chains, dtype):
     assert torch.equal(d, K().rel_bias_bwd(dy, b, pq, pk, cq, ck))  # a fixed order of sums
 
 
+@pytest.mark.parametrize("M", [5, 77, 130])
+def test_rel_bias_numbers_past_32_bits(M):
+    """Neighbouring keys 2^45 positions apart, groups whose numbers differ in their upper halves alone, queries of a group that
+    no key has; one bucket for pairs of different groups that the edges reach too, and one that they do not."""
+    H, N = 3, 70
+    g = torch.Generator(device="cuda").manual_seed(4)
+    big = lambda n: torch.randint(-3, 4, (n,), generator=g, device="cuda") * 2 ** 45 + torch.randint(0, 9, (n,), generator=g, device="cuda")
+    near = lambda n: torch.randint(0, 40, (n,), generator=g, device="cuda") + 2 ** 45
+    group = lambda n: torch.randint(0, 3, (n,), generator=g, device="cuda") * 2 ** 32 + 7
+    few = lambda n: (torch.arange(n, device="cuda") * 3 // n) % 3
+    for pos, ids in ((big, None), (near, group), (big, few), (near, few)):
+        for other in (True, False):
+            edges = K().clipped_edges(6)
+            b = K().rel_buckets(edges, other)
+            pq, pk = pos(N), pos(M)
+            cq, ck = (None, None) if ids is None else (ids(N), ids(M))
+            if ids is not None:
+                cq[3], cq[9] = 2 ** 40, -1
+            np_ = lambda *t: [x.cpu().numpy() for x in t]
+            at = T.buckets(edges, *np_(pq, pk)) if not other or ids is None else T.buckets(edges, *np_(pq, pk, cq, ck))
+            table, dy = rand(1, b.count, H), rand(3, H, N, M)
+            assert np.array_equal(np64(K().rel_bias(table, b, pq, pk, cq, ck)), T.rel_bias(np64(table), at))
+            close(K().rel_bias_bwd(dy, b, pq, pk, cq, ck), T.rel_bias_grad(np64(dy), at, b.count),
+                  grad_depth(1, H, N, M) * U * T.rel_bias_grad(np.abs(np64(dy)), at, b.count))
+
+
 def test_rel_bias_unordered_positions_and_shared_batches():
     """Positions in any order (chunks whose ends say nothing), a batch from one side alone, or from the pair bias alone."""
     H, N, M = 3, 50, 77
