@@ -54,7 +54,7 @@ __device__ __forceinline__ void exponentials(f16x& x, const Exponent& ex, bool s
   for (int i = 0; i < 16; i++) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], ex.by, -at));
 }
 
-// How a launch's waves work (attn_form chooses): in the wide form the four waves of a workgroup hold 32 rows each and share
+// How a launch's waves work (attn_split chooses): in the wide form the four waves of a workgroup hold 32 rows each and share
 // tiles of the other side's rows, in two buffers; in the split form they hold the same 32 rows, each with every fourth block
 // of the other side and tiles of its own (no barrier: a wave's LDS accesses keep their order), and meet at the end.
 template <typename T, bool SPLIT>
@@ -78,11 +78,13 @@ struct Form {
   }
 };
 
-// Split where 128-row workgroups would not give two to each compute unit; heads past 96 channels have the wide form alone
-// (their split form needs more registers than there are).
+// Split where 128-row workgroups would be fewer than 300 (half types; 512 in fp32, whose products are long enough to hide the
+// rest). dk/dv in us, wide and split, of n such workgroups: 48 channels fp16 n = 64: 25, 13; 192: 27, 27; 256: 28, 32; 288: 82,
+// 79; 320: 36, 40; 432: 91, 110; 24 channels fp32 n = 64: 44, 19; 288: 184, 137; 432: 202, 199; 512: 377, 389; 1024: 701, 754.
+// Heads past 96 channels have the wide form alone (their split form needs more registers than there are).
 constexpr int SPLIT_STEPS = 6;
 static inline bool attn_split(int64_t rows, const Attn& a) {
-  return a.C <= 16 * SPLIT_STEPS && (rows + 127) / 128 * a.S * a.H < 512;
+  return a.C <= 16 * SPLIT_STEPS && (rows + 127) / 128 * a.S * a.H < (a.dt == DT_F32 ? 512 : 300);
 }
 // Calls fn(true_type) or fn(false_type) for it.
 template <int KS, typename Fn>
