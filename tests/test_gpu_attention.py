@@ -490,6 +490,16 @@ def test_attention_larger(S, mult, H, C, N, M, dtype):
     check(inputs(1, S, mult, H, C, N, M, dtype, "same", True, "tail"), H)
 
 
+@pytest.mark.parametrize("S, mult, H, C, N, M", [
+    (3, 1, 4, 72, 40, 41), (2, 2, 3, 96, 70, 66), (6, 1, 2, 104, 35, 96), (3, 3, 2, 128, 96, 63), (7, 1, 2, 56, 33, 1), (7, 1, 1, 16, 31, 33),
+    (1, 1, 8, 8, 100, 100), (25, 5, 2, 120, 33, 7), (13, 1, 3, 88, 6, 200),
+])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_attention_tiles(S, mult, H, C, N, M, dtype):
+    """More than 192 rows in all: 32 x 32 tiles, every number of channel steps."""
+    test_attention(S, mult, H, C, N, M, dtype)
+
+
 @pytest.mark.parametrize("bias", [F16, BF16])
 def test_attention_half_bias_with_fp32(bias):
     check(inputs(3, 4, 2, 3, 24, 50, 61, F32, bias), 3)
@@ -506,7 +516,7 @@ def test_attention_few_queries(S, mult, H, C, N, M, dtype):
         check(inputs(10 * n + C, S, mult, H, C, N, M, dtype, bias, gate, mask), H, backward=M < 3000)
 
 
-@pytest.mark.parametrize("N", [1, 40])
+@pytest.mark.parametrize("N", [1, 40, 200])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_attention_bars_of_different_sizes(N, dtype):
     """Rows that the bias bars altogether, with the type's lowest value in some places and -1e30 in others: a softmax over
@@ -567,10 +577,11 @@ def test_attention_is_seq_attention():
         assert (np.abs(np64(o) - np64(call(a, H)[0])[0]) <= lim).all()
 
 
+@pytest.mark.parametrize("N", [45, 5])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-def test_attention_masked_places_hold_anything(dtype):
+def test_attention_masked_places_hold_anything(dtype, N):
     """Infinities and NaN in keys, values and biases that the mask leaves out; their gradients are 0."""
-    S, H, C, N, M = 2, 3, 24, 45, 70
+    S, H, C, M = 2, 3, 24, 70
     a = inputs(5, S, 1, H, C, N, M, dtype, mask="tail")
     a["mask"][0, 10], a["mask"][1, 0] = 0, 0
     o, stats = call(a, H)
@@ -591,12 +602,12 @@ def test_attention_masked_places_hold_anything(dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("mult", [1, 2])
-def test_attention_rows_without_keys(dtype, mult):
+@pytest.mark.parametrize("mult, S", [(1, 2), (2, 2), (1, 6), (2, 6)])
+def test_attention_rows_without_keys(dtype, mult, S):
     """A bias that is -inf over a row (the row gives 0 and takes no gradient), over some of one, or the type's lowest value
     over a whole row (a softmax over equals) or over some."""
     H, C, N, M = 2, 32, 40, 77
-    a = inputs(6, 2, mult, H, C, N, M, dtype, mask="tail")
+    a = inputs(6, S, mult, H, C, N, M, dtype, mask="tail")
     low = torch.finfo(dtype).min
     a["bias"][:, 0, 3] = -float("inf")
     a["bias"][:, 1, 4, 5:] = -float("inf")
@@ -618,7 +629,7 @@ def test_attention_rows_without_keys(dtype, mult):
     close(d["bias"][:, :, keep], grads["bias"][:, :, rowsel], tol["bias"][:, :, rowsel])
     if dtype != F16:
         on = a["mask"] != 0
-        for s in range(2):
+        for s in range(S):
             v = a["v"][s, on[s], :C].double().mean(0) * torch.sigmoid(a["g"][s, 6, :C].double())
             lim = float(a["v"].abs().max()) * (STEP[dtype] * 2 + 1e-5)
             assert (o[s, 6, :C].double() - v).abs().max() <= lim
