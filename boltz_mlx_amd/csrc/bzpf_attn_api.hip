@@ -105,6 +105,7 @@ int bzpf_rel_bias_bwd(const void* dout, int dt, const unsigned char* lut, int64_
   const int rc = make_rel("bzpf_rel_bias_bwd", dout, dt, lut, lo, span, count, pos_q, pos_k, group_q, group_k, wide, batch_q,
                           batch_k, B, H, N, M, &a);
   if (rc != BZPF_OK) return rc;
+  REQUIRE(B * ((H + 15) / 16) <= 65535, "bzpf_rel_bias_bwd: at most 65535 groups of 16 heads over the batch (B=%lld H=%d)", (long long)B, H);
   REQUIRE_EL(dtable, BZPF_F32);
   REQUIRE_EL(ws, BZPF_F32);
   const int64_t need = bzpf::rel_bias_bwd_ws_bytes(B, H, N, M, count);
@@ -213,6 +214,7 @@ int bzpf_qk_norm_rope_bwd(const void* dqn, const void* dkn, int y_dt, const void
 namespace {
 
 constexpr int64_t ATT_LEN = 1 << 22, ATT_PITCH = 1 << 23;  // what the kernels' 32-bit offsets within a block hold
+constexpr int64_t WORKGROUPS = (1 << 24) - 8;              // a launch has fewer than 2^32 threads, 256 a workgroup
 
 int make_attn(const char* who, const void* q, int64_t ldq, int64_t sq, const void* k, int64_t ldk, int64_t sk, const void* v,
               int64_t ldv, int64_t sv, const void* g, int64_t ldg, int64_t sg, const void* bias, int bias_dt, int mult,
@@ -226,6 +228,8 @@ int make_attn(const char* who, const void* q, int64_t ldq, int64_t sq, const voi
           who, S, H, mult);
   REQUIRE(N >= 1 && M >= 1 && N <= ATT_LEN && M <= ATT_LEN && product(S, H, N, M) >= 0 && product(S, N > M ? N : M, H, 4 * C) >= 0,
           "%s: 1 to 2^22 queries and keys (N=%lld M=%lld)", who, (long long)N, (long long)M);
+  REQUIRE(product(S, H, ((N > M ? N : M) + 31) / 32, 1) <= WORKGROUPS && product(S, H, N, (C + 7) / 8) < (int64_t)1 << 31,
+          "%s: too many samples, heads and rows for a launch (S=%d H=%d N=%lld M=%lld)", who, S, H, (long long)N, (long long)M);
   REQUIRE(q && k && v && out && stats, "%s: NULL pointer", who);
   for (const void* p : {q, k, v, g, out}) REQUIRE(aligned_el(p, dt), "%s: a tensor is misaligned", who);
   REQUIRE(aligned_el(bias, bias_dt) && aligned_el(mask, BZPF_F32) && aligned_el(stats, BZPF_F32), "%s: a tensor is misaligned", who);
@@ -295,6 +299,8 @@ int bzpf_attention_bwd(const void* dout, const void* q, int64_t ldq, int64_t sq,
   REQUIRE_EL(dv, dt);
   REQUIRE(!g == !dg && (bias || !dbias) && aligned_el(dg, dt) && aligned_el(dbias, bias_dt),
           "bzpf_attention_bwd: dg goes with g, dbias with bias");
+  REQUIRE(!dbias || mult == 1 || product(S_ / mult, H, (N + 63) / 64, (M + 63) / 64) <= WORKGROUPS,
+          "bzpf_attention_bwd: a shared bias of too many tiles for a launch");
   const int64_t need = bzpf::attention_bwd_ws_bytes(dt, S_, N, H, C, g != nullptr);
   REQUIRE_PTR(ws);
   REQUIRE(ws_bytes >= need, "bzpf_attention_bwd: ws holds %lld bytes of %lld", (long long)ws_bytes, (long long)need);

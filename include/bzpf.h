@@ -433,7 +433,7 @@ int bzpf_qk_norm_rope_bwd(const void* dqn, const void* dkn, int y_dt, const void
  *   x[h][i][j] = q_i . k_j / sqrt(C) + bias[h][i][j] over the keys with mask[j] != 0 (all of them where the sample has none);
  *   out[i][h C + c] = sigmoid(g[i][h C + c]) * sum_j softmax_j(x)[j] v[j][h C + c]   (0 for a row whose logits are all -inf).
  * q, g [S][N] and k, v [S][M] are rows of H heads of C channels (C a multiple of 8, 8 to 128) of pitch ld*, samples s*
- * elements apart, in dt; pitches below 2^23, N and M up to 2^22; g NULL: no gate. bias (or NULL) [S / mult][H][N][M] in
+ * elements apart, in dt; pitches below 2^23, N and M up to 2^22, S H ceil(max(N, M) / 32) below 2^24; g NULL: no gate. bias (or NULL) [S / mult][H][N][M] in
  * bias_dt (dt, or fp16 / bf16 with fp32 operands), shared by consecutive groups of mult samples; mask (or NULL) fp32 [S][M]. out [S][N][H C] in dt; stats fp32
  * [S][H][N][2]: a row's largest logit and the sum of exp(logit - that). What bzpf_seq_attention_batched computes, for any N
  * and M, in bf16 too. ws: bzpf_attention_ws bytes, 16-byte aligned (NULL where that is 0): few queries split a long key axis. */

@@ -54,7 +54,7 @@ REL_BWD = dict(dout=AT[0], dt=F32, lut=AT[1], lo=-3, span=7, count=8, pos_q=AT[2
 
 @pytest.mark.parametrize("change", [
     {"dout": None}, {"dout": AT[0] + 2}, {"dtable": None}, {"ws": None}, {"dtable": AT[4] + 1}, {"ws_bytes": 4}, {"dt": 4},
-    {"B": 0}, {"N": 0}, {"M": 0}, {"count": 300}, {"group_q": AT[6]}, {"dtable": AT[0] + 28000}, {"ws": AT[4]}, {"ws": AT[0]},
+    {"B": 0}, {"N": 0}, {"M": 0}, {"count": 300}, {"group_q": AT[6]}, {"dtable": AT[0] + 28000}, {"ws": AT[4]}, {"ws": AT[0]}, {"B": 65535, "H": 17, "N": 1, "M": 1, "ws_bytes": 1 << 40},
 ])
 def test_rel_bias_bwd_refuses(change):
     assert rc("bzpf_rel_bias_bwd", REL_BWD, change) == -1
@@ -100,6 +100,7 @@ ATT = dict(q=AT[0], ldq=48, sq=240, k=AT[1], ldk=48, sk=336, v=AT[2], ldv=48, sv
     {"M": 0}, {"N": -1}, {"N": 2 ** 22 + 1}, {"M": 2 ** 22 + 1}, {"ldq": 47}, {"ldk": 40}, {"ldv": 0}, {"ldg": 1}, {"sq": -1}, {"sv": -8},
     {"sk": 2 ** 62}, {"ldk": 2 ** 23}, {"ldg": 2 ** 60}, {"out": AT[0]}, {"out": AT[1] + 600}, {"out": AT[4]}, {"stats": AT[6]}, {"stats": AT[5]},
     {"out": AT[3] + 900}, {"ws": AT[8] + 8}, {"ws_bytes": -1},
+    {"S": 2 ** 20, "H": 16, "sq": 0, "sk": 0, "sv": 0, "sg": 0}, {"N": 2 ** 22, "H": 129, "C": 8, "S": 4, "mult": 4}, {"M": 2 ** 22, "S": 128},
 ])
 def test_attention_refuses(change):
     assert rc("bzpf_attention", ATT, change) == -1
