@@ -294,7 +294,10 @@ struct Att {
   at::IntArrayRef shape(const Tensor& x) const { return batched ? x.sizes() : x.sizes().slice(1); }
   int bias_type() const { return bias.defined() ? type_code(bias) : type_code(q); }
 };
-#define BZPF_ROWS(t) in(t), (t).defined() ? (t).stride(1) : 0, (t).defined() ? (t).stride(0) : 0
+// An operand's pointer, row pitch and sample stride (a dimension of one has any stride).
+#define BZPF_ROWS(t)                                                              \
+  in(t), !(t).defined() ? 0 : (t).size(1) == 1 ? (t).size(2) : (t).stride(1),     \
+      !(t).defined() || (t).size(0) == 1 ? 0 : (t).stride(0)
 
 std::tuple<Tensor, Tensor> attention(const Att& a) {
   on_gpu("attention", a.q);

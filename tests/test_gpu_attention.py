@@ -887,6 +887,73 @@ def test_captured_and_replayed():
             assert all(torch.equal(a, b) for a, b in zip(got, want)), (turn, n)
 
 
+def test_few_queries_captured_and_on_streams():
+    """One query against a long axis, whose parts meet in a workspace: replays of two graphs in turn with eager calls between,
+    two threads at once."""
+    import threading
+
+    H, C, M = 3, 40, 9000
+    graphs = []
+    for seed in (1, 2):
+        a = inputs(seed, 2, 1, H, C, 1, M, BF16, mask="tail")
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call(a, H)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(a, H)
+        graphs.append((graph, a, out))
+    for turn in range(4):
+        for n, (graph, a, out) in enumerate(graphs):
+            new = inputs(100 * turn + n, 2, 1, H, C, 1, M, BF16, mask="tail")
+            for name in ("q", "k", "v", "g", "bias", "mask"):
+                a[name].copy_(new[name])
+            graph.replay()
+            got = [t.clone() for t in out]
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(got, call(new, H))), (turn, n)
+    data = [inputs(s, 1, 1, H, C, 2, M, F16) for s in (5, 6)]
+    want = [call(a, H) for a in data]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got[i] = call(data[i], H)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(x, y) for g, w in zip(got, want) for x, y in zip(g, w))
+
+
+def test_attention_one_row_has_any_pitch():
+    """Dimensions of one, whose strides say nothing: one query, one key, one sample; samples that share a query or keys."""
+    S, H, C, M = 3, 2, 16, 20
+    a = inputs(3, S, 1, H, C, 1, M, F32)
+    want = call(a, H)
+    odd = dict(a)
+    for n in ("q", "g"):
+        odd[n] = torch.as_strided(a[n], a[n].shape, (H * C, 2 ** 40, 1))
+    assert all(torch.equal(x, y) for x, y in zip(call(odd, H), want))
+    dout = rand(9, S, 1, H * C)
+    d, dodd = call_bwd(dout, a, H, *want), call_bwd(dout, odd, H, *want)
+    assert all(torch.equal(d[n], dodd[n]) for n in d)
+    one = inputs(4, 1, 1, H, C, 50, 1, F32, mask=None)
+    odd = dict(one)
+    for n in ("k", "v"):
+        odd[n] = torch.as_strided(one[n], one[n].shape, (2 ** 41, 2 ** 40, 1))
+    assert all(torch.equal(x, y) for x, y in zip(call(odd, H), call(one, H)))
+    same = dict(a, q=a["q"][:1].expand(S, -1, -1), k=a["k"][:1].expand(S, -1, -1))
+    check(same, H)
+
+
 def test_streams_and_threads():
     """Calls on other streams and from two threads at once: the bits of the calls alone."""
     import threading
