@@ -293,6 +293,37 @@ struct KeyTile {
   }
 };
 
+// Eight neighbouring values on their way. ODD: 16-bit ones that may begin inside a dword, where a load of 16 bytes takes twice
+// as long: it begins at the dword then, with the value before them, and the last one comes by itself.
+template <typename T, bool ODD>
+struct EightOf {
+  typedef T V __attribute__((ext_vector_type(GK)));
+  typedef T U __attribute__((ext_vector_type(GK), aligned(sizeof(T))));
+  V v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const U*>(p); }
+  __device__ __forceinline__ V get() const { return v; }
+};
+template <typename T>
+struct EightOf<T, true> {
+  typedef T V __attribute__((ext_vector_type(GK)));
+  typedef uint32_t D __attribute__((ext_vector_type(4), aligned(4)));
+  D x;
+  uint16_t last;
+  uint32_t shift;
+  __device__ __forceinline__ void load(const T* p) {
+    const int odd = (int)(reinterpret_cast<uintptr_t>(p) >> 1 & 1);
+    x = *reinterpret_cast<const D*>(p - odd);
+    last = __builtin_bit_cast(uint16_t, p[GK - 1]);
+    shift = 16u * odd;
+  }
+  __device__ __forceinline__ V get() const {
+    D y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = __builtin_amdgcn_alignbit(e < 3 ? x[e + 1] : (uint32_t)last, x[e], shift);
+    return __builtin_bit_cast(V, y);
+  }
+};
+
 // grid (blocks of 128 keys, row blocks, batch times groups of 16 heads); partial sums [row block, key block, batch][H][count].
 // BT: groups of 16 buckets.
 template <typename T, int BT>
@@ -376,12 +407,17 @@ __global__ __launch_bounds__(256) void rel_bias_bwd_k(RelBias a, const T* __rest
       else if (k == LAST) run[LAST] += s;
       else run[OTHER] += s;
     };
-    if (a.M >= GK && !keys.rare) {
-      // 64 rows' distances, kinds and reached buckets at once, a lane a row; then row by row, some rows' values on their way.
+    // 64 rows' distances, kinds and reached buckets at once, a lane a row; then row by row, some rows' values on their way.
+    const auto all_rows = [&](auto odd_rows) {
+      constexpr bool ODD = decltype(odd_rows)::value;
       constexpr int U = BT > 5 ? 2 : 4;
       const bool whole_tile = j0 + 4 * GK <= a.M;
-      const auto fetch = [&](int64_t i) { return *reinterpret_cast<const TU*>(col + min(i, r1 - 1) * a.M); };
-      TU f[U];
+      const auto fetch = [&](int64_t i) {
+        EightOf<T, ODD> f;
+        f.load(col + min(i, r1 - 1) * a.M);
+        return f;
+      };
+      EightOf<T, ODD> f[U];
 #pragma unroll
       for (int u = 0; u < U; u++) f[u] = fetch(r0 + u);
       for (int64_t c0 = r0; c0 < r1; c0 += 64) {
@@ -405,7 +441,7 @@ __global__ __launch_bounds__(256) void rel_bias_bwd_k(RelBias a, const T* __rest
         for (int i0 = 0; i0 < n; i0 += U) {
 #pragma unroll
           for (int u = 0; u < U; u++) {
-            TV v = f[u];
+            TV v = f[u].get();
             f[u] = fetch(c0 + i0 + u + U);
             const int i = i0 + u;
             if (i >= n) continue;
@@ -429,6 +465,16 @@ __global__ __launch_bounds__(256) void rel_bias_bwd_k(RelBias a, const T* __rest
             }
           }
         }
+      }
+    };
+    if (a.M >= GK && !keys.rare) {
+      // Rows of an odd number of 16-bit values begin inside a dword every other time (16 x 4001 x 4001 bf16 158 us, 213 with
+      // loads that begin there). The tensor has to begin at one: the value before it is not read.
+      if constexpr (sizeof(T) == 2) {
+        if (a.M % 2 && (reinterpret_cast<uintptr_t>(dy) & 3) == 0) all_rows(std::true_type());
+        else all_rows(std::false_type());
+      } else {
+        all_rows(std::false_type());
       }
     } else {
       // Fewer than 8 keys, or such as 32 bits do not hold: one row after the other, all buckets.

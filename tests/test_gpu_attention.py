@@ -124,6 +124,21 @@ def test_rel_bias(B, H, N, M, edges, chains, dtype):
     assert torch.equal(d, K().rel_bias_bwd(dy, b, pq, pk, cq, ck))  # a fixed order of sums
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("N, M", [(31, 65), (70, 77), (9, 8), (40, 129), (33, 96), (5, 7)])
+def test_rel_bias_values_inside_dwords(N, M, dtype):
+    """Rows of odd lengths in 16-bit types, tensors that begin inside a dword."""
+    H, b = 5, K().rel_buckets(K().clipped_edges(7))
+    pq, pk = positions(1, N)[0], positions(2, M)[0]
+    at = T.buckets(K().clipped_edges(7), pq.cpu().numpy(), pk.cpu().numpy())
+    table = rand(3, b.count, H, dtype=dtype)
+    for offset in (0, 1, 2):
+        dy, add = (rand(s, offset + H * N * M, scale=0.1, dtype=dtype)[offset:].view(H, N, M) for s in (4, 5))
+        close(K().rel_bias_bwd(dy, b, pq, pk), T.rel_bias_grad(np64(dy), at, b.count),
+              grad_depth(1, H, N, M) * U * T.rel_bias_grad(np.abs(np64(dy)), at, b.count))
+        close(K().rel_bias(table, b, pq, pk, add=add), T.rel_bias(np64(table), at, np64(add)), 0.0)
+
+
 @pytest.mark.parametrize("M", [5, 77, 130])
 def test_rel_bias_numbers_past_32_bits(M):
     """Neighbouring keys 2^45 positions apart, groups whose numbers differ in their upper halves alone, queries of a group that
