@@ -43,11 +43,12 @@ struct Exponent {
   }
 };
 
-// 16 logits' exponentials for a row a lane, where waves without big rows have one instruction each.
-__device__ __forceinline__ void exponentials(f16x& x, const Exponent& ex, bool some_big) {
+// 16 logits' exponentials for a row a lane, where waves without big rows have one instruction each; `less`: powers of two off
+// those of big rows.
+__device__ __forceinline__ void exponentials(f16x& x, const Exponent& ex, bool some_big, float less = 0.f) {
   if (some_big) {
 #pragma unroll
-    for (int i = 0; i < 16; i++) x[i] = ex.big() ? (x[i] - ex.at) * LOG2E : x[i];
+    for (int i = 0; i < 16; i++) x[i] = ex.big() ? fmaf(x[i] - ex.at, LOG2E, -less) : x[i];
   }
   const float at = ex.big() ? 0.f : ex.at;
 #pragma unroll

@@ -67,10 +67,18 @@ struct RowStat {
   Exponent ex;
   float inv, delta;
   __device__ __forceinline__ explicit RowStat(f4 v) { ex.at = v[0], ex.by = v[3], inv = v[1], delta = v[2]; }
+  // Exponentials of a row smaller by 2^n, at most the root of the sum and of C; what is then left of its reciprocal; n.
+  __device__ __forceinline__ float root(int C) {
+    const float n = inv == 0.f ? 0.f : (float)(max((127 - (int)(__float_as_uint(inv) >> 23)) / 2, 0) + (31 - __builtin_clz(C)) / 2);
+    const float at = ex.big() ? ex.at : ex.at + n;
+    inv *= __builtin_amdgcn_exp2f(ex.big() ? n : at - ex.at);
+    ex.at = at;
+    return n;
+  }
 };
 
 // dq: a wave holds 32 queries as the columns of S^T, as the forward pass does. The sum's reciprocal is a row's own, so that it
-// scales dq at the end and ds is rounded before it. TWO: dO has a second part.
+// (in fp16: what root() leaves of it) scales dq at the end and ds is rounded before it. TWO: dO has a second part.
 template <typename T, typename BT, int KS, bool SPLIT, bool TWO>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_dq_k(Attn a, int64_t per_xcd) {
   typedef Form<T, SPLIT> F;
@@ -100,7 +108,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
   u4* const Bt = reinterpret_cast<u4*>(bias_lds + wave * BiasRows<BT, BK>::BYTES);
   const float* mask = a.mask ? a.mask + un.smp * a.M : nullptr;
   const int64_t srow = ((int64_t)un.smp * a.H + un.h) * a.N + jc;
-  const RowStat rs(static_cast<const f4*>(a.rows)[srow]);
+  RowStat rs(static_cast<const f4*>(a.rows)[srow]);
+  // A sum of K terms of a size is some sqrt(K) of it: with p at sqrt(K / C) times its size, ds leaves fp16's range where dq does.
+  float less = 0.f;
+  if constexpr (std::is_same<T, half_t>::value) less = rs.root(a.C);
   const bool some_big = __any(rs.ex.big());
 
   // dO's second part waits in LDS in the wide form (in registers 64 channels spill: dq of 2 x 16 x 2000 x
@@ -173,7 +184,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
       if (bias) b = BiasRows<BT, BK>::get(Bt, kt);
 #pragma unroll
       for (int i = 0; i < 16; i++) x[i] = fmaf(x[i], a.scale, b[i]);
-      exponentials(x, rs.ex, some_big);
+      exponentials(x, rs.ex, some_big, less);
 #pragma unroll
       for (int i = 0; i < 16; i++) dp[i] = x[i] * (dp[i] - rs.delta);
       if (keep != all_rows(BK)) {

@@ -439,7 +439,7 @@ def tolerances(a, H, dtype, dout=None):
     # what out's rounding leaves of delta before it is mended, which meets p k rounded
     raw = heads(np.abs(dout) * ((t_out + h * (np.abs(out) + t_out) + tiny) * 1.0), H).sum(-1, keepdims=True)
     scale = 1 / np.sqrt(C)
-    low = tiny / total
+    low = tiny * np.sqrt(C / total)  # fp16's ds at p total / 2^n, 2^n <= sqrt(C total): its 2^-25 counts 2^n / total at most
     # Half types take the rounded ds' own sum off dq: with e_j the rounding of ds_j, (sum of e_j ds_j) (sum of p k) on top of the
     # (sum of e_j ds_j k_j) that the products have, together sum of e_j ds_j (k_j - sum of p k); raw's part of ds as there.
     taken = (h * (np.abs(ds) + p * raw) + low * np.ones_like(ds)).sum(-1, keepdims=True) * np.abs(p @ heads(k, H)) * (1 + h)
@@ -648,6 +648,24 @@ def test_attention_rows_without_keys(dtype, mult, S):
             v = a["v"][s, on[s], :C].double().mean(0) * torch.sigmoid(a["g"][s, 6, :C].double())
             lim = float(a["v"].abs().max()) * (STEP[dtype] * 2 + 1e-5)
             assert (o[s, 6, :C].double() - v).abs().max() <= lim
+
+
+@pytest.mark.parametrize("S, N, M", [(1, 64, 600), (4, 64, 600), (1, 5, 900)])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_attention_large_gradients(dtype, S, N, M):
+    """Gradients of an output that are thousands: products with v pass fp16's largest number, no gradient does."""
+    H, C = 3, 64
+    a = inputs(8, S, 1, H, C, N, M, dtype)
+    a["v"] = rand(10, S, M, H * C, scale=4.0, dtype=dtype)
+    o, stats = call(a, H)
+    dout = rand(9, *o.shape, scale=4e3, dtype=dtype)
+    want, _, tol, grads = tolerances(a, H, dtype, dout)
+    d = call_bwd(dout, a, H, o, stats)
+    s = 1 / (1 + np.exp(-np64(a["g"])))
+    assert np.abs(heads(np64(dout) * s, H) @ heads(np64(a["v"]), H).swapaxes(-1, -2)).max() > 65504
+    for n, x in grads.items():
+        assert np.abs(x).max() < 65504
+        close(d[n], x, tol[n])
 
 
 def test_attention_large_logits():
