@@ -329,11 +329,10 @@ def rel_buckets(edges, other: bool = False, device="cuda") -> RelBuckets:
     lo, hi = (edges[0] - 1, edges[-1]) if edges else (0, 0)
     if count > 256 or hi - lo >= 16384:
         raise ValueError(f"rel_buckets: at most 256 buckets over 16384 distances, got {count} over {hi - lo + 1}")
-    lut, k = [], 0
-    for d in range(lo, hi + 1):
-        k += k < len(edges) and edges[k] <= d
-        lut.append(k)
-    return RelBuckets(torch.tensor(lut, dtype=torch.uint8, device=device), lo, count, bool(other))
+    lut = bytearray(1)  # one distance below the first edge, then those from each edge to the next, the last edge alone
+    for k, e in enumerate(edges, 1):
+        lut += bytes([k]) * ((edges[k] if k < len(edges) else e + 1) - e)
+    return RelBuckets(torch.frombuffer(lut, dtype=torch.uint8).to(device), lo, count, bool(other))
 
 
 def clipped_edges(reach: int) -> list:
