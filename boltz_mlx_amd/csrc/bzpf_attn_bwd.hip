@@ -20,7 +20,7 @@ namespace bzpf {
 namespace {
 
 // What the other kernels need of a row (p = Exponent(by, at).of(x) inv), [S][H][N], and with a gate dO (two parts in half types) and
-// dg. L lanes a head, 8 channels each.
+// dg. L lanes a head, 8 channels each. Bound by memory: 2 x 16 x 2000 rows of 64 channels bf16 with a gate 13.6 us (4.1 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void attn_rows_k(Attn a, int L) {
   const int l = threadIdx.x % L, heads = 256 / L;
@@ -78,7 +78,9 @@ struct RowStat {
 };
 
 // dq: a wave holds 32 queries as the columns of S^T, as the forward pass does. The sum's reciprocal is a row's own, so that it
-// (in fp16: what root() leaves of it) scales dq at the end and ds is rounded before it. TWO: dO has a second part.
+// (in fp16: what root() leaves of it) scales dq at the end and ds is rounded before it. TWO: dO has a second part. 2 x 16 x 2000 x 2000 in 64 channels bf16 with a
+// gate 133 to 146 us (matrix cores 38% busy, some pipe issuing 77% of the time), without 123; 16 x 400 x 400 in 24 channels
+// fp32 15 us, latency.
 template <typename T, typename BT, int KS, bool SPLIT, bool TWO>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_dq_k(Attn a, int64_t per_xcd) {
   typedef Form<T, SPLIT> F;
@@ -257,7 +259,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
 }
 
 // dk and dv (and dbias): a wave holds 32 keys as the columns of S = Q K^T, so that dk^T = q^T ds and dv^T = dO^T p take p and
-// ds from their lanes; the queries' statistics come from LDS, four rows a read.
+// ds from their lanes; the queries' statistics come from LDS, four rows a read. 2 x 16 x 2000 x 2000 in 64 channels bf16 with a
+// gate 189 to 201 us with dbias, 179 without, 139 without a bias; matrix cores 29% busy, LDS 32%, some pipe issuing 76% of the
+// time: two waves a SIMD take turns. 16 x 400 x 400 in 24 channels fp32 20 us, latency.
 template <typename T, typename BT, int KS, bool SPLIT, bool TWO>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_dkv_k(Attn a, int64_t per_xcd) {
   typedef Form<T, SPLIT> F;
@@ -445,7 +449,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
 }
 
 // dbias of a bias that `mult` samples share: a wave sums ds of one 32 x 32 tile over them in registers, the workgroup's four a
-// 64 x 64 one whose rows of q, dO, k and v go through LDS, the next sample's on their way meanwhile.
+// 64 x 64 one whose rows of q, dO, k and v go through LDS, the next sample's on their way meanwhile (5 x 16 x 400 x 400 in 48 channels
+// fp16 28 us; operands from L2 to each wave 41 us). Bound by latency, two barriers a sample.
 template <typename T, typename BT, int KS, bool TWO>
 __global__ __launch_bounds__(256, 1) void attn_dbias_k(Attn a, uint32_t tiles_k, uint32_t tiles_q) {
   constexpr int TILE = 64 * TILE_LD<T, KS>;

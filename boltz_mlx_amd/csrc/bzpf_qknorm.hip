@@ -82,7 +82,9 @@ __device__ __forceinline__ float rsqrt_of(float v) {
 }
 
 // grid.y = 2: a workgroup takes the queries or the keys alone (few rows). Waves: lanes are (token, head, part of a head),
-// tokens' heads in turns of `hp`, split over `sub` waves where tokens are few.
+// tokens' heads in turns of `hp`, split over `sub` waves where tokens are few. Backward pass of 32,008 tokens of 16 + 4 heads of
+// 128 bf16 120 us (4.1 TB/s; with the next turn's values on their way the same); 400 tokens of 16 + 16 heads of 24 fp32 5.2 us
+// forward, 10 us backward, one token 4.0 us: latency.
 template <bool BWD, typename TX, typename TY, int V, int K, bool INTER>
 __global__ __launch_bounds__(256) void qk_norm_k(QKNorm a) {
   typedef Pairs<V, K, INTER> PR;
