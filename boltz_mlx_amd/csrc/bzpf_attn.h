@@ -240,8 +240,8 @@ __device__ __forceinline__ u4 load_all(const BT* p) {
 }
 
 // The biases of a wave's 32 rows against BK keys, on their way through LDS: from memory in whole rows (a lane for each row
-// would take 32 lines an instruction: forward pass of 2 x 16 x 2000 x 2000 bfloat16 227 us instead of 171), to the lanes that own the rows.
-// 16-byte pieces lie at places that keep the lanes' reads of one column on different banks.
+// would take 32 lines an instruction: forward pass of 4096 x 4096, 16 heads bf16 227 us instead of 171), to the lanes that own
+// the rows. 16-byte pieces lie at places that keep the lanes' reads of one column on different banks.
 template <typename BT, int BK>
 struct BiasRows {
   static constexpr int CPR = BK * (int)sizeof(BT) / 16, NV = 32 * CPR / 64, E = 16 / (int)sizeof(BT), BYTES = 32 * CPR * 16;

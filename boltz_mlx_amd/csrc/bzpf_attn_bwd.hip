@@ -12,15 +12,16 @@
 //   leaves of each rounding what its key differs from the row's mean key by.
 // - dO is not a value of the type: it goes as two of them, the rounded one and the rest, in the products of dp and dv.
 // Without these the gradients were 1.7 to 2.3 times as far from the exact ones as their own rounding puts them, now 1.0
-// (dbias), 1.3 (dq), 1.4 (dk, dv) and 1.5 times (dg, from the output as it was rounded).
+// (dbias), 1.3 (dq), 1.4 (dk, dv) and 1.5 times (dg, from the output as it was rounded). Where ds is below fp16's 2^-14, dq errs
+// by about one of the type's smallest steps and dk by sqrt(N / C) of them.
 #include "bzpf_attn.h"
 
 namespace bzpf {
 
 namespace {
 
-// What the other kernels need of a row (p = Exponent(by, at).of(x) inv), [S][H][N], and with a gate dO (two parts in half types) and
-// dg. L lanes a head, 8 channels each. Bound by memory: 2 x 16 x 2000 rows of 64 channels bf16 with a gate 13.6 us (4.1 TB/s).
+// What the other kernels need of a row (p = Exponent(by, at).of(x) inv), [S][H][N], and with a gate dO (two parts in half
+// types) and dg. L lanes a head, 8 channels each. Bound by memory: 2 x 16 x 2000 rows of 64 channels bf16 with a gate 13.6 us (4.1 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void attn_rows_k(Attn a, int L) {
   const int l = threadIdx.x % L, heads = 256 / L;
@@ -78,9 +79,9 @@ struct RowStat {
 };
 
 // dq: a wave holds 32 queries as the columns of S^T, as the forward pass does. The sum's reciprocal is a row's own, so that it
-// (in fp16: what root() leaves of it) scales dq at the end and ds is rounded before it. TWO: dO has a second part. 2 x 16 x 2000 x 2000 in 64 channels bf16 with a
-// gate 133 to 146 us (matrix cores 38% busy, some pipe issuing 77% of the time), without 123; 16 x 400 x 400 in 24 channels
-// fp32 15 us, latency.
+// (in fp16: what root() leaves of it) scales dq at the end and ds is rounded before it. TWO: dO has a second part.
+// 2 x 16 x 2000 x 2000 in 64 channels bf16 with a gate 133 to 146 us (matrix cores 38% busy, some pipe issuing 77% of the
+// time), without 123; 16 x 400 x 400 in 24 channels fp32 15 us, latency.
 template <typename T, typename BT, int KS, bool SPLIT, bool TWO>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_dq_k(Attn a, int64_t per_xcd) {
   typedef Form<T, SPLIT> F;
