@@ -456,7 +456,7 @@ template <typename T, typename BT, int KS, bool TWO>
 __global__ __launch_bounds__(256, 1) void attn_dbias_k(Attn a, uint32_t tiles_k, uint32_t tiles_q) {
   constexpr int TILE = 64 * TILE_LD<T, KS>;
   __shared__ LDS_ALIGN T tiles[(TWO ? 5 : 4) * TILE];
-  __shared__ LDS_ALIGN char bias_lds[4 * BiasRows<BT, 32>::BYTES];
+  static_assert(sizeof(tiles) >= 4 * BiasRows<BT, 32>::BYTES, "the biases go through them first");
   T* const Qt = tiles;
   T* const Dt = Qt + TILE;
   T* const Kt = Dt + TILE;
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(256, 1) void attn_dbias_k(Attn a, uint32_t tiles_k,
   {
     const int64_t r0 = min(q0 + qw, a.N - 1), c0 = min(k0 + kw, a.M - 1);
     BiasRows<BT, 32> bs;
-    u4* const Bt = reinterpret_cast<u4*>(bias_lds + wave * BiasRows<BT, 32>::BYTES);
+    u4* const Bt = reinterpret_cast<u4*>(reinterpret_cast<char*>(tiles) + wave * BiasRows<BT, 32>::BYTES);
     bs.load(static_cast<const BT*>(a.bias) + ((int64_t)bh * a.N + r0) * a.M, (int)min(a.N - r0, (int64_t)32), (int)a.M, (int)c0);
     bs.store(Bt, (int)a.M, (int)c0);
     Form<T, true>::order();
@@ -521,12 +521,17 @@ __global__ __launch_bounds__(256, 1) void attn_dbias_k(Attn a, uint32_t tiles_k,
       dp = mma(vm, row_frag<T, KS>(Dt, qw + (l & 31), m), dp);
       if constexpr (TWO) dp = mma(vm, row_frag<T, KS>(Lt, qw + (l & 31), m), dp);
     }
+#pragma unroll
+    for (int i = 0; i < 16; i++) x[i] = fmaf(x[i], a.scale, bias[i]);
+    exponentials(x, rs.ex, __any(rs.ex.big()));
     const uint32_t on = (uint32_t)(keep >> kw) >> (16 * hl);
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const float d = rs.ex.of(fmaf(x[i], a.scale, bias[i])) * rs.inv * (dp[i] - rs.delta);
-      sum[i] += on >> i & 1 ? d : 0.f;
+    for (int i = 0; i < 16; i++) dp[i] = x[i] * rs.inv * (dp[i] - rs.delta);
+    if (keep != all_rows(64)) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) dp[i] = on >> i & 1 ? dp[i] : 0.f;
     }
+    sum += dp;
   }
   if (j >= a.N || first >= a.M) return;
   BT* const out = static_cast<BT*>(a.dbias) + ((int64_t)bh * a.N + j) * a.M + first;
