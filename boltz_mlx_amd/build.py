@@ -54,11 +54,8 @@ def binding_sources() -> list[str]:
 
 
 # Per-source additions. The fp16 attention core is VALU-bound; without NaN semantics its fmaxf reductions over MFMA
-# results need no canonicalising v_max_f32 per logit (its inputs are finite or -inf by construction). The backward attention
-# keeps its uniform branches as they are: made into a structure for divergent ones, each has a path past both sides, and the
-# waits after it are for every load and store in flight (dk/dv of 2 x 16 x 2000 x 2000 bf16 200 us instead of 205).
-FILE_FLAGS = {"bzpf_triattn_mfma.hip": ["-fno-honor-nans"],
-              "bzpf_attn_bwd.hip": ["-mllvm", "-structurizecfg-skip-uniform-regions"]}
+# results need no canonicalising v_max_f32 per logit (its inputs are finite or -inf by construction).
+FILE_FLAGS = {"bzpf_triattn_mfma.hip": ["-fno-honor-nans"]}
 
 
 def torch_flags() -> list[str]:
