@@ -124,6 +124,25 @@ def test_rel_bias(B, H, N, M, edges, chains, dtype):
     assert torch.equal(d, K().rel_bias_bwd(dy, b, pq, pk, cq, ck))  # a fixed order of sums
 
 
+@pytest.mark.parametrize("lut, count", [([0, 1, 2], 3), ([1, 1, 4, 4, 4, 20], 21), ([0], 1), ([2, 2], 40), ([0, 17, 33, 90], 91)])
+def test_rel_bias_look_up_tables_of_ones_own(lut, count):
+    """A table that skips buckets, has equal entries, or shares the bucket of other groups' pairs with its end."""
+    H, N, M = 18, 70, 100
+    g = torch.Generator(device="cuda").manual_seed(2)
+    pq, pk = (torch.randint(-8, 8, (n,), generator=g, device="cuda") for n in (N, M))
+    cq, ck = ((torch.arange(n, device="cuda") * 2) // n for n in (N, M))
+    for other in (False, True):
+        b = K().RelBuckets(torch.tensor(lut, dtype=torch.uint8, device="cuda"), -2, count, other)
+        d = (pq[:, None] - pk[None]).cpu().numpy()
+        at = np.array(lut)[np.clip(d + 2, 0, len(lut) - 1)]
+        if other:
+            at = np.where((cq[:, None] == ck[None]).cpu().numpy(), at, count - 1)
+        table, dy = rand(1, count, H), rand(3, H, N, M)
+        assert np.array_equal(np64(K().rel_bias(table, b, pq, pk, cq, ck)), T.rel_bias(np64(table), at))
+        close(K().rel_bias_bwd(dy, b, pq, pk, cq, ck), T.rel_bias_grad(np64(dy), at, count),
+              grad_depth(1, H, N, M) * U * T.rel_bias_grad(np.abs(np64(dy)), at, count))
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("N, M", [(31, 65), (70, 77), (9, 8), (40, 129), (33, 96), (5, 7)])
 def test_rel_bias_values_inside_dwords(N, M, dtype):
