@@ -13,7 +13,7 @@
 // - dO is not a value of the type: it goes as two of them, the rounded one and the rest, in the products of dp and dv.
 // Without these the gradients were 1.7 to 2.3 times as far from the exact ones as their own rounding puts them, now 1.0
 // (dbias), 1.3 (dq), 1.4 (dk, dv) and 1.5 times (dg, from the output as it was rounded). Where ds is below fp16's 2^-14, dq errs
-// by about one of the type's smallest steps and dk by sqrt(N / C) of them.
+// by about one of the type's smallest steps and dk by sqrt(N / C) of them; where it is past its largest number, Scale.
 #include "bzpf_attn.h"
 
 namespace bzpf {
@@ -78,6 +78,52 @@ struct RowStat {
   }
 };
 
+// ds on its way into a product, for a lane's key (dk) or row (dq). In fp16 it may pass the type's largest number where the product
+// does not: a ds of 10^6 meets a query of 0.01 under 1 / sqrt(C). The accumulators are infinite or NaN then, and the lanes
+// that have such go over the other axis again with ds times 2^-12, at last 2^-24 (finite operands give |ds| below 2^40). The
+// largest scaled ds is 2^4 or more then, so that what others lose below 2^-14 is 2^-29 of it. Operands that are not finite take
+// the two rounds too (2 x 16 x 2000 x 2000 in 64 channels without a gate 540 us instead of 209). The other types' ds have fp32's
+// range. The multiplication and the check cost the backward pass 4% at that size (with a gate and a bias 323 -> 336 us), 11%
+// where the registers of the split form were full (16 x 400 x 400, 64 channels with both 30.2 -> 33.7 us).
+template <typename T>
+struct Scale {
+  static constexpr bool ON = std::is_same<T, half_t>::value;
+  float by = 1.f;
+  // Accumulator rows 16 s .. 16 s + 15 as the products take them.
+  __device__ __forceinline__ frag<T> as_frag(const f16x& c, int s) const {
+    if constexpr (!ON) return bzpf::as_frag<T>(c, s);
+    frag<T> f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) f[j] = (T)(c[8 * s + j] * by);
+    return f;
+  }
+  __device__ __forceinline__ float back() const { return ON ? 1.f / by : 1.f; }
+  // Where a round begins, unknown to the compiler: addresses of a second round's first loads, formed before the first round and
+  // kept over it, took 15 registers and spilled.
+  static __device__ __forceinline__ int first(int at) {
+    if constexpr (ON) asm volatile("" : "+s"(at));
+    return at;
+  }
+  // Whether the workgroup has to go over the axis again (the same in all of its threads). Channels past C hold what lay in LDS
+  // and do not count, nor does a lane's column unless it is `mine`.
+  template <int NT>
+  __device__ __forceinline__ bool again(const f16x (&acc)[NT], int C, bool mine) {
+    if constexpr (!ON) return false;
+    f4 bad = f4{};  // stays 0 over finite numbers
+#pragma unroll
+    for (int tt = 0; tt < NT; tt++)
+#pragma unroll
+      for (int qq = 0; qq < 4; qq++) {
+        if (32 * tt + 8 * qq >= C) break;
+#pragma unroll
+        for (int e = 0; e < 4; e++) bad[e] = fmaf(acc[tt][4 * qq + e], 0.f, bad[e]);
+      }
+    const bool more = !(both_sum((bad[0] + bad[1]) + (bad[2] + bad[3])) == 0.f) && mine && by > 0x1p-24f;
+    by = more ? by * 0x1p-12f : by;
+    return __syncthreads_or(more);
+  }
+};
+
 // dq: a wave holds 32 queries as the columns of S^T, as the forward pass does. The sum's reciprocal is a row's own, so that it
 // (in fp16: what root() leaves of it) scales dq at the end and ds is rounded before it. TWO: dO has a second part.
 // 2 x 16 x 2000 x 2000 in 64 channels bf16 with a gate 133 to 146 us (matrix cores 38% busy, some pipe issuing 77% of the
@@ -112,7 +158,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
   const float* mask = a.mask ? a.mask + un.smp * a.M : nullptr;
   const int64_t srow = ((int64_t)un.smp * a.H + un.h) * a.N + jc;
   RowStat rs(static_cast<const f4*>(a.rows)[srow]);
-  // A sum of K terms of a size is some sqrt(K) of it: with p at sqrt(K / C) times its size, ds leaves fp16's range where dq does.
+  // A sum of K terms of a size is some sqrt(K) of it: with p at sqrt(K / C) times its size, ds leaves fp16's range where dq of
+  // keys of size one does.
   float less = 0.f;
   if constexpr (std::is_same<T, half_t>::value) less = rs.root(a.C);
   const bool some_big = __any(rs.ex.big());
@@ -134,12 +181,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
     }
   }
   f16x dq[NT], pk[MEND ? NT : 1];
-  float off = 0.f, taken = 0.f;  // the row's sums of ds and of what its products take for it
-#pragma unroll
-  for (int tt = 0; tt < NT; tt++) {
-    dq[tt] = f16x{};
-    if constexpr (MEND) pk[tt] = f16x{};
-  }
+  float off, taken;  // the row's sums of ds and of what its products take for it
+  Scale<T> scale;
 
   Stage<T, KS, BK, F::NTH, true> ks, vs;
   BiasRows<BT, BK> bs;
@@ -153,75 +196,89 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
     if (bias) bs.load(bias, brows, (int)a.M, (int)k0);
   };
   constexpr int STEP = F::GROUPS * BK;
-  int64_t k0 = group * BK;
-  if (k0 < a.M) {
-    fetch(k0);
-    fetch_bias(k0);
-  }
-  const bool masked = mask && any_key(mask, a.M);  // the first loads are on their way
-  for (int buf = 0; k0 < a.M; k0 += STEP, buf = (buf + 1) % F::BUFS) {
-    const uint64_t keep = __ballot(k0 + l < a.M && l < BK && (!masked || mk != 0.f));
-    T* const Kb = Kt + buf * TILE;
-    T* const Vb = Vt + buf * TILE;
-    ks.store(Kb, keep, a.C, t);
-    vs.store(Vb, keep, a.C, t);
-    if (bias) bs.store(Bt, (int)a.M, (int)k0);
-    F::sync();
-    const bool more = k0 + STEP < a.M;
-    if (more) {
-      fetch(k0 + STEP);
-      fetch_bias(k0 + STEP);
+  int64_t k0;
+  const auto start = [&] {
+    off = taken = 0.f;
+#pragma unroll
+    for (int tt = 0; tt < NT; tt++) {
+      dq[tt] = f16x{};
+      if constexpr (MEND) pk[tt] = f16x{};
     }
-#pragma unroll
-    for (int kt = 0; kt < KT; kt++) {
-      f16x x = f16x{}, dp = f16x{};
-#pragma unroll
-      for (int m = 0; m < KS; m++) {
-        x = mma(row_frag<T, KS>(Kb, 32 * kt + (l & 31), m), qf[m], x);
-        const frag<T> vm = row_frag<T, KS>(Vb, 32 * kt + (l & 31), m);
-        dp = mma(vm, df[m], dp);
-        if constexpr (ASIDE) dp = mma(vm, aside[(wave * KS + m) * 64 + l], dp);
-        else if constexpr (TWO) dp = mma(vm, dl[m], dp);
+    k0 = Scale<T>::first(group * BK);
+    if (k0 < a.M) {
+      fetch(k0);
+      fetch_bias(k0);
+    }
+  };
+  start();
+  const bool masked = mask && any_key(mask, a.M);  // the first loads are on their way
+  bool more;
+  do {
+    for (int buf = 0; k0 < a.M; k0 += STEP, buf = (buf + 1) % F::BUFS) {
+      const uint64_t keep = __ballot(k0 + l < a.M && l < BK && (!masked || mk != 0.f));
+      T* const Kb = Kt + buf * TILE;
+      T* const Vb = Vt + buf * TILE;
+      ks.store(Kb, keep, a.C, t);
+      vs.store(Vb, keep, a.C, t);
+      if (bias) bs.store(Bt, (int)a.M, (int)k0);
+      F::sync();
+      if (k0 + STEP < a.M) {
+        fetch(k0 + STEP);
+        fetch_bias(k0 + STEP);
       }
-      f16x b = f16x{};
-      if (bias) b = BiasRows<BT, BK>::get(Bt, kt);
 #pragma unroll
-      for (int i = 0; i < 16; i++) x[i] = fmaf(x[i], a.scale, b[i]);
-      exponentials(x, rs.ex, some_big, less);
+      for (int kt = 0; kt < KT; kt++) {
+        f16x x = f16x{}, dp = f16x{};
 #pragma unroll
-      for (int i = 0; i < 16; i++) dp[i] = x[i] * (dp[i] - rs.delta);
-      if (keep != all_rows(BK)) {
-        const uint32_t w = (uint32_t)(keep >> (32 * kt)) >> (16 * hl);
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const bool on = w >> i & 1;
-          x[i] = on ? x[i] : 0.f;
-          dp[i] = on ? dp[i] : 0.f;
+        for (int m = 0; m < KS; m++) {
+          x = mma(row_frag<T, KS>(Kb, 32 * kt + (l & 31), m), qf[m], x);
+          const frag<T> vm = row_frag<T, KS>(Vb, 32 * kt + (l & 31), m);
+          dp = mma(vm, df[m], dp);
+          if constexpr (ASIDE) dp = mma(vm, aside[(wave * KS + m) * 64 + l], dp);
+          else if constexpr (TWO) dp = mma(vm, dl[m], dp);
         }
-      }
+        f16x b = f16x{};
+        if (bias) b = BiasRows<BT, BK>::get(Bt, kt);
 #pragma unroll
-      for (int s = 0; s < 2; s++) {
-        const frag<T> d = as_frag<T>(dp, s), p = as_frag<T>(x, s);
-        if constexpr (MEND) {
+        for (int i = 0; i < 16; i++) x[i] = fmaf(x[i], a.scale, b[i]);
+        exponentials(x, rs.ex, some_big, less);
 #pragma unroll
-          for (int e = 0; e < 8; e++) {
-            off += dp[8 * s + e];
-            taken += (float)d[e];
+        for (int i = 0; i < 16; i++) dp[i] = x[i] * (dp[i] - rs.delta);
+        if (keep != all_rows(BK)) {
+          const uint32_t w = (uint32_t)(keep >> (32 * kt)) >> (16 * hl);
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const bool on = w >> i & 1;
+            x[i] = on ? x[i] : 0.f;
+            dp[i] = on ? dp[i] : 0.f;
           }
         }
 #pragma unroll
-        for (int tt = 0; tt < NT; tt++) {
-          const frag<T> kf = col_frag<T, KS>(Kb, 32 * kt + 16 * s, tt);
-          dq[tt] = mma(kf, d, dq[tt]);
-          if constexpr (MEND) pk[tt] = mma(kf, p, pk[tt]);
+        for (int s = 0; s < 2; s++) {
+          const frag<T> d = scale.as_frag(dp, s), p = as_frag<T>(x, s);
+          if constexpr (MEND) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              off += dp[8 * s + e];
+              taken += (float)d[e];
+            }
+          }
+#pragma unroll
+          for (int tt = 0; tt < NT; tt++) {
+            const frag<T> kf = col_frag<T, KS>(Kb, 32 * kt + 16 * s, tt);
+            dq[tt] = mma(kf, d, dq[tt]);
+            if constexpr (MEND) pk[tt] = mma(kf, p, pk[tt]);
+          }
         }
       }
+      F::again();
+      if constexpr (!SPLIT) F::order();  // the biases are the wave's own
     }
-    F::again();
-    if constexpr (!SPLIT) F::order();  // the biases are the wave's own
-  }
+    more = scale.again(dq, a.C, true);
+    if (more) start();
+  } while (more);
   if constexpr (MEND) {
-    off = both_sum(off), taken = both_sum(taken);
+    off = both_sum(off), taken = both_sum(taken) * scale.back();
     if constexpr (SPLIT) {
       float* const sums = reinterpret_cast<float*>(lds);
       __syncthreads();
@@ -233,7 +290,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
     }
     off *= rs.inv, taken *= rs.inv;
 #pragma unroll
-    for (int tt = 0; tt < NT; tt++) dq[tt] -= taken * pk[tt];
+    for (int tt = 0; tt < NT; tt++) dq[tt] = dq[tt] * scale.back() - taken * pk[tt];
     // no other workgroup reads this row's, and this one's waves have what they need
     if (j < a.N && hl == 0 && (!SPLIT || wave == 0)) static_cast<float*>(a.rows)[4 * srow + 2] = rs.delta + off;
   }
@@ -303,8 +360,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
   }
   const float mk = mask ? mask[kc] : 1.f;
   f16x dk[NT], dv[NT];
-#pragma unroll
-  for (int tt = 0; tt < NT; tt++) dk[tt] = dv[tt] = f16x{};
+  Scale<T> scale;
 
   Stage<T, KS, BQ, F::NTH, false> qs, ds, ls;
   BT bs[16] = {};  // the next tile's biases, a row's 32 keys a half wave and instruction; zero where there are none
@@ -331,9 +387,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
     }
   };
   constexpr int STEP = F::GROUPS * BQ;
-  int64_t q0 = group * BQ;
-  fetch(q0);
-  fetch_bias(q0);
+  int64_t q0;
+  const auto start = [&] {
+#pragma unroll
+    for (int tt = 0; tt < NT; tt++) dk[tt] = dv[tt] = f16x{};
+    q0 = Scale<T>::first(group * BQ);
+    fetch(q0);
+    fetch_bias(q0);
+  };
+  start();
   const bool masked = mask && any_key(mask, a.M);  // of the whole workgroup; the first loads are on their way
   const bool on = key < a.M && (!masked || mk != 0.f);
 #pragma unroll
@@ -356,74 +418,79 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
       for (int i = 0; i < 16; i++) at.put(to, 8 * (i >> 2) + (i & 3), false, v[i]);
     }
   };
-  for (int buf = 0; q0 < a.N; q0 += STEP, buf = (buf + 1) % F::BUFS) {
-    const uint64_t rows = all_rows((int)min(a.N - q0, (int64_t)BQ));
-    T* const Qb = Qt + buf * TILE;
-    T* const Db = Dt + buf * TILE;
-    T* const Lb = Lt + buf * TILE;
-    float(*const Sb)[BQ] = St[group][buf];
-    qs.store(Qb, rows, a.C, t);
-    ds.store(Db, rows, a.C, t);
-    if constexpr (TWO) ls.store(Lb, rows, a.C, t);
-    if (t < BQ) {
-      if (q0 + t >= a.N) st = f4{INFINITY, 0.f, 0.f, LOG2E};  // past the end: 2^(y by - inf) = 0
+  bool more;
+  do {
+    for (int buf = 0; q0 < a.N; q0 += STEP, buf = (buf + 1) % F::BUFS) {
+      const uint64_t rows = all_rows((int)min(a.N - q0, (int64_t)BQ));
+      T* const Qb = Qt + buf * TILE;
+      T* const Db = Dt + buf * TILE;
+      T* const Lb = Lt + buf * TILE;
+      float(*const Sb)[BQ] = St[group][buf];
+      qs.store(Qb, rows, a.C, t);
+      ds.store(Db, rows, a.C, t);
+      if constexpr (TWO) ls.store(Lb, rows, a.C, t);
+      if (t < BQ) {
+        if (q0 + t >= a.N) st = f4{INFINITY, 0.f, 0.f, LOG2E};  // past the end: 2^(y by - inf) = 0
 #pragma unroll
-      for (int i = 0; i < 4; i++) Sb[i][t] = st[i];
-      Big[group][buf] = __any(st[3] != LOG2E);
-    }
-    F::sync();
-    const bool big = __builtin_amdgcn_readfirstlane(Big[group][buf]);  // a big row (Exponent)
-    fetch(q0 + STEP);
-#pragma unroll
-    for (int qt = 0; qt < QT; qt++) {
-      const int64_t r0 = q0 + 32 * qt;
-      if (r0 >= a.N) break;
-      const int64_t next = qt + 1 < QT ? r0 + 32 : q0 + STEP;
-      f16x x = f16x{}, dp = f16x{};
-#pragma unroll
-      for (int m = 0; m < KS; m++) {
-        x = mma(row_frag<T, KS>(Qb, 32 * qt + (l & 31), m), kf[m], x);
-        dp = mma(row_frag<T, KS>(Db, 32 * qt + (l & 31), m), vf[m], dp);
-        if constexpr (TWO) dp = mma(row_frag<T, KS>(Lb, 32 * qt + (l & 31), m), vf[m], dp);
+        for (int i = 0; i < 4; i++) Sb[i][t] = st[i];
+        Big[group][buf] = __any(st[3] != LOG2E);
       }
-      // A key that takes no part has what it has in its own column alone, which ends as zeros.
-      const auto probs = [&](auto any) {
+      F::sync();
+      const bool big = __builtin_amdgcn_readfirstlane(Big[group][buf]);  // a big row (Exponent)
+      fetch(q0 + STEP);
 #pragma unroll
-        for (int qq = 0; qq < 4; qq++) {
-          const int r = 32 * qt + 8 * qq + 4 * hl;
-          const f4 at = *reinterpret_cast<const f4*>(&Sb[0][r]);
-          const f4 inv = *reinterpret_cast<const f4*>(&Sb[1][r]);
-          const f4 delta = *reinterpret_cast<const f4*>(&Sb[2][r]);
-          f4 by = f4{LOG2E, LOG2E, LOG2E, LOG2E};
-          if constexpr (any()) by = *reinterpret_cast<const f4*>(&Sb[3][r]);
+      for (int qt = 0; qt < QT; qt++) {
+        const int64_t r0 = q0 + 32 * qt;
+        if (r0 >= a.N) break;
+        const int64_t next = qt + 1 < QT ? r0 + 32 : q0 + STEP;
+        f16x x = f16x{}, dp = f16x{};
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int i = 4 * qq + e;
-            float z = fmaf(fmaf(x[i], a.scale, (float)bs[i]), by[e], -at[e]);
-            if constexpr (any()) z = by[e] == 1.0f ? z * LOG2E : z;
-            x[i] = __builtin_amdgcn_exp2f(z) * inv[e];
-            dp[i] = x[i] * (dp[i] - delta[e]);
+        for (int m = 0; m < KS; m++) {
+          x = mma(row_frag<T, KS>(Qb, 32 * qt + (l & 31), m), kf[m], x);
+          dp = mma(row_frag<T, KS>(Db, 32 * qt + (l & 31), m), vf[m], dp);
+          if constexpr (TWO) dp = mma(row_frag<T, KS>(Lb, 32 * qt + (l & 31), m), vf[m], dp);
+        }
+        // A key that takes no part has what it has in its own column alone, which ends as zeros.
+        const auto probs = [&](auto any) {
+#pragma unroll
+          for (int qq = 0; qq < 4; qq++) {
+            const int r = 32 * qt + 8 * qq + 4 * hl;
+            const f4 at = *reinterpret_cast<const f4*>(&Sb[0][r]);
+            const f4 inv = *reinterpret_cast<const f4*>(&Sb[1][r]);
+            const f4 delta = *reinterpret_cast<const f4*>(&Sb[2][r]);
+            f4 by = f4{LOG2E, LOG2E, LOG2E, LOG2E};
+            if constexpr (any()) by = *reinterpret_cast<const f4*>(&Sb[3][r]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const int i = 4 * qq + e;
+              float z = fmaf(fmaf(x[i], a.scale, (float)bs[i]), by[e], -at[e]);
+              if constexpr (any()) z = by[e] == 1.0f ? z * LOG2E : z;
+              x[i] = __builtin_amdgcn_exp2f(z) * inv[e];
+              dp[i] = x[i] * (dp[i] - delta[e]);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // sixteen rows' statistics at once would not fit in the registers
           }
-          __builtin_amdgcn_sched_barrier(0);  // sixteen rows' statistics at once would not fit in the registers
-        }
-      };
-      if (big) probs(std::true_type());
-      else probs(std::false_type());
-      fetch_bias(next);
-      if (db) put_bias(r0, dp);
+        };
+        if (big) probs(std::true_type());
+        else probs(std::false_type());
+        fetch_bias(next);
+        if (db) put_bias(r0, dp);
 #pragma unroll
-      for (int s = 0; s < 2; s++) {
-        const frag<T> p = as_frag<T>(x, s), d = as_frag<T>(dp, s);
+        for (int s = 0; s < 2; s++) {
+          const frag<T> p = as_frag<T>(x, s), d = scale.as_frag(dp, s);
 #pragma unroll
-        for (int tt = 0; tt < NT; tt++) {
-          dv[tt] = mma(col_frag<T, KS>(Db, 32 * qt + 16 * s, tt), p, dv[tt]);
-          if constexpr (TWO) dv[tt] = mma(col_frag<T, KS>(Lb, 32 * qt + 16 * s, tt), p, dv[tt]);
-          dk[tt] = mma(col_frag<T, KS>(Qb, 32 * qt + 16 * s, tt), d, dk[tt]);
+          for (int tt = 0; tt < NT; tt++) {
+            dv[tt] = mma(col_frag<T, KS>(Db, 32 * qt + 16 * s, tt), p, dv[tt]);
+            if constexpr (TWO) dv[tt] = mma(col_frag<T, KS>(Lb, 32 * qt + 16 * s, tt), p, dv[tt]);
+            dk[tt] = mma(col_frag<T, KS>(Qb, 32 * qt + 16 * s, tt), d, dk[tt]);
+          }
         }
       }
+      F::again();
     }
-    F::again();
-  }
+    more = scale.again(dk, a.C, on);
+    if (more) start();
+  } while (more);
   const int64_t at = (un.smp * a.M + kc) * pitch + hc;
   const auto put = [&](void* to, int tt, int qq, f4 r, float by) {
     const int c = 32 * tt + 8 * qq + 4 * hl;
@@ -432,7 +499,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
   };
   if constexpr (SPLIT) {
     f4 r[NT];
-    meet4<NT>(dk, reinterpret_cast<f4*>(lds), wave, l, 1.f, r);
+    meet4<NT>(dk, reinterpret_cast<f4*>(lds), wave, l, scale.back(), r);
 #pragma unroll
     for (int tt = 0; tt < NT; tt++) put(a.dk, tt, wave, r[tt], a.scale);
     meet4<NT>(dv, reinterpret_cast<f4*>(lds), wave, l, 1.f, r);
@@ -443,7 +510,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
     for (int tt = 0; tt < NT; tt++)
 #pragma unroll
       for (int qq = 0; qq < 4; qq++) {
-        put(a.dk, tt, qq, f4{dk[tt][4 * qq], dk[tt][4 * qq + 1], dk[tt][4 * qq + 2], dk[tt][4 * qq + 3]}, a.scale);
+        put(a.dk, tt, qq, f4{dk[tt][4 * qq], dk[tt][4 * qq + 1], dk[tt][4 * qq + 2], dk[tt][4 * qq + 3]}, a.scale * scale.back());
         put(a.dv, tt, qq, f4{dv[tt][4 * qq], dv[tt][4 * qq + 1], dv[tt][4 * qq + 2], dv[tt][4 * qq + 3]}, 1.f);
       }
   }
