@@ -57,6 +57,12 @@ __device__ __forceinline__ void numbers(const void* p, bool wide, int64_t i, int
   }
 }
 
+// The distance d from the lowest one, lo, held to `most` either way (past it all are alike: edges are at most 2^14 apart). Numbers
+// are below 2^62 in size, so that d takes 63 bits and d - lo may take 64.
+__device__ __forceinline__ int from_lowest(int64_t d, int64_t lo, int64_t most) {
+  return (int)(d < lo - most ? -most : d > lo + most ? most : d - lo);
+}
+
 // Where a chunk of keys lies for a query: in one bucket (the first, the last, other groups') or in several.
 enum { FIRST, LAST, OTHER, MIXED };
 
@@ -96,8 +102,7 @@ struct Query {
   int from, kind;  // distance - lo of the chunk's first key, at most 2^30 either way
   bool same0, same1;
   __device__ __forceinline__ Query(const RelBias& a, const Keys<V>& k, int64_t pos, int64_t group) {
-    const int64_t d = pos - a.lo - k.base;
-    from = (int)(d < -2 * Keys<V>::FAR ? -2 * Keys<V>::FAR : d > 2 * Keys<V>::FAR ? 2 * Keys<V>::FAR : d);
+    from = from_lowest(pos - k.base, a.lo, 2 * Keys<V>::FAR);
     same0 = !a.group_k || group == k.group0;
     same1 = k.cut == V ? same0 : group == k.group1;
     kind = !same0 && !same1 ? OTHER : !same0 || !same1 ? MIXED : from - k.least <= 0 ? FIRST : from - k.most >= a.span - 1 ? LAST : MIXED;
@@ -122,8 +127,8 @@ struct Query {
 // The bucket of query i and key j from memory.
 __device__ __forceinline__ int bucket_of(const RelBias& a, const uint8_t* lut, int64_t i, int64_t j) {
   if (a.group_q && whole(a.group_q, a.wide, i) != whole(a.group_k, a.wide, j)) return a.count - 1;
-  const int64_t d = whole(a.pos_q, a.wide, i) - a.lo - whole(a.pos_k, a.wide, j);
-  return lut[d < 0 ? 0 : d >= a.span ? a.span - 1 : (int)d];
+  const int d = from_lowest(whole(a.pos_q, a.wide, i) - whole(a.pos_k, a.wide, j), a.lo, a.span);
+  return lut[min(max(d, 0), a.span - 1)];
 }
 
 // The batch element's own positions and groups.
@@ -252,8 +257,7 @@ typedef bf16_t b8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ f4 mma16(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f4 mma16(b8 a, b8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-constexpr int64_t BOUND = (int64_t)1 << 30;  // distances past it are all alike (edges are at most 2^14 apart)
-__device__ __forceinline__ int bounded(int64_t d) { return (int)(d < -BOUND ? -BOUND : d > BOUND ? BOUND : d); }
+constexpr int64_t BOUND = (int64_t)1 << 30;  // of distances from the lowest one
 
 constexpr int GK = 8;  // keys of a lane: a product's k = 8 (lane / 16) .. + 7
 
@@ -424,7 +428,7 @@ __global__ __launch_bounds__(256) void rel_bias_bwd_k(RelBias a, const T* __rest
       for (int u = 0; u < U; u++) f[u] = fetch(r0 + u);
       for (int64_t c0 = r0; c0 < r1; c0 += 64) {
         const int64_t r = min(c0 + l, r1 - 1);
-        const int at = bounded(whole(a.pos_q, a.wide, r) - a.lo - keys.base), n = (int)min(r1 - c0, (int64_t)64);
+        const int at = from_lowest(whole(a.pos_q, a.wide, r) - keys.base, a.lo, BOUND), n = (int)min(r1 - c0, (int64_t)64);
         const int64_t group = a.group_q ? whole(a.group_q, a.wide, r) : 0;
         const bool alien = group != (int)group, same = group == keys.first_group;  // alien: no key's group
         const bool low = same && at - keys.least <= 0, high = same && !low && at - keys.most >= a.span - 1;
@@ -499,7 +503,7 @@ __global__ __launch_bounds__(256) void rel_bias_bwd_k(RelBias a, const T* __rest
         for (int e = 0; e < GK; e++) {
           const int64_t j = min(keys.j + e, a.M - 1);
           const bool other = a.group_k && whole(a.group_k, a.wide, j) != group;
-          d[e] = other ? others : bounded(pos - a.lo - whole(a.pos_k, a.wide, j));
+          d[e] = other ? others : from_lowest(pos - whole(a.pos_k, a.wide, j), a.lo, BOUND);
         }
         products(v, d, ~0u);
       }
