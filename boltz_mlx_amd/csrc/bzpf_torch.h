@@ -55,6 +55,11 @@ inline void check(int rc, const char* name) {
   if (rc != BZPF_OK) throw Failure(c10::str(name, " failed (", rc, "): ", lib.last_error()));
 }
 
+// A count as the entry points take it, in 32 bits: one that they do not hold is refused here, as they would see another.
+inline void count_fits(const char* name, const char* what, int64_t n) {
+  TORCH_CHECK_VALUE(n <= INT32_MAX, name, ": too many ", what, " (", n, ")");
+}
+
 template <typename... Ts>
 void on_gpu(const char* name, const Ts&... ts) {
   TORCH_CHECK_VALUE((... && (!ts.defined() || ts.is_cuda())), name, ": need ROCm device tensors");

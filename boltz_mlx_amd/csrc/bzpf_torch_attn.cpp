@@ -22,6 +22,8 @@ struct Rel {
         lo(lo_), count(count_), other(other_) {
     TORCH_CHECK_VALUE(lut.scalar_type() == at::kByte && lut.dim() == 1 && lut.is_contiguous() && lut.size(0) >= 1, name,
                       ": buckets must be made by rel_buckets");
+    count_fits(name, "distances", lut.size(0));
+    count_fits(name, "buckets", count);
     TORCH_CHECK_VALUE((pos_q.dim() == 1 || pos_q.dim() == 2) && (pos_k.dim() == 1 || pos_k.dim() == 2), name,
                       ": positions must be [n] or [B, n], got ", pos_q.sizes(), " and ", pos_k.sizes());
     TORCH_CHECK_VALUE(group_q.defined() == group_k.defined(), name, ": groups must be given for queries and keys, or for neither");
@@ -47,6 +49,7 @@ struct Rel {
                       name, ": ", what, " must be [", batched ? "B, " : "", "H, ", N, ", ", M, "], got ", t.sizes());
     TORCH_CHECK_VALUE(t.device() == lut.device(), name, ": ", what, " must be on ", lut.device());
     if (t.dim() == 4) batched = true, B = t.size(0);
+    count_fits(name, "heads", t.size(-3));
     return t.size(-3);
   }
   bool wide() const { return pos_q.scalar_type() == at::kLong; }
@@ -61,6 +64,7 @@ Tensor rel_bias(const Tensor& table, Rel r, const Tensor& add_, at::ScalarType t
   type_code(table);
   const int dt = type_code(to);
   const int64_t H = table.size(1);
+  count_fits(name, "heads", H);
   if (add_.defined()) {
     TORCH_CHECK_VALUE(r.meet(name, add_, "add") == H && add_.scalar_type() == to, name, ": add must have ", H,
                       " heads and the output's type");
@@ -157,6 +161,7 @@ struct QK {
                       name, ": k must have q's rows and heads of ", C, " channels, got ", k.sizes());
     TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type() && k.device() == q.device(), name, ": q and k must be of one type on one device");
     Hk = k.size(-1) / C;
+    count_fits(name, "heads", H > Hk ? H : Hk);
     for (int64_t i = 0; i + 1 < q.dim(); i++) rows *= q.size(i);
     rotary = rotary_.value_or(C);
     TORCH_CHECK_VALUE(rotary >= 0 && rotary <= C && rotary % 2 == 0, name, ": rotary must be even, 0 to ", C, ", got ", rotary);
@@ -268,6 +273,8 @@ struct Att {
     batched = q_.dim() == 3;
     S = batched ? q_.size(0) : 1, N = q_.size(-2), M = k_.size(-2), C = q_.size(-1) / H;
     TORCH_CHECK_VALUE(C % 8 == 0 && C <= 128, name, ": heads of 8 to 128 channels, a multiple of 8, got ", C);
+    count_fits(name, "samples", S);
+    count_fits(name, "heads", H);
     type_code(q_);
     TORCH_CHECK_VALUE(!g_.defined() || g_.sizes() == q_.sizes(), name, ": g must have q's shape");
     for (const Tensor& t : {k_, v_, g_})
