@@ -385,7 +385,9 @@ __global__ __launch_bounds__(256) void rel_bias_bwd_k(RelBias a, const T* __rest
         if constexpr (OH::PARTS == 1) {
           x[0][e] = v[e];
         } else {
-          const float hi = (float)(P)v[e], mid = (float)(P)(v[e] - hi);
+          // cut off, not rounded: the largest numbers would round to infinity
+          const auto cut = [](float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); };
+          const float hi = cut(v[e]), mid = cut(v[e] - hi);
           x[0][e] = (P)hi;
           x[1][e] = (P)mid;
           x[2][e] = (P)(v[e] - hi - mid);

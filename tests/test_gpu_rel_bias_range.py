@@ -55,3 +55,23 @@ def test_rel_bias_borders_far_from_zero(N, M):
         pq, pk = [sign * (2 ** 61 + i) for i in range(N)], [-sign * (2 ** 61 - 1) - sign * (i % 60) + sign * 40 for i in range(M)]
         at = check(EDGES[edges], pq, pk, F32)
         assert len(np.unique(at)) > 1
+
+
+@pytest.mark.parametrize("value", [float(np.finfo(np.float32).max), -3.395e38, 3e38, 2.0 ** -126, 1.5 * 2.0 ** -130])
+@pytest.mark.parametrize("M", [5, 40])
+def test_rel_bias_gradient_of_the_largest_and_smallest_numbers(value, M):
+    """One gradient in each bucket that is as large (or as small) as fp32 has them: the table's gradient is itself. Numbers below
+    2^-126 + 16 bits may lose what lies below bf16's smallest, 2^-133, in each of three parts."""
+    b = K().rel_buckets(list(range(-6, 8)))
+    pos = torch.arange(30, device="cuda")
+    dy = torch.zeros(2, 30, M, device="cuda")
+    want = np.zeros((b.count, 2))
+    for h in range(2):
+        for bucket in range(b.count):
+            j = (12 if M > 20 else 2) + (0 if h else 2)
+            i = j + bucket - 7  # the pair of the bucket's distance
+            if 0 <= i < 30:
+                dy[h, i, j] = value
+                want[bucket, h] = np.float32(value)
+    got = np64(K().rel_bias_bwd(dy, b, pos, torch.arange(M, device="cuda")))
+    assert np.abs(got - want).max() <= (0 if abs(value) > 1 else 3 * 2.0 ** -133)
