@@ -101,8 +101,11 @@ class AttentionPairBias(torch.nn.Module):
         """The update [B, N, c_s] with gradients for s, k_in, z or pair_bias, and the parameters, in s's type (fp32, fp16 or
         bf16; forward() carries none): torch's products around the attention kernels. Arguments as in forward(); k_in: s by
         default; z [B / multiplicity, N, M, c_z], or pair_bias [B / multiplicity, H, N, M], or neither. qk_norm and rel_bias
-        (QKNorm and RelativeBias of layers.positions) add the tokens' positions pos and chains chain ([N] or [B, N]; the
-        samples of a group share its first one's bias): queries and keys are the same tokens then."""
+        (QKNorm and RelativeBias of layers.positions) add the tokens' positions pos, [N] or [B, N], and chains chain, of pos's
+        shape and type (the samples of a group share its first one's bias): queries and keys are the same tokens then. A
+        position bias needs pos; norms without it do not rotate."""
+        if rel_bias is not None and pos is None:
+            raise ValueError("with_grad: rel_bias needs pos")
         linear, t = torch.nn.functional.linear, s.dtype
         B, N, _ = s.shape
         projs = (self.proj_q, self.proj_k, self.proj_v, self.proj_g)

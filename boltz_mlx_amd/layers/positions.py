@@ -27,7 +27,7 @@ class RelativeBias(torch.nn.Module):
         return K.RelBuckets(self.lut, self.lo, self.count, True)
 
     def forward(self, pos: torch.Tensor, chain=None, add=None, out_dtype=None) -> torch.Tensor:
-        """pos, chain: int32 or int64 [N] or [B, N]; add: a pair bias of the output's shape and type, added in the same pass.
+        """pos: int32 or int64 [N] or [B, N]; chain: of pos's shape and type; add: a pair bias of the output's shape and type, added in the same pass.
         With gradients for the table and add."""
         return A.rel_bias(self.table, self.buckets(), pos, group_q=chain, add=add, out_dtype=out_dtype)
 
