@@ -12,8 +12,9 @@
 //   leaves of each rounding what its key differs from the row's mean key by.
 // - dO is not a value of the type: it goes as two of them, the rounded one and the rest, in the products of dp and dv.
 // Without these the gradients were 1.7 to 2.3 times as far from the exact ones as their own rounding puts them, now 1.0
-// (dbias), 1.3 (dq), 1.4 (dk, dv) and 1.5 times (dg, from the output as it was rounded). Where ds is below fp16's 2^-14, dq errs
-// by about one of the type's smallest steps and dk by sqrt(N / C) of them; where it is past its largest number, Scale.
+// (dbias), 1.3 (dq), 1.4 (dk, dv) and 1.5 times (dg, from the output as it was rounded). Where ds is below fp16's 2^-14, dq and
+// dk err by about one of the type's smallest steps; where it is past its largest number, Scale. p below 2^-14 (tens of thousands of
+// keys) costs dv some sqrt(N) 2^-25 of dO.
 #include "bzpf_attn.h"
 
 namespace bzpf {
@@ -80,15 +81,19 @@ struct RowStat {
 
 // ds on its way into a product, for a lane's key (dk) or row (dq). In fp16 it may pass the type's largest number where the product
 // does not: a ds of 10^6 meets a query of 0.01 under 1 / sqrt(C). The accumulators are infinite or NaN then, and the lanes
-// that have such go over the other axis again with ds times 2^-12, at last 2^-24 (finite operands give |ds| below 2^40). The
+// that have such go over the other axis again with ds times 2^-12, and so on to 2^-23 (finite operands give |ds| below 2^38). The
 // largest scaled ds is 2^4 or more then, so that what others lose below 2^-14 is 2^-29 of it. Operands that are not finite take
-// the two rounds too (2 x 16 x 2000 x 2000 in 64 channels without a gate 540 us instead of 209). The other types' ds have fp32's
-// range. The multiplication and the check cost the backward pass 4% at that size (with a gate and a bias 323 -> 336 us), 11%
+// two or three rounds more too (2 x 16 x 2000 x 2000 in 64 channels without a gate 632 us instead of 207). The other types' ds have fp32's
+// range. The multiplication and the check cost the backward pass 4% at that size (with a gate and a bias 320 -> 331 us), 11%
 // where the registers of the split form were full (16 x 400 x 400, 64 channels with both 30.2 -> 33.7 us).
 template <typename T>
 struct Scale {
   static constexpr bool ON = std::is_same<T, half_t>::value;
-  float by = 1.f;
+  float by;
+  // n terms of a size in C channels: their product is some sqrt(n / C) of them where that is more than they are, and so small ones
+  // are lost where the product is.
+  __device__ __forceinline__ Scale(int64_t n, int C)
+      : by(ON && n > C ? (float)(1 << (31 - __builtin_clz((uint32_t)(n / C))) / 2) : 1.f) {}
   // Accumulator rows 16 s .. 16 s + 15 as the products take them.
   __device__ __forceinline__ frag<T> as_frag(const f16x& c, int s) const {
     if constexpr (!ON) return bzpf::as_frag<T>(c, s);
@@ -118,7 +123,7 @@ struct Scale {
 #pragma unroll
         for (int e = 0; e < 4; e++) bad[e] = fmaf(acc[tt][4 * qq + e], 0.f, bad[e]);
       }
-    const bool more = !(both_sum((bad[0] + bad[1]) + (bad[2] + bad[3])) == 0.f) && mine && by > 0x1p-24f;
+    const bool more = !(both_sum((bad[0] + bad[1]) + (bad[2] + bad[3])) == 0.f) && mine && by > 0x1p-23f;
     by = more ? by * 0x1p-12f : by;
     return __syncthreads_or(more);
   }
@@ -182,7 +187,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
   }
   f16x dq[NT], pk[MEND ? NT : 1];
   float off, taken;  // the row's sums of ds and of what its products take for it
-  Scale<T> scale;
+  Scale<T> scale(0, a.C);  // root() is what dq needs
 
   Stage<T, KS, BK, F::NTH, true> ks, vs;
   BiasRows<BT, BK> bs;
@@ -360,7 +365,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && KS <= 4 ? 2 : 1) void attn_d
   }
   const float mk = mask ? mask[kc] : 1.f;
   f16x dk[NT], dv[NT];
-  Scale<T> scale;
+  Scale<T> scale(a.N, a.C);
 
   Stage<T, KS, BQ, F::NTH, false> qs, ds, ls;
   BT bs[16] = {};  // the next tile's biases, a row's 32 keys a half wave and instruction; zero where there are none

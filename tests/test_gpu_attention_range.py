@@ -126,6 +126,29 @@ def test_attention_small_gradients_of_few_keys(N, M):
         close(d[n], x, tol[n])
 
 
+@pytest.mark.parametrize("N, M, C", [(4000, 40, 8), (9000, 3, 24), (2500, 300, 16)])
+def test_attention_small_gradients_of_many_queries(N, M, C):
+    """dk as a sum of many ds far below 2^-14, each off by fp16's 2^-25 after its scaling by 2^k <= sqrt(N / C): 2^-25 / 2^k. Errors
+    of independent roundings within bounds b have squares of at most the sum of b^2 (b^2 / 3 where they are even)."""
+    H = 2
+    a = inputs(6, 1, 1, H, C, N, M, F16, "same", False, None)
+    dout = rand(8, 1, N, H * C, scale=2.0 ** -9 / N ** 0.5 * M ** 0.5, dtype=F16)
+    o, stats = call(a, H)
+    d = call_bwd(dout, a, H, o, stats)
+    _, _, _, grads = tolerances(a, H, F16, dout)
+    q, k, v, bias = (np64(a[n]) for n in ("q", "k", "v", "bias"))
+    x = heads(q, H) @ heads(k, H).swapaxes(-1, -2) / np.sqrt(C) + bias
+    p = np.exp(x - x.max(-1, keepdims=True))
+    p /= p.sum(-1, keepdims=True)
+    dp = heads(np64(dout), H) @ heads(v, H).swapaxes(-1, -2)
+    ds = p * (dp - (p * dp).sum(-1, keepdims=True))
+    assert np.median(np.abs(ds)) < 2.0 ** -14
+    h, tiny = 2.0 ** -11, 2.0 ** -25
+    b = (h * np.abs(ds) + tiny / 2.0 ** (int(np.log2(N // C)) // 2)) ** 2
+    bound = rows(b.swapaxes(-1, -2) @ heads(q, H) ** 2) / C + (h * np.abs(grads["k"]) + tiny) ** 2
+    assert ((np64(d["k"]) - grads["k"]) ** 2).sum() <= bound.sum()
+
+
 def test_attention_fp32_as_before():
     """fp32 operands have no such step."""
     a, dout = aligned(7, 1, 1, 2, 64, 8, 2, None, False, 0.02, 16.0, 2000.0)
