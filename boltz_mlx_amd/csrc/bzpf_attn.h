@@ -79,10 +79,14 @@ struct Form {
   }
 };
 
-// Split where 128-row workgroups would be fewer than 300 (half types; 512 in fp32, whose products are long enough to hide the
-// rest). dk/dv in us, wide and split, of n such workgroups: 48 channels fp16 n = 64: 25, 13; 192: 27, 27; 256: 28, 32; 288: 82,
-// 79; 320: 36, 40; 432: 91, 110; 24 channels fp32 n = 64: 44, 19; 288: 184, 137; 432: 202, 199; 512: 377, 389; 1024: 701, 754.
-// Heads past 96 channels have the wide form alone (their split form needs more registers than there are).
+// Split where 128-row workgroups would be fewer than 300 (half types; 512 in fp32). dk/dv in us, wide and split, with bias and
+// gate, of S H = 16, 48, 64, 72, 80, 128 heads of 400 x 400, which are 64, 192, 256, 288, 320, 512 such workgroups:
+//   48 channels fp16: 29, 14; 30, 29; 31, 33; 38, 34; 39, 42; 42, 57.   24 channels fp32: 44, 18; 45, 39; 47, 49; 72, 49; 72, 59; 74, 80.
+//   64 channels fp16: 29, 17; 30, 35; 31, 39; 39, 41; 40, 52; 44, 74.   64 channels fp32: 69, 29; 71, 82; 74, 109; 122, 110; 121, 135; 126, 190.
+// The forward pass and dq turn at about the same places. One limit for all loses where the wide form fills the chip once, at 192 to 256
+// workgroups of 64 and more channels (96 channels fp16 at 256: 42, 76), in fp32 of 64 channels at 320 and more too, and where a head's
+// last workgroup is nearly empty. Heads past 96 channels have the wide form alone (their split form needs more registers than
+// there are; the gated split form of 64 channels spills 5 to 14 of them in fp16).
 constexpr int SPLIT_STEPS = 6;
 static inline bool attn_split(int64_t rows, const Attn& a) {
   return a.C <= 16 * SPLIT_STEPS && (rows + 127) / 128 * a.S * a.H < (a.dt == DT_F32 ? 512 : 300);

@@ -71,10 +71,10 @@ enum { FIRST, LAST, OTHER, MIXED };
 template <int V>
 struct Keys {
   int rel[V], least, most, cut;
-  int64_t base, group0, group1, at;
+  int64_t base, group0, group1;
   bool rare;
-  __device__ __forceinline__ void load(const RelBias& a, int64_t at_, int n) {
-    at = at_, rare = false, cut = V, least = most = 0;
+  __device__ __forceinline__ void load(const RelBias& a, int64_t at, int n) {
+    rare = false, cut = V, least = most = 0;
     int64_t pos[V], group[V];
     numbers(a.pos_k, a.wide, at, n, pos);
     if (a.group_k) numbers(a.group_k, a.wide, at, n, group);

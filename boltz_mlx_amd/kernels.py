@@ -321,7 +321,7 @@ class RelBuckets(NamedTuple):
 def rel_buckets(edges, other: bool = False, device="cuda") -> RelBuckets:
     """Buckets between the integers `edges` (rising): a distance pos_q - pos_k lies in the bucket with the number of edges at
     or below it, so that clipped_edges(32) gives each distance from -32 to 32 its own and those beyond the last ones; one more
-    bucket for pairs of different groups (chains) where `other`. At most 256 buckets, edges at most 16384 apart."""
+    bucket for pairs of different groups (chains) where `other`. At most 256 buckets, edges at most 16382 apart."""
     edges = [int(e) for e in edges]
     if any(b <= a for a, b in zip(edges, edges[1:])):
         raise ValueError("rel_buckets: edges must rise")

@@ -397,7 +397,7 @@ int bzpf_pair_bias(const float* z, const float* ln_w, const float* ln_b, float e
  * [count][H] and add (or NULL) of out's type and shape [B][H][N][M]. k is the bucket of the pair's distance d = pos_q[i] -
  * pos_k[j]: lut[d - lo], lut[0] below and lut[span - 1] above (lut uint8 [span] on the device, not falling, entries below
  * count); where groups are given, pairs of different groups lie in bucket count - 1. pos_q / group_q [N], pos_k / group_k
- * [M], int64 where wide, else int32, of absolute value below 2^62; batch element b's start b * batch_q (b * batch_k) elements
+ * [M], int64 where wide, else int32, of absolute value below 2^62, as is lo; batch element b's start b * batch_q (b * batch_k) elements
  * on (0: shared). 1 <= count <= 256, 1 <= span <= 16384. */
 int bzpf_rel_bias(const float* table, const unsigned char* lut, int64_t lo, int span, int count, const void* pos_q,
                   const void* pos_k, const void* group_q, const void* group_k, int wide, int64_t batch_q, int64_t batch_k,
