@@ -90,7 +90,7 @@ int bzpf_rel_bias(const float* table, const unsigned char* lut, int64_t lo, int 
 
 int64_t bzpf_rel_bias_bwd_ws(int64_t B, int H, int64_t N, int64_t M, int count) {
   if (B < 1 || B > 65535 || H < 1 || H > 65535 || N < 1 || M < 1 || N > INT32_MAX || M > INT32_MAX || count < 1 || count > 256 ||
-      product(B, H, N, M) < 0)
+      product(B, H, N, M) < 0 || B * ((H + 15) / 16) > 65535)
     return -1;
   return bzpf::rel_bias_bwd_ws_bytes(B, H, N, M, count);
 }
@@ -216,6 +216,14 @@ namespace {
 constexpr int64_t ATT_LEN = 1 << 22, ATT_PITCH = 1 << 23;  // what the kernels' 32-bit offsets within a block hold
 constexpr int64_t WORKGROUPS = (1 << 24) - 8;              // a launch has fewer than 2^32 threads, 256 a workgroup
 
+// Whether sizes are such that no product of them below overflows, and a launch holds them.
+bool attn_sizes(int S, int H, int C, int64_t N, int64_t M) {
+  if (S < 1 || H < 1 || H > 65535 || C < 8 || C > 128 || C % 8 || N < 1 || M < 1 || N > ATT_LEN || M > ATT_LEN) return false;
+  const int64_t most = N > M ? N : M, groups = product(S, H, (most + 31) / 32, 1), chunks = product(S, H, N, (C + 7) / 8);
+  return groups >= 0 && groups <= WORKGROUPS && chunks >= 0 && chunks < (int64_t)1 << 31 && product(S, H, N, M) >= 0 &&
+         product(S, most, H, 4 * C) >= 0;
+}
+
 int make_attn(const char* who, const void* q, int64_t ldq, int64_t sq, const void* k, int64_t ldk, int64_t sk, const void* v,
               int64_t ldv, int64_t sv, const void* g, int64_t ldg, int64_t sg, const void* bias, int bias_dt, int mult,
               const float* mask, const void* out, const float* stats, int dt, int S, int H, int C, int64_t N, int64_t M,
@@ -226,10 +234,9 @@ int make_attn(const char* who, const void* q, int64_t ldq, int64_t sq, const voi
   REQUIRE(C >= 8 && C <= 128 && C % 8 == 0, "%s: heads of 8 to 128 channels, a multiple of 8 (C=%d)", who, C);
   REQUIRE(S >= 1 && H >= 1 && H <= 65535 && mult >= 1 && S % mult == 0, "%s: bad sample or head counts (S=%d H=%d mult=%d)",
           who, S, H, mult);
-  REQUIRE(N >= 1 && M >= 1 && N <= ATT_LEN && M <= ATT_LEN && product(S, H, N, M) >= 0 && product(S, N > M ? N : M, H, 4 * C) >= 0,
-          "%s: 1 to 2^22 queries and keys (N=%lld M=%lld)", who, (long long)N, (long long)M);
-  REQUIRE(product(S, H, ((N > M ? N : M) + 31) / 32, 1) <= WORKGROUPS && product(S, H, N, (C + 7) / 8) < (int64_t)1 << 31,
-          "%s: too many samples, heads and rows for a launch (S=%d H=%d N=%lld M=%lld)", who, S, H, (long long)N, (long long)M);
+  REQUIRE(N >= 1 && M >= 1 && N <= ATT_LEN && M <= ATT_LEN, "%s: 1 to 2^22 queries and keys (N=%lld M=%lld)", who, (long long)N,
+          (long long)M);
+  REQUIRE(attn_sizes(S, H, C, N, M), "%s: too many samples, heads and rows for a launch (S=%d H=%d N=%lld M=%lld)", who, S, H, (long long)N, (long long)M);
   REQUIRE(q && k && v && out && stats, "%s: NULL pointer", who);
   for (const void* p : {q, k, v, g, out}) REQUIRE(aligned_el(p, dt), "%s: a tensor is misaligned", who);
   REQUIRE(aligned_el(bias, bias_dt) && aligned_el(mask, BZPF_F32) && aligned_el(stats, BZPF_F32), "%s: a tensor is misaligned", who);
@@ -252,7 +259,7 @@ int make_attn(const char* who, const void* q, int64_t ldq, int64_t sq, const voi
 extern "C" {
 
 int64_t bzpf_attention_ws(int S_, int H, int C, int64_t N, int64_t M) {
-  if (S_ < 1 || H < 1 || H > 65535 || C < 8 || C > 128 || C % 8 || N < 1 || N > ATT_LEN || M < 1 || M > ATT_LEN) return -1;
+  if (!attn_sizes(S_, H, C, N, M)) return -1;
   bzpf::Attn a{};
   a.S = S_, a.H = H, a.C = C, a.N = N, a.M = M;
   return bzpf::attention_ws_bytes(a);
@@ -278,9 +285,7 @@ int bzpf_attention(const void* q, int64_t ldq, int64_t sq, const void* k, int64_
 }
 
 int64_t bzpf_attention_bwd_ws(int dt, int S_, int H, int C, int64_t N, int64_t M, int gate) {
-  if (!dt3_ok(dt) || S_ < 1 || H < 1 || H > 65535 || C < 8 || C > 128 || C % 8 || N < 1 || N > ATT_LEN || M < 1 || M > ATT_LEN ||
-      product(S_, N > M ? N : M, H, 4 * C) < 0)
-    return -1;
+  if (!dt3_ok(dt) || !attn_sizes(S_, H, C, N, M)) return -1;
   return bzpf::attention_bwd_ws_bytes(dt, S_, N, H, C, gate != 0);
 }
 

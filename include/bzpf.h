@@ -436,7 +436,7 @@ int bzpf_qk_norm_rope_bwd(const void* dqn, const void* dkn, int y_dt, const void
  * elements apart, in dt; pitches below 2^23, N and M up to 2^22, S H ceil(max(N, M) / 32) below 2^24; g NULL: no gate. bias (or NULL) [S / mult][H][N][M] in
  * bias_dt (dt, or fp16 / bf16 with fp32 operands), shared by consecutive groups of mult samples; mask (or NULL) fp32 [S][M]. out [S][N][H C] in dt; stats fp32
  * [S][H][N][2]: a row's largest logit and the sum of exp(logit - that). What bzpf_seq_attention_batched computes, for any N
- * and M, in bf16 too. ws: bzpf_attention_ws bytes, 16-byte aligned (NULL where that is 0): few queries split a long key axis. */
+ * and M, in bf16 too. ws: bzpf_attention_ws bytes (-1 for sizes that are refused), 16-byte aligned (NULL where that is 0): few queries split a long key axis. */
 int64_t bzpf_attention_ws(int S, int H, int C, int64_t N, int64_t M);
 int bzpf_attention(const void* q, int64_t ldq, int64_t sq, const void* k, int64_t ldk, int64_t sk, const void* v, int64_t ldv,
                    int64_t sv, const void* g, int64_t ldg, int64_t sg, const void* bias, int bias_dt, int mult,
@@ -445,7 +445,7 @@ int bzpf_attention(const void* q, int64_t ldq, int64_t sq, const void* k, int64_
 
 /* Its gradients for dout [S][N][H C] (dt, contiguous) at its output and statistics: dq, dk, dv, dg contiguous in dt (dg NULL
  * where g is), dbias in bias_dt (NULL where not wanted), summed over the samples that share it. ws: bzpf_attention_bwd_ws
- * bytes (gate: g is given), 16-byte aligned. No atomics: equal inputs give equal bits. */
+ * bytes (gate: g is given; -1 as above), 16-byte aligned. No atomics: equal inputs give equal bits. */
 int64_t bzpf_attention_bwd_ws(int dt, int S, int H, int C, int64_t N, int64_t M, int gate);
 int bzpf_attention_bwd(const void* dout, const void* q, int64_t ldq, int64_t sq, const void* k, int64_t ldk, int64_t sk,
                        const void* v, int64_t ldv, int64_t sv, const void* g, int64_t ldg, int64_t sg, const void* bias,

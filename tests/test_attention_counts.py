@@ -6,6 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from boltz_mlx_amd import _lib
 from boltz_mlx_amd import autograd as A
 from boltz_mlx_amd import kernels as K
 
@@ -50,3 +51,15 @@ def test_rel_bias_counts(of):
 def test_rel_bias_bwd_counts():
     b, pos = K.rel_buckets([0], device="cpu"), torch.arange(1)
     refused("heads", lambda: K.rel_bias_bwd(torch.zeros(1, 1, 1).expand(MANY, 1, 1), b, pos))
+
+
+def test_workspace_sizes_of_what_is_refused():
+    """Sizes whose products pass 64 bits, and such as no launch holds: -1, from the questions as from the calls."""
+    lib = _lib.load()
+    for S, H, N, M in ((1 << 27, 1 << 15, 1 << 22, 1), (1 << 26, 1 << 15, 1 << 22, 1), (2 ** 31 - 1, 65535, 1 << 22, 1 << 22), (2 ** 31 - 1, 65535, 1, 1),
+                       (1 << 20, 16, 5, 7), (4, 129, 1 << 22, 7), (128, 3, 5, 1 << 22)):
+        assert lib.bzpf_attention_ws(S, H, 8, N, M) == -1, (S, H, N, M)
+        assert lib.bzpf_attention_bwd_ws(1, S, H, 8, N, M, 1) == -1, (S, H, N, M)
+    assert lib.bzpf_attention_ws(1, 1, 128, 1 << 22, 1 << 22) == 0 < lib.bzpf_attention_bwd_ws(0, 1, 1, 128, 1 << 22, 1 << 22, 1)
+    assert lib.bzpf_rel_bias_bwd_ws(65535, 65535, 1, 1 << 29, 256) == -1 == lib.bzpf_rel_bias_bwd_ws(65535, 17, 1, 1, 8)
+    assert lib.bzpf_rel_bias_bwd_ws(65535, 16, 1, 1, 8) > 0
