@@ -348,7 +348,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> attention_bwd(const Tensor& d
     return {dq, dk, dv, dg, db};
   }
   const int64_t bytes = lib.attention_bwd_ws(type_code(a.q), (int)a.S, (int)a.H, (int)a.C, a.N, a.M, a.g.defined());
-  const Tensor ws = at::empty({bytes}, a.q.options().dtype(at::kByte));
+  const Tensor ws = at::empty({bytes > 0 ? bytes : 0}, a.q.options().dtype(at::kByte));  // none for sizes that the call refuses
   check(lib.attention_bwd(in(dout), BZPF_ROWS(a.q), BZPF_ROWS(a.k), BZPF_ROWS(a.v), BZPF_ROWS(a.g), in(a.bias), a.bias_type(),
                           (int)a.mult, f32(a.mask), in(o), f32(stats), out(dq), out(dk), out(dv), out(dg), out(db), out(ws), bytes,
                           type_code(a.q), (int)a.S, (int)a.H, (int)a.C, a.N, a.M, dev.stream),

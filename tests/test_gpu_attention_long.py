@@ -85,3 +85,15 @@ def test_attention_gradients_of_long_axes(S, mult, H, C, N, M, dtype):
     """Few queries against many keys, and few keys that many queries see."""
     for n, (bias, gate, mask) in enumerate([("same", True, "tail"), (None, False, None), ("same", False, "holes")]):
         check(inputs(10 * n + C, S, mult, H, C, N, M, dtype, bias, gate, mask), H)
+
+
+def test_attention_refuses_too_many_rows_by_name():
+    """More than 2^22 queries or keys: the package's own error from both directions."""
+    from boltz_mlx_amd._lib import BzpfError
+
+    many, one = torch.zeros(2 ** 22 + 1, 8, device="cuda", dtype=F16), torch.zeros(1, 8, device="cuda", dtype=F16)
+    for q, k in ((many, one), (one, many)):
+        with pytest.raises(BzpfError, match="1 to 2\\^22 queries and keys"):
+            K().attention(q, k, k, 1)
+        with pytest.raises(BzpfError, match="1 to 2\\^22 queries and keys"):
+            K().attention_bwd(q, q, k, k, 1, q, torch.zeros(1, len(q), 2, device="cuda"))
